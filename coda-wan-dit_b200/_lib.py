@@ -81,6 +81,10 @@ _SIGNATURES = {
     "wdit_rms_apply_layers": (c_int, [P, I, I, P, I, I, P, F, I, c_longlong, I, I, P]),
     "wdit_patch_rows": (c_int, [P, I, I, I, I, I, I, I, c_longlong, I, I, P, P]),
     "wdit_rope_table": (c_int, [P, I, I, I, I, I, P, P, P]),
+    "wdit_rel_pos_bias": (c_int, [P, I, P, I, I, I, I, I, I, P, P]),
+    "wdit_rel_pos_bias_grad_workspace_bytes": (c_longlong, [I, I, I, I, I, I]),
+    "wdit_rel_pos_bias_grad": (c_int, [P, I, I, I, I, I, c_longlong, c_longlong, c_longlong, P, I, I, I, P, P,
+                                       c_longlong, P]),
     "wdit_ulysses_pack": (c_int, [P, I, I, I, I, I, I, I, P, P]),
     "wdit_seq_gather": (c_int, [P, I, I, I, I, I, P, P]),
     "wdit_seq_scatter": (c_int, [P, c_longlong, c_longlong, I, I, I, I, P, P]),
@@ -155,6 +159,7 @@ _LAUNCHING = {
     "wdit_layernorm_modulation", "wdit_rmsnorm", "wdit_qk_rms_rope_from_partials", "wdit_rope_table",
     "wdit_ulysses_pack", "wdit_seq_gather", "wdit_seq_scatter", "wdit_ulysses_unpack",
     "wdit_p2p_qkv_exchange", "wdit_p2p_out_exchange", "wdit_p2p_wait",
+    "wdit_rel_pos_bias", "wdit_rel_pos_bias_grad",
 }
 launch_counter = {"n": 0}
 
@@ -167,7 +172,7 @@ def call(name: str, *args, kernels: int = 1) -> int:
     if name in _LAUNCHING:
         launch_counter["n"] += kernels
     rc = getattr(lib, name)(*args)
-    if isinstance(rc, int) and name not in ("wdit_gemm_norm_workspace_bytes", "wdit_static_scratch_bytes"):
+    if isinstance(rc, int) and not name.endswith("_bytes"):
         check(rc, name)
     return rc
 

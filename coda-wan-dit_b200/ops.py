@@ -551,3 +551,9 @@ def linear_bias_residual_fixed(A, B, C, bias, *, inplace: bool = False):
     assert A.shape[0] == C.shape[0] and B.shape[1] == C.shape[1]
     out = C if inplace else torch.empty_like(C)
     return gemm_residual(A, _weight_nk(B), C, out=out, bias=bias)
+
+
+# ---------------------------------------------------------------------------
+# Text-encoder operators
+# ---------------------------------------------------------------------------
+from .encoder_ops import rel_pos_bias, rel_pos_bias_grad, rel_pos_bounds  # noqa: E402,F401

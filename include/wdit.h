@@ -306,6 +306,29 @@ int wdit_qk_rms_rope_from_partials(void* qk, int ldqk, const float* partial, int
 int wdit_rope_table(const double* freqs_ri, int max_pos, int f, int h, int w, int pair_major, float* cos_out,
                     float* sin_out, void* stream);
 
+/* ---- text-encoder operators (no reference counterpart: the reference takes the encoder's
+ * output as given) ----
+ * dtype codes: 0 fp32, 1 bf16, 2 fp16.
+ *
+ * Relative position buckets: relative position d = key - (query + q_offset); its distance n = |d|
+ * (bidirectional != 0; keys ahead of the query, d > 0, take the upper half of the buckets) or
+ * max(-d, 0). bounds is a HOST array of n_bounds (1 .. 255) ascending distances >= 1; the bucket
+ * of n is the number of bounds <= n. The table has n_bounds + 1 rows, twice that if bidirectional.
+ */
+
+/* out[H, Lq, Lk] (contiguous, dtype) = table[bucket(j - (i + q_offset)), h], table [buckets, H]
+ * contiguous of the same dtype. */
+int wdit_rel_pos_bias(const void* table, int dtype, const int* bounds, int n_bounds, int bidirectional, int H, int Lq,
+                      int Lk, int q_offset, void* out, void* stream);
+
+/* Gradient of the table: dtable[buckets, H] (fp32) = sum of dbias[b, h, i, j] over b, i, j by
+ * bucket. dbias of dtype with element strides (>= 0) for b, h, i and unit stride for j. The
+ * workspace needs no initialization. Two launches; sums are fp32 in a fixed order. */
+long long wdit_rel_pos_bias_grad_workspace_bytes(int B, int H, int Lq, int Lk, int n_bounds, int bidirectional);
+int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, int Lk, long long stride_b,
+                           long long stride_h, long long stride_i, const int* bounds, int n_bounds, int bidirectional,
+                           int q_offset, float* dtable, void* workspace, long long workspace_bytes, void* stream);
+
 /* ---- sequence-parallel (Ulysses) regrouping; no reference counterpart (the reference is
  * single-GPU), these serve the token-sharded multi-GPU forward ----
  * Units: u = b*H + h over the B*H (batch, head) pairs, U = B*H/P units per rank, unit u on
