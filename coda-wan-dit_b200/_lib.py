@@ -85,6 +85,10 @@ _SIGNATURES = {
     "wdit_rel_pos_bias_grad_workspace_bytes": (c_longlong, [I, I, I, I, I, I]),
     "wdit_rel_pos_bias_grad": (c_int, [P, I, I, I, I, I, c_longlong, c_longlong, c_longlong, P, I, I, I, P, P,
                                        c_longlong, P]),
+    "wdit_linear_act_residual": (c_int, [P, c_longlong, I, P, c_longlong, I, I, I, I, I, P, I, I, P, c_longlong, P,
+                                         c_longlong, P, c_longlong, P]),
+    "wdit_act_backward_workspace_bytes": (c_longlong, [I, I]),
+    "wdit_act_backward": (c_int, [P, c_longlong, P, c_longlong, I, I, I, I, P, c_longlong, P, I, P, c_longlong, P]),
     "wdit_ulysses_pack": (c_int, [P, I, I, I, I, I, I, I, P, P]),
     "wdit_seq_gather": (c_int, [P, I, I, I, I, I, P, P]),
     "wdit_seq_scatter": (c_int, [P, c_longlong, c_longlong, I, I, I, I, P, P]),
@@ -159,7 +163,7 @@ _LAUNCHING = {
     "wdit_layernorm_modulation", "wdit_rmsnorm", "wdit_qk_rms_rope_from_partials", "wdit_rope_table",
     "wdit_ulysses_pack", "wdit_seq_gather", "wdit_seq_scatter", "wdit_ulysses_unpack",
     "wdit_p2p_qkv_exchange", "wdit_p2p_out_exchange", "wdit_p2p_wait",
-    "wdit_rel_pos_bias", "wdit_rel_pos_bias_grad",
+    "wdit_rel_pos_bias", "wdit_rel_pos_bias_grad", "wdit_linear_act_residual", "wdit_act_backward",
 }
 launch_counter = {"n": 0}
 

@@ -53,7 +53,9 @@
 #include <cstring>
 #include <mutex>
 
+#define WDIT_OWNS_ERROR_RECORD
 #include "ptx.cuh"
+#include "tmap.h"
 #include "wdit_internal.h"
 
 namespace wdit {
@@ -1296,6 +1298,27 @@ int error_record_ptr(unsigned int** out) {
 }
 
 unsigned long long wait_limit_ns() { return g_wait_limit_host; }
+
+int encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* ptr, const unsigned long long* dims,
+                 const unsigned long long* strides_bytes, const unsigned int* box, CUtensorMapSwizzle sw) {
+  if (!get_encoder()) return WDIT_ERR_DRIVER;
+  if (rank < 2 || rank > 5) return WDIT_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(ptr) & 15) != 0) return WDIT_ERR_ALIGN;
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], es[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    es[i] = 1;
+    if (i + 1 < rank) {
+      if ((strides_bytes[i] & 15) != 0) return WDIT_ERR_ALIGN;
+      st[i] = strides_bytes[i];
+    }
+  }
+  const CUresult r = g_encode(map, dt, rank, const_cast<void*>(ptr), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? WDIT_OK : WDIT_ERR_TMAP;
+}
 
 }  // namespace wdit
 

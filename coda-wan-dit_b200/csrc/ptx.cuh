@@ -16,12 +16,6 @@ namespace wdit {
 // Error reporting: the first failure wins; the host reads and clears it.
 // word 0 = error code, word 1 = site, word 2 = block index, word 3 = extra.
 // ---------------------------------------------------------------------------
-// Defined here (whole-program compilation without -rdc): this header is included by
-// exactly one translation unit (gemm.cu); other device code that needs bounded waits is
-// #included into that unit.
-__device__ unsigned int g_wdit_error[4];
-__device__ unsigned long long g_wdit_wait_limit_ns = 2000000000ull;  // 2 s
-
 enum ErrSite : unsigned int {
   kSiteProducerEmpty = 1,
   kSiteMmaFull = 2,
@@ -34,15 +28,34 @@ enum ErrSite : unsigned int {
 };
 constexpr unsigned int kErrTimeout = 0x7117;
 
-__device__ __forceinline__ void report_error(unsigned int code, unsigned int site,
-                                             unsigned int extra) {
-  if (atomicCAS(&g_wdit_error[0], 0u, code) == 0u) {
-    g_wdit_error[1] = site;
-    g_wdit_error[2] = blockIdx.x;
-    g_wdit_error[3] = extra;
+// Error record and wait limit as kernel arguments (error_record_ptr, wait_limit_ns), for kernels
+// outside the translation unit that owns the record.
+struct WaitCtx {
+  unsigned int* rec;
+  unsigned long long limit_ns;
+};
+
+__device__ __forceinline__ void report_error_to(unsigned int* rec, unsigned int code, unsigned int site,
+                                                unsigned int extra) {
+  if (atomicCAS(&rec[0], 0u, code) == 0u) {
+    rec[1] = site;
+    rec[2] = blockIdx.x;
+    rec[3] = extra;
     __threadfence();
   }
 }
+
+// The record itself lives in the translation unit that defines WDIT_OWNS_ERROR_RECORD (gemm.cu;
+// whole-program compilation without -rdc, so a second copy would never be read).
+#ifdef WDIT_OWNS_ERROR_RECORD
+__device__ unsigned int g_wdit_error[4];
+__device__ unsigned long long g_wdit_wait_limit_ns = 2000000000ull;  // 2 s
+
+__device__ __forceinline__ void report_error(unsigned int code, unsigned int site,
+                                             unsigned int extra) {
+  report_error_to(g_wdit_error, code, site, extra);
+}
+#endif
 
 __device__ __forceinline__ uint64_t globaltimer_ns() {
   uint64_t t;
@@ -102,6 +115,23 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 
 // Bounded wait for the phase with the given parity to complete.
 template <bool kCluster = false>
+__device__ __forceinline__ bool wait_parity(uint64_t* bar, uint32_t parity, unsigned int site, const WaitCtx& ctx) {
+  if (mbar_try_wait<kCluster>(bar, parity)) return true;
+  const uint64_t start = globaltimer_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i) {
+      if (mbar_try_wait<kCluster>(bar, parity)) return true;
+    }
+    if (globaltimer_ns() - start > ctx.limit_ns) {
+      report_error_to(ctx.rec, kErrTimeout, site, parity);
+      return false;
+    }
+  }
+}
+
+#ifdef WDIT_OWNS_ERROR_RECORD
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_parity(uint64_t* bar, uint32_t parity, unsigned int site) {
   if (mbar_try_wait<kCluster>(bar, parity)) return true;
   const uint64_t start = globaltimer_ns();
@@ -117,6 +147,7 @@ __device__ __forceinline__ bool wait_parity(uint64_t* bar, uint32_t parity, unsi
     }
   }
 }
+#endif
 
 // ---------------------------------------------------------------------------
 // Proxy fences / named barriers

@@ -33,7 +33,7 @@ __device__ __forceinline__ int rel_bucket(const int* bounds, int n_bounds, int b
   return bidirectional && d > 0 ? lo + n_bounds + 1 : lo;
 }
 
-inline int rel_num_buckets(int n_bounds, int bidirectional) { return (n_bounds + 1) * (bidirectional ? 2 : 1); }
+__host__ __device__ inline int rel_num_buckets(int n_bounds, int bidirectional) { return (n_bounds + 1) * (bidirectional ? 2 : 1); }
 
 // Host check and copy of the caller's bounds; false = not ascending positive distances.
 inline bool rel_fill(RelBuckets* rb, const int* bounds, int n_bounds, int bidirectional) {

@@ -2,6 +2,7 @@
 
 * ``rel_pos_bias`` / ``rel_pos_bias_grad``: a learned relative position bias by buckets and the
   gradient of its table.
+* ``linear_act_residual``: act(x W^T + bias) + residual in one kernel, with its gradients.
 
 Public names are re-exported by ``ops``, beside the GEMM and position-table ops of the block.
 Differentiable ops take part in autograd (first order); the others do not.
@@ -164,3 +165,152 @@ def rel_pos_bias(table: torch.Tensor, q_len: int, k_len: int, *, bidirectional: 
     if torch.is_grad_enabled() and table.requires_grad:
         return _RelPosBias.apply(table, q_len, k_len, bidirectional, max_distance, q_offset)
     return _rel_pos_bias(table, q_len, k_len, bidirectional, max_distance, q_offset)
+
+
+# ---------------------------------------------------------------------------
+# act(x W^T + bias) + residual
+# ---------------------------------------------------------------------------
+_ACT = {"none": 0, "gelu_tanh": 1, "relu": 2, "silu": 3, "gelu": 4}
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """2-D operand the kernels take as it is (unit column stride, rows on 16-byte boundaries),
+    or a contiguous copy."""
+    if t.shape[0] <= 1 and t.stride(1) == 1 and t.data_ptr() % 16 == 0:
+        return t.as_strided(t.shape, (t.shape[1], 1))  # a single row's stride says nothing
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _product(a, a_mn, b, b_mn, M, N, K, out, *, bias=None, act=0, res=None, pre=None):
+    call("wdit_linear_act_residual", ptr(a), a.stride(0), int(a_mn), ptr(b), b.stride(0), int(b_mn), M, N, K,
+         _DTYPE[a.dtype], ptr(bias), 0 if bias is None else _DTYPE[bias.dtype], act,
+         ptr(res), 0 if res is None else res.stride(0), ptr(out), out.stride(0),
+         ptr(pre), 0 if pre is None else pre.stride(0), stream_ptr())
+
+
+def _linear_forward(x2, w, bias, act, res2, out2, pre):
+    M, K = x2.shape
+    N = w.shape[0]
+    _product(_rows(x2), False, _rows(w), False, M, N, K, out2, bias=None if bias is None else bias.contiguous(),
+             act=_ACT[act], res=None if res2 is None else _rows(res2), pre=pre)
+
+
+class _LinearActResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, act, residual):
+        N = w.shape[0]
+        x2 = x.reshape(-1, x.shape[-1])
+        with torch.cuda.device(x.device):
+            out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+            out2 = out.view(-1, N)
+            # The derivative needs pre = x W^T + bias: kept in the operands' type (half a step of
+            # it moves act' by no more than rounding the gradient itself does).
+            need = any(ctx.needs_input_grad[:3]) and act != "none"
+            pre = torch.empty_like(out2) if need else None
+            res2 = None if residual is None else residual.reshape(-1, N)
+            _linear_forward(x2, w, bias, act, res2, out2, pre)
+        ctx.save_for_backward(x, w, pre)
+        ctx.act = act
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, w, pre = ctx.saved_tensors
+        need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
+        N, K = w.shape
+        x2 = x.reshape(-1, K)
+        M = x2.shape[0]
+        dx = dw = db = None
+        with torch.cuda.device(x.device):
+            g = _rows(dout.reshape(-1, N)) if need_x or need_w or need_b else None
+            if g is not None:
+                dpre = torch.empty((M, N), dtype=x.dtype, device=x.device) if pre is not None else g
+                ws, nbytes = None, 0
+                if need_b:
+                    db = torch.empty(N, dtype=ctx.bias_dtype, device=x.device)
+                    nbytes = call("wdit_act_backward_workspace_bytes", M, N)
+                    ws = _workspace(nbytes, x.device)
+                if need_b or pre is not None:
+                    call("wdit_act_backward", ptr(g), g.stride(0), ptr(pre), N, _ACT[ctx.act] if pre is not None else 0,
+                         _DTYPE[x.dtype], M, N, ptr(dpre), dpre.stride(0), ptr(db),
+                         0 if db is None else _DTYPE[db.dtype], ptr(ws), nbytes, stream_ptr(),
+                         kernels=2 if need_b else 1)
+                if need_x:
+                    dx = torch.empty((M, K), dtype=x.dtype, device=x.device)
+                    _product(dpre, False, _rows(w), True, M, K, N, dx)
+                    dx = dx.view(x.shape)
+                if need_w:
+                    if M == 0:
+                        dw = torch.zeros((N, K), dtype=w.dtype, device=w.device)
+                    else:
+                        dw = torch.empty((N, K), dtype=w.dtype, device=w.device)
+                        _product(dpre, True, _rows(x2), True, N, K, M, dw)
+        return dx, dw, db, None, dout if need_r else None
+
+
+def linear_act_residual(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *, act: str = "none",
+                        residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x @ w.T + bias) + residual in one kernel, summed in fp32 and rounded once.
+
+    x [..., K] and w [N, K] (nn.Linear.weight) bf16 or fp16, N and K multiples of 8; bias [N] of
+    fp32, bf16 or fp16; residual [..., N] and out of x's dtype; act one of "none", "relu",
+    "silu", "gelu" (erf), "gelu_tanh". Any number of rows, one included. out (contiguous; may be
+    the residual itself) is for calls outside autograd. Differentiable in x, w, bias and
+    residual. Operands whose rows do not start on 16-byte boundaries are copied first."""
+    if act not in _ACT:
+        raise ValueError(f"unknown activation {act!r} ({', '.join(_ACT)})")
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"x [..., K] and w [N, K] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
+    if x.dtype not in (torch.bfloat16, torch.float16) or w.dtype != x.dtype:
+        raise ValueError(f"x and w must both be bf16 or both fp16, got {x.dtype} and {w.dtype}")
+    N, K = w.shape
+    if N % 8 != 0 or K % 8 != 0 or N == 0 or K == 0:
+        raise ValueError(f"N and K must be multiples of 8, got N {N}, K {K}")
+    shape = (*x.shape[:-1], N)
+    if bias is not None and (bias.shape != (N,) or bias.dtype not in _DTYPE):
+        raise ValueError(f"bias must be [{N}] of fp32, bf16 or fp16, got {tuple(bias.shape)} {bias.dtype}")
+    for name, t in (("residual", residual), ("out", out)):
+        if t is not None and (t.shape != shape or t.dtype != x.dtype):
+            raise ValueError(f"{name} must be {shape} of {x.dtype}, got {tuple(t.shape)} {t.dtype}")
+    _require_cuda(x, w, bias, residual, out)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual, out))
+    if grad:
+        if out is not None:
+            raise ValueError("out= is not supported where a gradient is recorded")
+        return _LinearActResidual.apply(x, w, bias, act, residual)
+    with torch.cuda.device(x.device):
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        elif not out.is_contiguous() or out.data_ptr() % 16 != 0:
+            raise ValueError("out must be contiguous and start on a 16-byte boundary")
+        _check_out_overlap(out, residual, x, w, bias)
+        res2 = None if residual is None else residual.reshape(-1, N)
+        _linear_forward(x.reshape(-1, K), w, bias, act, res2, out.view(-1, N), None)
+    return out
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    if t.numel() == 0:
+        return (t.data_ptr(), t.data_ptr())
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return (t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size())
+
+
+def _check_out_overlap(out, residual, *inputs) -> None:
+    """out may be exactly the residual (every element is read before it is written); any other
+    overlap with an input would be read after it was overwritten."""
+    lo, hi = _extent(out)
+    for t in inputs:
+        if t is not None:
+            a, b = _extent(t)
+            if a < hi and lo < b:
+                raise ValueError("out overlaps an operand")
+    if residual is not None:
+        a, b = _extent(residual)
+        same = residual.data_ptr() == out.data_ptr() and residual.stride() == out.stride()
+        if a < hi and lo < b and not same:
+            raise ValueError("out partly overlaps the residual")

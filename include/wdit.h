@@ -329,6 +329,29 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
                            long long stride_h, long long stride_i, const int* bounds, int n_bounds, int bidirectional,
                            int q_offset, float* dtable, void* workspace, long long workspace_bytes, void* stream);
 
+/*
+ * out[M, N] = act(A . B^T + bias) + res, operands and out of dtype (bf16 or fp16), fp32 sums, one
+ * rounding. A is [M, K] with rows of lda elements (a_mn = 0) or stored transposed, [K, M] with rows
+ * of lda (a_mn = 1); B is [N, K] (b_mn = 0) or stored [K, N] (b_mn = 1); a_mn = 1 needs b_mn = 1.
+ * bias[N] of bias_dtype, res[M, N] and pre_out[M, N] (= A . B^T + bias, rounded) may be NULL; out
+ * may be res exactly (same pointer and leading dimension).
+ * act: 0 none, 1 tanh-GELU, 2 ReLU, 3 SiLU, 4 GELU (erf). N % 8 == 0; leading dimensions in
+ * elements, multiples of 8; pointers 16-byte aligned (bias: of its element).
+ */
+int wdit_linear_act_residual(const void* A, long long lda, int a_mn, const void* B, long long ldb, int b_mn, int M,
+                             int N, int K, int dtype, const void* bias, int bias_dtype, int act, const void* res,
+                             long long ldr, void* out, long long ldo, void* pre_out, long long ldp, void* stream);
+
+/*
+ * dpre[M, N] = dout * act'(pre) and, unless dbias is NULL, dbias[N] (dbias_dtype) = the column sums
+ * of dpre before its rounding (fp32 sums in a fixed order). act = 0: dpre is dout, pre and dpre are
+ * not looked at. The workspace (only with dbias) needs no initialization.
+ */
+long long wdit_act_backward_workspace_bytes(int M, int N);
+int wdit_act_backward(const void* dout, long long ldd, const void* pre, long long ldp, int act, int dtype, int M, int N,
+                      void* dpre, long long ldq, void* dbias, int dbias_dtype, void* workspace,
+                      long long workspace_bytes, void* stream);
+
 /* ---- sequence-parallel (Ulysses) regrouping; no reference counterpart (the reference is
  * single-GPU), these serve the token-sharded multi-GPU forward ----
  * Units: u = b*H + h over the B*H (batch, head) pairs, U = B*H/P units per rank, unit u on
