@@ -85,6 +85,12 @@ _SIGNATURES = {
     "wdit_rel_pos_bias_grad_workspace_bytes": (c_longlong, [I, I, I, I, I, I]),
     "wdit_rel_pos_bias_grad": (c_int, [P, I, I, I, I, I, c_longlong, c_longlong, c_longlong, P, I, I, I, P, P,
                                        c_longlong, P]),
+    "wdit_rel_attention_workspace_bytes": (c_longlong, [I, I, I, I, I]),
+    "wdit_rel_attention": (c_int, [P, P, P, P, P, P, I, I, I, I, I, I, P, P, I, P, I, I, I, I, F, P, P, P, c_longlong,
+                                   P]),
+    "wdit_rel_attention_backward_workspace_bytes": (c_longlong, [I, I, I, I, I]),
+    "wdit_rel_attention_backward": (c_int, [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, P, P, I, P, I, I, I, I, F,
+                                            P, P, P, P, P, c_longlong, P]),
     "wdit_linear_act_residual": (c_int, [P, c_longlong, I, P, c_longlong, I, I, I, I, I, P, I, I, P, c_longlong, P,
                                          c_longlong, P, c_longlong, P]),
     "wdit_act_backward_workspace_bytes": (c_longlong, [I, I]),
@@ -164,6 +170,7 @@ _LAUNCHING = {
     "wdit_ulysses_pack", "wdit_seq_gather", "wdit_seq_scatter", "wdit_ulysses_unpack",
     "wdit_p2p_qkv_exchange", "wdit_p2p_out_exchange", "wdit_p2p_wait",
     "wdit_rel_pos_bias", "wdit_rel_pos_bias_grad", "wdit_linear_act_residual", "wdit_act_backward",
+    "wdit_rel_attention", "wdit_rel_attention_backward",
 }
 launch_counter = {"n": 0}
 

@@ -1,0 +1,1389 @@
+// Attention that reads a learned relative position bias from its table.
+//
+//   S = scale q k^T + table[bucket(j - i - q_offset), h],  key j visible for j < k_lens[b] (and
+//   j <= i + q_offset when causal),  P = softmax(S) over the visible keys,  O = P v
+//   (a row that sees no key gives 0 and lse = -inf).
+//
+// Backward, with delta = rowsum(dO O) and lse kept by the forward:
+//   dV = P^T dO,  dP = dO v^T,  dS = P (dP - delta),  dQ = scale dS k,  dK = scale dS^T q,
+//   dtable[bucket, h] = the sum of dS over its cells.
+//
+// The bias is a function of the diagonal d = key - query, so a warp's tile of 32 rows needs 31 +
+// columns table values: they are looked up once per tile into a short line of shared memory (a
+// thread's row then reads consecutive entries, free of bank conflicts), or are one value when the
+// whole tile falls into one bucket, as it does away from the diagonal.
+//
+// All products run on the tensor cores (tcgen05, operands by TMA with the 128-byte swizzle,
+// accumulators in TMEM); the score tile is read from TMEM one row per thread, transformed in
+// registers and written back to TMEM in 16 bits as the A operand of the next product, so nothing
+// of size Lq x Lk leaves the SM.
+//
+//   attn_fwd_kernel  CTA = 128 query rows of one head; key tiles of 64; warp 0 loads, warp 1
+//                    issues MMAs, warps 2-5 softmax (one row per thread). Two score buffers: the
+//                    next tile's scores are computed while this one's are exponentiated. With few
+//                    CTAs the keys are split over several, whose parts attn_combine_kernel joins.
+//   attn_dq_kernel   same rows; computes delta, dQ and the table's partial sums. No atomics.
+//   attn_dkv_kernel  CTA = 128 keys; runs over query tiles of 64 with the scores transposed, so
+//                    P^T and dS^T are the A operands; dK and dV stay in TMEM.
+//
+// Keys past k_lens may hold anything (NaN included): their scores are replaced, and their rows of
+// an operand that is summed over are overwritten with zeros in shared memory.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "ptx.cuh"
+#include "relpos.cuh"
+#include "tmap.h"
+#include "wdit_internal.h"
+
+namespace wdit {
+
+int launch_rel_table_sum(const float* part, int parts, int buckets, int H, float* out, void* stream);
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_huge_valf();
+constexpr int kRows = 128;  // accumulator rows of a CTA
+constexpr int kCols = 64;   // columns of a score tile
+enum : unsigned int { kSiteAttn = 16, kSiteAttnDq = 32, kSiteAttnDkv = 48 };
+
+struct AttnArgs {
+  int B, H, Lq, Lk;
+  int causal, q_offset;
+  float scale;
+  const int* k_lens;   // [B] or nullptr
+  const void* table;   // [buckets, H]
+  int table_dtype;
+  RelBuckets rb;
+  void* out;           // [B, Lq, H, D] contiguous
+  float* lse;          // [B, H, Lq], log2 units; nullable
+  int splits;          // forward: key splits; > 1 writes part_o / part_lse instead
+  float* part_o;       // [splits][B * H * Lq][D]
+  float* part_lse;     // [splits][B * H * Lq]
+  // backward
+  const void* dout;    // element strides below, unit along D
+  long long do_b, do_l, do_h;
+  float* delta;        // [B, H, Lq]
+  void* dq;            // [B, Lq, H, D]
+  void* dk;            // [B, Lk, H, D]
+  void* dv;
+  float* table_part;   // [H][B * q tiles][buckets]
+  WaitCtx ctx;
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (BF16) return pack_bf16x2(a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+  if constexpr (BF16) return unpack_bf16x2(w);
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float table_value(const AttnArgs& p, int b, int h) {
+  const long long i = static_cast<long long>(b) * p.H + h;
+  if (p.table_dtype == 0) return static_cast<const float*>(p.table)[i];
+  if (p.table_dtype == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(p.table)[i]);
+  return __half2float(static_cast<const __half*>(p.table)[i]);
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int h, int l,
+                                            int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(h), "r"(l), "r"(b)
+      : "memory");
+}
+
+// D[tmem] (+)= A[tmem, 16-bit, two K elements per column] * B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32f(uint32_t taddr, const float* v) {
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+  tmem_st16(taddr, r);
+  tmem_st16(taddr + 16, r + 16);
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// MN-major operand tile: rows of 64 elements (128 B) along M or N, one row per K index; pieces of
+// 64 elements are 64 rows x 128 B apart.
+__device__ __forceinline__ uint64_t smem_desc_mn64(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(8192u >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+__host__ __device__ constexpr uint32_t idesc16(int m, int n, bool bf16, bool b_mn) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Score product of a 128-row tile (pieces of 64 columns 16 KB apart) and a 64-row tile (8 KB
+// apart), both K-major over D.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t a128, uint32_t b64, uint32_t idesc) {
+  const uint64_t a = smem_desc_sw128(a128), b = smem_desc_sw128(b64);
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k)
+    mma_bf16(d_tmem, a + (k >> 2) * 1024 + (k & 3) * 2, b + (k >> 2) * 512 + (k & 3) * 2, idesc, k != 0 ? 1u : 0u);
+}
+
+// acc[128, D] (+)= A[128 x 64, TMEM] * B[64 x D, shared memory rows]. SPREAD: the two 32-column
+// halves of A lie 32 TMEM columns apart (written by different warps), else 16.
+template <bool SPREAD>
+__device__ __forceinline__ void issue_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b64, uint32_t idesc, bool accum) {
+  const uint64_t b = smem_desc_mn64(b64);
+#pragma unroll
+  for (int k = 0; k < kCols / 16; ++k)
+    mma_ts(d_tmem, a_tmem + (SPREAD ? (k >> 1) * 32 + (k & 1) * 8 : k * 8), b + 128 * k, idesc,
+           accum || k != 0 ? 1u : 0u);
+}
+
+// Zero rows [first, 64) of a 64-row tile (whole 128-byte rows: the swizzle stays inside a row).
+template <int D>
+__device__ __forceinline__ void zero_tail(uint8_t* tile, int first, int lane) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+    for (int x = first * 8 + lane; x < 64 * 8; x += 32)
+      *reinterpret_cast<uint4*>(tile + c * 8192 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// The head's table column (times `mult`) and the bucket bounds in shared memory.
+__device__ __forceinline__ void load_table(const AttnArgs& p, int h, float mult, int* bounds, float* col, int buckets,
+                                           int threads) {
+  for (int t = threadIdx.x; t < p.rb.n_bounds; t += threads) bounds[t] = p.rb.bounds[t];
+  for (int t = threadIdx.x; t < buckets; t += threads) col[t] = table_value(p, t, h) * mult;
+}
+
+__device__ __forceinline__ int sample_len(const AttnArgs& p, int b) {
+  if (p.k_lens == nullptr) return p.Lk;
+  const int n = p.k_lens[b];
+  return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
+}
+
+__host__ __device__ constexpr int align_up(int x, int a) { return (x + a - 1) / a * a; }
+
+// ---------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------
+template <int D>
+struct Fwd {
+  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kThreads = 192;
+  static constexpr uint32_t kQ = kRows * D * 2;
+  static constexpr uint32_t kTile = kCols * D * 2;
+  static constexpr uint32_t kTmem = 256;  // two score buffers of 64 columns, O at 128
+  static constexpr int kLine = 96;        // per-warp bias line (31 + 64 diagonals)
+  static int smem(int buckets) {
+    return 1024 + kQ + kStages * 2 * kTile + 256 + 4 * kLine * 4 + 1024 + align_up(buckets * 4, 16);
+  }
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
+    attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs p) {
+  using C = Fwd<D>;
+  constexpr int ST = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + C::kQ;
+  uint8_t* sV = sK + ST * C::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * C::kTile);
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = bars + ST;
+  uint64_t* v_full = bars + 2 * ST;
+  uint64_t* v_empty = bars + 3 * ST;
+  uint64_t* q_full = bars + 4 * ST;
+  uint64_t* s_full = q_full + 1;  // 2
+  uint64_t* p_ready = s_full + 2;  // 2: a warp may finish its rows of t + 1 before another's of t
+  uint64_t* pv_done = p_ready + 2;
+  uint64_t* last = pv_done + 1;  // every product is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
+  float* lines = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
+  int* bounds = reinterpret_cast<int*>(lines + 4 * C::kLine);
+  float* col = reinterpret_cast<float*>(bounds + 256);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int q_tiles = (p.Lq + kRows - 1) / kRows;
+  // q tile fastest (its CTAs share K and V in L2), then split, head, sample; the last rows first,
+  // since under a causal mask they see most keys
+  int x = blockIdx.x;
+  const int qt = q_tiles - 1 - x % q_tiles;
+  x /= q_tiles;
+  const int split = x % p.splits;
+  x /= p.splits;
+  const int h = x % p.H;
+  const int b = x / p.H;
+  const int i0 = qt * kRows;
+  const int klen = sample_len(p, b);
+  int visible = klen;  // keys any row of the tile sees
+  if (p.causal) visible = min(visible, min(i0 + kRows, p.Lq) + p.q_offset);
+  int t0 = 0, t1 = (visible + kCols - 1) / kCols;
+  if (p.splits > 1) {
+    const int tiles = (klen + kCols - 1) / kCols;
+    const int per = (tiles + p.splits - 1) / p.splits;
+    t0 = split * per;
+    t1 = min(t1, t0 + per);
+  }
+  const int n = max(0, t1 - t0);
+  const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(&p_ready[0], 4);
+    mbar_init(&p_ready[1], 4);
+    mbar_init(pv_done, 1);
+    mbar_init(last, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kTmem);
+    tmem_relinquish();
+  }
+  load_table(p, h, kLog2e, bounds, col, buckets, C::kThreads);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem_o = tmem + 2 * kCols;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(q_full, C::kQ);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) tma_load_4d(sQ + c * 16384, &tmQ, q_full, c * 64, h, i0, b);
+      int k_loaded = 0, v_loaded = 0;
+      for (int t = 0; t < n; ++t) {
+        const int st = t % ST;
+        const uint32_t ph = (t / ST) & 1;
+        const int j0 = (t0 + t) * kCols;
+        if (!wait_parity(&k_empty[st], ph ^ 1u, kSiteAttn, p.ctx)) break;
+        mbar_arrive_expect_tx(&k_full[st], C::kTile);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(sK + st * C::kTile + c * 8192, &tmK, &k_full[st], c * 64, h, j0, b);
+        k_loaded = t + 1;
+        if (!wait_parity(&v_empty[st], ph ^ 1u, kSiteAttn + 1, p.ctx)) break;
+        mbar_arrive_expect_tx(&v_full[st], C::kTile);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(sV + st * C::kTile + c * 8192, &tmV, &v_full[st], c * 64, h, j0, b);
+        v_loaded = t + 1;
+      }
+      // Do not leave while a copy into this CTA's shared memory is in flight.
+      wait_parity(q_full, 0, kSiteAttn + 2, p.ctx);
+      for (int t = max(0, k_loaded - ST); t < k_loaded; ++t)
+        wait_parity(&k_full[t % ST], (t / ST) & 1, kSiteAttn + 2, p.ctx);
+      for (int t = max(0, v_loaded - ST); t < v_loaded; ++t)
+        wait_parity(&v_full[t % ST], (t / ST) & 1, kSiteAttn + 2, p.ctx);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t id_s = idesc16(kRows, kCols, BF16, false);
+    constexpr uint32_t id_o = idesc16(kRows, D, BF16, true);
+    auto scores = [&](int t) {
+      const int st = t % ST;
+      const bool ok = wait_parity(&k_full[st], (t / ST) & 1, kSiteAttn + 3, p.ctx);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        issue_scores<D>(tmem + (t & 1) * kCols, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
+        mma_commit(&k_empty[st]);
+        mma_commit(&s_full[t & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = true;
+    if (n > 0) {
+      ok = wait_parity(q_full, 0, kSiteAttn + 4, p.ctx);
+      ok = __all_sync(0xffffffffu, ok) && scores(0);
+    }
+    for (int t = 0; t < n && ok; ++t) {
+      if (t + 1 < n) {
+        // scores(t + 1) overwrite the buffer whose P the product of t - 1 reads: products into
+        // different accumulators are ordered by their completion only
+        if (t > 0) ok = __all_sync(0xffffffffu, wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 10, p.ctx));
+        if (!ok || !scores(t + 1)) break;
+      }
+      const int st = t % ST;
+      ok = wait_parity(&v_full[st], (t / ST) & 1, kSiteAttn + 5, p.ctx);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      const int j0 = (t0 + t) * kCols;
+      if (j0 + kCols > klen) zero_tail<D>(sV + st * C::kTile, klen - j0, lane);
+      ok = wait_parity(&p_ready[t & 1], (t >> 1) & 1, kSiteAttn + 6, p.ctx);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      if (lane == 0) {
+        issue_ts<false>(tmem_o, tmem + (t & 1) * kCols, smem_u32(sV + st * C::kTile), id_o, t > 0);
+        mma_commit(&v_empty[st]);
+        mma_commit(pv_done);
+        if (t + 1 == n) mma_commit(last);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int wq = warp & 3;
+    const int r = wq * 32 + lane;
+    const int i = i0 + r;
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    float* line = lines + wq * C::kLine;
+    const float scale2 = p.scale * kLog2e;
+    const int row_end = p.causal ? min(klen, i + p.q_offset + 1) : klen;  // keys this row sees
+    const int warp_first = i0 + wq * 32 + p.q_offset;                      // the warp's first position
+    float m_used = -kInf, l = 0.f;
+    bool ok = true;
+    for (int t = 0; t < n; ++t) {
+      const int j0 = (t0 + t) * kCols;
+      // the tile's bias: one value, or a line over its 31 + 64 diagonals
+      const int d_lo = j0 - warp_first - 31, d_hi = j0 + kCols - 1 - warp_first;
+      const int b_lo = rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo);
+      const bool flat = b_lo == rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_hi);
+      if (!flat) {
+        __syncwarp();  // the previous tile's reads are done
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          const int dd = lane + 32 * q;
+          line[dd] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + min(dd, 94))];
+        }
+        __syncwarp();
+      }
+      ok = wait_parity(&s_full[t & 1], (t >> 1) & 1, kSiteAttn + 7, p.ctx);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const uint32_t ts = tmem + lane_off + (t & 1) * kCols;
+      float z[kCols];
+      tmem_ld32(ts, z);
+      tmem_ld32(ts + 32, z + 32);
+      if (flat) {
+        const float c = col[b_lo];
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) z[e] = fmaf(z[e], scale2, c);
+      } else {
+        const float* ln = line + 31 - lane;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) z[e] = fmaf(z[e], scale2, ln[e]);
+      }
+      if (__any_sync(0xffffffffu, row_end < j0 + kCols)) {
+        const int keep = row_end - j0;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) z[e] = e < keep ? z[e] : -kInf;
+      }
+      float m4[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+      for (int e = 4; e < kCols; ++e) m4[e & 3] = fmaxf(m4[e & 3], z[e]);
+      const float m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      // The running maximum in use moves only when it is exceeded by more than 8 (a factor of 256
+      // in P, harmless in fp32 sums and in 16-bit P), so O is rarely rescaled.
+      if (__any_sync(0xffffffffu, m_tile > m_used + 8.f || (m_used == -kInf && m_tile > -kInf))) {
+        const float m_new = fmaxf(m_used, m_tile);
+        const float f = m_new == -kInf ? 1.f : exp2_approx(m_used - m_new);
+        l *= f;
+        m_used = m_new;
+        if (t > 0) {
+          ok = wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 8, p.ctx);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tmem_ld32(tmem_o + lane_off + c * 32, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= f;
+            tmem_st32f(tmem_o + lane_off + c * 32, o);
+          }
+        }
+      }
+      const float m_sub = m_used == -kInf ? 0.f : m_used;
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t w[kCols / 2];
+#pragma unroll
+      for (int e = 0; e < kCols; e += 2) {
+        const float a = exp2_approx(z[e] - m_sub), c = exp2_approx(z[e + 1] - m_sub);
+        s4[e & 2] += a;
+        s4[(e & 2) + 1] += c;
+        w[e >> 1] = pack16<BF16>(a, c);
+      }
+      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      tmem_st16(ts, w);
+      tmem_st16(ts + 16, w + 16);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[t & 1]);
+    }
+    if (ok && n > 0) {
+      ok = wait_parity(last, 0, kSiteAttn + 9, p.ctx);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const float lse = l > 0.f || l != l ? m_used + log2f(l) : -kInf;
+    const long long hrow = (static_cast<long long>(b) * p.H + h) * p.Lq + i;
+    if (p.splits > 1) {
+      const long long slot = static_cast<long long>(split) * p.B * p.H * p.Lq + hrow;
+      if (i < p.Lq) p.part_lse[slot] = lse;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (n > 0 && ok) {
+          tmem_ld32(tmem_o + lane_off + c * 32, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (i >= p.Lq) continue;
+        float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + c * 32);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          dst[q] = inv == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                              : make_float4(o[4 * q] * inv, o[4 * q + 1] * inv, o[4 * q + 2] * inv, o[4 * q + 3] * inv);
+      }
+    } else {
+      if (i < p.Lq && p.lse != nullptr) p.lse[hrow] = lse;
+      uint16_t* dst = static_cast<uint16_t*>(p.out) + ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (n > 0 && ok) {
+          tmem_ld32(tmem_o + lane_off + c * 32, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (i >= p.Lq) continue;
+        // a row without keys is 0 whatever its accumulator holds
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = inv == 0.f ? 0.f : o[e] * inv;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          st_global_v4(dst + c * 32 + q * 8, pack16<BF16>(o[8 * q], o[8 * q + 1]),
+                       pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
+                       pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, C::kTmem);
+}
+
+// out = sum_s 2^(lse_s - lse) part_o[s], lse = log2 sum_s 2^lse_s: one warp per row.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant__ AttnArgs p) {
+  const long long rows = static_cast<long long>(p.B) * p.H * p.Lq;
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  float m = -kInf;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_lse[s * rows + row]);
+  const float ms = m == -kInf ? 0.f : m;
+  float total = 0.f;
+  constexpr int V = D / 32;  // columns per lane
+  float acc[V];
+#pragma unroll
+  for (int q = 0; q < V; ++q) acc[q] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float w = exp2f(p.part_lse[s * rows + row] - ms);
+    total += w;
+    const float* src = p.part_o + (s * rows + row) * D + lane * V;
+    if (w == 0.f) continue;
+#pragma unroll
+    for (int q = 0; q < V; ++q) acc[q] = fmaf(w, src[q], acc[q]);
+  }
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  const int i = static_cast<int>(row % p.Lq);
+  const int h = static_cast<int>(row / p.Lq % p.H);
+  const long long b = row / p.Lq / p.H;
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + ((b * p.Lq + i) * p.H + h) * D + lane * V;
+#pragma unroll
+  for (int q = 0; q < V; q += 2)
+    *reinterpret_cast<uint32_t*>(dst + q) = pack16<BF16>(acc[q] * inv, acc[q + 1] * inv);
+  if (lane == 0 && p.lse != nullptr) p.lse[row] = inv == 0.f ? -kInf : ms + log2f(total);
+}
+
+// ---------------------------------------------------------------------------
+// Backward
+// ---------------------------------------------------------------------------
+// Eight compute warps: warp w reads TMEM lanes [32 (w % 4), + 32), warps 2-5 columns 0-31 of a
+// score tile, warps 6-9 columns 32-63. D = 64: two CTAs per SM overlap each other; D = 128: one
+// CTA per SM with two score buffers.
+template <int D>
+struct Bwd {
+  static constexpr int kThreads = 320;
+  static constexpr int kCtas = D == 64 ? 2 : 1;
+  static constexpr int kBuf = D == 64 ? 1 : 2;
+  static constexpr int kStages = 2;
+  static constexpr uint32_t kTmem = D == 64 ? 256 : 512;
+  static constexpr uint32_t kBig = kRows * D * 2;
+  static constexpr uint32_t kTile = kCols * D * 2;
+  static constexpr int kWarp = 64 + 96 + 64;  // floats per warp: bias line, diagonals, row values
+  static int smem(int buckets) {
+    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 1024 + align_up(buckets * 4, 16) +
+           8 * align_up(buckets * 4, 16) + kRows * 4;
+  }
+};
+
+// Adds v into the warp's bucket sums: lanes with a bucket of their own directly, equal ones
+// through a fixed-order sum over the lanes.
+__device__ __forceinline__ void add_buckets(float* acc, int bucket, float v, int lane) {
+  const unsigned same = __match_any_sync(0xffffffffu, bucket);
+  const bool alone = same == (1u << lane);
+  if (alone && bucket >= 0) acc[bucket] += v;
+  unsigned todo = __ballot_sync(0xffffffffu, !alone && bucket >= 0);
+  while (todo != 0) {
+    const int bb = __shfl_sync(0xffffffffu, bucket, __ffs(todo) - 1);
+    float s = bucket == bb ? v : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) acc[bb] += s;
+    todo &= ~__ballot_sync(0xffffffffu, bucket == bb);
+  }
+  __syncwarp();
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
+    attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                   const __grid_constant__ AttnArgs p) {
+  using C = Bwd<D>;
+  constexpr int ST = C::kStages;
+  constexpr int NB = C::kBuf;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sO = sQ + C::kBig;  // dO
+  uint8_t* sK = sO + C::kBig;
+  uint8_t* sV = sK + ST * C::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * C::kTile);
+  uint64_t* full = bars;          // K and V of a stage
+  uint64_t* empty = bars + ST;
+  uint64_t* q_full = bars + 2 * ST;
+  uint64_t* s_full = q_full + 1;  // NB
+  uint64_t* ds_ready = s_full + 2;  // NB
+  uint64_t* done = ds_ready + 2;
+  uint64_t* last = done + 1;  // every product is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
+  const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
+  float* warps = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
+  int* bounds = reinterpret_cast<int*>(warps + 8 * C::kWarp);
+  float* col = reinterpret_cast<float*>(bounds + 256);
+  const int bpad = align_up(buckets * 4, 16) / 4;
+  float* sums = col + bpad;           // [8][bpad]
+  float* sdelta = sums + 8 * bpad;    // [128]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int q_tiles = (p.Lq + kRows - 1) / kRows;
+  int x = blockIdx.x;
+  const int qt = q_tiles - 1 - x % q_tiles;
+  x /= q_tiles;
+  const int h = x % p.H;
+  const int b = x / p.H;
+  const int i0 = qt * kRows;
+  const int klen = sample_len(p, b);
+  int visible = klen;
+  if (p.causal) visible = min(visible, min(i0 + kRows, p.Lq) + p.q_offset);
+  const int n = (visible + kCols - 1) / kCols;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(&ds_ready[0], 8);
+    mbar_init(&ds_ready[1], 8);
+    mbar_init(done, 1);
+    mbar_init(last, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kTmem);
+    tmem_relinquish();
+  }
+  load_table(p, h, kLog2e, bounds, col, buckets, C::kThreads);
+  for (int t = threadIdx.x; t < 8 * bpad; t += C::kThreads) sums[t] = 0.f;
+  // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too
+  if (threadIdx.x < kRows) {
+    const int i = i0 + threadIdx.x;
+    float s = 0.f;
+    if (i < p.Lq) {
+      const uint4* g = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.dout) + b * p.do_b + i * p.do_l +
+                                                      h * p.do_h);
+      const uint4* o = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.out) +
+                                                      ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D);
+#pragma unroll
+      for (int q = 0; q < D / 8; ++q) {
+        const uint4 a = __ldg(g + q), c = __ldg(o + q);
+        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack16<BF16>(aw[e]), v = unpack16<BF16>(cw[e]);
+          s = fmaf(f.x, v.x, fmaf(f.y, v.y, s));
+        }
+      }
+      p.delta[(static_cast<long long>(b) * p.H + h) * p.Lq + i] = s;
+    }
+    sdelta[threadIdx.x] = s;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem_acc = tmem + NB * 2 * kCols;  // buffers of (scores, dP), then dQ
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(q_full, 2 * C::kBig);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        tma_load_4d(sQ + c * 16384, &tmQ, q_full, c * 64, h, i0, b);
+        tma_load_4d(sO + c * 16384, &tmO, q_full, c * 64, h, i0, b);
+      }
+      int loaded = 0;
+      for (int t = 0; t < n; ++t) {
+        const int st = t % ST;
+        if (!wait_parity(&empty[st], ((t / ST) & 1) ^ 1u, kSiteAttnDq, p.ctx)) break;
+        mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          tma_load_4d(sK + st * C::kTile + c * 8192, &tmK, &full[st], c * 64, h, t * kCols, b);
+          tma_load_4d(sV + st * C::kTile + c * 8192, &tmV, &full[st], c * 64, h, t * kCols, b);
+        }
+        loaded = t + 1;
+      }
+      wait_parity(q_full, 0, kSiteAttnDq + 1, p.ctx);
+      for (int t = max(0, loaded - ST); t < loaded; ++t) wait_parity(&full[t % ST], (t / ST) & 1, kSiteAttnDq + 1, p.ctx);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t id_s = idesc16(kRows, kCols, BF16, false);
+    constexpr uint32_t id_acc = idesc16(kRows, D, BF16, true);
+    auto scores = [&](int t) {
+      const int st = t % ST;
+      const bool ok = wait_parity(&full[st], (t / ST) & 1, kSiteAttnDq + 2, p.ctx);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      // rows past the sample's keys would enter dQ as 0 * anything
+      if (t * kCols + kCols > klen) zero_tail<D>(sK + st * C::kTile, klen - t * kCols, lane);
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t d = tmem + (t % NB) * 2 * kCols;
+        issue_scores<D>(d, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
+        issue_scores<D>(d + kCols, smem_u32(sO), smem_u32(sV + st * C::kTile), id_s);
+        mma_commit(&s_full[t % NB]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = true;
+    if (n > 0) {
+      ok = wait_parity(q_full, 0, kSiteAttnDq + 3, p.ctx);
+      ok = __all_sync(0xffffffffu, ok) && scores(0);
+    }
+    for (int t = 0; t < n && ok; ++t) {
+      if (NB == 2 && t + 1 < n) {
+        // the buffer's previous content is still read until the products of t - 1 are done
+        if (t > 0) ok = __all_sync(0xffffffffu, wait_parity(done, (t - 1) & 1, kSiteAttnDq + 7, p.ctx));
+        if (!ok || !scores(t + 1)) break;
+      }
+      ok = wait_parity(&ds_ready[t % NB], (t / NB) & 1, kSiteAttnDq + 4, p.ctx);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const int st = t % ST;
+      if (lane == 0) {
+        issue_ts<true>(tmem_acc, tmem + (t % NB) * 2 * kCols, smem_u32(sK + st * C::kTile), id_acc, t > 0);
+        mma_commit(&empty[st]);
+        mma_commit(done);
+        if (t + 1 == n) mma_commit(last);
+      }
+      __syncwarp();
+      if (NB == 1 && t + 1 < n)
+        ok = __all_sync(0xffffffffu, wait_parity(done, t & 1, kSiteAttnDq + 7, p.ctx)) && scores(t + 1);
+    }
+  } else {
+    const int wq = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const int r = wq * 32 + lane;
+    const int i = i0 + r;
+    const bool row_ok = i < p.Lq;
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    float* line = warps + (warp - 2) * C::kWarp;
+    float* diag = line + 64;
+    float* mine = sums + (warp - 2) * bpad;
+    const float scale2 = p.scale * kLog2e;
+    const int row_end = !row_ok ? 0 : (p.causal ? min(klen, i + p.q_offset + 1) : klen);
+    const int warp_first = i0 + wq * 32 + p.q_offset;
+    float lse = kInf;
+    if (row_ok) lse = p.lse[(static_cast<long long>(b) * p.H + h) * p.Lq + i];
+    if (lse == -kInf) lse = kInf;  // no keys: every P is 0
+    const float delta = sdelta[r];
+    bool ok = true;
+    for (int t = 0; t < n; ++t) {
+      const int j0 = t * kCols + half * 32;
+      const int d_lo = j0 - warp_first - 31, d_hi = j0 + 31 - warp_first;
+      const int b_lo = rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo);
+      const bool flat = b_lo == rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_hi);
+      if (!flat) {
+        __syncwarp();
+        line[lane] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + lane)];
+        line[lane + 32] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + min(lane + 32, 62))];
+        __syncwarp();
+      }
+      ok = wait_parity(&s_full[t % NB], (t / NB) & 1, kSiteAttnDq + 5, p.ctx);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const uint32_t ts = tmem + lane_off + (t % NB) * 2 * kCols + half * 32;
+      float s[32], g[32];
+      tmem_ld32(ts, s);
+      tmem_ld32(ts + kCols, g);
+      if (flat) {
+        const float c = col[b_lo] - lse;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[e] = exp2_approx(fmaf(s[e], scale2, c)) * (g[e] - delta);
+      } else {
+        const float* ln = line + 31 - lane;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[e] = exp2_approx(fmaf(s[e], scale2, ln[e] - lse)) * (g[e] - delta);
+      }
+      if (__any_sync(0xffffffffu, row_end < j0 + 32)) {
+        const int keep = row_end - j0;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[e] = e < keep ? s[e] : 0.f;
+      }
+      uint32_t w[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[e] = pack16<BF16>(s[2 * e], s[2 * e + 1]);
+      tmem_st16(ts, w);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ds_ready[t % NB]);
+      // The table's gradient: the sum of dS by bucket.
+      if (flat) {
+        float a[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int e = 4; e < 32; ++e) a[e & 3] += s[e];
+        float tot = (a[0] + a[1]) + (a[2] + a[3]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+        if (lane == 0) mine[b_lo] += tot;
+      } else {
+        // Diagonal sums: from a column to the next a diagonal moves one lane up, so a running sum
+        // passed from lane to lane follows it. Two chains of 16 columns; entry d + 31 of a chain.
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float a = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            a = __shfl_up_sync(0xffffffffu, a, 1);
+            a = (lane == 0 ? 0.f : a) + s[16 * c + e];
+            if (lane == 31) diag[48 * c + e] = a;
+          }
+          if (lane < 31) diag[48 * c + 46 - lane] = a;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int idx = lane + 32 * q;
+          const float v = (idx < 47 ? diag[idx] : 0.f) + (idx >= 16 && idx < 63 ? diag[48 + idx - 16] : 0.f);
+          const int bk = idx < 63 ? rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + idx) : -1 - lane;
+          add_buckets(mine, bk, v, lane);
+        }
+      }
+      __syncwarp();
+    }
+    if (ok && n > 0) {
+      ok = wait_parity(last, 0, kSiteAttnDq + 6, p.ctx);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    uint16_t* dst = static_cast<uint16_t*>(p.dq) + ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D;
+#pragma unroll 1
+    for (int c = half; c < D / 32; c += 2) {
+      float o[32];
+      if (n > 0 && ok) {
+        tmem_ld32(tmem_acc + lane_off + c * 32, o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+      }
+      if (!row_ok) continue;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] *= p.scale;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        st_global_v4(dst + c * 32 + q * 8, pack16<BF16>(o[8 * q], o[8 * q + 1]),
+                     pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
+                     pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, C::kTmem);
+  for (int t = threadIdx.x; t < buckets; t += C::kThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += sums[w * bpad + t];
+    p.table_part[(static_cast<long long>(h) * p.B * q_tiles + static_cast<long long>(b) * q_tiles + qt) * buckets + t] = s;
+  }
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
+    attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmO,
+                    const __grid_constant__ AttnArgs p) {
+  using C = Bwd<D>;
+  constexpr int ST = C::kStages;
+  constexpr int NB = C::kBuf;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + C::kBig;
+  uint8_t* sQ = sV + C::kBig;
+  uint8_t* sO = sQ + ST * C::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sO + ST * C::kTile);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + ST;
+  uint64_t* k_full = bars + 2 * ST;
+  uint64_t* s_full = k_full + 1;
+  uint64_t* ds_ready = s_full + 2;  // NB
+  uint64_t* done = ds_ready + 2;
+  uint64_t* last = done + 1;  // every product is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
+  const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
+  float* warps = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
+  int* bounds = reinterpret_cast<int*>(warps + 8 * C::kWarp);
+  float* col = reinterpret_cast<float*>(bounds + 256);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k_tiles = (p.Lk + kRows - 1) / kRows;
+  int x = blockIdx.x;
+  const int kt = x % k_tiles;
+  x /= k_tiles;
+  const int h = x % p.H;
+  const int b = x / p.H;
+  const int j0 = kt * kRows;
+  const int klen = sample_len(p, b);
+  // query tiles with a row that sees one of these keys
+  const int q_tiles = (p.Lq + kCols - 1) / kCols;
+  const int first = p.causal ? max(0, j0 - p.q_offset) / kCols : 0;
+  const int n = j0 < klen ? max(0, q_tiles - first) : 0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(k_full, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(&ds_ready[0], 8);
+    mbar_init(&ds_ready[1], 8);
+    mbar_init(done, 1);
+    mbar_init(last, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kTmem);
+    tmem_relinquish();
+  }
+  load_table(p, h, kLog2e, bounds, col, buckets, C::kThreads);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem_dv = tmem + NB * 2 * kCols;
+  const uint32_t tmem_dk = tmem_dv + D;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(k_full, 2 * C::kBig);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        tma_load_4d(sK + c * 16384, &tmK, k_full, c * 64, h, j0, b);
+        tma_load_4d(sV + c * 16384, &tmV, k_full, c * 64, h, j0, b);
+      }
+      int loaded = 0;
+      for (int t = 0; t < n; ++t) {
+        const int st = t % ST;
+        const int i0 = (first + t) * kCols;
+        if (!wait_parity(&empty[st], ((t / ST) & 1) ^ 1u, kSiteAttnDkv, p.ctx)) break;
+        mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          tma_load_4d(sQ + st * C::kTile + c * 8192, &tmQ, &full[st], c * 64, h, i0, b);
+          tma_load_4d(sO + st * C::kTile + c * 8192, &tmO, &full[st], c * 64, h, i0, b);
+        }
+        loaded = t + 1;
+      }
+      wait_parity(k_full, 0, kSiteAttnDkv + 1, p.ctx);
+      for (int t = max(0, loaded - ST); t < loaded; ++t) wait_parity(&full[t % ST], (t / ST) & 1, kSiteAttnDkv + 1, p.ctx);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t id_s = idesc16(kRows, kCols, BF16, false);
+    constexpr uint32_t id_acc = idesc16(kRows, D, BF16, true);
+    auto scores = [&](int t) {
+      const int st = t % ST;
+      const bool ok = wait_parity(&full[st], (t / ST) & 1, kSiteAttnDkv + 2, p.ctx);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t d = tmem + (t % NB) * 2 * kCols;
+        issue_scores<D>(d, smem_u32(sK), smem_u32(sQ + st * C::kTile), id_s);
+        issue_scores<D>(d + kCols, smem_u32(sV), smem_u32(sO + st * C::kTile), id_s);
+        mma_commit(&s_full[t % NB]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = true;
+    if (n > 0) {
+      ok = wait_parity(k_full, 0, kSiteAttnDkv + 3, p.ctx);
+      ok = __all_sync(0xffffffffu, ok) && scores(0);
+    }
+    for (int t = 0; t < n && ok; ++t) {
+      if (NB == 2 && t + 1 < n) {
+        // the buffer's previous content is still read until the products of t - 1 are done
+        if (t > 0) ok = __all_sync(0xffffffffu, wait_parity(done, (t - 1) & 1, kSiteAttnDkv + 7, p.ctx));
+        if (!ok || !scores(t + 1)) break;
+      }
+      ok = wait_parity(&ds_ready[t % NB], (t / NB) & 1, kSiteAttnDkv + 4, p.ctx);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const int st = t % ST;
+      if (lane == 0) {
+        const uint32_t d = tmem + (t % NB) * 2 * kCols;
+        issue_ts<true>(tmem_dv, d, smem_u32(sO + st * C::kTile), id_acc, t > 0);
+        issue_ts<true>(tmem_dk, d + kCols, smem_u32(sQ + st * C::kTile), id_acc, t > 0);
+        mma_commit(&empty[st]);
+        mma_commit(done);
+        if (t + 1 == n) mma_commit(last);
+      }
+      __syncwarp();
+      if (NB == 1 && t + 1 < n)
+        ok = __all_sync(0xffffffffu, wait_parity(done, t & 1, kSiteAttnDkv + 7, p.ctx)) && scores(t + 1);
+    }
+  } else {
+    const int wq = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const int r = wq * 32 + lane;
+    const int j = j0 + r;  // this thread's key
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    float* line = warps + (warp - 2) * C::kWarp;
+    float* rowv = line + 160;  // lse and delta of the half tile's 32 query rows
+    const float scale2 = p.scale * kLog2e;
+    const bool key_ok = j < klen;
+    const long long hbase = (static_cast<long long>(b) * p.H + h) * p.Lq;
+    bool ok = true;
+    for (int t = 0; t < n; ++t) {
+      const int i0 = (first + t) * kCols + half * 32;
+      const int pos = i0 + p.q_offset;
+      // diagonal of (key lane, query e): j - i - off = d_lo + 31 + lane - e
+      const int d_lo = j0 + wq * 32 - pos - 31, d_hi = j0 + wq * 32 + 31 - pos;
+      const int b_lo = rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo);
+      const bool flat = b_lo == rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_hi);
+      float my_lse = kInf, my_delta = 0.f;
+      if (i0 + lane < p.Lq) {
+        my_lse = p.lse[hbase + i0 + lane];
+        my_delta = p.delta[hbase + i0 + lane];
+        if (my_lse == -kInf) my_lse = kInf;
+      }
+      __syncwarp();
+      rowv[lane] = my_lse;
+      rowv[32 + lane] = my_delta;
+      if (!flat) {
+        line[lane] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + lane)];
+        line[lane + 32] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + min(lane + 32, 62))];
+      }
+      __syncwarp();
+      ok = wait_parity(&s_full[t % NB], (t / NB) & 1, kSiteAttnDkv + 5, p.ctx);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const uint32_t ts = tmem + lane_off + (t % NB) * 2 * kCols + half * 32;
+      float s[32], g[32];
+      tmem_ld32(ts, s);
+      tmem_ld32(ts + kCols, g);
+      // visible to this key: query rows i >= j - off (causal), i < Lq
+      const int from = !key_ok ? 32 : (p.causal ? j - pos : 0);
+      const int to = p.Lq - i0;
+      const bool masked = __any_sync(0xffffffffu, from > 0) || to < 32;
+      const float flat_c = flat ? col[b_lo] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const float4 ls = *reinterpret_cast<const float4*>(rowv + e);
+        const float4 dl = *reinterpret_cast<const float4*>(rowv + 32 + e);
+        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dlv[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float bias = flat ? flat_c : line[31 + lane - (e + u)];
+          float pr = exp2_approx(fmaf(s[e + u], scale2, bias - lsv[u]));
+          float ds = pr * (g[e + u] - dlv[u]);
+          if (masked && (e + u < from || e + u >= to)) {
+            pr = 0.f;
+            ds = 0.f;
+          }
+          s[e + u] = pr;
+          g[e + u] = ds;
+        }
+      }
+      uint32_t w[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[e] = pack16<BF16>(s[2 * e], s[2 * e + 1]);
+      tmem_st16(ts, w);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[e] = pack16<BF16>(g[2 * e], g[2 * e + 1]);
+      tmem_st16(ts + kCols, w);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ds_ready[t % NB]);
+    }
+    if (ok && n > 0) {
+      ok = wait_parity(last, 0, kSiteAttnDkv + 6, p.ctx);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    // Warps 2-5 write dV, warps 6-9 dK; keys past the sample's length get 0.
+    uint16_t* dst = static_cast<uint16_t*>(half == 0 ? p.dv : p.dk) +
+                    ((static_cast<long long>(b) * p.Lk + j) * p.H + h) * D;
+    const uint32_t src = (half == 0 ? tmem_dv : tmem_dk) + lane_off;
+    const float mult = half == 0 ? 1.f : p.scale;
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+      float o[32];
+      if (n > 0 && ok) {
+        tmem_ld32(src + c * 32, o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+      }
+      if (j >= p.Lk) continue;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = key_ok ? o[e] * mult : 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        st_global_v4(dst + c * 32 + q * 8, pack16<BF16>(o[8 * q], o[8 * q + 1]),
+                     pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
+                     pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, C::kTmem);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int cuda_rc(cudaError_t e) { return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e); }
+
+int attn_sms() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  return n;
+}
+
+// Key splits of the forward: with fewer CTAs than two per SM (a few query rows of a few heads)
+// one CTA would walk a long cache alone, so the keys are divided until the SMs are full, at least
+// four tiles a part.
+int attn_splits(int B, int H, int Lq, int Lk) {
+  const long long ctas = static_cast<long long>(B) * H * ((Lq + kRows - 1) / kRows);
+  const int tiles = (Lk + kCols - 1) / kCols;
+  if (ctas <= 0) return 1;
+  long long s = 2ll * attn_sms() / ctas;
+  if (s > tiles / 4) s = tiles / 4;
+  return s < 1 ? 1 : (s > 64 ? 64 : static_cast<int>(s));
+}
+
+struct Strides {
+  long long b, l, h;
+};
+
+// [B, L, H, D] with element strides, unit along D; box of 64 columns x rows of one head
+int map_heads(CUtensorMap* m, bool bf16, const void* ptr, int B, int L, int H, int D, Strides s, int rows) {
+  const unsigned long long dims[4] = {static_cast<unsigned long long>(D), static_cast<unsigned long long>(H),
+                                      static_cast<unsigned long long>(L), static_cast<unsigned long long>(B)};
+  const unsigned long long st[3] = {static_cast<unsigned long long>(s.h) * 2, static_cast<unsigned long long>(s.l) * 2,
+                                    static_cast<unsigned long long>(s.b) * 2};
+  const unsigned int box[4] = {64, 1, static_cast<unsigned>(rows), 1};
+  return encode_tiled(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, ptr, dims, st,
+                      box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int check_attn(const int* bounds, int n_bounds, int B, int H, int Lq, int Lk, int D, int dtype, int table_dtype,
+               int q_offset, const void* table) {
+  if (bounds == nullptr || table == nullptr) return WDIT_ERR_ARG;
+  if (dtype != 1 && dtype != 2) return WDIT_ERR_ARG;
+  if (table_dtype < 0 || table_dtype > 2) return WDIT_ERR_ARG;
+  if (n_bounds < 1 || n_bounds > kMaxRelBounds) return WDIT_ERR_SHAPE;
+  if (B < 0 || H < 1 || Lq < 0 || Lk < 0 || (D != 64 && D != 128)) return WDIT_ERR_SHAPE;
+  if (q_offset < 0 || static_cast<long long>(q_offset) + Lq > (1ll << 30) || Lk > (1 << 30)) return WDIT_ERR_SHAPE;
+  return WDIT_OK;
+}
+
+int check_heads(const void* p, const long long* s) {
+  if (p == nullptr || s == nullptr) return WDIT_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return WDIT_ERR_ALIGN;
+  for (int i = 0; i < 3; ++i) {
+    if (s[i] <= 0) return WDIT_ERR_SHAPE;
+    if (s[i] % 8 != 0) return WDIT_ERR_ALIGN;
+  }
+  return WDIT_OK;
+}
+
+template <typename K>
+int set_smem(K kernel, int bytes, int (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_rc(e);
+  if (done[dev & 63] < bytes) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return cuda_rc(e);
+    done[dev & 63] = bytes;
+  }
+  return WDIT_OK;
+}
+
+template <int D, bool BF16>
+int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& p, int buckets,
+            cudaStream_t st) {
+  static int done[64] = {};
+  const int smem = Fwd<D>::smem(buckets);
+  int rc = set_smem(attn_fwd_kernel<D, BF16>, smem, done);
+  if (rc) return rc;
+  const long long grid = static_cast<long long>((p.Lq + kRows - 1) / kRows) * p.splits * p.H * p.B;
+  if (grid > 0x7fffffffll) return WDIT_ERR_SHAPE;
+  attn_fwd_kernel<D, BF16><<<static_cast<unsigned>(grid), Fwd<D>::kThreads, smem, st>>>(q, k, v, p);
+  rc = cuda_rc(cudaGetLastError());
+  if (rc || p.splits == 1) return rc;
+  const long long rows = static_cast<long long>(p.B) * p.H * p.Lq;
+  attn_combine_kernel<D, BF16><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(p);
+  return cuda_rc(cudaGetLastError());
+}
+
+template <int D, bool BF16>
+int run_bwd(const CUtensorMap (&big)[4], const CUtensorMap (&small)[4], const AttnArgs& p, int buckets,
+            float* dtable, cudaStream_t st) {
+  // order of the maps: q, k, v, dO
+  static int done_q[64] = {}, done_kv[64] = {};
+  const int smem = Bwd<D>::smem(buckets);
+  int rc = set_smem(attn_dq_kernel<D, BF16>, smem, done_q);
+  if (rc) return rc;
+  if ((rc = set_smem(attn_dkv_kernel<D, BF16>, smem, done_kv))) return rc;
+  const int q_tiles = (p.Lq + kRows - 1) / kRows;
+  const long long gq = static_cast<long long>(q_tiles) * p.H * p.B;
+  const long long gk = static_cast<long long>((p.Lk + kRows - 1) / kRows) * p.H * p.B;
+  if (gq > 0x7fffffffll || gk > 0x7fffffffll) return WDIT_ERR_SHAPE;
+  attn_dq_kernel<D, BF16><<<static_cast<unsigned>(gq), Bwd<D>::kThreads, smem, st>>>(big[0], small[1], small[2],
+                                                                                    big[3], p);
+  if ((rc = cuda_rc(cudaGetLastError()))) return rc;
+  attn_dkv_kernel<D, BF16><<<static_cast<unsigned>(gk), Bwd<D>::kThreads, smem, st>>>(big[1], big[2], small[0],
+                                                                                     small[3], p);
+  if ((rc = cuda_rc(cudaGetLastError()))) return rc;
+  return launch_rel_table_sum(p.table_part, p.B * q_tiles, buckets, p.H, dtable, st);
+}
+
+long long align16(long long x) { return (x + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace wdit
+
+using namespace wdit;
+
+extern "C" {
+
+long long wdit_rel_attention_workspace_bytes(int B, int H, int Lq, int Lk, int D) {
+  if (B <= 0 || H <= 0 || Lq <= 0 || Lk <= 0 || D <= 0) return 0;
+  const int s = attn_splits(B, H, Lq, Lk);
+  return s == 1 ? 0 : 4ll * s * B * H * Lq * (D + 1);
+}
+
+int wdit_rel_attention(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
+                       const void* v, const long long* v_strides, int B, int H, int Lq, int Lk, int D, int dtype,
+                       const int* k_lens, const void* table, int table_dtype, const int* bounds, int n_bounds,
+                       int bidirectional, int causal, int q_offset, float scale, void* out, float* lse,
+                       void* workspace, long long workspace_bytes, void* stream) {
+  int rc = check_attn(bounds, n_bounds, B, H, Lq, Lk, D, dtype, table_dtype, q_offset, table);
+  if (rc) return rc;
+  if (B == 0 || Lq == 0) return WDIT_OK;
+  if (out == nullptr) return WDIT_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0) return WDIT_ERR_ALIGN;
+  if (Lk == 0) return WDIT_ERR_SHAPE;  // the caller knows the answer: zeros
+  if ((rc = check_heads(q, q_strides)) || (rc = check_heads(k, k_strides)) || (rc = check_heads(v, v_strides)))
+    return rc;
+  AttnArgs p = {};
+  p.B = B;
+  p.H = H;
+  p.Lq = Lq;
+  p.Lk = Lk;
+  p.causal = causal != 0;
+  p.q_offset = q_offset;
+  p.scale = scale;
+  p.k_lens = k_lens;
+  p.table = table;
+  p.table_dtype = table_dtype;
+  if (!rel_fill(&p.rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
+  p.out = out;
+  p.lse = lse;
+  p.splits = attn_splits(B, H, Lq, Lk);
+  if (p.splits > 1) {
+    if (workspace == nullptr || workspace_bytes < wdit_rel_attention_workspace_bytes(B, H, Lq, Lk, D))
+      return WDIT_ERR_WORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return WDIT_ERR_ALIGN;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_lse = p.part_o + static_cast<long long>(p.splits) * B * H * Lq * D;
+  }
+  if ((rc = error_record_ptr(&p.ctx.rec))) return rc;
+  p.ctx.limit_ns = wait_limit_ns();
+  const bool bf16 = dtype == 1;
+  CUtensorMap mq, mk, mv;
+  if ((rc = map_heads(&mq, bf16, q, B, Lq, H, D, {q_strides[0], q_strides[1], q_strides[2]}, kRows)) ||
+      (rc = map_heads(&mk, bf16, k, B, Lk, H, D, {k_strides[0], k_strides[1], k_strides[2]}, kCols)) ||
+      (rc = map_heads(&mv, bf16, v, B, Lk, H, D, {v_strides[0], v_strides[1], v_strides[2]}, kCols)))
+    return rc;
+  const int buckets = rel_num_buckets(n_bounds, p.rb.bidirectional);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (D == 64)
+    return bf16 ? run_fwd<64, true>(mq, mk, mv, p, buckets, st) : run_fwd<64, false>(mq, mk, mv, p, buckets, st);
+  return bf16 ? run_fwd<128, true>(mq, mk, mv, p, buckets, st) : run_fwd<128, false>(mq, mk, mv, p, buckets, st);
+}
+
+long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional) {
+  if (B <= 0 || H <= 0 || Lq <= 0 || n_bounds < 1) return 0;
+  const long long q_tiles = (Lq + kRows - 1) / kRows;
+  return align16(4ll * B * H * Lq) + 4ll * H * B * q_tiles * rel_num_buckets(n_bounds, bidirectional);
+}
+
+int wdit_rel_attention_backward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
+                                const void* v, const long long* v_strides, const void* dout,
+                                const long long* dout_strides, const void* out, const float* lse, int B, int H, int Lq,
+                                int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
+                                const int* bounds, int n_bounds, int bidirectional, int causal, int q_offset,
+                                float scale, void* dq, void* dk, void* dv, float* dtable, void* workspace,
+                                long long workspace_bytes, void* stream) {
+  int rc = check_attn(bounds, n_bounds, B, H, Lq, Lk, D, dtype, table_dtype, q_offset, table);
+  if (rc) return rc;
+  if (B == 0 || Lq == 0 || Lk == 0) return WDIT_ERR_SHAPE;  // the caller knows the answer: zeros
+  if (out == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || dtable == nullptr)
+    return WDIT_ERR_ARG;
+  for (const void* t : {out, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
+    if ((reinterpret_cast<uintptr_t>(t) & 15) != 0) return WDIT_ERR_ALIGN;
+  if ((rc = check_heads(q, q_strides)) || (rc = check_heads(k, k_strides)) || (rc = check_heads(v, v_strides)) ||
+      (rc = check_heads(dout, dout_strides)))
+    return rc;
+  if (workspace == nullptr ||
+      workspace_bytes < wdit_rel_attention_backward_workspace_bytes(B, H, Lq, n_bounds, bidirectional))
+    return WDIT_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return WDIT_ERR_ALIGN;
+  AttnArgs p = {};
+  p.B = B;
+  p.H = H;
+  p.Lq = Lq;
+  p.Lk = Lk;
+  p.causal = causal != 0;
+  p.q_offset = q_offset;
+  p.scale = scale;
+  p.k_lens = k_lens;
+  p.table = table;
+  p.table_dtype = table_dtype;
+  if (!rel_fill(&p.rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
+  p.out = const_cast<void*>(out);
+  p.lse = const_cast<float*>(lse);
+  p.splits = 1;
+  p.dout = dout;
+  p.do_b = dout_strides[0];
+  p.do_l = dout_strides[1];
+  p.do_h = dout_strides[2];
+  p.delta = static_cast<float*>(workspace);
+  p.table_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align16(4ll * B * H * Lq));
+  p.dq = dq;
+  p.dk = dk;
+  p.dv = dv;
+  if ((rc = error_record_ptr(&p.ctx.rec))) return rc;
+  p.ctx.limit_ns = wait_limit_ns();
+  const bool bf16 = dtype == 1;
+  CUtensorMap big[4], small[4];
+  const void* ptrs[4] = {q, k, v, dout};
+  const long long* strides[4] = {q_strides, k_strides, v_strides, dout_strides};
+  for (int i = 0; i < 4; ++i) {
+    const int L = i == 1 || i == 2 ? Lk : Lq;
+    const Strides s = {strides[i][0], strides[i][1], strides[i][2]};
+    if ((rc = map_heads(&big[i], bf16, ptrs[i], B, L, H, D, s, kRows)) ||
+        (rc = map_heads(&small[i], bf16, ptrs[i], B, L, H, D, s, kCols)))
+      return rc;
+  }
+  const int buckets = rel_num_buckets(n_bounds, p.rb.bidirectional);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (D == 64)
+    return bf16 ? run_bwd<64, true>(big, small, p, buckets, dtable, st)
+                : run_bwd<64, false>(big, small, p, buckets, dtable, st);
+  return bf16 ? run_bwd<128, true>(big, small, p, buckets, dtable, st)
+              : run_bwd<128, false>(big, small, p, buckets, dtable, st);
+}
+
+}  // extern "C"

@@ -2,6 +2,7 @@
 
 * ``rel_pos_bias`` / ``rel_pos_bias_grad``: a learned relative position bias by buckets and the
   gradient of its table.
+* ``rel_pos_attention``: attention that reads that bias from its table, with its gradients.
 * ``linear_act_residual``: act(x W^T + bias) + residual in one kernel, with its gradients.
 
 Public names are re-exported by ``ops``, beside the GEMM and position-table ops of the block.
@@ -314,3 +315,115 @@ def _check_out_overlap(out, residual, *inputs) -> None:
         same = residual.data_ptr() == out.data_ptr() and residual.stride() == out.stride()
         if a < hi and lo < b and not same:
             raise ValueError("out partly overlaps the residual")
+
+
+# ---------------------------------------------------------------------------
+# Attention with the relative position bias
+# ---------------------------------------------------------------------------
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """[B, L, H, D] the kernels take as it is (unit stride along D, the other strides positive
+    multiples of 8 elements, 16-byte aligned), or a contiguous copy."""
+    if t.data_ptr() % 16 == 0 and t.stride(3) == 1 and all(
+            n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3])):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor):
+    # a dimension of size 1 has no meaningful stride; any valid one does
+    return (ctypes.c_longlong * 3)(*(t.stride(i) if t.shape[i] > 1 else t.shape[3] for i in range(3)))
+
+
+def _attention_args(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale):
+    B, Lq, H, D = q.shape
+    bounds, n = _bounds_arg(table.shape[0], max_distance, bidirectional)
+    shape = (B, H, Lq, k.shape[1], D, _DTYPE[q.dtype])
+    pos = (ptr(k_lens), ptr(table), _DTYPE[table.dtype], bounds, n, int(bidirectional), int(causal), q_offset,
+           float(scale))
+    return shape, pos
+
+
+def _attention_forward(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale, with_lse):
+    B, Lq, H, D = q.shape
+    Lk = k.shape[1]
+    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if with_lse else None
+    if out.numel() == 0 or Lk == 0:
+        return out.zero_(), None
+    shape, pos = _attention_args(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale)
+    nbytes = call("wdit_rel_attention_workspace_bytes", *shape[:5])
+    ws = _workspace(nbytes, q.device)
+    call("wdit_rel_attention", ptr(q), _strides(q), ptr(k), _strides(k), ptr(v), _strides(v), *shape, *pos, ptr(out),
+         ptr(lse), ptr(ws), nbytes, stream_ptr(), kernels=1 if nbytes == 0 else 2)
+    return out, lse
+
+
+class _RelPosAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale):
+        with torch.cuda.device(q.device):
+            qc, kc, vc, tc = _heads(q), _heads(k), _heads(v), table.contiguous()
+            out, lse = _attention_forward(qc, kc, vc, tc, k_lens, bidirectional, causal, max_distance, q_offset, scale,
+                                          True)
+        ctx.save_for_backward(qc, kc, vc, tc, k_lens, out, lse)
+        ctx.args = (bidirectional, causal, max_distance, q_offset, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, k_lens, out, lse = ctx.saved_tensors
+        nothing = (None,) * 6
+        if lse is None:  # no queries or no keys
+            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(table), *nothing)
+        with torch.cuda.device(q.device):
+            g = _heads(dout)
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+            dtable = torch.empty(table.shape, dtype=torch.float32, device=table.device)
+            shape, pos = _attention_args(q, k, v, table, k_lens, *ctx.args)
+            nbytes = call("wdit_rel_attention_backward_workspace_bytes", *shape[:3], pos[4], pos[5])
+            ws = _workspace(nbytes, q.device)
+            call("wdit_rel_attention_backward", ptr(q), _strides(q), ptr(k), _strides(k), ptr(v), _strides(v), ptr(g),
+                 _strides(g), ptr(out), ptr(lse), *shape, *pos, ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws), nbytes,
+                 stream_ptr(), kernels=3)
+        return (dq, dk, dv, dtable.to(table.dtype), *nothing)
+
+
+def rel_pos_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, *,
+                      k_lens: torch.Tensor | None = None, scale: float | None = None, causal: bool = False,
+                      bidirectional: bool = True, max_distance: int = 128, q_offset: int = 0) -> torch.Tensor:
+    """softmax(scale q k^T + bias) v with rel_pos_bias's bias read from its table: [B, Lq, H, D].
+
+    q [B, Lq, H, D], k and v [B, Lk, H, D] (bf16 or fp16, D 64 or 128; any strides, rows of a head
+    contiguous and on 16-byte boundaries, others are copied); table [num_buckets, H] (fp32, bf16
+    or fp16). k_lens [B] int32: sample b's first k_lens[b] keys are valid (clamped to [0, Lk]; what
+    lies behind them is not looked at). causal: query i sees the keys up to i + q_offset. A row
+    that sees no key gives 0. scale defaults to D ** -0.5. One token after a cache of n keys:
+    Lq 1, q_offset n - 1 if the cache holds the token's own key, n otherwise. Differentiable in
+    q, k, v and table; results repeat bit for bit."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"q [B, Lq, H, D], k and v [B, Lk, H, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    B, Lq, H, D = q.shape
+    if k.shape[0] != B or k.shape[2:] != q.shape[2:]:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, heads or head size")
+    if D not in (64, 128):
+        raise ValueError(f"head size 64 or 128, got {D}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v must all be bf16 or all fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    _check_table(table)
+    if table.shape[1] != H:
+        raise ValueError(f"table for {table.shape[1]} heads, q has {H}")
+    _check_positions(Lq, k.shape[1], q_offset)
+    rel_pos_bounds(table.shape[0], max_distance, bidirectional)
+    if k_lens is not None and (k_lens.shape != (B,) or k_lens.dtype != torch.int32):
+        raise ValueError(f"k_lens must be [{B}] int32, got {tuple(k_lens.shape)} {k_lens.dtype}")
+    _require_cuda(q, k, v, table, k_lens)
+    scale = D**-0.5 if scale is None else float(scale)
+    if k_lens is not None:
+        k_lens = k_lens.contiguous()
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table)):
+        return _RelPosAttention.apply(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale)
+    with torch.cuda.device(q.device):
+        return _attention_forward(_heads(q), _heads(k), _heads(v), table.contiguous(), k_lens, bidirectional, causal,
+                                  max_distance, q_offset, scale, False)[0]

@@ -556,4 +556,10 @@ def linear_bias_residual_fixed(A, B, C, bias, *, inplace: bool = False):
 # ---------------------------------------------------------------------------
 # Text-encoder operators
 # ---------------------------------------------------------------------------
-from .encoder_ops import linear_act_residual, rel_pos_bias, rel_pos_bias_grad, rel_pos_bounds  # noqa: E402,F401
+from .encoder_ops import (  # noqa: E402,F401
+    linear_act_residual,
+    rel_pos_attention,
+    rel_pos_bias,
+    rel_pos_bias_grad,
+    rel_pos_bounds,
+)

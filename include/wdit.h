@@ -330,6 +330,37 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
                            int q_offset, float* dtable, void* workspace, long long workspace_bytes, void* stream);
 
 /*
+ * Attention with that bias: out[B, Lq, H, D] (contiguous) = softmax(scale q k^T + table[bucket, h]) v.
+ * q, k, v (and dout) are [B, L, H, D] of dtype (bf16 or fp16), D 64 or 128, unit stride along D;
+ * *_strides are HOST arrays of the element strides of (b, l, h), multiples of 8 (dimensions of
+ * size 1 too). k_lens (device, [B], NULL = all of Lk): valid keys per sample, clamped to [0, Lk];
+ * causal != 0: key j <= i + q_offset. A row that sees no key gives 0. lse (fp32 [B, H, Lq], may be
+ * NULL) receives log2 of the softmax sums (-inf for such a row) for the backward pass.
+ * The workspace (0 bytes unless the keys are split over several CTAs) needs no initialization.
+ * Lk = 0 is WDIT_ERR_SHAPE (the result is zeros).
+ */
+long long wdit_rel_attention_workspace_bytes(int B, int H, int Lq, int Lk, int D);
+int wdit_rel_attention(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
+                       const void* v, const long long* v_strides, int B, int H, int Lq, int Lk, int D, int dtype,
+                       const int* k_lens, const void* table, int table_dtype, const int* bounds, int n_bounds,
+                       int bidirectional, int causal, int q_offset, float scale, void* out, float* lse,
+                       void* workspace, long long workspace_bytes, void* stream);
+
+/*
+ * Its gradients: dq [B, Lq, H, D], dk, dv [B, Lk, H, D] (contiguous, dtype; 0 for keys past
+ * k_lens) and dtable [buckets, H] (fp32). out and lse are the forward's. Three launches, no atomics:
+ * sums have a fixed order. Empty dimensions are WDIT_ERR_SHAPE (the results are zeros).
+ */
+long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional);
+int wdit_rel_attention_backward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
+                                const void* v, const long long* v_strides, const void* dout,
+                                const long long* dout_strides, const void* out, const float* lse, int B, int H, int Lq,
+                                int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
+                                const int* bounds, int n_bounds, int bidirectional, int causal, int q_offset,
+                                float scale, void* dq, void* dk, void* dv, float* dtable, void* workspace,
+                                long long workspace_bytes, void* stream);
+
+/*
  * out[M, N] = act(A . B^T + bias) + res, operands and out of dtype (bf16 or fp16), fp32 sums, one
  * rounding. A is [M, K] with rows of lda elements (a_mn = 0) or stored transposed, [K, M] with rows
  * of lda (a_mn = 1); B is [N, K] (b_mn = 0) or stored [K, N] (b_mn = 1); a_mn = 1 needs b_mn = 1.

@@ -85,3 +85,115 @@ def test_rel_pos_entry_points_validate_without_device(pkg):
     assert grad(ws=ctypes.c_void_p(0x1004)) == 3
     assert lib.wdit_rel_pos_bias_grad_workspace_bytes(0, 2, 4, 4, 3, 1) == 0
     assert lib.wdit_rel_pos_bias_grad_workspace_bytes(1, 2, 4, 4, 3, 1) == 4 * 1 * 2 * 8
+
+
+def test_linear_refused(pkg):
+    f = pkg.ops.linear_act_residual
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        f(bf(4, 64), bf(32, 64))
+    with pytest.raises(ValueError, match="unknown activation"):
+        f(bf(4, 64), bf(32, 64), act="tanh")
+    with pytest.raises(ValueError, match="expected"):
+        f(bf(4, 64), bf(32, 72))
+    with pytest.raises(ValueError, match="both be bf16 or both fp16"):
+        f(bf(4, 64), bf(32, 64).half())
+    with pytest.raises(ValueError, match="both be bf16 or both fp16"):
+        f(torch.zeros(4, 64), torch.zeros(32, 64))
+    for n, k in [(33, 64), (32, 60), (0, 64), (32, 0)]:
+        with pytest.raises(ValueError, match="multiples of 8"):
+            f(bf(4, k), bf(n, k))
+    with pytest.raises(ValueError, match="bias must be"):
+        f(bf(4, 64), bf(32, 64), bf(64))
+    with pytest.raises(ValueError, match="residual must be"):
+        f(bf(4, 64), bf(32, 64), residual=bf(1, 32))
+    with pytest.raises(ValueError, match="out must be"):
+        f(bf(4, 64), bf(32, 64), out=torch.zeros(4, 32))
+
+
+def test_attention_refused(pkg):
+    f = pkg.ops.rel_pos_attention
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    q, t = bf(2, 5, 3, 64), torch.zeros(32, 3)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        f(q, q, q, t)
+    with pytest.raises(ValueError, match="expected"):
+        f(q, q, bf(2, 6, 3, 64), t)
+    with pytest.raises(ValueError, match="differ in batch"):
+        f(q, bf(2, 5, 1, 64), bf(2, 5, 1, 64), t)
+    with pytest.raises(ValueError, match="head size"):
+        f(bf(2, 5, 3, 80), bf(2, 5, 3, 80), bf(2, 5, 3, 80), t)
+    with pytest.raises(ValueError, match="all be bf16"):
+        f(q, q.half(), q, t)
+    with pytest.raises(ValueError, match="table for 4 heads"):
+        f(q, q, q, torch.zeros(32, 4))
+    with pytest.raises(ValueError, match="even number"):
+        f(q, q, q, torch.zeros(31, 3))
+    with pytest.raises(ValueError, match="k_lens must be"):
+        f(q, q, q, t, k_lens=torch.zeros(2))
+    with pytest.raises(ValueError, match="k_lens must be"):
+        f(q, q, q, t, k_lens=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="negative"):
+        f(q, q, q, t, q_offset=-1)
+
+
+def test_linear_entry_points_validate_without_device(pkg):
+    lib = pkg._lib.load()
+    null, d = ctypes.c_void_p(None), ctypes.c_void_p(0x1000)
+
+    def lin(A=d, lda=64, a_mn=0, B=d, ldb=64, b_mn=0, M=4, N=32, K=64, dtype=1, bias=d, bd=0, act=0, res=d, ldr=32,
+            out=d, ldo=32, pre=null, ldp=0):
+        return lib.wdit_linear_act_residual(A, lda, a_mn, B, ldb, b_mn, M, N, K, dtype, bias, bd, act, res, ldr, out,
+                                            ldo, pre, ldp, null)
+
+    assert lin(A=null) == 1 and lin(B=null) == 1 and lin(out=null) == 1
+    assert lin(dtype=0) == 1 and lin(act=5) == 1 and lin(bd=3) == 1 and lin(a_mn=1) == 1
+    assert lin(N=36) == 2 and lin(K=0) == 2 and lin(M=-1) == 2
+    assert lin(lda=56) == 2 and lin(ldb=56) == 2 and lin(ldo=24) == 2 and lin(ldr=24) == 2
+    assert lin(pre=d, ldp=24) == 2
+    assert lin(lda=68) == 3 and lin(A=ctypes.c_void_p(0x1008)) == 3 and lin(res=ctypes.c_void_p(0x1002)) == 3
+    assert lin(A=null, out=null, M=0) == 0
+
+    def back(dout=d, pre=d, act=3, dtype=1, M=4, N=32, dpre=d, db=d, dbt=0, ws=d, nb=1 << 20, ld=32):
+        return lib.wdit_act_backward(dout, ld, pre, ld, act, dtype, M, N, dpre, ld, db, dbt, ws, nb, null)
+
+    assert back(dout=null) == 1 and back(pre=null) == 1 and back(dpre=null) == 1 and back(act=9) == 1
+    assert back(dtype=0) == 1 and back(dbt=3) == 1
+    assert back(N=30) == 2 and back(M=-1) == 2 and back(ld=24) == 2
+    assert back(ld=36) == 3 and back(ws=null) == 5 and back(nb=16) == 5
+    assert back(act=0, db=null, dout=null) == 0  # dpre is dout, no bias: nothing to do
+    assert lib.wdit_act_backward_workspace_bytes(65, 32) == 4 * 2 * 32
+
+
+def test_attention_entry_points_validate_without_device(pkg):
+    lib = pkg._lib.load()
+    null, d = ctypes.c_void_p(None), ctypes.c_void_p(0x1000)
+    bounds = (ctypes.c_int * 3)(1, 2, 8)
+    st = (ctypes.c_longlong * 3)(5 * 3 * 64, 3 * 64, 64)
+    bad = (ctypes.c_longlong * 3)(5 * 3 * 64, 3 * 64 + 4, 64)
+    zero = (ctypes.c_longlong * 3)(5 * 3 * 64, 0, 64)
+
+    def fwd(q=d, qs=st, B=2, H=3, Lq=5, Lk=5, D=64, dtype=1, table=d, td=0, b=bounds, n=3, off=0, out=d, ws=null,
+            nb=0):
+        return lib.wdit_rel_attention(q, qs, d, st, d, st, B, H, Lq, Lk, D, dtype, null, table, td, b, n, 1, 0, off,
+                                      1.0, out, null, ws, nb, null)
+
+    assert fwd(q=null) == 1 and fwd(qs=None) == 1 and fwd(table=null) == 1 and fwd(out=null) == 1 and fwd(b=None) == 1
+    assert fwd(dtype=0) == 1 and fwd(td=3) == 1
+    assert fwd(D=96) == 2 and fwd(H=0) == 2 and fwd(n=0) == 2 and fwd(off=-1) == 2 and fwd(Lk=0) == 2
+    assert fwd(qs=zero) == 2 and fwd(qs=bad) == 3 and fwd(q=ctypes.c_void_p(0x1008)) == 3
+    assert fwd(out=ctypes.c_void_p(0x1008)) == 3
+    assert fwd(B=0, q=null, out=null) == 0 and fwd(Lq=0, q=null, out=null) == 0
+    need = lib.wdit_rel_attention_workspace_bytes(1, 1, 1, 4096, 64)
+    assert need > 0 and fwd(B=1, H=1, Lq=1, Lk=4096) == 5
+    assert fwd(B=1, H=1, Lq=1, Lk=4096, ws=d, nb=need - 1) == 5
+    assert lib.wdit_rel_attention_workspace_bytes(64, 64, 512, 512, 64) == 0
+
+    def back(lse=d, out=d, dq=d, dt=d, ws=d, nb=1 << 30, Lq=5, Lk=5, gs=st):
+        return lib.wdit_rel_attention_backward(d, st, d, st, d, st, d, gs, out, lse, 2, 3, Lq, Lk, 64, 1, null, d, 0,
+                                               bounds, 3, 1, 0, 0, 1.0, dq, d, d, dt, ws, nb, null)
+
+    assert back(lse=null) == 1 and back(out=null) == 1 and back(dq=null) == 1 and back(dt=null) == 1
+    assert back(Lq=0) == 2 and back(Lk=0) == 2 and back(gs=zero) == 2 and back(gs=bad) == 3
+    assert back(dq=ctypes.c_void_p(0x1004)) == 3
+    assert back(ws=null) == 5 and back(nb=16) == 5
