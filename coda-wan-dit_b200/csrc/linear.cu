@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t make_idesc(int m, int n, int is_bf16, bool t
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 // x / (1 + exp(-2 z)) = 0.5 x (1 + tanh z): no cancellation for negative x
 constexpr float kGeluA = 2.f * 0.7978845608028654f;

@@ -8,10 +8,11 @@
 //   dV = P^T dO,  dP = dO v^T,  dS = P (dP - delta),  dQ = scale dS k,  dK = scale dS^T q,
 //   dtable[bucket, h] = the sum of dS over its cells.
 //
-// The bias is a function of the diagonal d = key - query, so a warp's tile of 32 rows needs 31 +
-// columns table values: they are looked up once per tile into a short line of shared memory (a
-// thread's row then reads consecutive entries, free of bank conflicts), or are one value when the
-// whole tile falls into one bucket, as it does away from the diagonal.
+// The bias is a function of the diagonal d = key - query and constant from the last bound on, so
+// the CTA looks every diagonal up to it up once. A warp's tile of 32 rows then copies its 31 +
+// columns values into a short line of its own (a thread's row reads consecutive entries, free of
+// bank conflicts), or uses one value when the whole tile lies past the last bound, as it does away
+// from the diagonal.
 //
 // All products run on the tensor cores (tcgen05, operands by TMA with the 128-byte swizzle,
 // accumulators in TMEM); the score tile is read from TMEM one row per thread, transformed in
@@ -140,6 +141,46 @@ __device__ __forceinline__ void tmem_st32f(uint32_t taddr, const float* v) {
   tmem_st16(taddr + 16, r + 16);
 }
 
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+      "[%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// The wait names the registers, so that no use of them is moved before it.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+// 32 columns from each of two places with one wait: both loads are in flight together.
+__device__ __forceinline__ void tmem_ld32x2(uint32_t a, float* v, uint32_t b, float* w) {
+  uint32_t r[32], q[32];
+  tmem_ld32_nowait(a, r);
+  tmem_ld32_nowait(b, q);
+  tmem_wait_ld(r);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(q[i]));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    v[i] = __uint_as_float(r[i]);
+    w[i] = __uint_as_float(q[i]);
+  }
+}
+
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) { tmem_ld32x2(taddr, v, taddr + 32, v + 32); }
+
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // MN-major operand tile: rows of 64 elements (128 B) along M or N, one row per K index; pieces of
@@ -191,11 +232,56 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int first, int lane) {
   __syncwarp();
 }
 
-// The head's table column (times `mult`) and the bucket bounds in shared memory.
-__device__ __forceinline__ void load_table(const AttnArgs& p, int h, float mult, int* bounds, float* col, int buckets,
-                                           int threads) {
+// The head's bias by diagonal: the table's values (times log2 e) and buckets of d = -reach .. reach,
+// constant past both ends, in shared memory. reach is the last bound, at most kReach: a table with
+// longer ones is searched per diagonal instead.
+constexpr int kReach = 1024;
+
+struct BiasLine {
+  const int* bounds;
+  const float* col;    // [buckets] table column * log2 e
+  const float* value;  // [2 reach + 1], nullptr: search
+  int n_bounds, bidirectional, reach;
+
+  __device__ __forceinline__ int bucket(int d) const { return rel_bucket(bounds, n_bounds, bidirectional, d); }
+  __device__ __forceinline__ float at(int d) const {
+    if (value == nullptr) return col[bucket(d)];
+    return value[min(max(d, -reach), reach) + reach];
+  }
+  // Whether d_lo .. d_hi share one bucket for certain (past the last bound on either side, or
+  // ahead of the query in one direction).
+  __device__ __forceinline__ bool flat(int d_lo, int d_hi) const {
+    return d_hi <= -reach || d_lo >= (bidirectional ? reach : 0);
+  }
+};
+
+__host__ __device__ inline int bias_reach(const RelBuckets& rb) { return rb.bounds[rb.n_bounds - 1]; }
+
+// Shared memory of load_bias in bytes (16-byte multiples).
+inline int bias_smem(const RelBuckets& rb) {
+  const int buckets = rel_num_buckets(rb.n_bounds, rb.bidirectional);
+  const int reach = bias_reach(rb);
+  return (1024 + buckets * 4 + (reach <= kReach ? (2 * reach + 1) * 4 : 0) + 15) / 16 * 16;
+}
+
+__device__ __forceinline__ BiasLine load_bias(const AttnArgs& p, int h, void* mem, int threads) {
+  int* bounds = static_cast<int*>(mem);
+  float* col = reinterpret_cast<float*>(bounds + 256);
+  const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
+  BiasLine l;
+  l.bounds = bounds;
+  l.col = col;
+  l.n_bounds = p.rb.n_bounds;
+  l.bidirectional = p.rb.bidirectional;
+  l.reach = bias_reach(p.rb);
+  l.value = l.reach <= kReach ? col + buckets : nullptr;
   for (int t = threadIdx.x; t < p.rb.n_bounds; t += threads) bounds[t] = p.rb.bounds[t];
-  for (int t = threadIdx.x; t < buckets; t += threads) col[t] = table_value(p, t, h) * mult;
+  for (int t = threadIdx.x; t < buckets; t += threads) col[t] = table_value(p, t, h) * kLog2e;
+  if (l.value != nullptr) {
+    __syncthreads();
+    for (int t = threadIdx.x; t < 2 * l.reach + 1; t += threads) col[buckets + t] = col[l.bucket(t - l.reach)];
+  }
+  return l;
 }
 
 __device__ __forceinline__ int sample_len(const AttnArgs& p, int b) {
@@ -217,9 +303,7 @@ struct Fwd {
   static constexpr uint32_t kTile = kCols * D * 2;
   static constexpr uint32_t kTmem = 256;  // two score buffers of 64 columns, O at 128
   static constexpr int kLine = 96;        // per-warp bias line (31 + 64 diagonals)
-  static int smem(int buckets) {
-    return 1024 + kQ + kStages * 2 * kTile + 256 + 4 * kLine * 4 + 1024 + align_up(buckets * 4, 16);
-  }
+  static int smem(const RelBuckets& rb) { return 1024 + kQ + kStages * 2 * kTile + 256 + 4 * kLine * 4 + bias_smem(rb); }
 };
 
 template <int D, bool BF16>
@@ -246,8 +330,6 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
   uint64_t* last = pv_done + 1;  // every product is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
   float* lines = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
-  int* bounds = reinterpret_cast<int*>(lines + 4 * C::kLine);
-  float* col = reinterpret_cast<float*>(bounds + 256);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_tiles = (p.Lq + kRows - 1) / kRows;
@@ -272,7 +354,6 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     t1 = min(t1, t0 + per);
   }
   const int n = max(0, t1 - t0);
-  const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -294,7 +375,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
-  load_table(p, h, kLog2e, bounds, col, buckets, C::kThreads);
+  const BiasLine bias = load_bias(p, h, lines + 4 * C::kLine, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -387,19 +468,24 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     const int warp_first = i0 + wq * 32 + p.q_offset;                      // the warp's first position
     float m_used = -kInf, l = 0.f;
     bool ok = true;
+    // Few query rows (one token): a warp without any leaves its rows of P as they are; they only
+    // reach its own rows of O, which are not stored.
+    const bool idle = i0 + wq * 32 >= p.Lq;
     for (int t = 0; t < n; ++t) {
+      if (idle) {
+        ok = wait_parity(&s_full[t & 1], (t >> 1) & 1, kSiteAttn + 7, p.ctx);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        if (lane == 0) mbar_arrive(&p_ready[t & 1]);
+        continue;
+      }
       const int j0 = (t0 + t) * kCols;
       // the tile's bias: one value, or a line over its 31 + 64 diagonals
       const int d_lo = j0 - warp_first - 31, d_hi = j0 + kCols - 1 - warp_first;
-      const int b_lo = rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo);
-      const bool flat = b_lo == rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_hi);
+      const bool flat = bias.flat(d_lo, d_hi);
       if (!flat) {
         __syncwarp();  // the previous tile's reads are done
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
-          const int dd = lane + 32 * q;
-          line[dd] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + min(dd, 94))];
-        }
+        for (int q = 0; q < 3; ++q) line[lane + 32 * q] = bias.at(d_lo + lane + 32 * q);
         __syncwarp();
       }
       ok = wait_parity(&s_full[t & 1], (t >> 1) & 1, kSiteAttn + 7, p.ctx);
@@ -407,10 +493,9 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       tc_fence_after();
       const uint32_t ts = tmem + lane_off + (t & 1) * kCols;
       float z[kCols];
-      tmem_ld32(ts, z);
-      tmem_ld32(ts + 32, z + 32);
+      tmem_ld64(ts, z);
       if (flat) {
-        const float c = col[b_lo];
+        const float c = bias.at(d_lo);
 #pragma unroll
         for (int e = 0; e < kCols; ++e) z[e] = fmaf(z[e], scale2, c);
       } else {
@@ -573,29 +658,12 @@ struct Bwd {
   static constexpr uint32_t kBig = kRows * D * 2;
   static constexpr uint32_t kTile = kCols * D * 2;
   static constexpr int kWarp = 64 + 96 + 64;  // floats per warp: bias line, diagonals, row values
-  static int smem(int buckets) {
-    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 1024 + align_up(buckets * 4, 16) +
-           8 * align_up(buckets * 4, 16) + kRows * 4;
+  static int smem(const RelBuckets& rb) {
+    const int buckets = rel_num_buckets(rb.n_bounds, rb.bidirectional);
+    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 8 * align_up(buckets * 4, 16) + kRows * 4 +
+           bias_smem(rb);
   }
 };
-
-// Adds v into the warp's bucket sums: lanes with a bucket of their own directly, equal ones
-// through a fixed-order sum over the lanes.
-__device__ __forceinline__ void add_buckets(float* acc, int bucket, float v, int lane) {
-  const unsigned same = __match_any_sync(0xffffffffu, bucket);
-  const bool alone = same == (1u << lane);
-  if (alone && bucket >= 0) acc[bucket] += v;
-  unsigned todo = __ballot_sync(0xffffffffu, !alone && bucket >= 0);
-  while (todo != 0) {
-    const int bb = __shfl_sync(0xffffffffu, bucket, __ffs(todo) - 1);
-    float s = bucket == bb ? v : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) acc[bb] += s;
-    todo &= ~__ballot_sync(0xffffffffu, bucket == bb);
-  }
-  __syncwarp();
-}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
@@ -623,11 +691,9 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
   const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
   float* warps = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
-  int* bounds = reinterpret_cast<int*>(warps + 8 * C::kWarp);
-  float* col = reinterpret_cast<float*>(bounds + 256);
   const int bpad = align_up(buckets * 4, 16) / 4;
-  float* sums = col + bpad;           // [8][bpad]
-  float* sdelta = sums + 8 * bpad;    // [128]
+  float* sums = warps + 8 * C::kWarp;  // [8][bpad]
+  float* sdelta = sums + 8 * bpad;     // [128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_tiles = (p.Lq + kRows - 1) / kRows;
@@ -660,7 +726,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
-  load_table(p, h, kLog2e, bounds, col, buckets, C::kThreads);
+  const BiasLine bias = load_bias(p, h, sdelta + kRows, C::kThreads);
   for (int t = threadIdx.x; t < 8 * bpad; t += C::kThreads) sums[t] = 0.f;
   // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too
   if (threadIdx.x < kRows) {
@@ -780,12 +846,11 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     for (int t = 0; t < n; ++t) {
       const int j0 = t * kCols + half * 32;
       const int d_lo = j0 - warp_first - 31, d_hi = j0 + 31 - warp_first;
-      const int b_lo = rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo);
-      const bool flat = b_lo == rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_hi);
+      const bool flat = bias.flat(d_lo, d_hi);
       if (!flat) {
         __syncwarp();
-        line[lane] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + lane)];
-        line[lane + 32] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + min(lane + 32, 62))];
+        line[lane] = bias.at(d_lo + lane);
+        line[lane + 32] = bias.at(d_lo + lane + 32);
         __syncwarp();
       }
       ok = wait_parity(&s_full[t % NB], (t / NB) & 1, kSiteAttnDq + 5, p.ctx);
@@ -793,10 +858,9 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tc_fence_after();
       const uint32_t ts = tmem + lane_off + (t % NB) * 2 * kCols + half * 32;
       float s[32], g[32];
-      tmem_ld32(ts, s);
-      tmem_ld32(ts + kCols, g);
+      tmem_ld32x2(ts, s, ts + kCols, g);
       if (flat) {
-        const float c = col[b_lo] - lse;
+        const float c = bias.at(d_lo) - lse;
 #pragma unroll
         for (int e = 0; e < 32; ++e) s[e] = exp2_approx(fmaf(s[e], scale2, c)) * (g[e] - delta);
       } else {
@@ -825,7 +889,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
         float tot = (a[0] + a[1]) + (a[2] + a[3]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
-        if (lane == 0) mine[b_lo] += tot;
+        if (lane == 0) mine[bias.bucket(d_lo)] += tot;
       } else {
         // Diagonal sums: from a column to the next a diagonal moves one lane up, so a running sum
         // passed from lane to lane follows it. Two chains of 16 columns; entry d + 31 of a chain.
@@ -845,7 +909,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
         for (int q = 0; q < 2; ++q) {
           const int idx = lane + 32 * q;
           const float v = (idx < 47 ? diag[idx] : 0.f) + (idx >= 16 && idx < 63 ? diag[48 + idx - 16] : 0.f);
-          const int bk = idx < 63 ? rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + idx) : -1 - lane;
+          const int bk = idx < 63 ? bias.bucket(d_lo + idx) : -1 - lane;
           add_buckets(mine, bk, v, lane);
         }
       }
@@ -912,10 +976,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   uint64_t* done = ds_ready + 2;
   uint64_t* last = done + 1;  // every product is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
-  const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
   float* warps = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
-  int* bounds = reinterpret_cast<int*>(warps + 8 * C::kWarp);
-  float* col = reinterpret_cast<float*>(bounds + 256);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k_tiles = (p.Lk + kRows - 1) / kRows;
@@ -949,7 +1010,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
-  load_table(p, h, kLog2e, bounds, col, buckets, C::kThreads);
+  const BiasLine bias = load_bias(p, h, warps + 8 * C::kWarp, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1043,8 +1104,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const int pos = i0 + p.q_offset;
       // diagonal of (key lane, query e): j - i - off = d_lo + 31 + lane - e
       const int d_lo = j0 + wq * 32 - pos - 31, d_hi = j0 + wq * 32 + 31 - pos;
-      const int b_lo = rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo);
-      const bool flat = b_lo == rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_hi);
+      const bool flat = bias.flat(d_lo, d_hi);
       float my_lse = kInf, my_delta = 0.f;
       if (i0 + lane < p.Lq) {
         my_lse = p.lse[hbase + i0 + lane];
@@ -1055,8 +1115,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       rowv[lane] = my_lse;
       rowv[32 + lane] = my_delta;
       if (!flat) {
-        line[lane] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + lane)];
-        line[lane + 32] = col[rel_bucket(bounds, p.rb.n_bounds, p.rb.bidirectional, d_lo + min(lane + 32, 62))];
+        line[lane] = bias.at(d_lo + lane);
+        line[lane + 32] = bias.at(d_lo + lane + 32);
       }
       __syncwarp();
       ok = wait_parity(&s_full[t % NB], (t / NB) & 1, kSiteAttnDkv + 5, p.ctx);
@@ -1064,13 +1124,12 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tc_fence_after();
       const uint32_t ts = tmem + lane_off + (t % NB) * 2 * kCols + half * 32;
       float s[32], g[32];
-      tmem_ld32(ts, s);
-      tmem_ld32(ts + kCols, g);
+      tmem_ld32x2(ts, s, ts + kCols, g);
       // visible to this key: query rows i >= j - off (causal), i < Lq
       const int from = !key_ok ? 32 : (p.causal ? j - pos : 0);
       const int to = p.Lq - i0;
       const bool masked = __any_sync(0xffffffffu, from > 0) || to < 32;
-      const float flat_c = flat ? col[b_lo] : 0.f;
+      const float flat_c = flat ? bias.at(d_lo) : 0.f;
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const float4 ls = *reinterpret_cast<const float4*>(rowv + e);
@@ -1210,10 +1269,9 @@ int set_smem(K kernel, int bytes, int (&done)[64]) {
 }
 
 template <int D, bool BF16>
-int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& p, int buckets,
-            cudaStream_t st) {
+int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& p, cudaStream_t st) {
   static int done[64] = {};
-  const int smem = Fwd<D>::smem(buckets);
+  const int smem = Fwd<D>::smem(p.rb);
   int rc = set_smem(attn_fwd_kernel<D, BF16>, smem, done);
   if (rc) return rc;
   const long long grid = static_cast<long long>((p.Lq + kRows - 1) / kRows) * p.splits * p.H * p.B;
@@ -1231,7 +1289,7 @@ int run_bwd(const CUtensorMap (&big)[4], const CUtensorMap (&small)[4], const At
             float* dtable, cudaStream_t st) {
   // order of the maps: q, k, v, dO
   static int done_q[64] = {}, done_kv[64] = {};
-  const int smem = Bwd<D>::smem(buckets);
+  const int smem = Bwd<D>::smem(p.rb);
   int rc = set_smem(attn_dq_kernel<D, BF16>, smem, done_q);
   if (rc) return rc;
   if ((rc = set_smem(attn_dkv_kernel<D, BF16>, smem, done_kv))) return rc;
@@ -1306,11 +1364,10 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
       (rc = map_heads(&mk, bf16, k, B, Lk, H, D, {k_strides[0], k_strides[1], k_strides[2]}, kCols)) ||
       (rc = map_heads(&mv, bf16, v, B, Lk, H, D, {v_strides[0], v_strides[1], v_strides[2]}, kCols)))
     return rc;
-  const int buckets = rel_num_buckets(n_bounds, p.rb.bidirectional);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (D == 64)
-    return bf16 ? run_fwd<64, true>(mq, mk, mv, p, buckets, st) : run_fwd<64, false>(mq, mk, mv, p, buckets, st);
-  return bf16 ? run_fwd<128, true>(mq, mk, mv, p, buckets, st) : run_fwd<128, false>(mq, mk, mv, p, buckets, st);
+    return bf16 ? run_fwd<64, true>(mq, mk, mv, p, st) : run_fwd<64, false>(mq, mk, mv, p, st);
+  return bf16 ? run_fwd<128, true>(mq, mk, mv, p, st) : run_fwd<128, false>(mq, mk, mv, p, st);
 }
 
 long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional) {

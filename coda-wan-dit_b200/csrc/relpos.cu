@@ -32,7 +32,7 @@ constexpr int kRelThreads = 256;
 constexpr int kRelWarps = kRelThreads / 32;
 constexpr int kBiasRows = 32;    // rows of a forward tile
 constexpr int kBiasCols = 2048;  // columns of a forward tile
-constexpr int kGradRows = 128;   // rows of a gradient strip
+constexpr int kGradRows = 64;    // rows of a gradient strip
 constexpr int kGradCols = 256;   // columns of a gradient strip (8 per lane)
 
 template <typename T>
@@ -217,16 +217,8 @@ __global__ void __launch_bounds__(kRelThreads)
     for (int t0 = 0; t0 < nd; t0 += 32) {
       const int t = t0 + lane;
       const float val = t < nd ? diag[base + t] : 0.f;
-      const int b = t < nd ? rel_bucket(bounds, rb.n_bounds, rb.bidirectional, d_first + t) : -1;
-      unsigned todo = __ballot_sync(0xffffffffu, b >= 0);
-      while (todo != 0) {
-        const int bb = __shfl_sync(0xffffffffu, b, __ffs(todo) - 1);
-        float s = b == bb ? val : 0.f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) mine[bb] += s;
-        todo &= ~__ballot_sync(0xffffffffu, b == bb);
-      }
+      const int b = t < nd ? rel_bucket(bounds, rb.n_bounds, rb.bidirectional, d_first + t) : -1 - lane;
+      add_buckets(mine, b, val, lane);
     }
     __syncwarp();  // diag and mine are reused by the next strip
   }

@@ -33,6 +33,24 @@ __device__ __forceinline__ int rel_bucket(const int* bounds, int n_bounds, int b
   return bidirectional && d > 0 ? lo + n_bounds + 1 : lo;
 }
 
+// Adds v into the warp's bucket sums: lanes with a bucket of their own directly, equal ones
+// through a fixed-order sum over the lanes.
+__device__ __forceinline__ void add_buckets(float* acc, int bucket, float v, int lane) {
+  const unsigned same = __match_any_sync(0xffffffffu, bucket);
+  const bool alone = same == (1u << lane);
+  if (alone && bucket >= 0) acc[bucket] += v;
+  unsigned todo = __ballot_sync(0xffffffffu, !alone && bucket >= 0);
+  while (todo != 0) {
+    const int bb = __shfl_sync(0xffffffffu, bucket, __ffs(todo) - 1);
+    float s = bucket == bb ? v : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) acc[bb] += s;
+    todo &= ~__ballot_sync(0xffffffffu, bucket == bb);
+  }
+  __syncwarp();
+}
+
 __host__ __device__ inline int rel_num_buckets(int n_bounds, int bidirectional) { return (n_bounds + 1) * (bidirectional ? 2 : 1); }
 
 // Host check and copy of the caller's bounds; false = not ascending positive distances.

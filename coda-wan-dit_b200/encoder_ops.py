@@ -17,30 +17,61 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, ptr, stream_ptr
+from ._lib import call, ptr
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_BUCKETS = 256  # table rows of one direction (kMaxRelBounds + 1 in csrc/relpos.cuh)
 
 
-def _require_cuda(*ts: torch.Tensor | None) -> torch.device:
-    """The tensors' common device."""
-    dev = None
+def _require_cuda(*ts: torch.Tensor | None) -> int:
+    """Index of the tensors' common device."""
+    dev = -1
     for t in ts:
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError("wdit ops run on CUDA tensors only (no CPU implementation)")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-        dev = t.device
+        i = t.get_device()
+        if dev >= 0 and i != dev:
+            raise ValueError(f"tensors on different devices: cuda:{dev} and cuda:{i}")
+        dev = i
     return dev
+
+
+class _on_device:
+    """Makes a device current around a launch; free when it is already (torch.cuda.device is not:
+    several microseconds a call)."""
+
+    __slots__ = ("dev", "prev")
+
+    def __init__(self, dev: int):
+        self.dev = dev
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)  # the handle without a Stream object
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor | None:
     # From torch's caching allocator on the current stream: calls never share one, and a captured
     # graph keeps its own.
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+@lru_cache(maxsize=512)
+def _workspace_bytes(dev: int, name: str, *shape: int) -> int:
+    """Workspace query of an entry point (a function of the shape and the device)."""
+    return call(name, *shape)
 
 
 # ---------------------------------------------------------------------------
@@ -97,13 +128,14 @@ def _check_table(table: torch.Tensor) -> None:
 
 
 def _rel_pos_bias(table, q_len, k_len, bidirectional, max_distance, q_offset):
-    H = table.shape[1]
-    bounds, n = _bounds_arg(table.shape[0], max_distance, bidirectional)
-    with torch.cuda.device(table.device):
+    dev = table.get_device()
+    nb, H = table.shape
+    bounds, n = _bounds_arg(nb, max_distance, bidirectional)
+    with _on_device(dev):
         table = table.contiguous()
         out = torch.empty((H, q_len, k_len), dtype=table.dtype, device=table.device)
-        call("wdit_rel_pos_bias", ptr(table), _DTYPE[table.dtype], bounds, n, int(bidirectional), H, q_len, k_len,
-             q_offset, ptr(out), stream_ptr())
+        call("wdit_rel_pos_bias", table.data_ptr(), _DTYPE[table.dtype], bounds, n, bidirectional, H, q_len, k_len,
+             q_offset, out.data_ptr(), _stream(dev))
     return out
 
 
@@ -124,15 +156,15 @@ def rel_pos_bias_grad(dbias: torch.Tensor, num_buckets: int, *, bidirectional: b
         raise ValueError("dbias has no heads")
     _check_positions(Lq, Lk, q_offset)
     bounds, n = _bounds_arg(num_buckets, max_distance, bidirectional)
-    if dbias.stride(3) != 1 and Lk > 1:
-        dbias = dbias.contiguous()
-    with torch.cuda.device(dev):
-        out = torch.empty((num_buckets, H), dtype=torch.float32, device=dev)
-        nbytes = call("wdit_rel_pos_bias_grad_workspace_bytes", B, H, Lq, Lk, n, int(bidirectional))
-        ws = _workspace(nbytes, dev)
-        call("wdit_rel_pos_bias_grad", ptr(dbias), _DTYPE[dbias.dtype], B, H, Lq, Lk, dbias.stride(0), dbias.stride(1),
-             dbias.stride(2), bounds, n, int(bidirectional), q_offset, ptr(out), ptr(ws), nbytes, stream_ptr(),
-             kernels=2)
+    with _on_device(dev):
+        if Lk > 1 and dbias.stride(3) != 1:
+            dbias = dbias.contiguous()
+        out = torch.empty((num_buckets, H), dtype=torch.float32, device=dbias.device)
+        nbytes = _workspace_bytes(dev, "wdit_rel_pos_bias_grad_workspace_bytes", B, H, Lq, Lk, n, int(bidirectional))
+        ws = _workspace(nbytes, dbias.device)
+        sb, sh, si, _ = dbias.stride()
+        call("wdit_rel_pos_bias_grad", dbias.data_ptr(), _DTYPE[dbias.dtype], B, H, Lq, Lk, sb, sh, si, bounds, n,
+             bidirectional, q_offset, out.data_ptr(), ptr(ws), nbytes, _stream(dev), kernels=2)
     return out
 
 
@@ -177,41 +209,44 @@ _ACT = {"none": 0, "gelu_tanh": 1, "relu": 2, "silu": 3, "gelu": 4}
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """2-D operand the kernels take as it is (unit column stride, rows on 16-byte boundaries),
     or a contiguous copy."""
-    if t.shape[0] <= 1 and t.stride(1) == 1 and t.data_ptr() % 16 == 0:
-        return t.as_strided(t.shape, (t.shape[1], 1))  # a single row's stride says nothing
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+    ld, one = t.stride()
+    if one == 1 and (t.shape[0] <= 1 or (ld % 8 == 0 and ld >= t.shape[1])) and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _product(a, a_mn, b, b_mn, M, N, K, out, *, bias=None, act=0, res=None, pre=None):
-    call("wdit_linear_act_residual", ptr(a), a.stride(0), int(a_mn), ptr(b), b.stride(0), int(b_mn), M, N, K,
-         _DTYPE[a.dtype], ptr(bias), 0 if bias is None else _DTYPE[bias.dtype], act,
-         ptr(res), 0 if res is None else res.stride(0), ptr(out), out.stride(0),
-         ptr(pre), 0 if pre is None else pre.stride(0), stream_ptr())
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]  # a single row's stride says nothing
 
 
-def _linear_forward(x2, w, bias, act, res2, out2, pre):
-    M, K = x2.shape
-    N = w.shape[0]
-    _product(_rows(x2), False, _rows(w), False, M, N, K, out2, bias=None if bias is None else bias.contiguous(),
-             act=_ACT[act], res=None if res2 is None else _rows(res2), pre=pre)
+def _product(dev, a, a_mn, b, b_mn, M, N, K, out, bias=None, act=0, res=None, pre=None):
+    call("wdit_linear_act_residual", a.data_ptr(), _ld(a), a_mn, b.data_ptr(), _ld(b), b_mn, M, N, K, _DTYPE[a.dtype],
+         None if bias is None else bias.data_ptr(), 0 if bias is None else _DTYPE[bias.dtype], act,
+         None if res is None else res.data_ptr(), 0 if res is None else _ld(res), out.data_ptr(), N,
+         None if pre is None else pre.data_ptr(), N, _stream(dev))
+
+
+def _linear_forward(dev, x, w, bias, act, residual, out, pre):
+    N, K = w.shape
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if residual is not None:
+        residual = _rows(residual if residual.dim() == 2 else residual.reshape(-1, N))
+    if bias is not None and bias.stride(0) != 1:
+        bias = bias.contiguous()
+    _product(dev, _rows(x2), 0, _rows(w), 0, x2.shape[0], N, K, out, bias, _ACT[act], residual, pre)
 
 
 class _LinearActResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, act, residual):
-        N = w.shape[0]
-        x2 = x.reshape(-1, x.shape[-1])
-        with torch.cuda.device(x.device):
-            out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-            out2 = out.view(-1, N)
+        dev = x.get_device()
+        with _on_device(dev):
+            out = torch.empty((*x.shape[:-1], w.shape[0]), dtype=x.dtype, device=x.device)
             # The derivative needs pre = x W^T + bias: kept in the operands' type (half a step of
             # it moves act' by no more than rounding the gradient itself does).
             need = any(ctx.needs_input_grad[:3]) and act != "none"
-            pre = torch.empty_like(out2) if need else None
-            res2 = None if residual is None else residual.reshape(-1, N)
-            _linear_forward(x2, w, bias, act, res2, out2, pre)
+            pre = torch.empty_like(out) if need else None
+            _linear_forward(dev, x, w, bias, act, residual, out, pre)
         ctx.save_for_backward(x, w, pre)
         ctx.act = act
         ctx.bias_dtype = None if bias is None else bias.dtype
@@ -226,30 +261,30 @@ class _LinearActResidual(torch.autograd.Function):
         x2 = x.reshape(-1, K)
         M = x2.shape[0]
         dx = dw = db = None
-        with torch.cuda.device(x.device):
+        dev = x.get_device()
+        with _on_device(dev):
             g = _rows(dout.reshape(-1, N)) if need_x or need_w or need_b else None
             if g is not None:
                 dpre = torch.empty((M, N), dtype=x.dtype, device=x.device) if pre is not None else g
                 ws, nbytes = None, 0
                 if need_b:
                     db = torch.empty(N, dtype=ctx.bias_dtype, device=x.device)
-                    nbytes = call("wdit_act_backward_workspace_bytes", M, N)
+                    nbytes = _workspace_bytes(dev, "wdit_act_backward_workspace_bytes", M, N)
                     ws = _workspace(nbytes, x.device)
                 if need_b or pre is not None:
-                    call("wdit_act_backward", ptr(g), g.stride(0), ptr(pre), N, _ACT[ctx.act] if pre is not None else 0,
-                         _DTYPE[x.dtype], M, N, ptr(dpre), dpre.stride(0), ptr(db),
-                         0 if db is None else _DTYPE[db.dtype], ptr(ws), nbytes, stream_ptr(),
-                         kernels=2 if need_b else 1)
+                    call("wdit_act_backward", ptr(g), _ld(g), ptr(pre), N, _ACT[ctx.act] if pre is not None else 0,
+                         _DTYPE[x.dtype], M, N, ptr(dpre), _ld(dpre), ptr(db), 0 if db is None else _DTYPE[db.dtype],
+                         ptr(ws), nbytes, _stream(dev), kernels=2 if need_b else 1)
                 if need_x:
                     dx = torch.empty((M, K), dtype=x.dtype, device=x.device)
-                    _product(dpre, False, _rows(w), True, M, K, N, dx)
+                    _product(dev, dpre, 0, _rows(w), 1, M, K, N, dx)
                     dx = dx.view(x.shape)
                 if need_w:
                     if M == 0:
                         dw = torch.zeros((N, K), dtype=w.dtype, device=w.device)
                     else:
                         dw = torch.empty((N, K), dtype=w.dtype, device=w.device)
-                        _product(dpre, True, _rows(x2), True, N, K, M, dw)
+                        _product(dev, dpre, 1, _rows(x2), 1, N, K, M, dw)
         return dx, dw, db, None, dout if need_r else None
 
 
@@ -264,33 +299,34 @@ def linear_act_residual(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | N
     residual. Operands whose rows do not start on 16-byte boundaries are copied first."""
     if act not in _ACT:
         raise ValueError(f"unknown activation {act!r} ({', '.join(_ACT)})")
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
-        raise ValueError(f"x [..., K] and w [N, K] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
-    if x.dtype not in (torch.bfloat16, torch.float16) or w.dtype != x.dtype:
+    xs, ws = x.shape, w.shape
+    if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[1]:
+        raise ValueError(f"x [..., K] and w [N, K] expected, got {tuple(xs)} and {tuple(ws)}")
+    dtype = x.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or w.dtype is not dtype:
         raise ValueError(f"x and w must both be bf16 or both fp16, got {x.dtype} and {w.dtype}")
-    N, K = w.shape
+    N, K = ws
     if N % 8 != 0 or K % 8 != 0 or N == 0 or K == 0:
         raise ValueError(f"N and K must be multiples of 8, got N {N}, K {K}")
-    shape = (*x.shape[:-1], N)
+    shape = (*xs[:-1], N)
     if bias is not None and (bias.shape != (N,) or bias.dtype not in _DTYPE):
         raise ValueError(f"bias must be [{N}] of fp32, bf16 or fp16, got {tuple(bias.shape)} {bias.dtype}")
     for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (t.shape != shape or t.dtype != x.dtype):
-            raise ValueError(f"{name} must be {shape} of {x.dtype}, got {tuple(t.shape)} {t.dtype}")
-    _require_cuda(x, w, bias, residual, out)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual, out))
-    if grad:
+        if t is not None and (t.shape != shape or t.dtype is not dtype):
+            raise ValueError(f"{name} must be {shape} of {dtype}, got {tuple(t.shape)} {t.dtype}")
+    dev = _require_cuda(x, w, bias, residual, out)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual, out)):
         if out is not None:
             raise ValueError("out= is not supported where a gradient is recorded")
         return _LinearActResidual.apply(x, w, bias, act, residual)
-    with torch.cuda.device(x.device):
+    with _on_device(dev):
         if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        elif not out.is_contiguous() or out.data_ptr() % 16 != 0:
-            raise ValueError("out must be contiguous and start on a 16-byte boundary")
-        _check_out_overlap(out, residual, x, w, bias)
-        res2 = None if residual is None else residual.reshape(-1, N)
-        _linear_forward(x.reshape(-1, K), w, bias, act, res2, out.view(-1, N), None)
+            out = torch.empty(shape, dtype=dtype, device=x.device)
+        else:
+            if not out.is_contiguous() or out.data_ptr() % 16 != 0:
+                raise ValueError("out must be contiguous and start on a 16-byte boundary")
+            _check_out_overlap(out, residual, x, w, bias)
+        _linear_forward(dev, x, w, bias, act, residual, out, None)
     return out
 
 
@@ -323,48 +359,54 @@ def _check_out_overlap(out, residual, *inputs) -> None:
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """[B, L, H, D] the kernels take as it is (unit stride along D, the other strides positive
     multiples of 8 elements, 16-byte aligned), or a contiguous copy."""
-    if t.data_ptr() % 16 == 0 and t.stride(3) == 1 and all(
-            n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3])):
+    (B, L, H, _), (sb, sl, sh, sd) = t.shape, t.stride()
+    if (sd == 1 and t.data_ptr() % 16 == 0 and (B == 1 or (sb > 0 and sb % 8 == 0))
+            and (L == 1 or (sl > 0 and sl % 8 == 0)) and (H == 1 or (sh > 0 and sh % 8 == 0))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
+_Strides = ctypes.c_longlong * 3
+
+
 def _strides(t: torch.Tensor):
     # a dimension of size 1 has no meaningful stride; any valid one does
-    return (ctypes.c_longlong * 3)(*(t.stride(i) if t.shape[i] > 1 else t.shape[3] for i in range(3)))
+    (B, L, H, D), (sb, sl, sh, _) = t.shape, t.stride()
+    return _Strides(sb if B > 1 else D, sl if L > 1 else D, sh if H > 1 else D)
 
 
-def _attention_args(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale):
+def _attention_args(q, k, table, k_lens, bidirectional, causal, max_distance, q_offset, scale):
     B, Lq, H, D = q.shape
     bounds, n = _bounds_arg(table.shape[0], max_distance, bidirectional)
-    shape = (B, H, Lq, k.shape[1], D, _DTYPE[q.dtype])
-    pos = (ptr(k_lens), ptr(table), _DTYPE[table.dtype], bounds, n, int(bidirectional), int(causal), q_offset,
-           float(scale))
+    shape = (B, H, Lq, k.shape[1], D)
+    pos = (_DTYPE[q.dtype], None if k_lens is None else k_lens.data_ptr(), table.data_ptr(), _DTYPE[table.dtype],
+           bounds, n, bidirectional, causal, q_offset, scale)
     return shape, pos
 
 
-def _attention_forward(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale, with_lse):
+def _attention_forward(dev, q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale, with_lse):
     B, Lq, H, D = q.shape
-    Lk = k.shape[1]
-    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if with_lse else None
-    if out.numel() == 0 or Lk == 0:
+    device = q.device
+    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=device)
+    if B == 0 or Lq == 0 or k.shape[1] == 0:
         return out.zero_(), None
-    shape, pos = _attention_args(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale)
-    nbytes = call("wdit_rel_attention_workspace_bytes", *shape[:5])
-    ws = _workspace(nbytes, q.device)
-    call("wdit_rel_attention", ptr(q), _strides(q), ptr(k), _strides(k), ptr(v), _strides(v), *shape, *pos, ptr(out),
-         ptr(lse), ptr(ws), nbytes, stream_ptr(), kernels=1 if nbytes == 0 else 2)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=device) if with_lse else None
+    shape, pos = _attention_args(q, k, table, k_lens, bidirectional, causal, max_distance, q_offset, scale)
+    nbytes = _workspace_bytes(dev, "wdit_rel_attention_workspace_bytes", *shape)
+    ws = _workspace(nbytes, device)
+    call("wdit_rel_attention", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), *shape,
+         *pos, out.data_ptr(), ptr(lse), ptr(ws), nbytes, _stream(dev), kernels=1 if nbytes == 0 else 2)
     return out, lse
 
 
 class _RelPosAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale):
-        with torch.cuda.device(q.device):
+        dev = q.get_device()
+        with _on_device(dev):
             qc, kc, vc, tc = _heads(q), _heads(k), _heads(v), table.contiguous()
-            out, lse = _attention_forward(qc, kc, vc, tc, k_lens, bidirectional, causal, max_distance, q_offset, scale,
-                                          True)
+            out, lse = _attention_forward(dev, qc, kc, vc, tc, k_lens, bidirectional, causal, max_distance, q_offset,
+                                          scale, True)
         ctx.save_for_backward(qc, kc, vc, tc, k_lens, out, lse)
         ctx.args = (bidirectional, causal, max_distance, q_offset, scale)
         return out
@@ -376,16 +418,18 @@ class _RelPosAttention(torch.autograd.Function):
         nothing = (None,) * 6
         if lse is None:  # no queries or no keys
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(table), *nothing)
-        with torch.cuda.device(q.device):
+        dev = q.get_device()
+        with _on_device(dev):
             g = _heads(dout)
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
             dtable = torch.empty(table.shape, dtype=torch.float32, device=table.device)
-            shape, pos = _attention_args(q, k, v, table, k_lens, *ctx.args)
-            nbytes = call("wdit_rel_attention_backward_workspace_bytes", *shape[:3], pos[4], pos[5])
+            shape, pos = _attention_args(q, k, table, k_lens, *ctx.args)
+            nbytes = _workspace_bytes(dev, "wdit_rel_attention_backward_workspace_bytes", *shape[:3], pos[5],
+                                      int(pos[6]))
             ws = _workspace(nbytes, q.device)
             call("wdit_rel_attention_backward", ptr(q), _strides(q), ptr(k), _strides(k), ptr(v), _strides(v), ptr(g),
                  _strides(g), ptr(out), ptr(lse), *shape, *pos, ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws), nbytes,
-                 stream_ptr(), kernels=3)
+                 _stream(dev), kernels=3)
         return (dq, dk, dv, dtable.to(table.dtype), *nothing)
 
 
@@ -401,29 +445,30 @@ def rel_pos_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
     that sees no key gives 0. scale defaults to D ** -0.5. One token after a cache of n keys:
     Lq 1, q_offset n - 1 if the cache holds the token's own key, n otherwise. Differentiable in
     q, k, v and table; results repeat bit for bit."""
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"q [B, Lq, H, D], k and v [B, Lk, H, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, "
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape:
+        raise ValueError(f"q [B, Lq, H, D], k and v [B, Lk, H, D] expected, got {tuple(qs)}, {tuple(ks)}, "
                          f"{tuple(v.shape)}")
-    B, Lq, H, D = q.shape
-    if k.shape[0] != B or k.shape[2:] != q.shape[2:]:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, heads or head size")
-    if D not in (64, 128):
+    B, Lq, H, D = qs
+    if ks[0] != B or ks[2] != H or ks[3] != D:
+        raise ValueError(f"q {tuple(qs)} and k {tuple(ks)} differ in batch, heads or head size")
+    if D != 64 and D != 128:
         raise ValueError(f"head size 64 or 128, got {D}")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError(f"q, k and v must all be bf16 or all fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
     _check_table(table)
     if table.shape[1] != H:
         raise ValueError(f"table for {table.shape[1]} heads, q has {H}")
-    _check_positions(Lq, k.shape[1], q_offset)
+    _check_positions(Lq, ks[1], q_offset)
     rel_pos_bounds(table.shape[0], max_distance, bidirectional)
-    if k_lens is not None and (k_lens.shape != (B,) or k_lens.dtype != torch.int32):
-        raise ValueError(f"k_lens must be [{B}] int32, got {tuple(k_lens.shape)} {k_lens.dtype}")
-    _require_cuda(q, k, v, table, k_lens)
-    scale = D**-0.5 if scale is None else float(scale)
     if k_lens is not None:
+        if k_lens.shape != (B,) or k_lens.dtype is not torch.int32:
+            raise ValueError(f"k_lens must be [{B}] int32, got {tuple(k_lens.shape)} {k_lens.dtype}")
         k_lens = k_lens.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table)):
+    dev = _require_cuda(q, k, v, table, k_lens)
+    scale = D**-0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
         return _RelPosAttention.apply(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale)
-    with torch.cuda.device(q.device):
-        return _attention_forward(_heads(q), _heads(k), _heads(v), table.contiguous(), k_lens, bidirectional, causal,
-                                  max_distance, q_offset, scale, False)[0]
+    with _on_device(dev):
+        return _attention_forward(dev, _heads(q), _heads(k), _heads(v), table.contiguous(), k_lens, bidirectional,
+                                  causal, max_distance, q_offset, scale, False)[0]
