@@ -20,7 +20,7 @@
 // of size Lq x Lk leaves the SM.
 //
 //   attn_fwd_kernel  CTA = 128 query rows of one head; key tiles of 64; warp 0 loads, warp 1
-//                    issues MMAs, warps 2-5 softmax (one row per thread). Two score buffers: the
+//                    issues MMAs, warps 2-9 softmax (half a row per thread). Two score buffers: the
 //                    next tile's scores are computed while this one's are exponentiated. With few
 //                    CTAs the keys are split over several, whose parts attn_combine_kernel joins.
 //   attn_dq_kernel   same rows; computes delta, dQ and the table's partial sums. No atomics.
@@ -179,8 +179,6 @@ __device__ __forceinline__ void tmem_ld32x2(uint32_t a, float* v, uint32_t b, fl
   }
 }
 
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) { tmem_ld32x2(taddr, v, taddr + 32, v + 32); }
-
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // MN-major operand tile: rows of 64 elements (128 B) along M or N, one row per K index; pieces of
@@ -295,16 +293,47 @@ __host__ __device__ constexpr int align_up(int x, int a) { return (x + a - 1) / 
 // ---------------------------------------------------------------------------
 // Forward
 // ---------------------------------------------------------------------------
+// Ten warps, two CTAs per SM. Warps 2-9 are the softmax: warp w reads TMEM lanes [32 (w % 4), + 32),
+// warps 2-5 columns 0-31 of a score tile, warps 6-9 columns 32-63; the two warps of a row agree
+// on the maximum in use through a named barrier of 64 threads.
 template <int D>
 struct Fwd {
   static constexpr int kStages = D == 64 ? 4 : 2;
-  static constexpr int kThreads = 192;
+  static constexpr int kThreads = 320;
   static constexpr uint32_t kQ = kRows * D * 2;
   static constexpr uint32_t kTile = kCols * D * 2;
   static constexpr uint32_t kTmem = 256;  // two score buffers of 64 columns, O at 128
-  static constexpr int kLine = 96;        // per-warp bias line (31 + 64 diagonals)
-  static int smem(const RelBuckets& rb) { return 1024 + kQ + kStages * 2 * kTile + 256 + 4 * kLine * 4 + bias_smem(rb); }
+  static constexpr int kLine = 64;        // per-warp bias line (31 + 32 diagonals)
+  static constexpr int kFloats = 8 * kLine + 2 * kRows;  // lines, the halves' row values
+  static int smem(const RelBuckets& rb) { return 1024 + kQ + kStages * 2 * kTile + 256 + kFloats * 4 + bias_smem(rb); }
 };
+
+// Linear block index -> (query tile, split, head, sample). Under a causal mask the last query rows
+// see most keys: all heads' last tiles go first, so that the short ones fill the end. Otherwise
+// the query tile is fastest: its CTAs share K and V in L2.
+struct FwdPlace {
+  int qt, split, h, b;
+};
+__device__ __forceinline__ FwdPlace fwd_place(const AttnArgs& p, int q_tiles) {
+  unsigned x = blockIdx.x;
+  FwdPlace f;
+  if (p.causal) {
+    f.h = x % p.H;
+    x /= p.H;
+    f.b = x % p.B;
+    x /= p.B;
+    f.split = x % p.splits;
+    f.qt = q_tiles - 1 - static_cast<int>(x / p.splits);
+  } else {
+    f.qt = x % q_tiles;
+    x /= q_tiles;
+    f.split = x % p.splits;
+    x /= p.splits;
+    f.h = x % p.H;
+    f.b = x / p.H;
+  }
+  return f;
+}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
@@ -324,25 +353,19 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
   uint64_t* v_full = bars + 2 * ST;
   uint64_t* v_empty = bars + 3 * ST;
   uint64_t* q_full = bars + 4 * ST;
-  uint64_t* s_full = q_full + 1;  // 2
+  uint64_t* s_full = q_full + 1;   // 2
   uint64_t* p_ready = s_full + 2;  // 2: a warp may finish its rows of t + 1 before another's of t
   uint64_t* pv_done = p_ready + 2;
   uint64_t* last = pv_done + 1;  // every product is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
   float* lines = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
+  float* row_x = lines + 8 * C::kLine;  // [2][kRows]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_tiles = (p.Lq + kRows - 1) / kRows;
-  // q tile fastest (its CTAs share K and V in L2), then split, head, sample; the last rows first,
-  // since under a causal mask they see most keys
-  int x = blockIdx.x;
-  const int qt = q_tiles - 1 - x % q_tiles;
-  x /= q_tiles;
-  const int split = x % p.splits;
-  x /= p.splits;
-  const int h = x % p.H;
-  const int b = x / p.H;
-  const int i0 = qt * kRows;
+  const FwdPlace at = fwd_place(p, q_tiles);
+  const int h = at.h, b = at.b, split = at.split;
+  const int i0 = at.qt * kRows;
   const int klen = sample_len(p, b);
   int visible = klen;  // keys any row of the tile sees
   if (p.causal) visible = min(visible, min(i0 + kRows, p.Lq) + p.q_offset);
@@ -355,6 +378,20 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
   }
   const int n = max(0, t1 - t0);
 
+  auto load_k = [&](int t) {
+    const int st = t % ST;
+    mbar_arrive_expect_tx(&k_full[st], C::kTile);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+      tma_load_4d(sK + st * C::kTile + c * 8192, &tmK, &k_full[st], c * 64, h, (t0 + t) * kCols, b);
+  };
+  auto load_v = [&](int t) {
+    const int st = t % ST;
+    mbar_arrive_expect_tx(&v_full[st], C::kTile);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+      tma_load_4d(sV + st * C::kTile + c * 8192, &tmV, &v_full[st], c * 64, h, (t0 + t) * kCols, b);
+  };
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1);
@@ -363,19 +400,30 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       mbar_init(&v_empty[i], 1);
     }
     mbar_init(q_full, 1);
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
-    mbar_init(&p_ready[0], 4);
-    mbar_init(&p_ready[1], 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 8);
+    }
     mbar_init(pv_done, 1);
     mbar_init(last, 1);
     fence_mbar_init();
+    // the first loads run under the rest of the set-up
+    if (n > 0) {
+      mbar_arrive_expect_tx(q_full, C::kQ);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) tma_load_4d(sQ + c * 16384, &tmQ, q_full, c * 64, h, i0, b);
+      for (int t = 0; t < min(n, ST); ++t) {
+        load_k(t);
+        load_v(t);
+      }
+    }
   }
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
-  const BiasLine bias = load_bias(p, h, lines + 4 * C::kLine, C::kThreads);
+  const BiasLine bias = load_bias(p, h, lines + C::kFloats, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -384,25 +432,14 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(q_full, C::kQ);
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) tma_load_4d(sQ + c * 16384, &tmQ, q_full, c * 64, h, i0, b);
-      int k_loaded = 0, v_loaded = 0;
-      for (int t = 0; t < n; ++t) {
-        const int st = t % ST;
+      int k_loaded = min(n, ST), v_loaded = k_loaded;
+      for (int t = ST; t < n; ++t) {
         const uint32_t ph = (t / ST) & 1;
-        const int j0 = (t0 + t) * kCols;
-        if (!wait_parity(&k_empty[st], ph ^ 1u, kSiteAttn, p.ctx)) break;
-        mbar_arrive_expect_tx(&k_full[st], C::kTile);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(sK + st * C::kTile + c * 8192, &tmK, &k_full[st], c * 64, h, j0, b);
+        if (!wait_parity(&k_empty[t % ST], ph ^ 1u, kSiteAttn, p.ctx)) break;
+        load_k(t);
         k_loaded = t + 1;
-        if (!wait_parity(&v_empty[st], ph ^ 1u, kSiteAttn + 1, p.ctx)) break;
-        mbar_arrive_expect_tx(&v_full[st], C::kTile);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(sV + st * C::kTile + c * 8192, &tmV, &v_full[st], c * 64, h, j0, b);
+        if (!wait_parity(&v_empty[t % ST], ph ^ 1u, kSiteAttn + 1, p.ctx)) break;
+        load_v(t);
         v_loaded = t + 1;
       }
       // Do not leave while a copy into this CTA's shared memory is in flight.
@@ -450,7 +487,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       if (lane == 0) {
-        issue_ts<false>(tmem_o, tmem + (t & 1) * kCols, smem_u32(sV + st * C::kTile), id_o, t > 0);
+        issue_ts<true>(tmem_o, tmem + (t & 1) * kCols, smem_u32(sV + st * C::kTile), id_o, t > 0);
         mma_commit(&v_empty[st]);
         mma_commit(pv_done);
         if (t + 1 == n) mma_commit(last);
@@ -459,11 +496,13 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     }
   } else {
     const int wq = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const uint32_t pair_bar = 1 + wq;  // the two warps that share these rows
     const int r = wq * 32 + lane;
     const int i = i0 + r;
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
-    float* line = lines + wq * C::kLine;
-    const float scale2 = p.scale * kLog2e;
+    float* line = lines + (warp - 2) * C::kLine;
+    const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     const int row_end = p.causal ? min(klen, i + p.q_offset + 1) : klen;  // keys this row sees
     const int warp_first = i0 + wq * 32 + p.q_offset;                      // the warp's first position
     float m_used = -kInf, l = 0.f;
@@ -478,53 +517,74 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
         if (lane == 0) mbar_arrive(&p_ready[t & 1]);
         continue;
       }
-      const int j0 = (t0 + t) * kCols;
-      // the tile's bias: one value, or a line over its 31 + 64 diagonals
-      const int d_lo = j0 - warp_first - 31, d_hi = j0 + kCols - 1 - warp_first;
+      const int j0 = (t0 + t) * kCols + half * 32;
+      // the tile's bias: one value, or a line over its 31 + 32 diagonals
+      const int d_lo = j0 - warp_first - 31, d_hi = j0 + 31 - warp_first;
       const bool flat = bias.flat(d_lo, d_hi);
-      if (!flat) {
+      float flat_c = 0.f;
+      if (flat) {
+        flat_c = bias.at(d_lo);
+      } else {
         __syncwarp();  // the previous tile's reads are done
-#pragma unroll
-        for (int q = 0; q < 3; ++q) line[lane + 32 * q] = bias.at(d_lo + lane + 32 * q);
+        line[lane] = bias.at(d_lo + lane);
+        line[lane + 32] = bias.at(d_lo + lane + 32);
         __syncwarp();
       }
       ok = wait_parity(&s_full[t & 1], (t >> 1) & 1, kSiteAttn + 7, p.ctx);
-      if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      tc_fence_after();
-      const uint32_t ts = tmem + lane_off + (t & 1) * kCols;
-      float z[kCols];
-      tmem_ld64(ts, z);
-      if (flat) {
-        const float c = bias.at(d_lo);
+      ok = __all_sync(0xffffffffu, ok);
+      const uint32_t ts = tmem + lane_off + (t & 1) * kCols + half * 32;
+      float z[32];
+      float m_tile = -kInf;
+      if (ok) {
+        tc_fence_after();
+        uint32_t raw[32];
+        tmem_ld32_nowait(ts, raw);
+        tmem_wait_ld(raw);
+        if (flat) {
+          const uint64_t c2 = f2_pack(flat_c, flat_c);
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) z[e] = fmaf(z[e], scale2, c);
-      } else {
-        const float* ln = line + 31 - lane;
+          for (int e = 0; e < 32; e += 2)
+            f2_unpack(ffma2(f2_pack(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), scale2, c2), z[e], z[e + 1]);
+        } else {
+          const float* ln = line + 31 - lane;
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) z[e] = fmaf(z[e], scale2, ln[e]);
+          for (int e = 0; e < 32; e += 2)
+            f2_unpack(ffma2(f2_pack(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), scale2,
+                            f2_pack(ln[e], ln[e + 1])),
+                      z[e], z[e + 1]);
+        }
+        if (__any_sync(0xffffffffu, row_end < j0 + 32)) {
+          const int keep = row_end - j0;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) z[e] = e < keep ? z[e] : -kInf;
+        }
+        float m4[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+        for (int e = 4; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], z[e]);
+        m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       }
-      if (__any_sync(0xffffffffu, row_end < j0 + kCols)) {
-        const int keep = row_end - j0;
-#pragma unroll
-        for (int e = 0; e < kCols; ++e) z[e] = e < keep ? z[e] : -kInf;
-      }
-      float m4[4] = {z[0], z[1], z[2], z[3]};
-#pragma unroll
-      for (int e = 4; e < kCols; ++e) m4[e & 3] = fmaxf(m4[e & 3], z[e]);
-      const float m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       // The running maximum in use moves only when it is exceeded by more than 8 (a factor of 256
       // in P, harmless in fp32 sums and in 16-bit P), so O is rarely rescaled.
-      if (__any_sync(0xffffffffu, m_tile > m_used + 8.f || (m_used == -kInf && m_tile > -kInf))) {
-        const float m_new = fmaxf(m_used, m_tile);
+      if (named_bar_any(pair_bar, 64, !ok || m_tile > m_used + 8.f)) {
+        if (named_bar_any(pair_bar, 64, !ok)) {
+          ok = false;
+          break;
+        }
+        row_x[half * kRows + r] = m_tile;
+        named_bar_sync(pair_bar, 64);
+        const float m_new = fmaxf(m_used, fmaxf(m_tile, row_x[(half ^ 1) * kRows + r]));
         const float f = m_new == -kInf ? 1.f : exp2_approx(m_used - m_new);
         l *= f;
         m_used = m_new;
         if (t > 0) {
           ok = wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 8, p.ctx);
-          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          if (named_bar_any(pair_bar, 64, !ok)) {
+            ok = false;
+            break;
+          }
           tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
+#pragma unroll 1
+          for (int c = half; c < D / 32; c += 2) {
             float o[32];
             tmem_ld32(tmem_o + lane_off + c * 32, o);
 #pragma unroll
@@ -533,67 +593,61 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
           }
         }
       }
-      const float m_sub = m_used == -kInf ? 0.f : m_used;
+      const float m_sub = m_used == -kInf ? 0.f : -m_used;
       float s4[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t w[kCols / 2];
+      uint32_t w[16];
 #pragma unroll
-      for (int e = 0; e < kCols; e += 2) {
-        const float a = exp2_approx(z[e] - m_sub), c = exp2_approx(z[e + 1] - m_sub);
+      for (int e = 0; e < 32; e += 2) {
+        const float a = exp2_approx(z[e] + m_sub), c = exp2_approx(z[e + 1] + m_sub);
         s4[e & 2] += a;
         s4[(e & 2) + 1] += c;
         w[e >> 1] = pack16<BF16>(a, c);
       }
       l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
       tmem_st16(ts, w);
-      tmem_st16(ts + 16, w + 16);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[t & 1]);
     }
-    if (ok && n > 0) {
-      ok = wait_parity(last, 0, kSiteAttn + 9, p.ctx);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-    }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const float lse = l > 0.f || l != l ? m_used + log2f(l) : -kInf;
+    // the row's sum over both halves (an idle pair's rows are not stored)
+    row_x[half * kRows + r] = l;
+    bool done = ok;
+    if (ok && n > 0) done = wait_parity(last, 0, kSiteAttn + 9, p.ctx);
+    ok = !named_bar_any(pair_bar, 64, !done);
+    tc_fence_after();
+    l += row_x[(half ^ 1) * kRows + r];
+    const bool any = l > 0.f || l != l;
+    const float inv = any ? 1.f / l : 0.f;
+    const float lse = any ? m_used + log2f(l) : -kInf;
     const long long hrow = (static_cast<long long>(b) * p.H + h) * p.Lq + i;
-    if (p.splits > 1) {
-      const long long slot = static_cast<long long>(split) * p.B * p.H * p.Lq + hrow;
-      if (i < p.Lq) p.part_lse[slot] = lse;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
-        if (n > 0 && ok) {
-          tmem_ld32(tmem_o + lane_off + c * 32, o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
-        }
-        if (i >= p.Lq) continue;
-        float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + c * 32);
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          dst[q] = inv == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                              : make_float4(o[4 * q] * inv, o[4 * q + 1] * inv, o[4 * q + 2] * inv, o[4 * q + 3] * inv);
+    const long long slot = static_cast<long long>(split) * p.B * p.H * p.Lq + hrow;
+    uint16_t* dst = static_cast<uint16_t*>(p.out) + ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D;
+    if (i < p.Lq && half == 0) {
+      if (p.splits > 1) {
+        p.part_lse[slot] = lse;
+      } else if (p.lse != nullptr) {
+        p.lse[hrow] = lse;
       }
-    } else {
-      if (i < p.Lq && p.lse != nullptr) p.lse[hrow] = lse;
-      uint16_t* dst = static_cast<uint16_t*>(p.out) + ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D;
+    }
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
-        if (n > 0 && ok) {
-          tmem_ld32(tmem_o + lane_off + c * 32, o);
-        } else {
+    for (int c = half; c < D / 32; c += 2) {
+      float o[32];
+      if (n > 0 && ok) {
+        tmem_ld32(tmem_o + lane_off + c * 32, o);
+      } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
-        }
-        if (i >= p.Lq) continue;
-        // a row without keys is 0 whatever its accumulator holds
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+      }
+      if (i >= p.Lq) continue;
+      // a row without keys is 0 whatever its accumulator holds
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = inv == 0.f ? 0.f : o[e] * inv;
+      for (int e = 0; e < 32; ++e) o[e] = any ? o[e] * inv : 0.f;
+      if (p.splits > 1) {
+        float4* po = reinterpret_cast<float4*>(p.part_o + slot * D + c * 32);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) po[q] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+      } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           st_global_v4(dst + c * 32 + q * 8, pack16<BF16>(o[8 * q], o[8 * q + 1]),
