@@ -114,20 +114,45 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // Bounded wait for the phase with the given parity to complete.
+// The waiting thread is suspended by the hardware for up to kSuspendNs at a time, so that waiting
+// warps take no issue slots from the working ones.
+constexpr uint32_t kSuspendNs = 100000;
+
+template <bool kCluster>
+__device__ __forceinline__ bool mbar_suspend_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  if constexpr (kCluster) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+  }
+  return done != 0;
+}
+
 template <bool kCluster = false>
 __device__ __forceinline__ bool wait_parity(uint64_t* bar, uint32_t parity, unsigned int site, const WaitCtx& ctx) {
-  if (mbar_try_wait<kCluster>(bar, parity)) return true;
+  if (mbar_suspend_wait<kCluster>(bar, parity)) return true;
   const uint64_t start = globaltimer_ns();
-  while (true) {
 #pragma unroll 1
-    for (int i = 0; i < 256; ++i) {
-      if (mbar_try_wait<kCluster>(bar, parity)) return true;
-    }
+  while (!mbar_suspend_wait<kCluster>(bar, parity)) {
     if (globaltimer_ns() - start > ctx.limit_ns) {
       report_error_to(ctx.rec, kErrTimeout, site, parity);
       return false;
     }
   }
+  return true;
 }
 
 #ifdef WDIT_OWNS_ERROR_RECORD
@@ -443,6 +468,12 @@ __device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 

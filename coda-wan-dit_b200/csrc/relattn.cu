@@ -20,8 +20,7 @@
 // of size Lq x Lk leaves the SM.
 //
 //   attn_fwd_kernel  CTA = 128 query rows of one head; key tiles of 64; warp 0 loads, warp 1
-//                    issues MMAs, warps 2-9 softmax (half a row per thread). Two score buffers: the
-//                    next tile's scores are computed while this one's are exponentiated. With few
+//                    issues MMAs, warps 2-9 softmax (half a row per thread). With few
 //                    CTAs the keys are split over several, whose parts attn_combine_kernel joins.
 //   attn_dq_kernel   same rows; computes delta, dQ and the table's partial sums. No atomics.
 //   attn_dkv_kernel  CTA = 128 keys; runs over query tiles of 64 with the scores transposed, so
@@ -181,12 +180,13 @@ __device__ __forceinline__ void tmem_ld32x2(uint32_t a, float* v, uint32_t b, fl
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// MN-major operand tile: rows of 64 elements (128 B) along M or N, one row per K index; pieces of
-// 64 elements are 64 rows x 128 B apart.
-__device__ __forceinline__ uint64_t smem_desc_mn64(uint32_t saddr) {
+// MN-major operand tile of ROWS K indices: rows of 64 elements (128 B) along M or N, one row per K
+// index; pieces of 64 elements are ROWS x 128 B apart.
+template <int ROWS>
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(8192u >> 4) << 16;
+  d |= static_cast<uint64_t>((ROWS * 128u) >> 4) << 16;
   d |= static_cast<uint64_t>(1024u >> 4) << 32;
   d |= static_cast<uint64_t>(1u) << 46;
   d |= static_cast<uint64_t>(2u) << 61;
@@ -198,34 +198,36 @@ __host__ __device__ constexpr uint32_t idesc16(int m, int n, bool bf16, bool b_m
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// Score product of a 128-row tile (pieces of 64 columns 16 KB apart) and a 64-row tile (8 KB
-// apart), both K-major over D.
-template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t a128, uint32_t b64, uint32_t idesc) {
-  const uint64_t a = smem_desc_sw128(a128), b = smem_desc_sw128(b64);
+// Score product of a 128-row tile and a COLS-row tile, both K-major over D (pieces of 64 columns,
+// 128 bytes a row).
+template <int D, int COLS>
+__device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t a128, uint32_t b_tile, uint32_t idesc) {
+  const uint64_t a = smem_desc_sw128(a128), b = smem_desc_sw128(b_tile);
 #pragma unroll
   for (int k = 0; k < D / 16; ++k)
-    mma_bf16(d_tmem, a + (k >> 2) * 1024 + (k & 3) * 2, b + (k >> 2) * 512 + (k & 3) * 2, idesc, k != 0 ? 1u : 0u);
+    mma_bf16(d_tmem, a + (k >> 2) * (kRows * 8) + (k & 3) * 2, b + (k >> 2) * (COLS * 8) + (k & 3) * 2, idesc,
+             k != 0 ? 1u : 0u);
 }
 
-// acc[128, D] (+)= A[128 x 64, TMEM] * B[64 x D, shared memory rows]. SPREAD: the two 32-column
-// halves of A lie 32 TMEM columns apart (written by different warps), else 16.
-template <bool SPREAD>
-__device__ __forceinline__ void issue_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b64, uint32_t idesc, bool accum) {
-  const uint64_t b = smem_desc_mn64(b64);
+// acc[128, D] (+)= A[128 x COLS, TMEM] * B[COLS x D, shared memory rows]. The two halves of A's
+// columns are written by different warps, each over the scores it read: COLS / 2 TMEM columns apart.
+template <int COLS>
+__device__ __forceinline__ void issue_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_tile, uint32_t idesc,
+                                         bool accum) {
+  const uint64_t b = smem_desc_mn<COLS>(b_tile);
+  constexpr int H = COLS / 32;  // MMAs of 16 K indices in a half
 #pragma unroll
-  for (int k = 0; k < kCols / 16; ++k)
-    mma_ts(d_tmem, a_tmem + (SPREAD ? (k >> 1) * 32 + (k & 1) * 8 : k * 8), b + 128 * k, idesc,
-           accum || k != 0 ? 1u : 0u);
+  for (int k = 0; k < COLS / 16; ++k)
+    mma_ts(d_tmem, a_tmem + (k / H) * (COLS / 2) + (k % H) * 8, b + 128 * k, idesc, accum || k != 0 ? 1u : 0u);
 }
 
-// Zero rows [first, 64) of a 64-row tile (whole 128-byte rows: the swizzle stays inside a row).
-template <int D>
+// Zero rows [first, ROWS) of a tile (whole 128-byte rows: the swizzle stays inside a row).
+template <int D, int ROWS>
 __device__ __forceinline__ void zero_tail(uint8_t* tile, int first, int lane) {
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
-    for (int x = first * 8 + lane; x < 64 * 8; x += 32)
-      *reinterpret_cast<uint4*>(tile + c * 8192 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+    for (int x = first * 8 + lane; x < ROWS * 8; x += 32)
+      *reinterpret_cast<uint4*>(tile + c * (ROWS * 128) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
   fence_proxy_async_smem();
   __syncwarp();
 }
@@ -294,8 +296,15 @@ __host__ __device__ constexpr int align_up(int x, int a) { return (x + a - 1) / 
 // Forward
 // ---------------------------------------------------------------------------
 // Ten warps, two CTAs per SM. Warps 2-9 are the softmax: warp w reads TMEM lanes [32 (w % 4), + 32),
-// warps 2-5 columns 0-31 of a score tile, warps 6-9 columns 32-63; the two warps of a row agree
-// on the maximum in use through a named barrier of 64 threads.
+// warps 2-5 columns 0-31 of a score tile, warps 6-9 columns 32-63; the two warps of a row share
+// the maximum in use. Two score buffers: the scores of t + 1 are computed while those of t are
+// exponentiated, so the softmax never waits for a product. (One buffer of 128 columns, with the
+// two CTAs left to alternate, measured 5% slower: they fall into step and wait together.)
+//
+// The maximum in use is that of the row's first tile. Later tiles are exponentiated against it
+// without looking for theirs; only when a tile's sum passes kSumLimit is the maximum taken anew,
+// O rescaled and the tile done again. 16-bit P keeps its relative precision up to there (fp16 up
+// to 2^15 of its 65504, bf16 far beyond), and the sums are fp32.
 template <int D>
 struct Fwd {
   static constexpr int kStages = D == 64 ? 4 : 2;
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
       if (lane == 0) {
-        issue_scores<D>(tmem + (t & 1) * kCols, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
+        issue_scores<D, kCols>(tmem + (t & 1) * kCols, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
         mma_commit(&k_empty[st]);
         mma_commit(&s_full[t & 1]);
       }
@@ -482,12 +491,12 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       ok = wait_parity(&v_full[st], (t / ST) & 1, kSiteAttn + 5, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       const int j0 = (t0 + t) * kCols;
-      if (j0 + kCols > klen) zero_tail<D>(sV + st * C::kTile, klen - j0, lane);
+      if (j0 + kCols > klen) zero_tail<D, kCols>(sV + st * C::kTile, klen - j0, lane);
       ok = wait_parity(&p_ready[t & 1], (t >> 1) & 1, kSiteAttn + 6, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       if (lane == 0) {
-        issue_ts<true>(tmem_o, tmem + (t & 1) * kCols, smem_u32(sV + st * C::kTile), id_o, t > 0);
+        issue_ts<kCols>(tmem_o, tmem + (t & 1) * kCols, smem_u32(sV + st * C::kTile), id_o, t > 0);
         mma_commit(&v_empty[st]);
         mma_commit(pv_done);
         if (t + 1 == n) mma_commit(last);
@@ -505,6 +514,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     const int row_end = p.causal ? min(klen, i + p.q_offset + 1) : klen;  // keys this row sees
     const int warp_first = i0 + wq * 32 + p.q_offset;                      // the warp's first position
+    constexpr float kSumLimit = BF16 ? 1.0995116e12f : 32768.f;  // 2^40, 2^15
     float m_used = -kInf, l = 0.f;
     bool ok = true;
     // Few query rows (one token): a warp without any leaves its rows of P as they are; they only
@@ -517,12 +527,15 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
         if (lane == 0) mbar_arrive(&p_ready[t & 1]);
         continue;
       }
+      const uint32_t ts = tmem + lane_off + (t & 1) * kCols + half * 32;
       const int j0 = (t0 + t) * kCols + half * 32;
       // the tile's bias: one value, or a line over its 31 + 32 diagonals
-      const int d_lo = j0 - warp_first - 31, d_hi = j0 + 31 - warp_first;
-      const bool flat = bias.flat(d_lo, d_hi);
+      const int d_lo = j0 - warp_first - 31;
+      const bool flat = bias.flat(d_lo, d_lo + 31 + 31);
+      const int keep = row_end - j0;
+      const bool masked = __any_sync(0xffffffffu, keep < 32);
       float flat_c = 0.f;
-      if (flat) {
+      if (flat && !masked) {
         flat_c = bias.at(d_lo);
       } else {
         __syncwarp();  // the previous tile's reads are done
@@ -530,59 +543,79 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
         line[lane + 32] = bias.at(d_lo + lane + 32);
         __syncwarp();
       }
+      const float* ln = line + 31 - lane;
       ok = wait_parity(&s_full[t & 1], (t >> 1) & 1, kSiteAttn + 7, p.ctx);
       ok = __all_sync(0xffffffffu, ok);
-      const uint32_t ts = tmem + lane_off + (t & 1) * kCols + half * 32;
-      float z[32];
-      float m_tile = -kInf;
-      if (ok) {
-        tc_fence_after();
+      tc_fence_after();
+      uint32_t w[16];
+      float sum = 0.f;
+      // P of the tile against the maximum in use: 16-bit pairs in w, their sum before rounding in
+      // `sum`. One instance for each kind of tile, so that nothing is decided per element.
+      auto exponentiate = [&](auto is_flat, auto is_masked) {
+        const float m = m_used == -kInf ? 0.f : m_used;
+        const uint64_t sub = decltype(is_flat)::value ? f2_pack(flat_c - m, flat_c - m) : f2_pack(-m, -m);
+        uint64_t s2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
         uint32_t raw[32];
         tmem_ld32_nowait(ts, raw);
         tmem_wait_ld(raw);
-        if (flat) {
-          const uint64_t c2 = f2_pack(flat_c, flat_c);
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            f2_unpack(ffma2(f2_pack(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), scale2, c2), z[e], z[e + 1]);
-        } else {
-          const float* ln = line + 31 - lane;
-#pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            f2_unpack(ffma2(f2_pack(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), scale2,
-                            f2_pack(ln[e], ln[e + 1])),
-                      z[e], z[e + 1]);
+        for (int e = 0; e < 16; ++e) {
+          uint64_t add = sub;
+          if constexpr (!decltype(is_flat)::value) add = fadd2(f2_pack(ln[2 * e], ln[2 * e + 1]), sub);
+          float x, y;
+          f2_unpack(ffma2(f2_pack(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])), scale2, add), x, y);
+          if constexpr (decltype(is_masked)::value) {
+            x = 2 * e < keep ? x : -kInf;
+            y = 2 * e + 1 < keep ? y : -kInf;
+          }
+          x = exp2_approx(x);
+          y = exp2_approx(y);
+          s2[e & 1] = fadd2(s2[e & 1], f2_pack(x, y));
+          w[e] = pack16<BF16>(x, y);
         }
-        if (__any_sync(0xffffffffu, row_end < j0 + 32)) {
-          const int keep = row_end - j0;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) z[e] = e < keep ? z[e] : -kInf;
+        float x, y;
+        f2_unpack(fadd2(s2[0], s2[1]), x, y);
+        sum = x + y;
+      };
+      const std::true_type yes;
+      const std::false_type no;
+      bool settled = false;
+      for (bool first = t == 0;; first = false) {
+        if (!first) {
+          if (ok) {
+            if (masked)
+              exponentiate(no, yes);  // the line serves flat tiles too
+            else if (flat)
+              exponentiate(yes, no);
+            else
+              exponentiate(no, no);
+          }
+          if (settled || !named_bar_any(pair_bar, 64, !ok || m_used == -kInf || sum > kSumLimit)) break;
         }
-        float m4[4] = {z[0], z[1], z[2], z[3]};
-#pragma unroll
-        for (int e = 4; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], z[e]);
-        m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-      }
-      // The running maximum in use moves only when it is exceeded by more than 8 (a factor of 256
-      // in P, harmless in fp32 sums and in 16-bit P), so O is rarely rescaled.
-      if (named_bar_any(pair_bar, 64, !ok || m_tile > m_used + 8.f)) {
+        // The row's maximum anew, over both halves; everything before is rescaled to it, once the
+        // product of t - 1 has left O at rest.
+        if (t > 0 && ok) ok = wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 8, p.ctx);
         if (named_bar_any(pair_bar, 64, !ok)) {
           ok = false;
           break;
         }
+        tc_fence_after();
+        float m_tile = -kInf;
+        {
+          float z[32];
+          tmem_ld32(ts, z);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x = fmaf(z[e], p.scale * kLog2e, flat && !masked ? flat_c : ln[e]);
+            m_tile = fmaxf(m_tile, e < keep ? x : -kInf);
+          }
+        }
         row_x[half * kRows + r] = m_tile;
         named_bar_sync(pair_bar, 64);
         const float m_new = fmaxf(m_used, fmaxf(m_tile, row_x[(half ^ 1) * kRows + r]));
-        const float f = m_new == -kInf ? 1.f : exp2_approx(m_used - m_new);
-        l *= f;
-        m_used = m_new;
         if (t > 0) {
-          ok = wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 8, p.ctx);
-          if (named_bar_any(pair_bar, 64, !ok)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+          const float f = m_new == -kInf ? 1.f : exp2_approx(m_used - m_new);
+          l *= f;
 #pragma unroll 1
           for (int c = half; c < D / 32; c += 2) {
             float o[32];
@@ -592,18 +625,11 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
             tmem_st32f(tmem_o + lane_off + c * 32, o);
           }
         }
+        m_used = m_new;
+        settled = true;
       }
-      const float m_sub = m_used == -kInf ? 0.f : -m_used;
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t w[16];
-#pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        const float a = exp2_approx(z[e] + m_sub), c = exp2_approx(z[e + 1] + m_sub);
-        s4[e & 2] += a;
-        s4[(e & 2) + 1] += c;
-        w[e >> 1] = pack16<BF16>(a, c);
-      }
-      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      if (!ok) break;
+      l += sum;
       tmem_st16(ts, w);
       tmem_wait_st();
       tc_fence_before();
@@ -843,12 +869,12 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const bool ok = wait_parity(&full[st], (t / ST) & 1, kSiteAttnDq + 2, p.ctx);
       if (!__all_sync(0xffffffffu, ok)) return false;
       // rows past the sample's keys would enter dQ as 0 * anything
-      if (t * kCols + kCols > klen) zero_tail<D>(sK + st * C::kTile, klen - t * kCols, lane);
+      if (t * kCols + kCols > klen) zero_tail<D, kCols>(sK + st * C::kTile, klen - t * kCols, lane);
       tc_fence_after();
       if (lane == 0) {
         const uint32_t d = tmem + (t % NB) * 2 * kCols;
-        issue_scores<D>(d, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
-        issue_scores<D>(d + kCols, smem_u32(sO), smem_u32(sV + st * C::kTile), id_s);
+        issue_scores<D, kCols>(d, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
+        issue_scores<D, kCols>(d + kCols, smem_u32(sO), smem_u32(sV + st * C::kTile), id_s);
         mma_commit(&s_full[t % NB]);
       }
       __syncwarp();
@@ -870,7 +896,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tc_fence_after();
       const int st = t % ST;
       if (lane == 0) {
-        issue_ts<true>(tmem_acc, tmem + (t % NB) * 2 * kCols, smem_u32(sK + st * C::kTile), id_acc, t > 0);
+        issue_ts<kCols>(tmem_acc, tmem + (t % NB) * 2 * kCols, smem_u32(sK + st * C::kTile), id_acc, t > 0);
         mma_commit(&empty[st]);
         mma_commit(done);
         if (t + 1 == n) mma_commit(last);
@@ -1107,8 +1133,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tc_fence_after();
       if (lane == 0) {
         const uint32_t d = tmem + (t % NB) * 2 * kCols;
-        issue_scores<D>(d, smem_u32(sK), smem_u32(sQ + st * C::kTile), id_s);
-        issue_scores<D>(d + kCols, smem_u32(sV), smem_u32(sO + st * C::kTile), id_s);
+        issue_scores<D, kCols>(d, smem_u32(sK), smem_u32(sQ + st * C::kTile), id_s);
+        issue_scores<D, kCols>(d + kCols, smem_u32(sV), smem_u32(sO + st * C::kTile), id_s);
         mma_commit(&s_full[t % NB]);
       }
       __syncwarp();
@@ -1131,8 +1157,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const int st = t % ST;
       if (lane == 0) {
         const uint32_t d = tmem + (t % NB) * 2 * kCols;
-        issue_ts<true>(tmem_dv, d, smem_u32(sO + st * C::kTile), id_acc, t > 0);
-        issue_ts<true>(tmem_dk, d + kCols, smem_u32(sQ + st * C::kTile), id_acc, t > 0);
+        issue_ts<kCols>(tmem_dv, d, smem_u32(sO + st * C::kTile), id_acc, t > 0);
+        issue_ts<kCols>(tmem_dk, d + kCols, smem_u32(sQ + st * C::kTile), id_acc, t > 0);
         mma_commit(&empty[st]);
         mma_commit(done);
         if (t + 1 == n) mma_commit(last);
