@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         coords(i, m_blk, n_blk);
         const int n_row = n_blk * p.bn + (PAIR ? cta_rank * b_rows : 0);
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!wait_parity<PAIR>(&empty_bar[stage], phase ^ 1u, kSiteProducerEmpty, p.ctx)) {
+          if (!wait_parity<PAIR, true>(&empty_bar[stage], phase ^ 1u, kSiteProducerEmpty, p.ctx)) {
             ok = false;
             break;
           }
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // Drain: do not leave the CTA while TMA writes into its shared memory are pending.
       for (int i = 0; i < stages; ++i) {
-        if (!wait_parity<PAIR>(&empty_bar[stage], phase ^ 1u, kSiteDrain, p.ctx)) break;
+        if (!wait_parity<PAIR, true>(&empty_bar[stage], phase ^ 1u, kSiteDrain, p.ctx)) break;
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
@@ -330,12 +330,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int it = 0; it < my_count; ++it) {
         const int buf = it & 1;
         const uint32_t tphase = (it >> 1) & 1;
-        if (!wait_parity<PAIR>(&tempty_bar[buf], tphase ^ 1u, kSiteMmaTmemEmpty, p.ctx)) break;
+        if (!wait_parity<PAIR, true>(&tempty_bar[buf], tphase ^ 1u, kSiteMmaTmemEmpty, p.ctx)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * 256;
         bool ok = true;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!wait_parity<PAIR>(&full_bar[stage], phase, kSiteMmaFull, p.ctx)) {
+          if (!wait_parity<PAIR, true>(&full_bar[stage], phase, kSiteMmaFull, p.ctx)) {
             ok = false;
             break;
           }
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int buf = it & 1;
       const uint32_t tphase = (it >> 1) & 1;
       const int row = m_blk * BM + r;
-      const bool ok = wait_parity<PAIR>(&tfull_bar[buf], tphase, kSiteEpiTmemFull, p.ctx);
+      const bool ok = wait_parity<PAIR, true>(&tfull_bar[buf], tphase, kSiteEpiTmemFull, p.ctx);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + lane_off + buf * 256;

@@ -20,7 +20,7 @@
 // of size Lq x Lk leaves the SM.
 //
 //   attn_fwd_kernel  CTA = 128 query rows of one head; key tiles of 64; warp 0 loads, warp 1
-//                    issues MMAs, warps 2-9 softmax (half a row per thread). With few
+//                    issues MMAs, warps 2-5 softmax (one row per thread). With few
 //                    CTAs the keys are split over several, whose parts attn_combine_kernel joins.
 //   attn_dq_kernel   same rows; computes delta, dQ and the table's partial sums. No atomics.
 //   attn_dkv_kernel  CTA = 128 keys; runs over query tiles of 64 with the scores transposed, so
@@ -295,11 +295,9 @@ __host__ __device__ constexpr int align_up(int x, int a) { return (x + a - 1) / 
 // ---------------------------------------------------------------------------
 // Forward
 // ---------------------------------------------------------------------------
-// Ten warps, two CTAs per SM. Warps 2-9 are the softmax: warp w reads TMEM lanes [32 (w % 4), + 32),
-// warps 2-5 columns 0-31 of a score tile, warps 6-9 columns 32-63; the two warps of a row share
-// the maximum in use. Two score buffers: the scores of t + 1 are computed while those of t are
-// exponentiated, so the softmax never waits for a product. (One buffer of 128 columns, with the
-// two CTAs left to alternate, measured 5% slower: they fall into step and wait together.)
+// Six warps, two CTAs per SM. Warps 2-5 are the softmax, one row per thread: warp w reads TMEM lanes
+// [32 (w % 4), + 32). Two score buffers: the scores of t + 1 are computed while those of t are
+// exponentiated, so the softmax never waits for a product.
 //
 // The maximum in use is that of the row's first tile. Later tiles are exponentiated against it
 // without looking for theirs; only when a tile's sum passes kSumLimit is the maximum taken anew,
@@ -308,13 +306,12 @@ __host__ __device__ constexpr int align_up(int x, int a) { return (x + a - 1) / 
 template <int D>
 struct Fwd {
   static constexpr int kStages = D == 64 ? 4 : 2;
-  static constexpr int kThreads = 320;
+  static constexpr int kThreads = 192;
   static constexpr uint32_t kQ = kRows * D * 2;
   static constexpr uint32_t kTile = kCols * D * 2;
   static constexpr uint32_t kTmem = 256;  // two score buffers of 64 columns, O at 128
-  static constexpr int kLine = 64;        // per-warp bias line (31 + 32 diagonals)
-  static constexpr int kFloats = 8 * kLine + 2 * kRows;  // lines, the halves' row values
-  static int smem(const RelBuckets& rb) { return 1024 + kQ + kStages * 2 * kTile + 256 + kFloats * 4 + bias_smem(rb); }
+  static constexpr int kLine = 96;        // per-warp bias line (31 + 64 diagonals)
+  static int smem(const RelBuckets& rb) { return 1024 + kQ + kStages * 2 * kTile + 256 + 4 * kLine * 4 + bias_smem(rb); }
 };
 
 // Linear block index -> (query tile, split, head, sample). Under a causal mask the last query rows
@@ -368,7 +365,6 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
   uint64_t* last = pv_done + 1;  // every product is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
   float* lines = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
-  float* row_x = lines + 8 * C::kLine;  // [2][kRows]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_tiles = (p.Lq + kRows - 1) / kRows;
@@ -411,7 +407,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 8);
+      mbar_init(&p_ready[i], 4);
     }
     mbar_init(pv_done, 1);
     mbar_init(last, 1);
@@ -432,7 +428,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
-  const BiasLine bias = load_bias(p, h, lines + C::kFloats, C::kThreads);
+  const BiasLine bias = load_bias(p, h, lines + 4 * C::kLine, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -505,12 +501,9 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     }
   } else {
     const int wq = warp & 3;
-    const int half = (warp - 2) >> 2;
-    const uint32_t pair_bar = 1 + wq;  // the two warps that share these rows
-    const int r = wq * 32 + lane;
-    const int i = i0 + r;
+    const int i = i0 + wq * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
-    float* line = lines + (warp - 2) * C::kLine;
+    float* line = lines + wq * C::kLine;
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     const int row_end = p.causal ? min(klen, i + p.q_offset + 1) : klen;  // keys this row sees
     const int warp_first = i0 + wq * 32 + p.q_offset;                      // the warp's first position
@@ -521,33 +514,31 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     // reach its own rows of O, which are not stored.
     const bool idle = i0 + wq * 32 >= p.Lq;
     for (int t = 0; t < n; ++t) {
-      if (idle) {
-        ok = wait_parity(&s_full[t & 1], (t >> 1) & 1, kSiteAttn + 7, p.ctx);
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        if (lane == 0) mbar_arrive(&p_ready[t & 1]);
-        continue;
-      }
-      const uint32_t ts = tmem + lane_off + (t & 1) * kCols + half * 32;
-      const int j0 = (t0 + t) * kCols + half * 32;
-      // the tile's bias: one value, or a line over its 31 + 32 diagonals
+      const int j0 = (t0 + t) * kCols;
+      const uint32_t ts = tmem + lane_off + (t & 1) * kCols;
+      // the tile's bias: one value, or a line over its 31 + 64 diagonals
       const int d_lo = j0 - warp_first - 31;
-      const bool flat = bias.flat(d_lo, d_lo + 31 + 31);
+      const bool flat = bias.flat(d_lo, d_lo + 31 + 63);
       const int keep = row_end - j0;
-      const bool masked = __any_sync(0xffffffffu, keep < 32);
+      const bool masked = __any_sync(0xffffffffu, keep < kCols);
       float flat_c = 0.f;
       if (flat && !masked) {
         flat_c = bias.at(d_lo);
-      } else {
+      } else if (!idle) {
         __syncwarp();  // the previous tile's reads are done
-        line[lane] = bias.at(d_lo + lane);
-        line[lane + 32] = bias.at(d_lo + lane + 32);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) line[lane + 32 * q] = bias.at(d_lo + lane + 32 * q);
         __syncwarp();
       }
       const float* ln = line + 31 - lane;
       ok = wait_parity(&s_full[t & 1], (t >> 1) & 1, kSiteAttn + 7, p.ctx);
-      ok = __all_sync(0xffffffffu, ok);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      if (idle) {
+        if (lane == 0) mbar_arrive(&p_ready[t & 1]);
+        continue;
+      }
       tc_fence_after();
-      uint32_t w[16];
+      uint32_t w[32];
       float sum = 0.f;
       // P of the tile against the maximum in use: 16-bit pairs in w, their sum before rounding in
       // `sum`. One instance for each kind of tile, so that nothing is decided per element.
@@ -555,23 +546,31 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
         const float m = m_used == -kInf ? 0.f : m_used;
         const uint64_t sub = decltype(is_flat)::value ? f2_pack(flat_c - m, flat_c - m) : f2_pack(-m, -m);
         uint64_t s2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-        uint32_t raw[32];
-        tmem_ld32_nowait(ts, raw);
-        tmem_wait_ld(raw);
+        uint32_t raw[2][32];
+        tmem_ld32_nowait(ts, raw[0]);
+        tmem_ld32_nowait(ts + 32, raw[1]);
+        tmem_wait_ld(raw[0]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          uint64_t add = sub;
-          if constexpr (!decltype(is_flat)::value) add = fadd2(f2_pack(ln[2 * e], ln[2 * e + 1]), sub);
-          float x, y;
-          f2_unpack(ffma2(f2_pack(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])), scale2, add), x, y);
-          if constexpr (decltype(is_masked)::value) {
-            x = 2 * e < keep ? x : -kInf;
-            y = 2 * e + 1 < keep ? y : -kInf;
+        for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(raw[1][e]));
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            uint64_t add = sub;
+            if constexpr (!decltype(is_flat)::value)
+              add = fadd2(f2_pack(ln[c * 32 + 2 * e], ln[c * 32 + 2 * e + 1]), sub);
+            float x, y;
+            f2_unpack(ffma2(f2_pack(__uint_as_float(raw[c][2 * e]), __uint_as_float(raw[c][2 * e + 1])), scale2, add),
+                      x, y);
+            if constexpr (decltype(is_masked)::value) {
+              x = c * 32 + 2 * e < keep ? x : -kInf;
+              y = c * 32 + 2 * e + 1 < keep ? y : -kInf;
+            }
+            x = exp2_approx(x);
+            y = exp2_approx(y);
+            s2[e & 1] = fadd2(s2[e & 1], f2_pack(x, y));
+            w[c * 16 + e] = pack16<BF16>(x, y);
           }
-          x = exp2_approx(x);
-          y = exp2_approx(y);
-          s2[e & 1] = fadd2(s2[e & 1], f2_pack(x, y));
-          w[e] = pack16<BF16>(x, y);
         }
         float x, y;
         f2_unpack(fadd2(s2[0], s2[1]), x, y);
@@ -582,42 +581,36 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       bool settled = false;
       for (bool first = t == 0;; first = false) {
         if (!first) {
-          if (ok) {
-            if (masked)
-              exponentiate(no, yes);  // the line serves flat tiles too
-            else if (flat)
-              exponentiate(yes, no);
-            else
-              exponentiate(no, no);
-          }
-          if (settled || !named_bar_any(pair_bar, 64, !ok || m_used == -kInf || sum > kSumLimit)) break;
+          if (masked)
+            exponentiate(no, yes);  // the line serves flat tiles too
+          else if (flat)
+            exponentiate(yes, no);
+          else
+            exponentiate(no, no);
+          if (settled || !__any_sync(0xffffffffu, m_used == -kInf || sum > kSumLimit)) break;
         }
-        // The row's maximum anew, over both halves; everything before is rescaled to it, once the
-        // product of t - 1 has left O at rest.
-        if (t > 0 && ok) ok = wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 8, p.ctx);
-        if (named_bar_any(pair_bar, 64, !ok)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+        // The row's maximum anew; everything before is rescaled to it, once the product of t - 1
+        // has left O at rest.
         float m_tile = -kInf;
-        {
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
           float z[32];
-          tmem_ld32(ts, z);
+          tmem_ld32(ts + c * 32, z);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float x = fmaf(z[e], p.scale * kLog2e, flat && !masked ? flat_c : ln[e]);
-            m_tile = fmaxf(m_tile, e < keep ? x : -kInf);
+            const float x = fmaf(z[e], p.scale * kLog2e, flat && !masked ? flat_c : ln[c * 32 + e]);
+            m_tile = fmaxf(m_tile, c * 32 + e < keep ? x : -kInf);
           }
         }
-        row_x[half * kRows + r] = m_tile;
-        named_bar_sync(pair_bar, 64);
-        const float m_new = fmaxf(m_used, fmaxf(m_tile, row_x[(half ^ 1) * kRows + r]));
+        const float m_new = fmaxf(m_used, m_tile);
         if (t > 0) {
+          ok = wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 8, p.ctx);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          tc_fence_after();
           const float f = m_new == -kInf ? 1.f : exp2_approx(m_used - m_new);
           l *= f;
 #pragma unroll 1
-          for (int c = half; c < D / 32; c += 2) {
+          for (int c = 0; c < D / 32; ++c) {
             float o[32];
             tmem_ld32(tmem_o + lane_off + c * 32, o);
 #pragma unroll
@@ -631,25 +624,24 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       if (!ok) break;
       l += sum;
       tmem_st16(ts, w);
+      tmem_st16(ts + 32, w + 16);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[t & 1]);
     }
-    // the row's sum over both halves (an idle pair's rows are not stored)
-    row_x[half * kRows + r] = l;
-    bool done = ok;
-    if (ok && n > 0) done = wait_parity(last, 0, kSiteAttn + 9, p.ctx);
-    ok = !named_bar_any(pair_bar, 64, !done);
-    tc_fence_after();
-    l += row_x[(half ^ 1) * kRows + r];
+    if (ok && n > 0) {
+      ok = wait_parity(last, 0, kSiteAttn + 9, p.ctx);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
     const bool any = l > 0.f || l != l;
     const float inv = any ? 1.f / l : 0.f;
     const float lse = any ? m_used + log2f(l) : -kInf;
     const long long hrow = (static_cast<long long>(b) * p.H + h) * p.Lq + i;
     const long long slot = static_cast<long long>(split) * p.B * p.H * p.Lq + hrow;
     uint16_t* dst = static_cast<uint16_t*>(p.out) + ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D;
-    if (i < p.Lq && half == 0) {
+    if (i < p.Lq) {
       if (p.splits > 1) {
         p.part_lse[slot] = lse;
       } else if (p.lse != nullptr) {
@@ -657,7 +649,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       }
     }
 #pragma unroll 1
-    for (int c = half; c < D / 32; c += 2) {
+    for (int c = 0; c < D / 32; ++c) {
       float o[32];
       if (n > 0 && ok) {
         tmem_ld32(tmem_o + lane_off + c * 32, o);
