@@ -112,6 +112,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int x, int h, int l, int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(src)), "r"(x), "r"(h), "r"(l), "r"(b)
+      : "memory");
+}
+
 // D[tmem] (+)= A[tmem, 16-bit, two K elements per column] * B[smem]
 __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                        uint32_t accumulate) {
@@ -240,19 +248,19 @@ constexpr int kReach = 1024;
 struct BiasLine {
   const int* bounds;
   const float* col;    // [buckets] table column * log2 e
-  const float* value;  // [2 reach + 1], nullptr: search
+  const float* value;  // [2 reach + 1] unless searched
   int n_bounds, bidirectional, reach;
+  bool searched;
 
   __device__ __forceinline__ int bucket(int d) const { return rel_bucket(bounds, n_bounds, bidirectional, d); }
   __device__ __forceinline__ float at(int d) const {
-    if (value == nullptr) return col[bucket(d)];
+    if (searched) return col[bucket(d)];
     return value[min(max(d, -reach), reach) + reach];
   }
-  // Whether d_lo .. d_hi share one bucket for certain (past the last bound on either side, or
-  // ahead of the query in one direction).
-  __device__ __forceinline__ bool flat(int d_lo, int d_hi) const {
-    return d_hi <= -reach || d_lo >= (bidirectional ? reach : 0);
-  }
+  // One bucket for certain: d <= -reach, or d >= ahead() (past the last bound, or ahead of the
+  // query in one direction).
+  __device__ __forceinline__ int ahead() const { return bidirectional ? reach : 0; }
+  __device__ __forceinline__ bool flat(int d_lo, int d_hi) const { return d_hi <= -reach || d_lo >= ahead(); }
 };
 
 __host__ __device__ inline int bias_reach(const RelBuckets& rb) { return rb.bounds[rb.n_bounds - 1]; }
@@ -274,10 +282,11 @@ __device__ __forceinline__ BiasLine load_bias(const AttnArgs& p, int h, void* me
   l.n_bounds = p.rb.n_bounds;
   l.bidirectional = p.rb.bidirectional;
   l.reach = bias_reach(p.rb);
-  l.value = l.reach <= kReach ? col + buckets : nullptr;
+  l.value = col + buckets;
+  l.searched = l.reach > kReach;
   for (int t = threadIdx.x; t < p.rb.n_bounds; t += threads) bounds[t] = p.rb.bounds[t];
   for (int t = threadIdx.x; t < buckets; t += threads) col[t] = table_value(p, t, h) * kLog2e;
-  if (l.value != nullptr) {
+  if (!l.searched) {
     __syncthreads();
     for (int t = threadIdx.x; t < 2 * l.reach + 1; t += threads) col[buckets + t] = col[l.bucket(t - l.reach)];
   }
@@ -344,7 +353,8 @@ __device__ __forceinline__ FwdPlace fwd_place(const AttnArgs& p, int q_tiles) {
 template <int D, bool BF16>
 __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs p) {
+                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmOut,
+                    const __grid_constant__ AttnArgs p) {
   using C = Fwd<D>;
   constexpr int ST = C::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -513,19 +523,23 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     // Few query rows (one token): a warp without any leaves its rows of P as they are; they only
     // reach its own rows of O, which are not stored.
     const bool idle = i0 + wq * 32 >= p.Lq;
+    // The warp's tiles by kind: bias of the last bucket on the left before t_left and on the right
+    // from t_right on, some rows' keys ending inside from t_mask on (row_end rises with the lane).
+    const int first_key = t0 * kCols;
+    const int t_left = (warp_first - bias.reach - (kCols - 1) - first_key + kCols) / kCols;
+    const int t_right = (warp_first + 31 + bias.ahead() - first_key + kCols - 1) / kCols;
+    const int t_mask = (__shfl_sync(0xffffffffu, row_end, 0) - first_key) / kCols;
+    const float c_left = bias.at(-bias.reach), c_right = bias.at(bias.reach);
     for (int t = 0; t < n; ++t) {
       const int j0 = (t0 + t) * kCols;
       const uint32_t ts = tmem + lane_off + (t & 1) * kCols;
-      // the tile's bias: one value, or a line over its 31 + 64 diagonals
-      const int d_lo = j0 - warp_first - 31;
-      const bool flat = bias.flat(d_lo, d_lo + 31 + 63);
+      const bool masked = t >= t_mask;
+      const bool flat = !masked && (t < t_left || t >= t_right);
+      const float flat_c = t < t_left ? c_left : c_right;
       const int keep = row_end - j0;
-      const bool masked = __any_sync(0xffffffffu, keep < kCols);
-      float flat_c = 0.f;
-      if (flat && !masked) {
-        flat_c = bias.at(d_lo);
-      } else if (!idle) {
-        __syncwarp();  // the previous tile's reads are done
+      if (!flat && !idle) {
+        const int d_lo = j0 - warp_first - 31;  // a line over the tile's 31 + 64 diagonals
+        __syncwarp();                           // the previous tile's reads are done
 #pragma unroll
         for (int q = 0; q < 3; ++q) line[lane + 32 * q] = bias.at(d_lo + lane + 32 * q);
         __syncwarp();
@@ -598,7 +612,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
           tmem_ld32(ts + c * 32, z);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float x = fmaf(z[e], p.scale * kLog2e, flat && !masked ? flat_c : ln[c * 32 + e]);
+            const float x = fmaf(z[e], p.scale * kLog2e, flat ? flat_c : ln[c * 32 + e]);
             m_tile = fmaxf(m_tile, c * 32 + e < keep ? x : -kInf);
           }
         }
@@ -640,7 +654,6 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     const float lse = any ? m_used + log2f(l) : -kInf;
     const long long hrow = (static_cast<long long>(b) * p.H + h) * p.Lq + i;
     const long long slot = static_cast<long long>(split) * p.B * p.H * p.Lq + hrow;
-    uint16_t* dst = static_cast<uint16_t*>(p.out) + ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D;
     if (i < p.Lq) {
       if (p.splits > 1) {
         p.part_lse[slot] = lse;
@@ -648,6 +661,9 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
         p.lse[hrow] = lse;
       }
     }
+    // The rows go out through the query tile's shared memory (every product that reads it is
+    // done), 32 rows x 128 bytes a TMA store and warp: rows past Lq are left out by the map.
+    uint8_t* stage = sQ + wq * 32 * 128;
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       float o[32];
@@ -657,21 +673,36 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = 0.f;
       }
-      if (i >= p.Lq) continue;
       // a row without keys is 0 whatever its accumulator holds
 #pragma unroll
       for (int e = 0; e < 32; ++e) o[e] = any ? o[e] * inv : 0.f;
       if (p.splits > 1) {
+        if (i >= p.Lq) continue;
         float4* po = reinterpret_cast<float4*>(p.part_o + slot * D + c * 32);
 #pragma unroll
         for (int q = 0; q < 8; ++q) po[q] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          st_global_v4(dst + c * 32 + q * 8, pack16<BF16>(o[8 * q], o[8 * q + 1]),
-                       pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
-                       pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
+        continue;
       }
+      const uint32_t row = smem_u32(stage + (c >> 1) * 16384) + lane * 128;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        st_shared_v4(row + ((((c & 1) * 4 + q) ^ (lane & 7)) << 4), pack16<BF16>(o[8 * q], o[8 * q + 1]),
+                     pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
+                     pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
+    }
+    if (p.splits == 1) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (i0 + wq * 32 < p.Lq) {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_store_4d(&tmOut, stage + c * 16384, c * 64, h, i0 + wq * 32, b);
+        }
+        bulk_commit();
+        bulk_wait_all<0>();
+      }
+      __syncwarp();
     }
   }
   tc_fence_before();
@@ -1341,14 +1372,15 @@ int set_smem(K kernel, int bytes, int (&done)[64]) {
 }
 
 template <int D, bool BF16>
-int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& p, cudaStream_t st) {
+int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, const AttnArgs& p,
+            cudaStream_t st) {
   static int done[64] = {};
   const int smem = Fwd<D>::smem(p.rb);
   int rc = set_smem(attn_fwd_kernel<D, BF16>, smem, done);
   if (rc) return rc;
   const long long grid = static_cast<long long>((p.Lq + kRows - 1) / kRows) * p.splits * p.H * p.B;
   if (grid > 0x7fffffffll) return WDIT_ERR_SHAPE;
-  attn_fwd_kernel<D, BF16><<<static_cast<unsigned>(grid), Fwd<D>::kThreads, smem, st>>>(q, k, v, p);
+  attn_fwd_kernel<D, BF16><<<static_cast<unsigned>(grid), Fwd<D>::kThreads, smem, st>>>(q, k, v, o, p);
   rc = cuda_rc(cudaGetLastError());
   if (rc || p.splits == 1) return rc;
   const long long rows = static_cast<long long>(p.B) * p.H * p.Lq;
@@ -1431,15 +1463,16 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
   if ((rc = error_record_ptr(&p.ctx.rec))) return rc;
   p.ctx.limit_ns = wait_limit_ns();
   const bool bf16 = dtype == 1;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   if ((rc = map_heads(&mq, bf16, q, B, Lq, H, D, {q_strides[0], q_strides[1], q_strides[2]}, kRows)) ||
       (rc = map_heads(&mk, bf16, k, B, Lk, H, D, {k_strides[0], k_strides[1], k_strides[2]}, kCols)) ||
-      (rc = map_heads(&mv, bf16, v, B, Lk, H, D, {v_strides[0], v_strides[1], v_strides[2]}, kCols)))
+      (rc = map_heads(&mv, bf16, v, B, Lk, H, D, {v_strides[0], v_strides[1], v_strides[2]}, kCols)) ||
+      (rc = map_heads(&mo, bf16, out, B, Lq, H, D, {1ll * Lq * H * D, 1ll * H * D, D}, 32)))
     return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (D == 64)
-    return bf16 ? run_fwd<64, true>(mq, mk, mv, p, st) : run_fwd<64, false>(mq, mk, mv, p, st);
-  return bf16 ? run_fwd<128, true>(mq, mk, mv, p, st) : run_fwd<128, false>(mq, mk, mv, p, st);
+    return bf16 ? run_fwd<64, true>(mq, mk, mv, mo, p, st) : run_fwd<64, false>(mq, mk, mv, mo, p, st);
+  return bf16 ? run_fwd<128, true>(mq, mk, mv, mo, p, st) : run_fwd<128, false>(mq, mk, mv, mo, p, st);
 }
 
 long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional) {

@@ -53,12 +53,13 @@ __device__ __forceinline__ void add_buckets(float* acc, int bucket, float v, int
 
 __host__ __device__ inline int rel_num_buckets(int n_bounds, int bidirectional) { return (n_bounds + 1) * (bidirectional ? 2 : 1); }
 
-// Host check and copy of the caller's bounds; false = not ascending positive distances.
+// Host check and copy of the caller's bounds; false = not ascending distances in 1 .. 2^29 (positions
+// go up to 2^30: their sums stay inside 32 bits).
 inline bool rel_fill(RelBuckets* rb, const int* bounds, int n_bounds, int bidirectional) {
   rb->n_bounds = n_bounds;
   rb->bidirectional = bidirectional != 0 ? 1 : 0;
   for (int i = 0; i < n_bounds; ++i) {
-    if (bounds[i] < 1 || (i > 0 && bounds[i] < bounds[i - 1])) return false;
+    if (bounds[i] < 1 || bounds[i] > (1 << 29) || (i > 0 && bounds[i] < bounds[i - 1])) return false;
     rb->bounds[i] = bounds[i];
   }
   return true;

@@ -90,8 +90,8 @@ def rel_pos_bounds(num_buckets: int, max_distance: int, bidirectional: bool) -> 
     if not 2 <= nb <= MAX_BUCKETS:
         raise ValueError(f"2 to {MAX_BUCKETS} buckets a direction, got {nb}")
     exact = nb // 2
-    if not exact < max_distance <= 1 << 30:
-        raise ValueError(f"max_distance must be above {exact} (the exact distances) and at most 2^30, got {max_distance}")
+    if not exact < max_distance <= 1 << 29:
+        raise ValueError(f"max_distance must be above {exact} (the exact distances) and at most 2^29, got {max_distance}")
     T = nb - exact
     bounds = list(range(1, exact + 1))
     for t in range(1, T):

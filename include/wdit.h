@@ -312,7 +312,7 @@ int wdit_rope_table(const double* freqs_ri, int max_pos, int f, int h, int w, in
  *
  * Relative position buckets: relative position d = key - (query + q_offset); its distance n = |d|
  * (bidirectional != 0; keys ahead of the query, d > 0, take the upper half of the buckets) or
- * max(-d, 0). bounds is a HOST array of n_bounds (1 .. 255) ascending distances >= 1; the bucket
+ * max(-d, 0). bounds is a HOST array of n_bounds (1 .. 255) ascending distances in 1 .. 2^29; the bucket
  * of n is the number of bounds <= n. The table has n_bounds + 1 rows, twice that if bidirectional.
  */
 
