@@ -11,14 +11,19 @@
 // with dpre = dout * act'(pre) from act_backward_kernel (one pass, which also sums the columns
 // for the bias gradient).
 //
-// The product is a persistent warp-specialized tcgen05 kernel: warp 0 loads tiles by TMA into a
-// shared-memory ring (128-byte swizzle, 64-wide K blocks), warp 1 issues the MMAs into one of two
-// TMEM accumulators, warps 2-9 apply the epilogue of the other. Three tile forms (plan()):
+// The product is a persistent warp-specialized tcgen05 kernel: warps 0 and 10 load the tiles of A
+// and B by TMA into a shared-memory ring (128-byte swizzle, 64-wide K blocks), warp 1 issues the
+// MMAs into one of two TMEM accumulators, warps 2-9 apply the epilogue of the other: 32 x 32
+// pieces, the residual in and the result out by TMA through the warp's own shared memory. The two
+// loading threads matter: one TMA instruction with its barrier arithmetic takes a single thread
+// about 220 clocks whatever the box size (measured: 37, 74 and 125 bytes per clock and SM for
+// boxes of 8, 16 and 32 KB), so one thread that loads both operands falls behind the MMAs.
+// Tile forms (plan()):
 //   pair    256 x bn tiles over CTA pairs (tcgen05 cta_group::2): many rows
-//   single  128 x bn tiles, bn 64 .. 256: few tiles to spread over the SMs
-//   split   128 x bn tiles whose K range is divided over a cluster of CTAs; the partial sums are
-//           exchanged through distributed shared memory and added in rank order: few rows, where
-//           reading B once is the bound and one CTA per tile cannot keep enough loads in flight
+//   single  128 x bn tiles
+//   split   either of them with the K range divided over a cluster; the partial tiles are exchanged
+//           through distributed shared memory and added in rank order: few tiles, where reading B
+//           once or filling the SMs is the bound
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -37,14 +42,17 @@ namespace {
 
 constexpr int BM = 128;
 constexpr int BK = 64;
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;  // warp 0 loads A, 1 MMA, 2-9 epilogue, 10 loads B
 constexpr int kEpiThreads = 256;
 constexpr uint32_t kTileABytes = BM * BK * 2;
 constexpr uint32_t kTmemCols = 512;  // two accumulators of up to 256 columns
 constexpr int kMaxStages = 8;
+constexpr uint32_t kPieceBytes = 32 * 32 * 2;
+constexpr uint32_t kWarpBytes = 4 * kPieceBytes;   // three rotating pieces and one of pre-activations
+constexpr uint32_t kEpiBytes = 8 * (kWarpBytes + 32 * 4);  // ... and a line of 32 bias values
+constexpr uint32_t kBarBytes = 512;
 constexpr uint32_t kSmemLimit = 232448;
-constexpr uint32_t kBarBytes = 256;
-constexpr uint32_t kRingBudget = kSmemLimit - 1024 - kBarBytes;
+constexpr uint32_t kRingBudget = kSmemLimit - 1024 - kBarBytes - kEpiBytes;
 constexpr int kRasterRows = 8;
 constexpr long long kRasterBytes = 64ll << 20;
 
@@ -54,6 +62,7 @@ struct LinArgs {
   int M, N, K;
   int m_blocks, n_blocks, k_blocks, tiles, raster_rows;
   int bn, stages, splits;
+  int a_one, b_one;  // MN-major operand whose 64-wide pieces come in one box (M or N % 64 == 0)
   int is_bf16, act, bias_dtype;
   const void* bias;
   const void* res;
@@ -86,57 +95,119 @@ __device__ __forceinline__ uint32_t make_idesc(int m, int n, int is_bf16, bool t
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-// x / (1 + exp(-2 z)) = 0.5 x (1 + tanh z): no cancellation for negative x
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint64_t splat2(float v) { return f2_pack(v, v); }
+
+__device__ __forceinline__ uint64_t exp2_2(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return f2_pack(exp2_approx(a), exp2_approx(b));
+}
+
+__device__ __forceinline__ uint64_t rcp_2(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return f2_pack(rcp_approx(a), rcp_approx(b));
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+// tanh-GELU as x / (1 + exp(-2 z)), z = sqrt(2/pi) (x + 0.044715 x^3): no cancellation for x < 0
 constexpr float kGeluA = 2.f * 0.7978845608028654f;
 constexpr float kGeluB = 2.f * 0.7978845608028654f * 0.044715f;
 
-template <int N>
-__device__ __forceinline__ void apply_act(float (&v)[N], int act) {
+// Q(u) = 1 - Phi(u) for u >= 0 as exp(-u^2 / 2) R(t), t = 1 / (1 + 0.312 u): R is a polynomial of
+// degree 6 fitted to Q exp(u^2 / 2) with relative error below 2^-17.3 for every u (a least-squares
+// fit with weights driven to equal ripple; half a step of fp16 is 2^-11). e receives exp(-u^2 / 2).
+// u is |x| cut at 30, where Q is 0 in fp32, so that infinities make no 0 * inf.
+constexpr float kQc = 0.312f;
+__device__ __forceinline__ uint64_t gauss_tail2(uint64_t u, uint64_t& e) {
+  const uint64_t t = rcp_2(ffma2(u, splat2(kQc), splat2(1.f)));
+  uint64_t r = ffma2(t, splat2(-0.07296360501607355f), splat2(0.17343308598567092f));
+  r = ffma2(r, t, splat2(0.021109508863869385f));
+  r = ffma2(r, t, splat2(0.1324384307670562f));
+  r = ffma2(r, t, splat2(0.12126615653403806f));
+  r = ffma2(r, t, splat2(0.12472093351055727f));
+  r = ffma2(r, t, splat2(-7.4565507634441656e-06f));
+  e = exp2_2(fmul2(fmul2(u, u), splat2(-0.5f * kLog2e)));
+  return fmul2(e, r);
+}
+
+// Two columns at a time (packed fp32).
+__device__ __forceinline__ uint64_t act2(uint64_t x, int act) {
+  float a, b;
   switch (act) {
     case kRelu:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];
-      break;
+      f2_unpack(x, a, b);
+      return f2_pack(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b);  // NaN stays
     case kSilu:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = __fdividef(v[i], 1.f + __expf(-v[i]));
-      break;
-    case kGeluTanh:
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float z = v[i] * (kGeluA + kGeluB * v[i] * v[i]);
-        v[i] = __fdividef(v[i], 1.f + __expf(-z));
-      }
-      break;
-    case kGelu:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * erfcf(-0.70710678118654752f * v[i]);
-      break;
+      return fmul2(x, rcp_2(fadd2(exp2_2(fmul2(x, splat2(-kLog2e))), splat2(1.f))));
+    case kGeluTanh: {
+      const uint64_t z = fmul2(x, ffma2(fmul2(x, x), splat2(-kLog2e * kGeluB), splat2(-kLog2e * kGeluA)));
+      return fmul2(x, rcp_2(fadd2(exp2_2(z), splat2(1.f))));
+    }
+    case kGelu: {  // max(x, 0) - |x| Q(|x|)
+      f2_unpack(x, a, b);
+      const uint64_t u = f2_pack(fminf(fabsf(a), 30.f), fminf(fabsf(b), 30.f));
+      uint64_t e;
+      const uint64_t q = gauss_tail2(u, e);
+      return ffma2(fmul2(u, splat2(-1.f)), q, f2_pack(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b));
+    }
     default:
-      break;
+      return x;
   }
 }
 
-__device__ __forceinline__ float act_grad(float x, int act) {
-  // Past |x| = 20 every act' here is 0 or 1 to fp32; the clamp keeps x^2 finite (NaN passes).
-  if (fabsf(x) > 20.f) x = copysignf(20.f, x);
-  switch (act) {
-    case kRelu:
-      return x > 0.f ? 1.f : 0.f;
-    case kSilu: {
-      const float s = sigmoid(x);
-      return s * (1.f + x * (1.f - s));
-    }
-    case kGeluTanh: {
-      const float s = sigmoid(x * (kGeluA + kGeluB * x * x));
-      return s + x * s * (1.f - s) * (kGeluA + 3.f * kGeluB * x * x);
-    }
-    case kGelu:
-      return 0.5f * erfcf(-0.70710678118654752f * x) + x * 0.3989422804014327f * __expf(-0.5f * x * x);
-    default:
-      return 1.f;
+template <int N>
+__device__ __forceinline__ void apply_act(float (&v)[N], int act) {
+  if (act == kNone) return;
+  // one branch for the whole piece
+  auto all = [&](auto kind) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) f2_unpack(act2(f2_pack(v[i], v[i + 1]), decltype(kind)::value), v[i], v[i + 1]);
+  };
+  if (act == kRelu) {
+    all(std::integral_constant<int, kRelu>{});
+  } else if (act == kSilu) {
+    all(std::integral_constant<int, kSilu>{});
+  } else if (act == kGeluTanh) {
+    all(std::integral_constant<int, kGeluTanh>{});
+  } else {
+    all(std::integral_constant<int, kGelu>{});
+  }
+}
+
+// act'(x) of two columns. Past |x| = 20 each is 0 or 1 to fp32; the cut keeps x^2 finite (NaN passes).
+template <int ACT>
+__device__ __forceinline__ uint64_t act_grad2(float a, float b) {
+  if constexpr (ACT == kRelu) return f2_pack(a > 0.f ? 1.f : 0.f, b > 0.f ? 1.f : 0.f);
+  if (fabsf(a) > 20.f) a = copysignf(20.f, a);
+  if (fabsf(b) > 20.f) b = copysignf(20.f, b);
+  const uint64_t x = f2_pack(a, b);
+  if constexpr (ACT == kSilu) {  // s + x s (1 - s)
+    const uint64_t s = rcp_2(fadd2(exp2_2(fmul2(x, splat2(-kLog2e))), splat2(1.f)));
+    return ffma2(fmul2(x, s), ffma2(s, splat2(-1.f), splat2(1.f)), s);
+  } else if constexpr (ACT == kGeluTanh) {  // s + x s (1 - s) (2 z)'
+    const uint64_t xx = fmul2(x, x);
+    const uint64_t s =
+        rcp_2(fadd2(exp2_2(fmul2(x, ffma2(xx, splat2(-kLog2e * kGeluB), splat2(-kLog2e * kGeluA)))), splat2(1.f)));
+    const uint64_t dz = ffma2(xx, splat2(3.f * kGeluB), splat2(kGeluA));
+    return ffma2(fmul2(fmul2(x, dz), s), ffma2(s, splat2(-1.f), splat2(1.f)), s);
+  } else {  // Phi(x) + x phi(x)
+    uint64_t e;
+    float q0, q1;
+    f2_unpack(gauss_tail2(f2_pack(fabsf(a), fabsf(b)), e), q0, q1);
+    return ffma2(fmul2(x, splat2(0.3989422804014327f)), e, f2_pack(a < 0.f ? q0 : 1.f - q0, b < 0.f ? q1 : 1.f - q1));
   }
 }
 
@@ -192,30 +263,53 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
-enum Form { kSingle = 0, kPair = 1, kSplit = 2 };
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
 
-template <int FORM, bool TA, bool TB>
+// Completes on the pair leader's barrier (a shared::cluster address).
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// Operand maps are 3-D in either storage: K-major {K, rows, 1}, box {64, rows of the tile, 1};
+// MN-major {64, K, pieces of 64} with all of a tile's pieces in one box, or, when M or N is no
+// multiple of 64, {M or N, K, 1} with one box per piece.
+template <bool PAIR, bool SPLIT, bool TA, bool TB>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                  const __grid_constant__ LinArgs p) {
-  constexpr bool PAIR = FORM == kPair;
-  constexpr bool SPLIT = FORM == kSplit;
+                  const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmRes,
+                  const __grid_constant__ CUtensorMap tmPre, const __grid_constant__ LinArgs p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int b_rows = PAIR ? p.bn / 2 : p.bn;  // B rows this CTA stages
-  const uint32_t SB = kTileABytes + static_cast<uint32_t>(b_rows) * (BK * 2);
+  const uint32_t b_bytes = static_cast<uint32_t>(b_rows) * (BK * 2);
+  const uint32_t SB = kTileABytes + b_bytes;
   const int stages = p.stages;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + stages * SB);
+  uint8_t* epi = smem + stages * SB;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(epi + kEpiBytes);
   uint64_t* empty_bar = full_bar + kMaxStages;
   uint64_t* tfull_bar = empty_bar + kMaxStages;
   uint64_t* tempty_bar = tfull_bar + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  uint64_t* res_bar = tempty_bar + 2;  // 3 per epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_bar + 24);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int cta_rank = FORM != kSingle ? static_cast<int>(cluster_ctarank()) : 0;
-  const int group = PAIR ? 2 : (SPLIT ? p.splits : 1);  // CTAs that share a tile
+  const int rank = PAIR || SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+  const int cta_rank = PAIR ? rank & 1 : 0;
+  const int split = SPLIT ? (PAIR ? rank >> 1 : rank) : 0;
+  const int leader = rank & ~1;  // pair: the even CTA arms barriers and issues the MMAs
+  const int group = (PAIR ? 2 : 1) * (SPLIT ? p.splits : 1);  // CTAs that share a tile
   const int t_first = static_cast<int>(blockIdx.x) / group;
   const int t_step = static_cast<int>(gridDim.x) / group;
   const int my_count = t_first < p.tiles ? (p.tiles - 1 - t_first) / t_step + 1 : 0;
@@ -223,8 +317,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   int kb0 = 0, kb1 = p.k_blocks;
   if constexpr (SPLIT) {
     const int base = p.k_blocks / p.splits, rem = p.k_blocks % p.splits;
-    kb0 = cta_rank * base + min(cta_rank, rem);
-    kb1 = kb0 + base + (cta_rank < rem ? 1 : 0);
+    kb0 = split * base + min(split, rem);
+    kb1 = kb0 + base + (split < rem ? 1 : 0);
   }
   auto coords = [&](int i, int& m_blk, int& n_blk) {
     const int t = t_first + i * t_step;
@@ -241,13 +335,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&full_bar[i], 1);
+      mbar_init(&full_bar[i], 2);  // armed by the loaders of A and B
       mbar_init(&empty_bar[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull_bar[i], 1);
       mbar_init(&tempty_bar[i], PAIR ? 2 * (kEpiThreads / 32) : kEpiThreads / 32);
     }
+    for (int i = 0; i < 24; ++i) mbar_init(&res_bar[i], 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
@@ -262,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   tc_fence_before();
-  if constexpr (FORM != kSingle) {
+  if constexpr (PAIR || SPLIT) {
     cluster_sync_all();
   } else {
     __syncthreads();
@@ -270,41 +365,46 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 10) {
+    // Loaders: warp 0 the A tiles, warp 10 the B tiles of the same stages.
     if (lane == 0) {
+      const bool is_a = warp == 0;
+      const CUtensorMap* map = is_a ? &tmA : &tmB;
+      const bool mn = is_a ? TA : TB;
+      const uint32_t bytes = is_a ? kTileABytes : b_bytes;
+      const int pieces = (is_a ? BM : b_rows) / 64;
+      const bool one = (is_a ? p.a_one : p.b_one) != 0;
+      const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full_bar), leader) : smem_u32(full_bar);
+      uint8_t* const dst0 = smem + (is_a ? 0 : kTileABytes);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int i = 0; i < my_count && ok; ++i) {
         int m_blk, n_blk;
         coords(i, m_blk, n_blk);
-        const int n_row = n_blk * p.bn + (PAIR ? cta_rank * b_rows : 0);
+        const int row = is_a ? m_blk * BM : n_blk * p.bn + cta_rank * b_rows;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!wait_parity<PAIR, true>(&empty_bar[stage], phase ^ 1u, kSiteProducerEmpty, p.ctx)) {
+          if (!wait_parity<PAIR>(&empty_bar[stage], phase ^ 1u, kSiteProducerEmpty, p.ctx)) {
             ok = false;
             break;
           }
-          uint8_t* st = smem + stage * SB;
-          // Pair: both CTAs' loads complete on the leader's full barrier; only the leader arms it.
-          const uint32_t fb = PAIR ? mapa_shared(smem_u32(&full_bar[stage]), 0) : smem_u32(&full_bar[stage]);
-          if (!PAIR || cta_rank == 0) mbar_arrive_expect_tx(&full_bar[stage], PAIR ? 2 * SB : SB);
-          auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
+          uint8_t* dst = dst0 + stage * SB;
+          const uint32_t bar = full0 + stage * 8;
+          // Pair: both CTAs' loads complete on the leader's barrier; only the leader arms it.
+          if (!PAIR || cta_rank == 0) mbar_arrive_expect_tx(&full_bar[stage], PAIR ? 2 * bytes : bytes);
+          auto load = [&](uint8_t* to, int x, int y, int z) {
             if constexpr (PAIR) {
-              tma_load_2d_pair(dst, map, fb, x, y);
+              tma_load_3d_pair(to, map, bar, x, y, z);
             } else {
-              tma_load_2d(dst, map, &full_bar[stage], x, y);
+              tma_load_3d(to, map, bar, x, y, z);
             }
           };
-          if constexpr (TA) {
-#pragma unroll
-            for (int c = 0; c < BM / 64; ++c) load(st + c * 8192, &tmA, m_blk * BM + c * 64, kb * BK);
+          if (!mn) {
+            load(dst, kb * BK, row, 0);
+          } else if (one) {
+            load(dst, 0, kb * BK, row / 64);
           } else {
-            load(st, &tmA, kb * BK, m_blk * BM);
-          }
-          if constexpr (TB) {
-            for (int c = 0; c < b_rows / 64; ++c) load(st + kTileABytes + c * 8192, &tmB, n_row + c * 64, kb * BK);
-          } else {
-            load(st + kTileABytes, &tmB, kb * BK, n_row);
+            for (int c = 0; c < pieces; ++c) load(dst + c * 8192, row + c * 64, kb * BK, 0);
           }
           if (++stage == stages) {
             stage = 0;
@@ -314,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // Drain: do not leave the CTA while TMA writes into its shared memory are pending.
       for (int i = 0; i < stages; ++i) {
-        if (!wait_parity<PAIR, true>(&empty_bar[stage], phase ^ 1u, kSiteDrain, p.ctx)) break;
+        if (!wait_parity<PAIR>(&empty_bar[stage], phase ^ 1u, kSiteDrain, p.ctx)) break;
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
@@ -323,24 +423,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && (!PAIR || cta_rank == 0)) {
+    if (lane == 0 && cta_rank == 0) {
       const uint32_t idesc = make_idesc(PAIR ? 2 * BM : BM, p.bn, p.is_bf16, TA, TB);
+      const uint32_t ring = smem_u32(smem);
+      const uint32_t empty0 = smem_u32(empty_bar), peer0 = PAIR ? mapa_shared(empty0, rank | 1) : 0u;
       int stage = 0;
       uint32_t phase = 0;
       for (int it = 0; it < my_count; ++it) {
         const int buf = it & 1;
         const uint32_t tphase = (it >> 1) & 1;
-        if (!wait_parity<PAIR, true>(&tempty_bar[buf], tphase ^ 1u, kSiteMmaTmemEmpty, p.ctx)) break;
+        if (!wait_parity<PAIR>(&tempty_bar[buf], tphase ^ 1u, kSiteMmaTmemEmpty, p.ctx)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * 256;
         bool ok = true;
+        uint32_t acc = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!wait_parity<PAIR, true>(&full_bar[stage], phase, kSiteMmaFull, p.ctx)) {
+          if (!wait_parity<PAIR>(&full_bar[stage], phase, kSiteMmaFull, p.ctx)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(smem + stage * SB);
+          const uint32_t a_addr = ring + stage * SB;
           const uint64_t a_desc = TA ? smem_desc_mn(a_addr) : smem_desc_sw128(a_addr);
           const uint64_t b_desc = TB ? smem_desc_mn(a_addr + kTileABytes) : smem_desc_sw128(a_addr + kTileABytes);
 #pragma unroll
@@ -348,16 +451,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             // 16 K elements on: 32 bytes inside a K-major row, 16 rows of 128 bytes MN-major
             const uint64_t ad = a_desc + (TA ? 128 : 2) * k;
             const uint64_t bd = b_desc + (TB ? 128 : 2) * k;
-            const uint32_t acc = kb != kb0 || k != 0 ? 1u : 0u;
             if constexpr (PAIR) {
               mma_bf16_pair(d_tmem, ad, bd, idesc, acc);
             } else {
               mma_bf16(d_tmem, ad, bd, idesc, acc);
             }
+            acc = 1;
           }
           if constexpr (PAIR) {
-            mma_commit_pair(smem_u32(&empty_bar[stage]));
-            mma_commit_pair(mapa_shared(smem_u32(&empty_bar[stage]), 1));
+            mma_commit_pair(empty0 + stage * 8);
+            mma_commit_pair(peer0 + stage * 8);
           } else {
             mma_commit(&empty_bar[stage]);
           }
@@ -369,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         if constexpr (PAIR) {
           mma_commit_pair(smem_u32(&tfull_bar[buf]));
-          mma_commit_pair(mapa_shared(smem_u32(&tfull_bar[buf]), 1));
+          mma_commit_pair(mapa_shared(smem_u32(&tfull_bar[buf]), rank | 1));
         } else {
           mma_commit(&tfull_bar[buf]);
         }
@@ -379,23 +482,43 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // Epilogue: warp w reads TMEM lanes [32 (w % 4), + 32) (its thread owns one accumulator row);
     // warps 2-5 take the even 32-column pieces of the tile, warps 6-9 the odd ones.
+    const int ew = warp - 2;
     const int wq = warp & 3;
-    const int half = (warp - 2) >> 2;
+    const int half = ew >> 2;
     const int r = wq * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
-    for (int it = 0; it < my_count; ++it) {
+    const int pieces = p.bn / 32;
+    uint8_t* const bufs = epi + ew * kWarpBytes;
+    float* const bias_line = reinterpret_cast<float*>(epi + 8 * kWarpBytes) + ew * 32;
+    uint64_t* const rbar = res_bar + ew * 3;
+    uint32_t rphase = 0;  // phase of each residual buffer's barrier
+    int cur = 0;          // rotating piece buffer
+    const bool has_res = !SPLIT && p.res != nullptr;
+    auto piece_at = [&](int it, int c, int& row0, int& n0) {  // false: outside the matrix
       int m_blk, n_blk;
       coords(it, m_blk, n_blk);
+      row0 = m_blk * BM + wq * 32;
+      n0 = n_blk * p.bn + c * 32;
+      return row0 < p.M && n0 < p.N;
+    };
+    auto fetch_res = [&](int it, int c, int buf) {  // lane 0
+      int row0, n0;
+      if (!piece_at(it, c, row0, n0)) return;
+      mbar_arrive_expect_tx(&rbar[buf], kPieceBytes);
+      tma_load_2d(bufs + buf * kPieceBytes, &tmRes, &rbar[buf], n0, row0);
+    };
+    if (has_res && lane == 0 && my_count > 0) fetch_res(0, half, 0);
+    for (int it = 0; it < my_count; ++it) {
       const int buf = it & 1;
       const uint32_t tphase = (it >> 1) & 1;
-      const int row = m_blk * BM + r;
-      const bool ok = wait_parity<PAIR, true>(&tfull_bar[buf], tphase, kSiteEpiTmemFull, p.ctx);
+      bool ok = wait_parity<PAIR>(&tfull_bar[buf], tphase, kSiteEpiTmemFull, p.ctx);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + lane_off + buf * 256;
-      const int pieces = p.bn / 32;
+#pragma unroll 1
       for (int c = half; c < pieces; c += 2) {
-        const int n0 = n_blk * p.bn + c * 32;
+        int row0, n0;
+        const bool inside = piece_at(it, c, row0, n0);
         float v[32];
         tmem_ld32(tbase + c * 32, v);
         if (c + 2 >= pieces) {
@@ -403,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) {
             if constexpr (PAIR) {
-              mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[buf]), 0));
+              mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[buf]), leader));
             } else {
               mbar_arrive(&tempty_bar[buf]);
             }
@@ -411,38 +534,88 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if constexpr (SPLIT) {
           // this rank's partial tile, rows of bn + 4 floats, over the drained ring
-          if (row < p.M) {
+          if (row0 + lane < p.M) {
             float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(smem) + r * (p.bn + 4) + c * 32);
 #pragma unroll
             for (int q = 0; q < 8; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
           }
         } else {
-          if (n0 >= p.N) continue;
-          float bias = 0.f;
-          if (p.bias != nullptr) {
-            if (n0 + lane < p.N) bias = load_scalar(p.bias, n0 + lane, p.bias_dtype);
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] += __shfl_sync(0xffffffffu, bias, q);
-          }
-          if (row < p.M) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if (n0 + 8 * q >= p.N) break;
-              float o[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) o[i] = v[8 * q + i];
-              finish8(p, o, row, n0 + 8 * q);
+          const int next = cur == 2 ? 0 : cur + 1;
+          if (lane == 0) {
+            bulk_wait_read<1>();  // every store but the last has left its buffer
+            if (has_res) {
+              if (c + 2 < pieces) {
+                fetch_res(it, c + 2, next);
+              } else if (it + 1 < my_count) {
+                fetch_res(it + 1, half, next);
+              }
             }
           }
+          if (inside) {
+            if (p.bias != nullptr) {
+              const float bv = n0 + lane < p.N ? load_scalar(p.bias, n0 + lane, p.bias_dtype) : 0.f;
+              __syncwarp();
+              bias_line[lane] = bv;
+            }
+            __syncwarp();
+            if (p.bias != nullptr) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float4 b4 = reinterpret_cast<const float4*>(bias_line)[q];
+                v[4 * q] += b4.x;
+                v[4 * q + 1] += b4.y;
+                v[4 * q + 2] += b4.z;
+                v[4 * q + 3] += b4.w;
+              }
+            }
+            auto stage_out = [&](uint8_t* to, const CUtensorMap* map) {
+              const uint32_t row = smem_u32(to) + lane * 64;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                st_shared_v4(row + ((q ^ ((lane >> 1) & 3)) << 4), pack2(v[8 * q], v[8 * q + 1], p.is_bf16),
+                             pack2(v[8 * q + 2], v[8 * q + 3], p.is_bf16), pack2(v[8 * q + 4], v[8 * q + 5], p.is_bf16),
+                             pack2(v[8 * q + 6], v[8 * q + 7], p.is_bf16));
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(map, to, n0, row0);
+                bulk_commit();
+              }
+            };
+            if (p.pre != nullptr) stage_out(bufs + 3 * kPieceBytes, &tmPre);
+            apply_act<32>(v, p.act);
+            uint8_t* mine = bufs + cur * kPieceBytes;
+            if (has_res) {
+              ok = wait_parity(&rbar[cur], (rphase >> cur) & 1u, kSiteEpiCLoad, p.ctx);
+              if (!__all_sync(0xffffffffu, ok)) break;
+              rphase ^= 1u << cur;
+              const uint32_t row = smem_u32(mine) + lane * 64;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint4 w = ld_shared_u4(row + ((q ^ ((lane >> 1) & 3)) << 4));
+                const uint32_t rw[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = unpack2(rw[e], p.is_bf16);
+                  v[8 * q + 2 * e] += f.x;
+                  v[8 * q + 2 * e + 1] += f.y;
+                }
+              }
+            }
+            stage_out(mine, &tmOut);
+          }
+          cur = next;
         }
       }
     }
+    if (lane == 0) bulk_wait_all<0>();
+    __syncwarp();
   }
   if constexpr (SPLIT) {
-    // One tile per cluster. Rank c adds columns [c * bn / splits, + bn / splits) of all ranks'
-    // partial tiles, rank 0 first.
+    // One tile per cluster. Split c adds columns [c * bn / splits, + bn / splits) of all the splits'
+    // partial tiles (pair: of its own 128 rows), split 0 first.
     cluster_sync_all();
-    if (warp >= 2) {
+    if (warp >= 2 && warp < 10 && my_count > 0) {
       int m_blk, n_blk;
       coords(0, m_blk, n_blk);
       const int cols = p.bn / p.splits;
@@ -451,25 +624,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t mine = smem_u32(smem);
       for (int x = threadIdx.x - 64; x < rows * per_row; x += kEpiThreads) {
         const int rr = x / per_row;
-        const int c = cta_rank * cols + (x - rr * per_row) * 8;
+        const int c = split * cols + (x - rr * per_row) * 8;
         const int n = n_blk * p.bn + c;
         if (n >= p.N) continue;
+        float4 f[8][2];  // all ranks' loads are in flight together
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          f[s][0] = f[s][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (s < p.splits) {
+            const uint32_t a = mapa_shared(mine + (rr * (p.bn + 4) + c) * 4, PAIR ? 2 * s + cta_rank : s);
+            f[s][0] = ld_cluster_f4(a);
+            f[s][1] = ld_cluster_f4(a + 16);
+          }
+        }
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i] = p.bias != nullptr ? load_scalar(p.bias, n + i, p.bias_dtype) : 0.f;
-        for (int s = 0; s < p.splits; ++s) {
-          const uint32_t a = mapa_shared(mine + (rr * (p.bn + 4) + c) * 4, s);
-          const float4 f = ld_cluster_f4(a), g = ld_cluster_f4(a + 16);
-          v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-          v[4] += g.x; v[5] += g.y; v[6] += g.z; v[7] += g.w;
+        for (int i = 0; i < 8; ++i) v[i] = p.bias != nullptr ? load_scalar(p.bias, n + i, p.bias_dtype) : 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          v[0] += f[s][0].x; v[1] += f[s][0].y; v[2] += f[s][0].z; v[3] += f[s][0].w;
+          v[4] += f[s][1].x; v[5] += f[s][1].y; v[6] += f[s][1].z; v[7] += f[s][1].w;
         }
         finish8(p, v, m_blk * BM + rr, n);
       }
     }
   }
   tc_fence_before();
-  if constexpr (FORM != kSingle) {
+  if constexpr (PAIR || SPLIT) {
     cluster_sync_all();  // peers may still read this CTA's shared memory / signal its barriers
   } else {
     __syncthreads();
@@ -490,10 +671,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kBackRows = 64;  // rows of one block
 constexpr int kBackCols = 256;
 
-template <bool BF16>
+template <bool BF16, int ACT>
 __global__ void __launch_bounds__(256)
     act_backward_kernel(const uint16_t* __restrict__ dout, long long ldd, const uint16_t* __restrict__ pre,
-                        long long ldp, int act, uint16_t* __restrict__ dpre, long long ldq,
+                        long long ldp, uint16_t* __restrict__ dpre, long long ldq,
                         float* __restrict__ part, int M, int N) {
   __shared__ float sums[8][kBackCols];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -515,14 +696,13 @@ __global__ void __launch_bounds__(256)
         d[2 * i] = f.x;
         d[2 * i + 1] = f.y;
       }
-      if (act != kNone) {
+      if constexpr (ACT != kNone) {
         const uint4 x = __ldg(reinterpret_cast<const uint4*>(pre + m * ldp + n));
         const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 f = unpack2(xw[i], BF16);
-          d[2 * i] *= act_grad(f.x, act);
-          d[2 * i + 1] *= act_grad(f.y, act);
+          f2_unpack(fmul2(f2_pack(d[2 * i], d[2 * i + 1]), act_grad2<ACT>(f.x, f.y)), d[2 * i], d[2 * i + 1]);
         }
         st_global_v4(dpre + m * ldq + n, pack2(d[0], d[1], BF16), pack2(d[2], d[3], BF16), pack2(d[4], d[5], BF16),
                      pack2(d[6], d[7], BF16));
@@ -583,70 +763,79 @@ int sm_count() {
 }
 
 struct Plan {
-  int form, bn, splits;
+  int pair, bn, splits;
 };
 
-// Cost of one K block of a tile per CTA, in clocks: its MMAs (2 clocks per column of a 128-row
-// accumulator) or its loads from L2 (about 48 bytes per clock and SM).
-double block_cost(int load_rows, int bn_mma) {
-  const double mma = 2.0 * bn_mma, ld = load_rows * BK * 2 / 48.0;
-  return mma > ld ? mma : ld;
+// Clocks of one K block of a tile in a CTA: its MMAs (bn columns: 2 bn for 128 accumulator rows), its
+// loads from L2 (about 64 bytes a clock when all SMs load), or one turn of the issuing threads.
+double block_cost(int load_rows, int bn) {
+  double c = 2.0 * bn;
+  const double ld = load_rows * BK * 2 / 64.0;
+  if (ld > c) c = ld;
+  return c < 280 ? 280 : c;
 }
 
-Plan plan(int M, int N, int K, int sms) {
+Plan plan(int M, int N, int K, int mn_b, int sms) {
   const int kb = (K + BK - 1) / BK;
-  Plan best = {kSingle, 128, 1};
+  Plan best = {0, 128, 1};
   double best_cost = 1e30;
-  auto consider = [&](int form, int bn, int splits, long long tiles, long long slots, double per_block, double fixed) {
-    const long long waves = (tiles + slots - 1) / slots;
-    const double cost = static_cast<double>(waves) * ((kb + splits - 1) / splits * per_block + fixed) + 2000;
+  auto consider = [&](int pair, int bn, int s) {
+    const long long mb = (M + BM - 1) / BM, nb = (N + bn - 1) / bn;
+    const long long tiles = (pair ? (mb + 1) / 2 : mb) * nb;
+    const long long slots = sms / (pair ? 2 : 1);
+    // clusters of more than two need their SMs inside one GPC: count 7/8 of them
+    if (s > 1 && tiles * s > slots * 7 / 8) return;
+    const long long waves = s > 1 ? 1 : (tiles + slots - 1) / slots;
+    const int rows = M < BM ? M : BM;
+    // epilogue of the last tile; split: partial tiles written, exchanged, added
+    const double end = (s > 1 ? 2500 + rows * bn * (1.0 + 1.0 / s) / 24 : rows * bn / 16.0) + (pair ? 500 : 0);
+    const double cost = waves * ((kb + s - 1) / s) * block_cost(BM + (pair ? bn / 2 : bn), bn) + end;
     if (cost < best_cost) {
       best_cost = cost;
-      best = {form, bn, splits};
+      best = {pair, bn, s};
     }
   };
-  const long long mb = (M + BM - 1) / BM;
-  for (int bn = 256; bn >= 64; bn -= 64) {
-    const long long nb = (N + bn - 1) / bn;
-    if (M > BM && (bn == 256 || bn == 128))
-      consider(kPair, bn, 1, (mb + 1) / 2 * nb, sms / 2, block_cost(BM + bn / 2, bn), 500);
-    consider(kSingle, bn, 1, mb * nb, sms, block_cost(BM + bn, bn), 500);
-    if (bn <= 128)
-      for (int s = 2; s <= 8 && s <= kb; s *= 2)
-        // one tile per cluster; 8 CTAs of a cluster need a GPC with room, so count 7/8 of the SMs
-        if (mb * nb * s <= sms * 7 / 8) consider(kSplit, bn, s, mb * nb, mb * nb, block_cost(BM + bn, bn), 1500);
-  }
+  for (int bn = 256; bn >= 64; bn -= 64)
+    for (int s = 1; s <= 8 && s <= kb; s *= 2) {
+      consider(0, bn, s);
+      if (M > BM && bn != 64 && s <= 4 && (!mn_b || bn != 192)) consider(1, bn, s);
+    }
   return best;
 }
 
 int launch_error(cudaError_t e) { return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e); }
 
-template <int FORM, bool TA, bool TB>
-int launch(const CUtensorMap& a, const CUtensorMap& b, LinArgs p, cudaStream_t stream) {
+struct Maps {
+  CUtensorMap a, b, out, res, pre;
+};
+
+template <bool PAIR, bool SPLIT, bool TA, bool TB>
+int launch(const Maps& m, LinArgs p, cudaStream_t stream) {
   static bool attr_set[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return launch_error(e);
-  const int b_rows = FORM == kPair ? p.bn / 2 : p.bn;
+  const int b_rows = PAIR ? p.bn / 2 : p.bn;
   const uint32_t sb = kTileABytes + static_cast<uint32_t>(b_rows) * BK * 2;
   p.stages = static_cast<int>(kRingBudget / sb);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   if (!attr_set[dev & 63]) {
-    e = cudaFuncSetAttribute(linear_kernel<FORM, TA, TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+    e = cudaFuncSetAttribute(linear_kernel<PAIR, SPLIT, TA, TB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kSmemLimit);
     if (e != cudaSuccess) return launch_error(e);
     attr_set[dev & 63] = true;
   }
-  const int group = FORM == kPair ? 2 : (FORM == kSplit ? p.splits : 1);
-  p.tiles = (FORM == kPair ? (p.m_blocks + 1) / 2 : p.m_blocks) * p.n_blocks;
+  const int group = (PAIR ? 2 : 1) * (SPLIT ? p.splits : 1);
+  p.tiles = (PAIR ? (p.m_blocks + 1) / 2 : p.m_blocks) * p.n_blocks;
   long long grid = static_cast<long long>(p.tiles) * group;
-  if (FORM != kSplit) {
+  if (!SPLIT) {
     const long long slots = sm_count() / group * group;
     if (grid > slots) grid = slots;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = 1024 + p.stages * sb + kBarBytes;
+  cfg.dynamicSmemBytes = 1024 + p.stages * sb + kEpiBytes + kBarBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -654,24 +843,46 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, LinArgs p, cudaStream_t s
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = FORM != kSingle ? 1 : 0;
-  return launch_error(cudaLaunchKernelEx(&cfg, linear_kernel<FORM, TA, TB>, a, b, p));
+  cfg.numAttrs = group > 1 ? 1 : 0;
+  return launch_error(
+      cudaLaunchKernelEx(&cfg, linear_kernel<PAIR, SPLIT, TA, TB>, m.a, m.b, m.out, m.res, m.pre, p));
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// rows x cols matrix (cols contiguous, row stride ld elements), box of box_cols x box_rows
-int map_2d(CUtensorMap* m, int is_bf16, const void* ptr, int cols, int rows, long long ld, int box_cols, int box_rows) {
+CUtensorMapDataType map_type(int is_bf16) {
+  return is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// Operand map (see linear_kernel): `rows` along M or N of which a CTA's tile takes `tile`.
+int map_operand(CUtensorMap* m, int is_bf16, const void* ptr, int rows, int K, long long ld, int mn, int tile,
+                int* one) {
+  typedef unsigned long long u64;
+  *one = mn && rows % 64 == 0 ? 1 : 0;
+  const u64 row_bytes = static_cast<u64>(ld) * 2;
+  if (!mn) {
+    const u64 dims[3] = {static_cast<u64>(K), static_cast<u64>(rows), 1};
+    const u64 st[2] = {row_bytes, row_bytes};
+    const unsigned box[3] = {64, static_cast<unsigned>(tile), 1};
+    return encode_tiled(m, map_type(is_bf16), 3, ptr, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  const u64 dims[3] = {static_cast<u64>(*one ? 64 : rows), static_cast<u64>(K), static_cast<u64>(*one ? rows / 64 : 1)};
+  const u64 st[2] = {row_bytes, 128};
+  const unsigned box[3] = {64, BK, static_cast<unsigned>(*one ? tile / 64 : 1)};
+  return encode_tiled(m, map_type(is_bf16), 3, ptr, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// 32 x 32 pieces of a row-major matrix, for the epilogue
+int map_pieces(CUtensorMap* m, int is_bf16, const void* ptr, int cols, int rows, long long ld) {
   const unsigned long long dims[2] = {static_cast<unsigned long long>(cols), static_cast<unsigned long long>(rows)};
-  const unsigned long long strides[1] = {static_cast<unsigned long long>(ld) * 2};
-  const unsigned int box[2] = {static_cast<unsigned>(box_cols), static_cast<unsigned>(box_rows)};
-  return encode_tiled(m, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, ptr, dims,
-                      strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const unsigned long long st[1] = {static_cast<unsigned long long>(ld) * 2};
+  const unsigned box[2] = {32, 32};
+  return encode_tiled(m, map_type(is_bf16), 2, ptr, dims, st, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 int run_linear(const void* A, long long lda, int a_mn, const void* B, long long ldb, int b_mn, LinArgs p,
                cudaStream_t stream) {
-  const Plan pl = plan(p.M, p.N, p.K, sm_count());
+  const Plan pl = plan(p.M, p.N, p.K, b_mn, sm_count());
   p.bn = pl.bn;
   p.splits = pl.splits;
   p.m_blocks = (p.M + BM - 1) / BM;
@@ -681,21 +892,24 @@ int run_linear(const void* A, long long lda, int a_mn, const void* B, long long 
   int rc = error_record_ptr(&p.ctx.rec);
   if (rc) return rc;
   p.ctx.limit_ns = wait_limit_ns();
-  const int b_rows = pl.form == kPair ? p.bn / 2 : p.bn;
-  CUtensorMap ma, mb;
-  rc = a_mn ? map_2d(&ma, p.is_bf16, A, p.M, p.K, lda, 64, BK) : map_2d(&ma, p.is_bf16, A, p.K, p.M, lda, BK, BM);
-  if (rc) return rc;
-  rc = b_mn ? map_2d(&mb, p.is_bf16, B, p.N, p.K, ldb, 64, BK) : map_2d(&mb, p.is_bf16, B, p.K, p.N, ldb, BK, b_rows);
-  if (rc) return rc;
-  auto go = [&](auto form) {
-    constexpr int F = decltype(form)::value;
-    if (a_mn) return launch<F, true, true>(ma, mb, p, stream);
-    if (b_mn) return launch<F, false, true>(ma, mb, p, stream);
-    return launch<F, false, false>(ma, mb, p, stream);
+  Maps m;
+  memset(&m, 0, sizeof(m));
+  if ((rc = map_operand(&m.a, p.is_bf16, A, p.M, p.K, lda, a_mn, BM, &p.a_one)) ||
+      (rc = map_operand(&m.b, p.is_bf16, B, p.N, p.K, ldb, b_mn, pl.pair ? p.bn / 2 : p.bn, &p.b_one)))
+    return rc;
+  if (pl.splits == 1) {
+    if ((rc = map_pieces(&m.out, p.is_bf16, p.out, p.N, p.M, p.ldo))) return rc;
+    if (p.res != nullptr && (rc = map_pieces(&m.res, p.is_bf16, p.res, p.N, p.M, p.ldr))) return rc;
+    if (p.pre != nullptr && (rc = map_pieces(&m.pre, p.is_bf16, p.pre, p.N, p.M, p.ldp))) return rc;
+  }
+  auto go = [&](auto pair, auto split) {
+    constexpr bool P = decltype(pair)::value, S = decltype(split)::value;
+    if (a_mn) return launch<P, S, true, true>(m, p, stream);
+    if (b_mn) return launch<P, S, false, true>(m, p, stream);
+    return launch<P, S, false, false>(m, p, stream);
   };
-  if (pl.form == kPair) return go(std::integral_constant<int, kPair>{});
-  if (pl.form == kSplit) return go(std::integral_constant<int, kSplit>{});
-  return go(std::integral_constant<int, kSingle>{});
+  if (pl.pair) return pl.splits > 1 ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+  return pl.splits > 1 ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
 }
 
 int check_operand(const void* p, long long ld, long long cols) {
@@ -776,10 +990,20 @@ int wdit_act_backward(const void* dout, long long ldd, const void* pre, long lon
   const uint16_t* g = static_cast<const uint16_t*>(dout);
   const uint16_t* x = static_cast<const uint16_t*>(pre);
   uint16_t* d = static_cast<uint16_t*>(dpre);
-  if (dtype == 1)
-    act_backward_kernel<true><<<grid, 256, 0, st>>>(g, ldd, x, ldp, act, d, ldq, part, M, N);
-  else
-    act_backward_kernel<false><<<grid, 256, 0, st>>>(g, ldd, x, ldp, act, d, ldq, part, M, N);
+  auto go = [&](auto kind) {
+    constexpr int A = decltype(kind)::value;
+    if (dtype == 1)
+      act_backward_kernel<true, A><<<grid, 256, 0, st>>>(g, ldd, x, ldp, d, ldq, part, M, N);
+    else
+      act_backward_kernel<false, A><<<grid, 256, 0, st>>>(g, ldd, x, ldp, d, ldq, part, M, N);
+  };
+  switch (act) {
+    case kRelu: go(std::integral_constant<int, kRelu>{}); break;
+    case kSilu: go(std::integral_constant<int, kSilu>{}); break;
+    case kGeluTanh: go(std::integral_constant<int, kGeluTanh>{}); break;
+    case kGelu: go(std::integral_constant<int, kGelu>{}); break;
+    default: go(std::integral_constant<int, kNone>{}); break;
+  }
   rc = launch_error(cudaGetLastError());
   if (rc || part == nullptr) return rc;
   col_sum_kernel<<<(N + 31) / 32, 256, 0, st>>>(part, chunks, N, dbias, dbias_dtype);
