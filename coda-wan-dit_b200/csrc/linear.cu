@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0 || warp == 10) {
     // Loaders: warp 0 the A tiles, warp 10 the B tiles of the same stages.
-    if (lane == 0) {
+    if (elect_one()) {
       const bool is_a = warp == 0;
       const CUtensorMap* map = is_a ? &tmA : &tmB;
       const bool mn = is_a ? TA : TB;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && cta_rank == 0) {
+    if (cta_rank == 0 && elect_one()) {
       const uint32_t idesc = make_idesc(PAIR ? 2 * BM : BM, p.bn, p.is_bf16, TA, TB);
       const uint32_t ring = smem_u32(smem);
       const uint32_t empty0 = smem_u32(empty_bar), peer0 = PAIR ? mapa_shared(empty0, rank | 1) : 0u;
@@ -612,19 +612,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   }
   if constexpr (SPLIT) {
-    // One tile per cluster. Split c adds columns [c * bn / splits, + bn / splits) of all the splits'
-    // partial tiles (pair: of its own 128 rows), split 0 first.
+    // One tile per cluster. The tile's valid rows, in pieces of eight columns, are shared out over
+    // the splits in order (whole rows, so that the remote reads are contiguous); each adds all the
+    // splits' partial values of its pieces (pair: of its own 128 rows), split 0 first.
     cluster_sync_all();
     if (warp >= 2 && warp < 10 && my_count > 0) {
       int m_blk, n_blk;
       coords(0, m_blk, n_blk);
-      const int cols = p.bn / p.splits;
-      const int rows = min(BM, p.M - m_blk * BM);
-      const int per_row = cols / 8;
+      const int per_row = p.bn / 8;
+      const int total = min(BM, p.M - m_blk * BM) * per_row;
+      const int share = (total + p.splits - 1) / p.splits;
+      const int end = min(total, (split + 1) * share);
       const uint32_t mine = smem_u32(smem);
-      for (int x = threadIdx.x - 64; x < rows * per_row; x += kEpiThreads) {
+      for (int x = split * share + threadIdx.x - 64; x < end; x += kEpiThreads) {
         const int rr = x / per_row;
-        const int c = split * cols + (x - rr * per_row) * 8;
+        const int c = (x - rr * per_row) * 8;
         const int n = n_blk * p.bn + c;
         if (n >= p.N) continue;
         float4 f[8][2];  // all ranks' loads are in flight together

@@ -57,6 +57,20 @@ __device__ __forceinline__ void report_error(unsigned int code, unsigned int sit
 }
 #endif
 
+// True in one lane of a converged warp. Code that only one lane runs (loading, issuing MMAs) is put
+// under this rather than under lane == 0: the compiler then knows that a single thread runs it and
+// keeps addresses and descriptors in uniform registers, which TMA and tcgen05 instructions take,
+// instead of moving each of them there one by one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 __device__ __forceinline__ uint64_t globaltimer_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));

@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
   const uint32_t tmem_o = tmem + 2 * kCols;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
+    if (elect_one() && n > 0) {
       int k_loaded = min(n, ST), v_loaded = k_loaded;
       for (int t = ST; t < n; ++t) {
         const uint32_t ph = (t / ST) & 1;
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       const bool ok = wait_parity(&k_full[st], (t / ST) & 1, kSiteAttn + 3, p.ctx);
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         issue_scores<D, kCols>(tmem + (t & 1) * kCols, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
         mma_commit(&k_empty[st]);
         mma_commit(&s_full[t & 1]);
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       ok = wait_parity(&p_ready[t & 1], (t >> 1) & 1, kSiteAttn + 6, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         issue_ts<kCols>(tmem_o, tmem + (t & 1) * kCols, smem_u32(sV + st * C::kTile), id_o, t > 0);
         mma_commit(&v_empty[st]);
         mma_commit(pv_done);
@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   const uint32_t tmem_acc = tmem + NB * 2 * kCols;  // buffers of (scores, dP), then dQ
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
+    if (elect_one() && n > 0) {
       mbar_arrive_expect_tx(q_full, 2 * C::kBig);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
@@ -894,7 +894,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       // rows past the sample's keys would enter dQ as 0 * anything
       if (t * kCols + kCols > klen) zero_tail<D, kCols>(sK + st * C::kTile, klen - t * kCols, lane);
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t d = tmem + (t % NB) * 2 * kCols;
         issue_scores<D, kCols>(d, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
         issue_scores<D, kCols>(d + kCols, smem_u32(sO), smem_u32(sV + st * C::kTile), id_s);
@@ -918,7 +918,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       const int st = t % ST;
-      if (lane == 0) {
+      if (elect_one()) {
         issue_ts<kCols>(tmem_acc, tmem + (t % NB) * 2 * kCols, smem_u32(sK + st * C::kTile), id_acc, t > 0);
         mma_commit(&empty[st]);
         mma_commit(done);
@@ -1122,7 +1122,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   const uint32_t tmem_dk = tmem_dv + D;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
+    if (elect_one() && n > 0) {
       mbar_arrive_expect_tx(k_full, 2 * C::kBig);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
@@ -1154,7 +1154,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const bool ok = wait_parity(&full[st], (t / ST) & 1, kSiteAttnDkv + 2, p.ctx);
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t d = tmem + (t % NB) * 2 * kCols;
         issue_scores<D, kCols>(d, smem_u32(sK), smem_u32(sQ + st * C::kTile), id_s);
         issue_scores<D, kCols>(d + kCols, smem_u32(sV), smem_u32(sO + st * C::kTile), id_s);
@@ -1178,7 +1178,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       const int st = t % ST;
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t d = tmem + (t % NB) * 2 * kCols;
         issue_ts<kCols>(tmem_dv, d, smem_u32(sO + st * C::kTile), id_acc, t > 0);
         issue_ts<kCols>(tmem_dk, d + kCols, smem_u32(sQ + st * C::kTile), id_acc, t > 0);
