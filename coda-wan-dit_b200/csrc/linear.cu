@@ -768,15 +768,14 @@ struct Plan {
   int pair, bn, splits;
 };
 
-// Clocks of one K block of a tile in a CTA: its MMAs (bn columns: 2 bn for 128 accumulator rows), its
-// loads from L2 (about 64 bytes a clock when all SMs load), or one turn of the issuing threads.
-double block_cost(int load_rows, int bn) {
-  double c = 2.0 * bn;
-  const double ld = load_rows * BK * 2 / 64.0;
-  if (ld > c) c = ld;
-  return c < 280 ? 280 : c;
-}
-
+// The tile form by estimated clocks. Measured at 1.9 GHz, one K block (64) of a tile takes a CTA 270
+// clocks at least (its issuing threads), 2.1 per column otherwise (the tensor pipe: 128 x 192 398,
+// 128 x 256 548; pairs 256 x 192 394, 256 x 256 530), and all CTAs together load about 11 KB a clock
+// from L2 (128 x 128 tiles on every SM: 418 instead of 270). The last tile's epilogue adds 17 clocks
+// per column, an exchange between splits 4200 and 0.45 per element that crosses. What that picks
+// (us; next best in brackets):   1 x 1536 x 8960 split 8 of 128 x 128 11.3 (one CTA a tile 46)
+//   256 x 1536 x 8960 split 4 15.6 (pairs, no split 47)   1024 x 1536 x 4096 128 x 128 15.6 (pairs 16.8)
+//   2048 x 1536 x 8960 pairs 256 x 192 42.5 (128 x 192 46.1)   1024 x 8960 x 1536 pairs 256 x 256 23.0
 Plan plan(int M, int N, int K, int mn_b, int sms) {
   const int kb = (K + BK - 1) / BK;
   Plan best = {0, 128, 1};
@@ -784,14 +783,20 @@ Plan plan(int M, int N, int K, int mn_b, int sms) {
   auto consider = [&](int pair, int bn, int s) {
     const long long mb = (M + BM - 1) / BM, nb = (N + bn - 1) / bn;
     const long long tiles = (pair ? (mb + 1) / 2 : mb) * nb;
-    const long long slots = sms / (pair ? 2 : 1);
-    // clusters of more than two need their SMs inside one GPC: count 7/8 of them
-    if (s > 1 && tiles * s > slots * 7 / 8) return;
-    const long long waves = s > 1 ? 1 : (tiles + slots - 1) / slots;
+    const int group = (pair ? 2 : 1) * s;
+    // co-resident clusters of this kernel on 148 SMs (cudaOccupancyMaxActiveClusters): 74, 33, 15
+    const long long slots =
+        group == 1 ? sms : (group == 2 ? sms / 2 : (group == 4 ? sms * 33 / 148 : sms * 15 / 148));
+    if (s > 1 && tiles > slots) return;
+    const long long waves = (tiles + slots - 1) / slots;
+    const double active = static_cast<double>(tiles < slots ? tiles : slots) * group;
+    double block = 2.1 * bn;
+    const double l2 = active * (BM + (pair ? bn / 2 : bn)) * BK * 2 / 11000;
+    if (l2 > block) block = l2;
+    if (block < 270) block = 270;
     const int rows = M < BM ? M : BM;
-    // epilogue of the last tile; split: partial tiles written, exchanged, added
-    const double end = (s > 1 ? 2500 + rows * bn * (1.0 + 1.0 / s) / 24 : rows * bn / 16.0) + (pair ? 500 : 0);
-    const double cost = waves * ((kb + s - 1) / s) * block_cost(BM + (pair ? bn / 2 : bn), bn) + end;
+    const double end = (s > 1 ? 4200 + 0.45 * rows * bn * (s - 1) / s : 17.0 * bn) + (pair ? 500 : 0);
+    const double cost = waves * ((kb + s - 1) / s) * block + end;
     if (cost < best_cost) {
       best_cost = cost;
       best = {pair, bn, s};
