@@ -8,19 +8,29 @@
 //
 // Forward (rel_bias_kernel). A CTA takes a tile of rows x columns of one head, looks the bucket of
 // each of the tile's rows + columns - 1 diagonals up once, keeps the table's values for them in
-// shared memory, and writes every row as a shifted window of that line with 16-byte stores.
+// shared memory, and writes every row as a shifted window of that line with 16-byte stores. The
+// line is kept as 32-bit words (16-bit types: one copy per element parity) with a word of padding
+// every 32, so that lanes four words apart read different banks.
 //
-// Gradient (rel_bias_grad_kernel). A warp walks down a strip of 256 columns; a lane's accumulators
-// follow the diagonals: from a row to the next every diagonal moves one column to the right, so
-// the accumulators shift by one column (a register renaming, plus one shuffle per lane boundary)
-// instead of being looked up. Only the diagonal that leaves the strip is stored per row. At the
-// strip's end each warp adds its 256 + rows diagonal sums into the buckets. Sums are fp32, the
-// order is fixed (no atomics), and a second small kernel adds the CTAs' partial buckets.
+// Gradient (rel_bias_grad_kernel). A warp takes some rows of a strip of columns, and a lane's
+// accumulators are diagonals, never looked up per cell:
+//   rows on 16-byte boundaries: a rectangle of 256 columns, 8 per lane, 8 rows at a time. Row u adds
+//     its column e to the lane's sum e - u; after 8 rows the sums move 8 columns on, to the next
+//     lane (one shuffle per row of the block), and those of the last lane leave the strip.
+//   other rows: a parallelogram of 256 diagonals; the columns read move one on per row, so each
+//     lane stays on its 8 diagonals. The rows come by 16-byte asynchronous copies of the aligned
+//     blocks that hold them, eight rows ahead, and are read from shared memory at any offset.
+// The diagonal sums then go to the warp's sums per diagonal, which reach from the last bound on
+// one side to the other; what lies past them goes into one sum per side. Buckets are formed once
+// per CTA. (A table whose last bound is above 512 has no room for that; its strips are added bucket
+// by bucket.) Sums are fp32, the order is fixed (no atomics), and a second small kernel adds the
+// CTAs' partial buckets.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "relpos.cuh"
 #include "wdit_internal.h"
@@ -32,8 +42,25 @@ constexpr int kRelThreads = 256;
 constexpr int kRelWarps = kRelThreads / 32;
 constexpr int kBiasRows = 32;    // rows of a forward tile
 constexpr int kBiasCols = 2048;  // columns of a forward tile
-constexpr int kGradRows = 64;    // rows of a gradient strip
+constexpr int kGradRowsMin = 32;   // rows of a gradient strip: few cells ...
+constexpr int kGradRowsMax = 64;   // ... and many
 constexpr int kGradCols = 256;   // columns of a gradient strip (8 per lane)
+constexpr int kGradReach = 512;  // sums per diagonal are kept up to this last bound
+constexpr int kFewBounds = 32;   // up to here bounds are counted straight from the kernel's arguments
+
+constexpr int kRing = 8;  // rows of a parallelogram strip in flight per warp
+
+// Shared memory of the gradient kernel: sums and bounds, then (unaligned rows) the warps' rings of
+// 256 columns and one more 16-byte block a row.
+__host__ __device__ constexpr int grad_fixed_bytes(int sums) {
+  return (kRelWarps * sums * 4 + kMaxRelBounds * 4 + 15) / 16 * 16;
+}
+__host__ __device__ constexpr int grad_row_bytes(int esize) { return kGradCols * esize + 16; }
+
+// Strips of a gradient chunk of `rows` rows: 256 columns each, or 256 of its Lk + rows - 1 diagonals.
+__host__ __device__ inline int grad_strips(int Lk, int rows, bool vec) {
+  return ((vec ? Lk : Lk + rows - 1) + kGradCols - 1) / kGradCols;
+}
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -50,183 +77,307 @@ __device__ __forceinline__ float to_f32<__half>(__half v) {
   return __half2float(v);
 }
 
-// Lines of table values per element parity, so that a 16-byte piece of 2-byte elements that
-// starts at an odd diagonal is still read as aligned 32-bit words.
+// The bucket of d without shared memory when there are few bounds (uniform constant reads, no
+// latency chain), by binary search otherwise.
+__device__ __forceinline__ int bucket_of(const RelBuckets& rb, const int* bounds, int d) {
+  if (rb.n_bounds > kFewBounds) return rel_bucket(bounds, rb.n_bounds, rb.bidirectional, d);
+  const int n = rb.bidirectional ? (d < 0 ? -d : d) : (d < 0 ? -d : 0);
+  int c = 0;
+  for (int i = 0; i < rb.n_bounds; ++i) c += rb.bounds[i] <= n ? 1 : 0;
+  return rb.bidirectional && d > 0 ? c + rb.n_bounds + 1 : c;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kRelThreads)
     rel_bias_kernel(const T* __restrict__ table, const __grid_constant__ RelBuckets rb, int H, int Lq, int Lk,
                     int q_offset, int rows, T* __restrict__ out) {
-  constexpr int V = 16 / static_cast<int>(sizeof(T));
-  constexpr int kCopies = sizeof(T) == 2 ? 2 : 1;
-  constexpr int kLine = kBiasCols + kBiasRows + 16;
-  __shared__ __align__(16) T line[kCopies][kLine];
+  constexpr int E = 4 / static_cast<int>(sizeof(T));  // elements of a word
+  constexpr int V = 4 * E;                            // elements of a 16-byte store
+  constexpr int kWords = (kBiasCols + kBiasRows) / E + 16;
+  __shared__ uint32_t line[E][kWords + kWords / 32 + 1];
   __shared__ int bounds[kMaxRelBounds];
+  auto slot = [](int w) { return w + (w >> 5); };
   const int h = blockIdx.z;
   const int i0 = static_cast<int>(blockIdx.y) * rows;
   const int i1 = min(i0 + rows, Lq);
   const int j0 = static_cast<int>(blockIdx.x) * kBiasCols;
   const int j1 = min(j0 + kBiasCols, Lk);
-  for (int t = threadIdx.x; t < rb.n_bounds; t += kRelThreads) bounds[t] = rb.bounds[t];
-  __syncthreads();
+  if (rb.n_bounds > kFewBounds) {
+    for (int t = threadIdx.x; t < rb.n_bounds; t += kRelThreads) bounds[t] = rb.bounds[t];
+    __syncthreads();
+  }
   const int d0 = j0 - (i1 - 1) - q_offset;  // the tile's first diagonal
   const int nd = (j1 - j0) + (i1 - i0) - 1;
   for (int t = threadIdx.x; t < nd; t += kRelThreads) {
-    const T v = table[static_cast<size_t>(rel_bucket(bounds, rb.n_bounds, rb.bidirectional, d0 + t)) * H + h];
-    line[0][t] = v;
-    if (kCopies == 2 && t > 0) line[kCopies - 1][t - 1] = v;
+    const T v = table[static_cast<size_t>(bucket_of(rb, bounds, d0 + t)) * H + h];
+    if constexpr (E == 1) {
+      line[0][slot(t)] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      reinterpret_cast<T*>(&line[0][slot(t >> 1)])[t & 1] = v;
+      if (t > 0) reinterpret_cast<T*>(&line[E - 1][slot((t - 1) >> 1)])[(t - 1) & 1] = v;
+    }
   }
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int segs = (j1 - j0 + V - 1 + 32 * V - 1) / (32 * V);  // warp-wide pieces of a row, any alignment
-  for (int it = warp; it < segs * (i1 - i0); it += kRelWarps) {
-    const int i = i0 + it / segs;
+  // few rows: the warps share a row's pieces instead of taking rows
+  const int by_row = i1 - i0 >= kRelWarps ? 1 : 0;
+  const int w0 = by_row ? 0 : warp, wstep = by_row ? 1 : kRelWarps;
+  for (int i = i0 + (by_row ? warp : 0); i < i1; i += by_row ? kRelWarps : 1) {
     T* row = out + (static_cast<size_t>(h) * Lq + i) * Lk;
     const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row + j0) & 15) / sizeof(T));
-    const int j = j0 - mis + ((it % segs) * 32 + lane) * V;  // 16-byte aligned in memory
-    const int s = j - j0 + (i1 - 1 - i);                      // its diagonal in the line
-    if (j >= j0 && j + V <= j1) {
-      uint32_t w[4];
-      if constexpr (sizeof(T) == 2) {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(&line[s & (kCopies - 1)][s & ~1]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) w[q] = src[q];
+    const int shift = i1 - 1 - i - j0;  // column j of this row is diagonal j + shift of the line
+    for (int j = j0 - mis + (w0 * 32 + lane) * V; j < j1; j += wstep * 32 * V) {  // 16-byte aligned
+      const int s = j + shift;
+      if (j >= j0 && j + V <= j1) {
+        const uint32_t* src = line[E == 2 ? s & 1 : 0];
+        const int w = E == 2 ? s >> 1 : s;
+        *reinterpret_cast<uint4*>(row + j) =
+            make_uint4(src[slot(w)], src[slot(w + 1)], src[slot(w + 2)], src[slot(w + 3)]);
       } else {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(&line[0][s]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) w[q] = src[q];
+        for (int q = 0; q < V; ++q)
+          if (j + q >= j0 && j + q < j1) {
+            const int e = s + q;
+            if constexpr (E == 1)
+              row[j + q] = *reinterpret_cast<const T*>(&line[0][slot(e)]);
+            else
+              row[j + q] = reinterpret_cast<const T*>(&line[0][slot(e >> 1)])[e & 1];
+          }
       }
-      *reinterpret_cast<uint4*>(row + j) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      for (int q = 0; q < V; ++q)
-        if (j + q >= j0 && j + q < j1) row[j + q] = line[0][s + q];
     }
   }
 }
 
+// Eight neighbouring elements as fp32 from loaded words.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+__device__ __forceinline__ void widen8(const uint32_t* w, float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const T* e = reinterpret_cast<const T*>(&a);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = to_f32<T>(e[q]);
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_f32<T>(reinterpret_cast<const T*>(w)[e]);
   }
 }
 
-// VEC: rows start on 16-byte boundaries and lane l holds columns 8 l .. 8 l + 7 of the strip;
-// otherwise lane l holds columns l + 32 e (coalesced single elements).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kRelThreads)
+__global__ void __launch_bounds__(kRelThreads, VEC ? 2 : 3)
     rel_bias_grad_kernel(const T* __restrict__ db, const __grid_constant__ RelBuckets rb, int B, int Lq, int Lk,
                          int q_offset, long long stride_b, long long stride_h, long long stride_i, int buckets,
-                         float* __restrict__ part) {
+                         int rows, float* __restrict__ part) {
   extern __shared__ float sm[];
-  constexpr int kDiag = kGradCols + kGradRows;
-  float* acc_b = sm;                                   // [warps][buckets]
-  float* diag_all = sm + kRelWarps * buckets;          // [warps][kDiag]
-  int* bounds = reinterpret_cast<int*>(diag_all + kRelWarps * kDiag);
+  // per warp: sums of the diagonals -reach .. reach (the ends hold all beyond), or of the buckets
+  const int reach = rb.bounds[rb.n_bounds - 1];
+  const bool by_diag = reach <= kGradReach;
+  const int ahead = rb.bidirectional ? reach : 0;  // from here on one bucket
+  const int sums = by_diag ? reach + ahead + 1 : buckets;
+  float* acc_b = sm;  // [warps][sums]
+  int* bounds = reinterpret_cast<int*>(sm + kRelWarps * sums);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kRowBytes = grad_row_bytes(sizeof(T));
+  uint8_t* const rows_smem =
+      reinterpret_cast<uint8_t*>(sm) + grad_fixed_bytes(sums) + (VEC ? 0 : warp * kRing * kRowBytes);
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(rows_smem));
   const int h = blockIdx.y;
   for (int t = threadIdx.x; t < rb.n_bounds; t += kRelThreads) bounds[t] = rb.bounds[t];
-  for (int t = threadIdx.x; t < kRelWarps * buckets; t += kRelThreads) acc_b[t] = 0.f;
+  for (int t = threadIdx.x; t < kRelWarps * sums; t += kRelThreads) acc_b[t] = 0.f;
   __syncthreads();
-  float* mine = acc_b + warp * buckets;
-  float* diag = diag_all + warp * kDiag;
-  const int chunks = (Lq + kGradRows - 1) / kGradRows;
-  const int strips = (Lk + kGradCols - 1) / kGradCols;
-  const long long items = static_cast<long long>(B) * chunks * strips;
-  for (long long it = static_cast<long long>(blockIdx.x) * kRelWarps + warp; it < items;
-       it += static_cast<long long>(gridDim.x) * kRelWarps) {
-    const int strip = static_cast<int>(it % strips);
-    const long long r = it / strips;
-    const int i0 = static_cast<int>(r % chunks) * kGradRows;
-    const int i1 = min(i0 + kGradRows, Lq);
-    const int j0 = strip * kGradCols;
-    const T* src = db + (r / chunks) * stride_b + h * stride_h + j0;
-    float acc[8];
+  float* mine = acc_b + warp * sums;
+  float left = 0.f, right = 0.f;  // this lane's share of the cells past the ends
+  // One value per lane, of 32 different diagonals.
+  auto add_diag = [&](int d, float val) {
+    if (by_diag) {
+      if (d <= -reach) {
+        left += val;
+      } else if (d >= ahead) {
+        right += val;
+      } else {
+        mine[d + reach] += val;
+      }
+      __syncwarp();
+    } else {
+      add_buckets(mine, rel_bucket(bounds, rb.n_bounds, rb.bidirectional, d), val, lane);
+    }
+  };
+  const int chunks = (Lq + rows - 1) / rows;
+  const int strips = grad_strips(Lk, rows, VEC);
+  // (2^31 strips would be more cells than any memory holds: the entry point refuses them)
+  const unsigned items = static_cast<unsigned>(B) * chunks * strips;
+  for (unsigned it = blockIdx.x * kRelWarps + warp; it < items; it += gridDim.x * kRelWarps) {
+    const unsigned r = it / strips;
+    const int strip = static_cast<int>(it - r * strips);
+    const unsigned smp = r / chunks;
+    const int i0 = static_cast<int>(r - smp * chunks) * rows;
+    const int i1 = min(i0 + rows, Lq);
+    const T* src = db + smp * stride_b + h * stride_h + i0 * stride_i;
+    if constexpr (VEC) {
+      constexpr int kW = static_cast<int>(sizeof(T)) * 2;  // loaded words of a lane and row
+      const int j = strip * kGradCols + 8 * lane;            // the lane's first column
+      float acc[15];  // acc[7 + s]: the diagonal of column s of the block's first row
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    // diag[t] holds the sum of diagonal d = j - i (row-relative) = t - (kGradRows - 1)
-    constexpr int kStep = VEC ? 8 : 4;  // rows whose loads are in flight together
-    for (int i = i0; i < i1; i += kStep) {
-      float v[kStep][8];
+      for (int e = 0; e < 15; ++e) acc[e] = 0.f;
+      for (int i = i0; i < i1; i += 8, src += 8 * stride_i) {
+        uint32_t raw[8][kW];
+        const T* p = src + j;
+        if (i + 8 <= i1 && j + 8 <= Lk) {
 #pragma unroll
-      for (int u = 0; u < kStep; ++u) {
-        const T* p = src + static_cast<long long>(i + u) * stride_i;
-        const bool row_ok = i + u < i1;
-        if constexpr (VEC) {
-          // rows are a multiple of 16 bytes long, so 8 columns are all inside or (past the row's
-          // end: at most one 16-byte piece of fp32 inside) checked one by one
-          if (row_ok && j0 + 8 * lane + 8 <= Lk) {
-            load8<T>(p + 8 * lane, v[u]);
-          } else {
+          for (int u = 0; u < 8; ++u, p += stride_i) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              v[u][e] = row_ok && j0 + 8 * lane + e < Lk ? to_f32<T>(p[8 * lane + e]) : 0.f;
+            for (int q = 0; q < kW; q += 4) {
+              const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p) + q / 4);
+              raw[u][q] = w.x, raw[u][q + 1] = w.y, raw[u][q + 2] = w.z, raw[u][q + 3] = w.w;
+            }
           }
         } else {
+          // past the last row, or the row's end inside this lane's eight columns or before them
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            v[u][e] = row_ok && j0 + lane + 32 * e < Lk ? to_f32<T>(p[lane + 32 * e]) : 0.f;
-        }
-      }
+          for (int u = 0; u < 8; ++u, p += stride_i) {
+            T e8[8];
 #pragma unroll
-      for (int u = 0; u < kStep; ++u) {
-        if (i + u >= i1) break;
-        if (i + u > i0) {
-          // next row: every diagonal moves one column right; the strip's last one leaves
-          const float out = acc[7];
-          if (lane == 31) diag[kGradCols - 1 - (i + u - 1 - i0) + kGradRows - 1] = out;
-          if constexpr (VEC) {
-            float in = __shfl_up_sync(0xffffffffu, acc[7], 1);
-            if (lane == 0) in = 0.f;
+            for (int e = 0; e < 8; ++e) e8[e] = i + u < i1 && j + e < Lk ? p[e] : T(0.f);
 #pragma unroll
-            for (int e = 7; e > 0; --e) acc[e] = acc[e - 1];
-            acc[0] = in;
-          } else {
-            float rot[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) rot[e] = __shfl_sync(0xffffffffu, acc[e], (lane + 31) & 31);
-#pragma unroll
-            for (int e = 7; e > 0; --e) acc[e] = lane == 0 ? rot[e - 1] : rot[e];
-            acc[0] = lane == 0 ? 0.f : rot[0];
+            for (int q = 0; q < kW; ++q) raw[u][q] = reinterpret_cast<const uint32_t*>(e8)[q];
           }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += v[u][e];
-      }
-    }
-    // the diagonals still in the strip at its last row
-    const int last = i1 - 1 - i0;
+        for (int u = 0; u < 8; ++u) {
+          float v[8];
+          widen8<T>(raw[u], v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = VEC ? 8 * lane + e : lane + 32 * e;
-      diag[c - last + kGradRows - 1] = acc[e];
+          for (int e = 0; e < 8; ++e) acc[7 + e - u] += v[e];
+        }
+        // Eight columns on: sums 0 .. 7 belong to the next lane, -7 .. -1 stay as 1 .. 7. The last
+        // lane's leave the strip, one after the other from one lane.
+        const int d = j - i - q_offset;
+        float up[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          up[e] = __shfl_up_sync(0xffffffffu, acc[7 + e], 1);
+          if (lane == 0) up[e] = 0.f;
+        }
+        float leaving = 0.f;  // lane e < 8 takes sum e of the last lane
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __shfl_sync(0xffffffffu, acc[7 + e], 31);
+          if (lane == e) leaving = x;
+        }
+        add_diag(__shfl_sync(0xffffffffu, d, 31) + lane, leaving);
+#pragma unroll
+        for (int e = 7; e > 0; --e) acc[7 + e] = acc[e - 1] + up[e];
+        acc[7] = up[0];
+#pragma unroll
+        for (int e = 0; e < 7; ++e) acc[e] = 0.f;
+      }
+      const int rows8 = (i1 - i0 + 7) / 8 * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) add_diag(j + e - (i0 + rows8) - q_offset, acc[7 + e]);
+    } else {
+      const int dw = strip * kGradCols - (i1 - 1);  // the strip's first diagonal (j - i)
+      const int d0 = dw + lane;
+      float acc[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+      // rows with a column of the strip
+      const int r0 = max(i0, -(dw + kGradCols - 1)), r1 = min(i1, Lk - dw);
+      const bool inside = dw + r0 >= 0 && dw + r1 - 1 + kGradCols <= Lk;  // all 256 of every row
+      const uint64_t step = static_cast<uint64_t>((stride_i + 1) * static_cast<int>(sizeof(T)));
+      // address of the strip's first column in the next row to load and in the next row to read
+      uint64_t load_at = reinterpret_cast<uint64_t>(src) +
+                         static_cast<uint64_t>(((r0 - i0) * stride_i + dw + r0) * static_cast<int>(sizeof(T)));
+      uint32_t read_at = static_cast<uint32_t>(load_at);
+      const uint32_t lane_to = ring + lane * 16;
+      // An aligned 16-byte block is loaded when it holds an element of the strip and of the row.
+      auto fetch = [&](int i, int slot) {
+        const uint64_t block = (load_at & ~15ull) + lane * 16;
+        const uint32_t to = lane_to + slot * kRowBytes;
+        if (inside || (dw + i >= 0 && dw + i + kGradCols <= Lk)) {
+#pragma unroll
+          for (int c = 0; c < kGradCols * static_cast<int>(sizeof(T)); c += 512)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + c), "l"(block + c) : "memory");
+          if (lane == 0 && (load_at & 15) != 0)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + kRowBytes - 16),
+                         "l"(block + kRowBytes - 16)
+                         : "memory");
+        } else {
+          // byte positions of the row's columns 0 and Lk from the strip's first block
+          const int off = static_cast<int>(load_at & 15) - (dw + i) * static_cast<int>(sizeof(T));
+          const int end = off + Lk * static_cast<int>(sizeof(T));
+#pragma unroll
+          for (int c = 0; c < kRowBytes; c += 512) {
+            const int at = c + lane * 16;
+            if (at < kRowBytes && at + 16 > off && at < end)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + c), "l"(block + c) : "memory");
+          }
+        }
+        load_at += step;
+      };
+      auto consume = [&](int k, int slot) {
+        const T* line = reinterpret_cast<const T*>(rows_smem + slot * kRowBytes + (read_at & 15u)) + lane;
+        if (inside || (dw + k >= 0 && dw + k + kGradCols <= Lk)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] += to_f32<T>(line[32 * e]);
+        } else {
+          const int j = d0 + k;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (static_cast<unsigned>(j + 32 * e) < static_cast<unsigned>(Lk)) acc[e] += to_f32<T>(line[32 * e]);
+        }
+        read_at += static_cast<uint32_t>(step);
+      };
+      for (int base = r0; base < r1 + kRing - 1; base += kRing) {
+#pragma unroll
+        for (int u = 0; u < kRing; ++u) {
+          const int i = base + u, k = i - (kRing - 1);  // the rows loaded and read now
+          if (i < r1) fetch(i, u);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          if (k >= r0 && k < r1) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+            __syncwarp();
+            consume(k, (u + 1) % kRing);
+            __syncwarp();  // the slot is loaded anew in the next turn
+          }
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+      for (int e = 0; e < 8; ++e) add_diag(d0 + 32 * e - q_offset, acc[e]);
     }
-    __syncwarp();
-    // Diagonals -last .. 255 into the buckets, 32 at a time: equal buckets are neighbours, so a
-    // piece usually has one or a few; each is summed over its lanes in a fixed order.
-    const int base = kGradRows - 1 - last;
-    const int nd = kGradCols + last;
-    const int d_first = j0 - (i0 + last) - q_offset;
-    for (int t0 = 0; t0 < nd; t0 += 32) {
-      const int t = t0 + lane;
-      const float val = t < nd ? diag[base + t] : 0.f;
-      const int b = t < nd ? rel_bucket(bounds, rb.n_bounds, rb.bidirectional, d_first + t) : -1 - lane;
-      add_buckets(mine, b, val, lane);
+  }
+  if (by_diag) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      left += __shfl_xor_sync(0xffffffffu, left, o);
+      right += __shfl_xor_sync(0xffffffffu, right, o);
     }
-    __syncwarp();  // diag and mine are reused by the next strip
+    if (lane == 0) {
+      mine[0] += left;
+      mine[reach + ahead] += right;
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < sums; t += kRelThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRelWarps; ++w) s += acc_b[w * sums + t];
+    acc_b[t] = s;  // (row 0 is read by this thread only)
   }
   __syncthreads();
   for (int b = threadIdx.x; b < buckets; b += kRelThreads) {
     float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRelWarps; ++w) s += acc_b[w * buckets + b];
+    if (by_diag) {
+      // the bucket's distances [lo, hi], on its side of the diagonal
+      const int side = rb.n_bounds + 1;
+      const bool up = b >= side;
+      const int k = up ? b - side : b;
+      const int lo = k == 0 ? 0 : bounds[k - 1];
+      const int hi = k == rb.n_bounds ? reach : bounds[k] - 1;
+      if (up) {
+        for (int n = max(lo, 1); n <= hi; ++n) s += acc_b[reach + n];
+      } else {
+        for (int n = lo; n <= hi; ++n) s += acc_b[reach - n];
+      }
+    } else {
+      s = acc_b[b];
+    }
     part[(static_cast<size_t>(h) * gridDim.x + blockIdx.x) * buckets + b] = s;
   }
 }
@@ -250,13 +401,24 @@ int rel_cta_target() {
   return n * 4;
 }
 
-// CTAs per head of the gradient: about four per SM over all heads, at least one strip per warp.
+// Rows of a strip: 64 when there are enough cells to give every warp two strips of that, else 32
+// (more warps with loads in flight).
+int grad_rows(int B, int H, int Lq, int Lk, int target) {
+  int rows = kGradRowsMax;
+  while (rows > kGradRowsMin && static_cast<long long>(B) * H * ((Lq + rows - 1) / rows) * grad_strips(Lk, rows, false) <
+                                    2ll * target * kRelWarps)
+    rows /= 2;
+  return rows;
+}
+
+// CTAs per head of the gradient: about four per SM over all heads, every warp the same number of
+// strips (the last may have fewer), at least one.
 int grad_parts(int B, int H, int Lq, int Lk, int target) {
-  const long long items = static_cast<long long>(B) * ((Lq + kGradRows - 1) / kGradRows) *
-                          ((Lk + kGradCols - 1) / kGradCols);
-  long long x = (target + H - 1) / H;
-  const long long most = (items + kRelWarps - 1) / kRelWarps;
-  if (x > most) x = most;
+  const int rows = grad_rows(B, H, Lq, Lk, target);
+  const long long items = static_cast<long long>(B) * ((Lq + rows - 1) / rows) * grad_strips(Lk, rows, false);
+  const long long most = (target + H - 1) / H * kRelWarps;  // warps per head
+  const long long per = (items + most - 1) / most;
+  const long long x = (items + per * kRelWarps - 1) / (per * kRelWarps);
   return x < 1 ? 1 : static_cast<int>(x);
 }
 
@@ -273,18 +435,27 @@ int launch_bias(const void* table, const RelBuckets& rb, int H, int Lq, int Lk, 
 
 template <typename T>
 int launch_grad(const void* db, const RelBuckets& rb, int B, int H, int Lq, int Lk, int q_offset, long long sb,
-                long long sh, long long si, int buckets, int parts, float* part, cudaStream_t st) {
+                long long sh, long long si, int buckets, int parts, int rows, float* part, cudaStream_t st) {
   constexpr long long V = 16 / static_cast<long long>(sizeof(T));
   const bool vec = (reinterpret_cast<uintptr_t>(db) & 15) == 0 && sb % V == 0 && sh % V == 0 && si % V == 0;
-  const size_t smem = (static_cast<size_t>(kRelWarps) * (buckets + kGradCols + kGradRows) + kMaxRelBounds) * 4;
+  const int reach = rb.bounds[rb.n_bounds - 1];
+  const int sums = reach <= kGradReach ? reach + (rb.bidirectional ? reach : 0) + 1 : buckets;
+  // at most 34 KB, and 65 KB of rings
+  const size_t smem =
+      grad_fixed_bytes(sums) + (vec ? 0 : kRelWarps * kRing * grad_row_bytes(static_cast<int>(sizeof(T))));
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(rel_bias_grad_kernel<T, false>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    if (e != cudaSuccess) return WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+  }
   const dim3 grid(parts, H);
   const T* p = static_cast<const T*>(db);
   if (vec)
     rel_bias_grad_kernel<T, true><<<grid, kRelThreads, smem, st>>>(p, rb, B, Lq, Lk, q_offset, sb, sh, si, buckets,
-                                                                  part);
+                                                                  rows, part);
   else
     rel_bias_grad_kernel<T, false><<<grid, kRelThreads, smem, st>>>(p, rb, B, Lq, Lk, q_offset, sb, sh, si, buckets,
-                                                                   part);
+                                                                   rows, part);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e);
 }
@@ -292,7 +463,9 @@ int launch_grad(const void* db, const RelBuckets& rb, int B, int H, int Lq, int 
 int check_rel(const int* bounds, int n_bounds, int H, int Lq, int Lk, int q_offset, int dtype) {
   if (bounds == nullptr) return WDIT_ERR_ARG;
   if (n_bounds < 1 || n_bounds > kMaxRelBounds || H < 1 || H > 65535 || Lq < 0 || Lk < 0) return WDIT_ERR_SHAPE;
-  if (q_offset < 0 || static_cast<long long>(q_offset) + Lq > (1ll << 30) || Lk > (1 << 30)) return WDIT_ERR_SHAPE;
+  // positions up to 2^30, rows up to 2^28 cells (byte offsets in a row stay inside 32 bits)
+  if (q_offset < 0 || static_cast<long long>(q_offset) + Lq > (1ll << 30) || Lq > (1 << 28) || Lk > (1 << 28))
+    return WDIT_ERR_SHAPE;
   if (dtype < 0 || dtype > 2) return WDIT_ERR_ARG;
   return WDIT_OK;
 }
@@ -348,6 +521,8 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
   }
   if (dbias == nullptr) return WDIT_ERR_ARG;
   if (stride_b < 0 || stride_h < 0 || stride_i < 0) return WDIT_ERR_SHAPE;
+  if (static_cast<long long>(B) * ((Lq + kGradRowsMin - 1) / kGradRowsMin) * grad_strips(Lk, kGradRowsMin, false) >= 1ll << 31)
+    return WDIT_ERR_SHAPE;
   if (workspace == nullptr ||
       workspace_bytes < wdit_rel_pos_bias_grad_workspace_bytes(B, H, Lq, Lk, n_bounds, bidirectional))
     return WDIT_ERR_WORKSPACE;
@@ -355,15 +530,14 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
   RelBuckets rb;
   if (!rel_fill(&rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
   const int parts = grad_parts(B, H, Lq, Lk, rel_cta_target());
+  const int rows = grad_rows(B, H, Lq, Lk, rel_cta_target());
   float* part = static_cast<float*>(workspace);
-  if (dtype == 0)
-    rc = launch_grad<float>(dbias, rb, B, H, Lq, Lk, q_offset, stride_b, stride_h, stride_i, buckets, parts, part, st);
-  else if (dtype == 1)
-    rc = launch_grad<__nv_bfloat16>(dbias, rb, B, H, Lq, Lk, q_offset, stride_b, stride_h, stride_i, buckets, parts,
-                                    part, st);
-  else
-    rc = launch_grad<__half>(dbias, rb, B, H, Lq, Lk, q_offset, stride_b, stride_h, stride_i, buckets, parts, part,
-                             st);
+  auto go = [&](auto* type) {
+    return launch_grad<std::remove_pointer_t<decltype(type)>>(dbias, rb, B, H, Lq, Lk, q_offset, stride_b, stride_h,
+                                                              stride_i, buckets, parts, rows, part, st);
+  };
+  rc = dtype == 0 ? go(static_cast<float*>(nullptr))
+                  : (dtype == 1 ? go(static_cast<__nv_bfloat16*>(nullptr)) : go(static_cast<__half*>(nullptr)));
   if (rc) return rc;
   return launch_rel_table_sum(part, parts, buckets, H, dtable, stream);
 }
