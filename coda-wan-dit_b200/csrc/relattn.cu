@@ -257,10 +257,9 @@ struct BiasLine {
     if (searched) return col[bucket(d)];
     return value[min(max(d, -reach), reach) + reach];
   }
-  // One bucket for certain: d <= -reach, or d >= ahead() (past the last bound, or ahead of the
-  // query in one direction).
+  // One bucket each: d <= -reach, and d >= ahead() (past the last bound, or ahead of the query in
+  // one direction).
   __device__ __forceinline__ int ahead() const { return bidirectional ? reach : 0; }
-  __device__ __forceinline__ bool flat(int d_lo, int d_hi) const { return d_hi <= -reach || d_lo >= ahead(); }
 };
 
 __host__ __device__ inline int bias_reach(const RelBuckets& rb) { return rb.bounds[rb.n_bounds - 1]; }
@@ -298,8 +297,6 @@ __device__ __forceinline__ int sample_len(const AttnArgs& p, int b) {
   const int n = p.k_lens[b];
   return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
 }
-
-__host__ __device__ constexpr int align_up(int x, int a) { return (x + a - 1) / a * a; }
 
 // ---------------------------------------------------------------------------
 // Forward
@@ -751,6 +748,7 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
 // Eight compute warps: warp w reads TMEM lanes [32 (w % 4), + 32), warps 2-5 columns 0-31 of a
 // score tile, warps 6-9 columns 32-63. D = 64: two CTAs per SM overlap each other; D = 128: one
 // CTA per SM with two score buffers.
+constexpr int kSumReach = 256;  // the table's gradient is summed by diagonal up to this last bound
 template <int D>
 struct Bwd {
   static constexpr int kThreads = 320;
@@ -762,17 +760,60 @@ struct Bwd {
   static constexpr uint32_t kTile = kCols * D * 2;
   static constexpr int kWarp = 64 + 96 + 64;  // floats per warp: bias line, diagonals, row values
   static int smem(const RelBuckets& rb) {
-    const int buckets = rel_num_buckets(rb.n_bounds, rb.bidirectional);
-    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 8 * align_up(buckets * 4, 16) + kRows * 4 +
+    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 8 * 4 * grad_sums(rb) + kRows * 4 +
            bias_smem(rb);
   }
+  // Floats of a warp's sums of the table's gradient: by diagonal, or by bucket.
+  __host__ __device__ static int grad_sums(const RelBuckets& rb) {
+    const int reach = bias_reach(rb);
+    const int n = reach <= kSumReach ? reach + (rb.bidirectional ? reach : 0) + 1
+                                     : rel_num_buckets(rb.n_bounds, rb.bidirectional);
+    return (n + 3) / 4 * 4;
+  }
 };
+
+// 32 rows of a warp's accumulator, 64 columns from `tmem` on, times `mult`, through shared memory (32
+// rows of 128 bytes, swizzled) out by TMA. zero: the rows of lanes without a result.
+template <bool BF16>
+__device__ __forceinline__ void store_rows64(const CUtensorMap* map, uint8_t* stage, uint32_t tmem, bool has, bool zero,
+                                             float mult, int lane, int x, int h, int l, int b, bool inside) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    float o[32];
+    if (has) {
+      tmem_ld32(tmem + c * 32, o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = zero ? 0.f : o[e] * mult;
+    const uint32_t row = smem_u32(stage) + lane * 128;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      st_shared_v4(row + (((c * 4 + q) ^ (lane & 7)) << 4), pack16<BF16>(o[8 * q], o[8 * q + 1]),
+                   pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
+                   pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (inside) tma_store_4d(map, stage, x, h, l, b);
+    bulk_commit();
+  }
+}
+
+__device__ __forceinline__ uint64_t exp2_2(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return f2_pack(exp2_approx(a), exp2_approx(b));
+}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
-                   const __grid_constant__ AttnArgs p) {
+                   const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ AttnArgs p) {
   using C = Bwd<D>;
   constexpr int ST = C::kStages;
   constexpr int NB = C::kBuf;
@@ -792,11 +833,12 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   uint64_t* done = ds_ready + 2;
   uint64_t* last = done + 1;  // every product is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
-  const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
   float* warps = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
-  const int bpad = align_up(buckets * 4, 16) / 4;
-  float* sums = warps + 8 * C::kWarp;  // [8][bpad]
-  float* sdelta = sums + 8 * bpad;     // [128]
+  const int reach = bias_reach(p.rb);
+  const bool by_diag = reach <= kSumReach;
+  const int nsum = C::grad_sums(p.rb);
+  float* sums = warps + 8 * C::kWarp;  // [8][nsum]
+  float* sdelta = sums + 8 * nsum;     // [128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_tiles = (p.Lq + kRows - 1) / kRows;
@@ -806,43 +848,63 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   const int h = x % p.H;
   const int b = x / p.H;
   const int i0 = qt * kRows;
-  const int klen = sample_len(p, b);
-  int visible = klen;
-  if (p.causal) visible = min(visible, min(i0 + kRows, p.Lq) + p.q_offset);
-  const int n = (visible + kCols - 1) / kCols;
 
+  auto load_kv = [&](int t) {
+    const int st = t % ST;
+    mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      tma_load_4d(sK + st * C::kTile + c * 8192, &tmK, &full[st], c * 64, h, t * kCols, b);
+      tma_load_4d(sV + st * C::kTile + c * 8192, &tmV, &full[st], c * 64, h, t * kCols, b);
+    }
+  };
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     mbar_init(q_full, 1);
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
-    mbar_init(&ds_ready[0], 8);
-    mbar_init(&ds_ready[1], 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&ds_ready[i], 8);
+    }
     mbar_init(done, 1);
     mbar_init(last, 1);
     fence_mbar_init();
   }
+  const int klen = sample_len(p, b);
+  int visible = klen;
+  if (p.causal) visible = min(visible, min(i0 + kRows, p.Lq) + p.q_offset);
+  const int n = (visible + kCols - 1) / kCols;
+  if (threadIdx.x == 0 && n > 0) {  // the first loads run under the rest of the set-up
+    mbar_arrive_expect_tx(q_full, 2 * C::kBig);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      tma_load_4d(sQ + c * 16384, &tmQ, q_full, c * 64, h, i0, b);
+      tma_load_4d(sO + c * 16384, &tmO, q_full, c * 64, h, i0, b);
+    }
+    for (int t = 0; t < min(n, ST); ++t) load_kv(t);
+  }
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
-  const BiasLine bias = load_bias(p, h, sdelta + kRows, C::kThreads);
-  for (int t = threadIdx.x; t < 8 * bpad; t += C::kThreads) sums[t] = 0.f;
-  // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too
-  if (threadIdx.x < kRows) {
-    const int i = i0 + threadIdx.x;
-    float s = 0.f;
-    if (i < p.Lq) {
-      const uint4* g = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.dout) + b * p.do_b + i * p.do_l +
-                                                      h * p.do_h);
-      const uint4* o = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.out) +
-                                                      ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D);
+  for (int t = threadIdx.x; t < 8 * nsum; t += C::kThreads) sums[t] = 0.f;
+  // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too: D / 8 lanes a row.
+  {
+    constexpr int kLanes = D / 8, kAtOnce = C::kThreads / kLanes;
+    const int part = threadIdx.x % kLanes;
 #pragma unroll
-      for (int q = 0; q < D / 8; ++q) {
-        const uint4 a = __ldg(g + q), c = __ldg(o + q);
+    for (int r0 = 0; r0 < kRows; r0 += kAtOnce) {
+      const int r = r0 + threadIdx.x / kLanes;
+      const int i = i0 + r;
+      float s = 0.f;
+      if (r < kRows && i < p.Lq) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.dout) + b * p.do_b +
+                                                             i * p.do_l + h * p.do_h) + part);
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.out) +
+                                                             ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D) + part);
         const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -850,10 +912,15 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
           s = fmaf(f.x, v.x, fmaf(f.y, v.y, s));
         }
       }
-      p.delta[(static_cast<long long>(b) * p.H + h) * p.Lq + i] = s;
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (part == 0 && r < kRows) {
+        sdelta[r] = s;
+        if (i < p.Lq) p.delta[(static_cast<long long>(b) * p.H + h) * p.Lq + i] = s;
+      }
     }
-    sdelta[threadIdx.x] = s;
   }
+  const BiasLine bias = load_bias(p, h, sdelta + kRows, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -862,22 +929,10 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
 
   if (warp == 0) {
     if (elect_one() && n > 0) {
-      mbar_arrive_expect_tx(q_full, 2 * C::kBig);
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        tma_load_4d(sQ + c * 16384, &tmQ, q_full, c * 64, h, i0, b);
-        tma_load_4d(sO + c * 16384, &tmO, q_full, c * 64, h, i0, b);
-      }
-      int loaded = 0;
-      for (int t = 0; t < n; ++t) {
-        const int st = t % ST;
-        if (!wait_parity(&empty[st], ((t / ST) & 1) ^ 1u, kSiteAttnDq, p.ctx)) break;
-        mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          tma_load_4d(sK + st * C::kTile + c * 8192, &tmK, &full[st], c * 64, h, t * kCols, b);
-          tma_load_4d(sV + st * C::kTile + c * 8192, &tmV, &full[st], c * 64, h, t * kCols, b);
-        }
+      int loaded = min(n, ST);
+      for (int t = ST; t < n; ++t) {
+        if (!wait_parity(&empty[t % ST], ((t / ST) & 1) ^ 1u, kSiteAttnDq, p.ctx)) break;
+        load_kv(t);
         loaded = t + 1;
       }
       wait_parity(q_full, 0, kSiteAttnDq + 1, p.ctx);
@@ -937,44 +992,60 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     float* line = warps + (warp - 2) * C::kWarp;
     float* diag = line + 64;
-    float* mine = sums + (warp - 2) * bpad;
-    const float scale2 = p.scale * kLog2e;
+    float* mine = sums + (warp - 2) * nsum;
+    float left = 0.f, right = 0.f;  // this row's share of the table's gradient past the last bounds
     const int row_end = !row_ok ? 0 : (p.causal ? min(klen, i + p.q_offset + 1) : klen);
     const int warp_first = i0 + wq * 32 + p.q_offset;
     float lse = kInf;
     if (row_ok) lse = p.lse[(static_cast<long long>(b) * p.H + h) * p.Lq + i];
     if (lse == -kInf) lse = kInf;  // no keys: every P is 0
-    const float delta = sdelta[r];
+    const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
+    const uint64_t neg_delta = f2_pack(-sdelta[r], -sdelta[r]);
+    // The warp's tiles by kind, as in the forward kernel, for its 32 columns of each tile.
+    const int t_left = (warp_first - bias.reach - 31 - half * 32 + kCols) / kCols;
+    const int t_right = (warp_first + 31 + bias.ahead() - half * 32 + kCols - 1) / kCols;
+    const int t_mask = ((__reduce_min_sync(0xffffffffu, row_end) - half * 32 - 32) >> 6) + 1;
+    static_assert(kCols == 64, "shift above");
+    const float c_left = bias.at(-bias.reach), c_right = bias.at(bias.reach);
     bool ok = true;
     for (int t = 0; t < n; ++t) {
       const int j0 = t * kCols + half * 32;
-      const int d_lo = j0 - warp_first - 31, d_hi = j0 + 31 - warp_first;
-      const bool flat = bias.flat(d_lo, d_hi);
+      const int d_lo = j0 - warp_first - 31;
+      const bool masked = t >= t_mask;
+      const bool flat = !masked && (t < t_left || t >= t_right);
       if (!flat) {
         __syncwarp();
         line[lane] = bias.at(d_lo + lane);
         line[lane + 32] = bias.at(d_lo + lane + 32);
         __syncwarp();
       }
+      const float* ln = line + 31 - lane;
       ok = wait_parity(&s_full[t % NB], (t / NB) & 1, kSiteAttnDq + 5, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       const uint32_t ts = tmem + lane_off + (t % NB) * 2 * kCols + half * 32;
       float s[32], g[32];
       tmem_ld32x2(ts, s, ts + kCols, g);
+      // dS in s
       if (flat) {
-        const float c = bias.at(d_lo) - lse;
+        const float c = (t < t_left ? c_left : c_right) - lse;
+        const uint64_t c2 = f2_pack(c, c);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = exp2_approx(fmaf(s[e], scale2, c)) * (g[e] - delta);
+        for (int e = 0; e < 32; e += 2)
+          f2_unpack(fmul2(exp2_2(ffma2(f2_pack(s[e], s[e + 1]), scale2, c2)), fadd2(f2_pack(g[e], g[e + 1]), neg_delta)),
+                    s[e], s[e + 1]);
       } else {
-        const float* ln = line + 31 - lane;
+        const uint64_t neg_lse = f2_pack(-lse, -lse);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = exp2_approx(fmaf(s[e], scale2, ln[e] - lse)) * (g[e] - delta);
-      }
-      if (__any_sync(0xffffffffu, row_end < j0 + 32)) {
-        const int keep = row_end - j0;
+        for (int e = 0; e < 32; e += 2)
+          f2_unpack(fmul2(exp2_2(ffma2(f2_pack(s[e], s[e + 1]), scale2, fadd2(f2_pack(ln[e], ln[e + 1]), neg_lse))),
+                          fadd2(f2_pack(g[e], g[e + 1]), neg_delta)),
+                    s[e], s[e + 1]);
+        if (masked) {
+          const int keep = row_end - j0;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = e < keep ? s[e] : 0.f;
+          for (int e = 0; e < 32; ++e) s[e] = e < keep ? s[e] : 0.f;
+        }
       }
       uint32_t w[16];
 #pragma unroll
@@ -984,81 +1055,108 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ds_ready[t % NB]);
-      // The table's gradient: the sum of dS by bucket.
+      // The table's gradient: the sum of dS by diagonal (the products run meanwhile).
       if (flat) {
-        float a[4] = {s[0], s[1], s[2], s[3]};
+        uint64_t a2 = f2_pack(s[0], s[1]), b2 = f2_pack(s[2], s[3]);
 #pragma unroll
-        for (int e = 4; e < 32; ++e) a[e & 3] += s[e];
-        float tot = (a[0] + a[1]) + (a[2] + a[3]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
-        if (lane == 0) mine[bias.bucket(d_lo)] += tot;
+        for (int e = 4; e < 32; e += 4) {
+          a2 = fadd2(a2, f2_pack(s[e], s[e + 1]));
+          b2 = fadd2(b2, f2_pack(s[e + 2], s[e + 3]));
+        }
+        float x0, x1;
+        f2_unpack(fadd2(a2, b2), x0, x1);
+        if (t < t_left) {
+          left += x0 + x1;
+        } else {
+          right += x0 + x1;
+        }
       } else {
-        // Diagonal sums: from a column to the next a diagonal moves one lane up, so a running sum
-        // passed from lane to lane follows it. Two chains of 16 columns; entry d + 31 of a chain.
+        // From a column to the next a diagonal moves one lane up, so a running sum passed from lane
+        // to lane follows it. Two chains of 16 columns; entry d + 31 of a chain.
+        float a[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float a = 0.f;
+        for (int e = 0; e < 16; ++e) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            a = __shfl_up_sync(0xffffffffu, a, 1);
-            a = (lane == 0 ? 0.f : a) + s[16 * c + e];
-            if (lane == 31) diag[48 * c + e] = a;
+          for (int c = 0; c < 2; ++c) {
+            a[c] = __shfl_up_sync(0xffffffffu, a[c], 1);
+            a[c] = (lane == 0 ? 0.f : a[c]) + s[16 * c + e];
+            if (lane == 31) diag[48 * c + e] = a[c];
           }
-          if (lane < 31) diag[48 * c + 46 - lane] = a;
+        }
+        if (lane < 31) {
+          diag[46 - lane] = a[0];
+          diag[48 + 46 - lane] = a[1];
         }
         __syncwarp();
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int idx = lane + 32 * q;
           const float v = (idx < 47 ? diag[idx] : 0.f) + (idx >= 16 && idx < 63 ? diag[48 + idx - 16] : 0.f);
-          const int bk = idx < 63 ? bias.bucket(d_lo + idx) : -1 - lane;
-          add_buckets(mine, bk, v, lane);
+          const int d = d_lo + idx;
+          if (!by_diag) {
+            add_buckets(mine, idx < 63 ? bias.bucket(d) : -1 - lane, v, lane);
+          } else if (idx < 63) {
+            if (d <= -reach) {
+              left += v;
+            } else if (d >= bias.ahead()) {
+              right += v;
+            } else {
+              mine[d + reach] += v;  // one lane per diagonal
+            }
+          }
         }
+        __syncwarp();
       }
-      __syncwarp();
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      left += __shfl_xor_sync(0xffffffffu, left, o);
+      right += __shfl_xor_sync(0xffffffffu, right, o);
+    }
+    if (lane == 0) {
+      if (by_diag) {
+        mine[0] += left;
+        mine[reach + bias.ahead()] += right;
+      } else {
+        mine[bias.bucket(-reach)] += left;
+        mine[bias.bucket(bias.ahead())] += right;
+      }
     }
     if (ok && n > 0) {
       ok = wait_parity(last, 0, kSiteAttnDq + 6, p.ctx);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
-    uint16_t* dst = static_cast<uint16_t*>(p.dq) + ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D;
-#pragma unroll 1
-    for (int c = half; c < D / 32; c += 2) {
-      float o[32];
-      if (n > 0 && ok) {
-        tmem_ld32(tmem_acc + lane_off + c * 32, o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0.f;
-      }
-      if (!row_ok) continue;
-#pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] *= p.scale;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        st_global_v4(dst + c * 32 + q * 8, pack16<BF16>(o[8 * q], o[8 * q + 1]),
-                     pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
-                     pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
+    // dQ through the query tile's shared memory: warps 2-5 write columns 0-63, 6-9 64-127.
+    if (half < D / 64) {
+      store_rows64<BF16>(&tmOut, sQ + half * 16384 + wq * 4096, tmem_acc + lane_off + half * 64, n > 0 && ok, false,
+                         p.scale, lane, half * 64, h, i0 + wq * 32, b, i0 + wq * 32 < p.Lq);
+      if (lane == 0) bulk_wait_all<0>();
     }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, C::kTmem);
-  for (int t = threadIdx.x; t < buckets; t += C::kThreads) {
+  for (int t = threadIdx.x; t < nsum; t += C::kThreads) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += sums[w * bpad + t];
-    p.table_part[(static_cast<long long>(h) * p.B * q_tiles + static_cast<long long>(b) * q_tiles + qt) * buckets + t] = s;
+    for (int w = 0; w < 8; ++w) s += sums[w * nsum + t];
+    sums[t] = s;  // (column t is this thread's)
   }
+  __syncthreads();
+  const int buckets = rel_num_buckets(p.rb.n_bounds, p.rb.bidirectional);
+  for (int t = threadIdx.x; t < buckets; t += C::kThreads)
+    p.table_part[(static_cast<long long>(h) * p.B * q_tiles + static_cast<long long>(b) * q_tiles + qt) * buckets + t] =
+        by_diag ? rel_bucket_sum(sums, reach, bias.bounds, p.rb.n_bounds, t) : sums[t];
 }
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmO,
+                    const __grid_constant__ CUtensorMap tmDk, const __grid_constant__ CUtensorMap tmDv,
                     const __grid_constant__ AttnArgs p) {
   using C = Bwd<D>;
   constexpr int ST = C::kStages;
@@ -1089,26 +1187,45 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   const int h = x % p.H;
   const int b = x / p.H;
   const int j0 = kt * kRows;
-  const int klen = sample_len(p, b);
   // query tiles with a row that sees one of these keys
   const int q_tiles = (p.Lq + kCols - 1) / kCols;
   const int first = p.causal ? max(0, j0 - p.q_offset) / kCols : 0;
-  const int n = j0 < klen ? max(0, q_tiles - first) : 0;
 
+  auto load_q = [&](int t) {
+    const int st = t % ST;
+    mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      tma_load_4d(sQ + st * C::kTile + c * 8192, &tmQ, &full[st], c * 64, h, (first + t) * kCols, b);
+      tma_load_4d(sO + st * C::kTile + c * 8192, &tmO, &full[st], c * 64, h, (first + t) * kCols, b);
+    }
+  };
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     mbar_init(k_full, 1);
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
-    mbar_init(&ds_ready[0], 8);
-    mbar_init(&ds_ready[1], 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&ds_ready[i], 8);
+    }
     mbar_init(done, 1);
     mbar_init(last, 1);
     fence_mbar_init();
   }
+  const int klen = sample_len(p, b);
+  const int n = j0 < klen ? max(0, q_tiles - first) : 0;
+  if (threadIdx.x == 0 && n > 0) {  // the first loads run under the rest of the set-up
+    mbar_arrive_expect_tx(k_full, 2 * C::kBig);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      tma_load_4d(sK + c * 16384, &tmK, k_full, c * 64, h, j0, b);
+      tma_load_4d(sV + c * 16384, &tmV, k_full, c * 64, h, j0, b);
+    }
+    for (int t = 0; t < min(n, ST); ++t) load_q(t);
+  }
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
@@ -1123,23 +1240,10 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
 
   if (warp == 0) {
     if (elect_one() && n > 0) {
-      mbar_arrive_expect_tx(k_full, 2 * C::kBig);
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        tma_load_4d(sK + c * 16384, &tmK, k_full, c * 64, h, j0, b);
-        tma_load_4d(sV + c * 16384, &tmV, k_full, c * 64, h, j0, b);
-      }
-      int loaded = 0;
-      for (int t = 0; t < n; ++t) {
-        const int st = t % ST;
-        const int i0 = (first + t) * kCols;
-        if (!wait_parity(&empty[st], ((t / ST) & 1) ^ 1u, kSiteAttnDkv, p.ctx)) break;
-        mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          tma_load_4d(sQ + st * C::kTile + c * 8192, &tmQ, &full[st], c * 64, h, i0, b);
-          tma_load_4d(sO + st * C::kTile + c * 8192, &tmO, &full[st], c * 64, h, i0, b);
-        }
+      int loaded = min(n, ST);
+      for (int t = ST; t < n; ++t) {
+        if (!wait_parity(&empty[t % ST], ((t / ST) & 1) ^ 1u, kSiteAttnDkv, p.ctx)) break;
+        load_q(t);
         loaded = t + 1;
       }
       wait_parity(k_full, 0, kSiteAttnDkv + 1, p.ctx);
@@ -1193,71 +1297,106 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   } else {
     const int wq = warp & 3;
     const int half = (warp - 2) >> 2;
-    const int r = wq * 32 + lane;
-    const int j = j0 + r;  // this thread's key
+    const int jw = j0 + wq * 32;  // the warp's first key
+    const int j = jw + lane;      // this thread's key
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     float* line = warps + (warp - 2) * C::kWarp;
-    float* rowv = line + 160;  // lse and delta of the half tile's 32 query rows
-    const float scale2 = p.scale * kLog2e;
+    float* rowv = line + 160;  // -lse and -delta of the half tile's 32 query rows
+    const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     const bool key_ok = j < klen;
     const long long hbase = (static_cast<long long>(b) * p.H + h) * p.Lq;
+    // Row values of tile t for this lane: loaded a tile ahead.
+    float next_lse = -kInf, next_delta = 0.f;
+    auto load_rows = [&](int t) {
+      const int i = (first + t) * kCols + half * 32 + lane;
+      next_lse = -kInf;  // (negated) no such row, or one without keys: every P is 0
+      next_delta = 0.f;
+      if (t < n && i < p.Lq) {
+        const float v = p.lse[hbase + i];
+        next_delta = -p.delta[hbase + i];
+        next_lse = v == -kInf ? -kInf : -v;
+      }
+    };
+    load_rows(0);
+    // Tile kinds: positions pos .. pos + 31 of the half tile's rows, pos = pos0 + t * kCols. Keys
+    // jw .. jw + 31 lie past the last bound on the left from t_left on, on the right before t_right.
+    const int pos0 = first * kCols + half * 32 + p.q_offset;
+    const int t_left = (jw + 31 + bias.reach - pos0 + kCols - 1) / kCols;
+    const int t_right = (jw - 31 - bias.ahead() - pos0 + kCols) / kCols;
+    // masked: rows past Lq, keys past klen, or (causal) a row before one of the keys
+    const int t_causal = p.causal ? (jw + 31 - pos0 + kCols - 1) / kCols : 0;
+    const bool all_keys = jw + 32 <= klen;
+    const float c_left = bias.at(-bias.reach), c_right = bias.at(bias.reach);
     bool ok = true;
     for (int t = 0; t < n; ++t) {
-      const int i0 = (first + t) * kCols + half * 32;
-      const int pos = i0 + p.q_offset;
-      // diagonal of (key lane, query e): j - i - off = d_lo + 31 + lane - e
-      const int d_lo = j0 + wq * 32 - pos - 31, d_hi = j0 + wq * 32 + 31 - pos;
-      const bool flat = bias.flat(d_lo, d_hi);
-      float my_lse = kInf, my_delta = 0.f;
-      if (i0 + lane < p.Lq) {
-        my_lse = p.lse[hbase + i0 + lane];
-        my_delta = p.delta[hbase + i0 + lane];
-        if (my_lse == -kInf) my_lse = kInf;
-      }
+      const int pos = pos0 + t * kCols;
+      const int i_half = pos - p.q_offset;
+      const bool masked = !all_keys || t < t_causal || i_half + 32 > p.Lq;
+      const bool flat = !masked && (t >= t_left || t < t_right);
       __syncwarp();
-      rowv[lane] = my_lse;
-      rowv[32 + lane] = my_delta;
+      rowv[lane] = next_lse;
+      rowv[32 + lane] = next_delta;
       if (!flat) {
+        // diagonal of (key lane, query e): d_lo + 31 + lane - e
+        const int d_lo = jw - pos - 31;
         line[lane] = bias.at(d_lo + lane);
         line[lane + 32] = bias.at(d_lo + lane + 32);
       }
       __syncwarp();
+      load_rows(t + 1);
       ok = wait_parity(&s_full[t % NB], (t / NB) & 1, kSiteAttnDkv + 5, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       const uint32_t ts = tmem + lane_off + (t % NB) * 2 * kCols + half * 32;
       float s[32], g[32];
       tmem_ld32x2(ts, s, ts + kCols, g);
-      // visible to this key: query rows i >= j - off (causal), i < Lq
-      const int from = !key_ok ? 32 : (p.causal ? j - pos : 0);
-      const int to = p.Lq - i0;
-      const bool masked = __any_sync(0xffffffffu, from > 0) || to < 32;
-      const float flat_c = flat ? bias.at(d_lo) : 0.f;
+      uint32_t wp[16], wd[16];
+      auto transform = [&](auto is_flat, auto is_masked) {
+        const float c = t >= t_left ? c_left : c_right;
+        const uint64_t c2 = f2_pack(c, c);
+        const float* ln = line + 31 + lane;
+        const int from = !key_ok ? 32 : (p.causal ? j - pos : 0), to = p.Lq - i_half;
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        const float4 ls = *reinterpret_cast<const float4*>(rowv + e);
-        const float4 dl = *reinterpret_cast<const float4*>(rowv + 32 + e);
-        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dlv[4] = {dl.x, dl.y, dl.z, dl.w};
+        for (int e = 0; e < 32; e += 4) {
+          const float4 l4 = *reinterpret_cast<const float4*>(rowv + e);
+          const float4 d4 = *reinterpret_cast<const float4*>(rowv + 32 + e);
+          const uint64_t nl[2] = {f2_pack(l4.x, l4.y), f2_pack(l4.z, l4.w)};
+          const uint64_t nd[2] = {f2_pack(d4.x, d4.y), f2_pack(d4.z, d4.w)};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float bias = flat ? flat_c : line[31 + lane - (e + u)];
-          float pr = exp2_approx(fmaf(s[e + u], scale2, bias - lsv[u]));
-          float ds = pr * (g[e + u] - dlv[u]);
-          if (masked && (e + u < from || e + u >= to)) {
-            pr = 0.f;
-            ds = 0.f;
+          for (int u = 0; u < 2; ++u) {
+            const int q = e + 2 * u;
+            uint64_t add;
+            if constexpr (decltype(is_flat)::value) {
+              add = fadd2(c2, nl[u]);
+            } else {
+              add = fadd2(f2_pack(ln[-q], ln[-q - 1]), nl[u]);
+            }
+            uint64_t pr = exp2_2(ffma2(f2_pack(s[q], s[q + 1]), scale2, add));
+            uint64_t ds = fmul2(pr, fadd2(f2_pack(g[q], g[q + 1]), nd[u]));
+            float p0, p1, d0, d1;
+            f2_unpack(pr, p0, p1);
+            f2_unpack(ds, d0, d1);
+            if constexpr (decltype(is_masked)::value) {
+              const bool a = q >= from && q < to, bb = q + 1 >= from && q + 1 < to;
+              p0 = a ? p0 : 0.f;
+              d0 = a ? d0 : 0.f;
+              p1 = bb ? p1 : 0.f;
+              d1 = bb ? d1 : 0.f;
+            }
+            wp[q >> 1] = pack16<BF16>(p0, p1);
+            wd[q >> 1] = pack16<BF16>(d0, d1);
           }
-          s[e + u] = pr;
-          g[e + u] = ds;
         }
+      };
+      if (masked) {
+        transform(std::false_type{}, std::true_type{});
+      } else if (flat) {
+        transform(std::true_type{}, std::false_type{});
+      } else {
+        transform(std::false_type{}, std::false_type{});
       }
-      uint32_t w[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) w[e] = pack16<BF16>(s[2 * e], s[2 * e + 1]);
-      tmem_st16(ts, w);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) w[e] = pack16<BF16>(g[2 * e], g[2 * e + 1]);
-      tmem_st16(ts + kCols, w);
+      tmem_st16(ts, wp);
+      tmem_st16(ts + kCols, wd);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -1268,29 +1407,15 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
-    // Warps 2-5 write dV, warps 6-9 dK; keys past the sample's length get 0.
-    uint16_t* dst = static_cast<uint16_t*>(half == 0 ? p.dv : p.dk) +
-                    ((static_cast<long long>(b) * p.Lk + j) * p.H + h) * D;
-    const uint32_t src = (half == 0 ? tmem_dv : tmem_dk) + lane_off;
-    const float mult = half == 0 ? 1.f : p.scale;
+    // Warps 2-5 write dV, warps 6-9 dK (through the tiles' shared memory); keys past the sample's
+    // length get 0.
 #pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      float o[32];
-      if (n > 0 && ok) {
-        tmem_ld32(src + c * 32, o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0.f;
-      }
-      if (j >= p.Lk) continue;
-#pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = key_ok ? o[e] * mult : 0.f;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        st_global_v4(dst + c * 32 + q * 8, pack16<BF16>(o[8 * q], o[8 * q + 1]),
-                     pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
-                     pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
-    }
+    for (int c = 0; c < D / 64; ++c)
+      store_rows64<BF16>(half == 0 ? &tmDv : &tmDk, (half == 0 ? sV : sK) + c * 16384 + wq * 4096,
+                         (half == 0 ? tmem_dv : tmem_dk) + lane_off + c * 64, n > 0 && ok, !key_ok,
+                         half == 0 ? 1.f : p.scale, lane, c * 64, h, jw, b, jw < p.Lk);
+    if (lane == 0) bulk_wait_all<0>();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -1389,9 +1514,9 @@ int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, co
 }
 
 template <int D, bool BF16>
-int run_bwd(const CUtensorMap (&big)[4], const CUtensorMap (&small)[4], const AttnArgs& p, int buckets,
-            float* dtable, cudaStream_t st) {
-  // order of the maps: q, k, v, dO
+int run_bwd(const CUtensorMap (&big)[4], const CUtensorMap (&small)[4], const CUtensorMap (&out)[3], const AttnArgs& p,
+            int buckets, float* dtable, cudaStream_t st) {
+  // order of the maps: q, k, v, dO; dq, dk, dv
   static int done_q[64] = {}, done_kv[64] = {};
   const int smem = Bwd<D>::smem(p.rb);
   int rc = set_smem(attn_dq_kernel<D, BF16>, smem, done_q);
@@ -1402,10 +1527,10 @@ int run_bwd(const CUtensorMap (&big)[4], const CUtensorMap (&small)[4], const At
   const long long gk = static_cast<long long>((p.Lk + kRows - 1) / kRows) * p.H * p.B;
   if (gq > 0x7fffffffll || gk > 0x7fffffffll) return WDIT_ERR_SHAPE;
   attn_dq_kernel<D, BF16><<<static_cast<unsigned>(gq), Bwd<D>::kThreads, smem, st>>>(big[0], small[1], small[2],
-                                                                                    big[3], p);
+                                                                                    big[3], out[0], p);
   if ((rc = cuda_rc(cudaGetLastError()))) return rc;
   attn_dkv_kernel<D, BF16><<<static_cast<unsigned>(gk), Bwd<D>::kThreads, smem, st>>>(big[1], big[2], small[0],
-                                                                                     small[3], p);
+                                                                                     small[3], out[1], out[2], p);
   if ((rc = cuda_rc(cudaGetLastError()))) return rc;
   return launch_rel_table_sum(p.table_part, p.B * q_tiles, buckets, p.H, dtable, st);
 }
@@ -1529,7 +1654,7 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
   if ((rc = error_record_ptr(&p.ctx.rec))) return rc;
   p.ctx.limit_ns = wait_limit_ns();
   const bool bf16 = dtype == 1;
-  CUtensorMap big[4], small[4];
+  CUtensorMap big[4], small[4], outs[3];
   const void* ptrs[4] = {q, k, v, dout};
   const long long* strides[4] = {q_strides, k_strides, v_strides, dout_strides};
   for (int i = 0; i < 4; ++i) {
@@ -1539,13 +1664,18 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
         (rc = map_heads(&small[i], bf16, ptrs[i], B, L, H, D, s, kCols)))
       return rc;
   }
+  void* const grads[3] = {dq, dk, dv};
+  for (int i = 0; i < 3; ++i) {
+    const int L = i == 0 ? Lq : Lk;
+    if ((rc = map_heads(&outs[i], bf16, grads[i], B, L, H, D, {1ll * L * H * D, 1ll * H * D, D}, 32))) return rc;
+  }
   const int buckets = rel_num_buckets(n_bounds, p.rb.bidirectional);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (D == 64)
-    return bf16 ? run_bwd<64, true>(big, small, p, buckets, dtable, st)
-                : run_bwd<64, false>(big, small, p, buckets, dtable, st);
-  return bf16 ? run_bwd<128, true>(big, small, p, buckets, dtable, st)
-              : run_bwd<128, false>(big, small, p, buckets, dtable, st);
+    return bf16 ? run_bwd<64, true>(big, small, outs, p, buckets, dtable, st)
+                : run_bwd<64, false>(big, small, outs, p, buckets, dtable, st);
+  return bf16 ? run_bwd<128, true>(big, small, outs, p, buckets, dtable, st)
+              : run_bwd<128, false>(big, small, outs, p, buckets, dtable, st);
 }
 
 }  // extern "C"

@@ -362,22 +362,7 @@ __global__ void __launch_bounds__(kRelThreads, VEC ? 2 : 3)
   }
   __syncthreads();
   for (int b = threadIdx.x; b < buckets; b += kRelThreads) {
-    float s = 0.f;
-    if (by_diag) {
-      // the bucket's distances [lo, hi], on its side of the diagonal
-      const int side = rb.n_bounds + 1;
-      const bool up = b >= side;
-      const int k = up ? b - side : b;
-      const int lo = k == 0 ? 0 : bounds[k - 1];
-      const int hi = k == rb.n_bounds ? reach : bounds[k] - 1;
-      if (up) {
-        for (int n = max(lo, 1); n <= hi; ++n) s += acc_b[reach + n];
-      } else {
-        for (int n = lo; n <= hi; ++n) s += acc_b[reach - n];
-      }
-    } else {
-      s = acc_b[b];
-    }
+    const float s = by_diag ? rel_bucket_sum(acc_b, reach, bounds, rb.n_bounds, b) : acc_b[b];
     part[(static_cast<size_t>(h) * gridDim.x + blockIdx.x) * buckets + b] = s;
   }
 }

@@ -51,6 +51,22 @@ __device__ __forceinline__ void add_buckets(float* acc, int bucket, float v, int
   __syncwarp();
 }
 
+// Sum of bucket b from sums by diagonal: sums[reach + d] for -reach <= d <= reach (bidirectional) or
+// <= 0, the ends holding everything past them; reach is the last bound.
+__device__ __forceinline__ float rel_bucket_sum(const float* sums, int reach, const int* bounds, int n_bounds, int b) {
+  const bool up = b > n_bounds;  // keys ahead of the query
+  const int k = up ? b - n_bounds - 1 : b;
+  const int lo = k == 0 ? 0 : bounds[k - 1];  // the bucket's distances
+  const int hi = k == n_bounds ? reach : bounds[k] - 1;
+  float s = 0.f;
+  if (up) {
+    for (int n = lo < 1 ? 1 : lo; n <= hi; ++n) s += sums[reach + n];
+  } else {
+    for (int n = lo; n <= hi; ++n) s += sums[reach - n];
+  }
+  return s;
+}
+
 __host__ __device__ inline int rel_num_buckets(int n_bounds, int bidirectional) { return (n_bounds + 1) * (bidirectional ? 2 : 1); }
 
 // Host check and copy of the caller's bounds; false = not ascending distances in 1 .. 2^29 (positions
