@@ -893,32 +893,45 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   for (int t = threadIdx.x; t < 8 * nsum; t += C::kThreads) sums[t] = 0.f;
   // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too: D / 8 lanes a row.
   {
-    constexpr int kLanes = D / 8, kAtOnce = C::kThreads / kLanes;
+    constexpr int kLanes = D / 8, kAtOnce = C::kThreads / kLanes, kTurns = (kRows + kAtOnce - 1) / kAtOnce;
     const int part = threadIdx.x % kLanes;
+    const uint16_t* go = static_cast<const uint16_t*>(p.dout) + b * p.do_b + h * p.do_h;
+    const uint16_t* oo = static_cast<const uint16_t*>(p.out) + (static_cast<long long>(b) * p.Lq * p.H + h) * D;
+    uint4 a[kTurns], c[kTurns];  // every row's loads are in flight together
 #pragma unroll
-    for (int r0 = 0; r0 < kRows; r0 += kAtOnce) {
-      const int r = r0 + threadIdx.x / kLanes;
-      const int i = i0 + r;
-      float s = 0.f;
+    for (int u = 0; u < kTurns; ++u) {
+      const int r = u * kAtOnce + threadIdx.x / kLanes;
+      const long long i = i0 + r;
+      a[u] = c[u] = make_uint4(0u, 0u, 0u, 0u);
       if (r < kRows && i < p.Lq) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.dout) + b * p.do_b +
-                                                             i * p.do_l + h * p.do_h) + part);
-        const uint4 c = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.out) +
-                                                             ((static_cast<long long>(b) * p.Lq + i) * p.H + h) * D) + part);
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
+        a[u] = __ldg(reinterpret_cast<const uint4*>(go + i * p.do_l) + part);
+        c[u] = __ldg(reinterpret_cast<const uint4*>(oo + i * p.H * D) + part);
+      }
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack16<BF16>(aw[e]), v = unpack16<BF16>(cw[e]);
-          s = fmaf(f.x, v.x, fmaf(f.y, v.y, s));
-        }
+    for (int u = 0; u < kTurns; ++u) {
+      const int r = u * kAtOnce + threadIdx.x / kLanes;
+      const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, cw[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack16<BF16>(aw[e]), v = unpack16<BF16>(cw[e]);
+        s = fmaf(f.x, v.x, fmaf(f.y, v.y, s));
       }
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (part == 0 && r < kRows) {
         sdelta[r] = s;
-        if (i < p.Lq) p.delta[(static_cast<long long>(b) * p.H + h) * p.Lq + i] = s;
+        if (i0 + r < p.Lq) p.delta[(static_cast<long long>(b) * p.H + h) * p.Lq + i0 + r] = s;
       }
     }
+  }
+  // this compute thread's row: its lse, loaded under the set-up too
+  float lse = kInf;
+  {
+    const int i = i0 + (warp & 3) * 32 + lane;
+    if (warp >= 2 && i < p.Lq) lse = p.lse[(static_cast<long long>(b) * p.H + h) * p.Lq + i];
+    if (lse == -kInf) lse = kInf;  // no keys: every P is 0
   }
   const BiasLine bias = load_bias(p, h, sdelta + kRows, C::kThreads);
   tc_fence_before();
@@ -996,9 +1009,6 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     float left = 0.f, right = 0.f;  // this row's share of the table's gradient past the last bounds
     const int row_end = !row_ok ? 0 : (p.causal ? min(klen, i + p.q_offset + 1) : klen);
     const int warp_first = i0 + wq * 32 + p.q_offset;
-    float lse = kInf;
-    if (row_ok) lse = p.lse[(static_cast<long long>(b) * p.H + h) * p.Lq + i];
-    if (lse == -kInf) lse = kInf;  // no keys: every P is 0
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     const uint64_t neg_delta = f2_pack(-sdelta[r], -sdelta[r]);
     // The warp's tiles by kind, as in the forward kernel, for its 32 columns of each tile.
@@ -1305,16 +1315,15 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     const bool key_ok = j < klen;
     const long long hbase = (static_cast<long long>(b) * p.H + h) * p.Lq;
-    // Row values of tile t for this lane: loaded a tile ahead.
+    // Row values of tile t for this lane: loaded a tile ahead, looked at when their tile begins.
+    // -inf: no such row, or one without keys; every P is 0.
     float next_lse = -kInf, next_delta = 0.f;
     auto load_rows = [&](int t) {
       const int i = (first + t) * kCols + half * 32 + lane;
-      next_lse = -kInf;  // (negated) no such row, or one without keys: every P is 0
-      next_delta = 0.f;
+      next_lse = -kInf;
       if (t < n && i < p.Lq) {
-        const float v = p.lse[hbase + i];
-        next_delta = -p.delta[hbase + i];
-        next_lse = v == -kInf ? -kInf : -v;
+        next_lse = p.lse[hbase + i];
+        next_delta = p.delta[hbase + i];
       }
     };
     load_rows(0);
@@ -1334,8 +1343,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const bool masked = !all_keys || t < t_causal || i_half + 32 > p.Lq;
       const bool flat = !masked && (t >= t_left || t < t_right);
       __syncwarp();
-      rowv[lane] = next_lse;
-      rowv[32 + lane] = next_delta;
+      rowv[lane] = next_lse == -kInf ? -kInf : -next_lse;
+      rowv[32 + lane] = -next_delta;
       if (!flat) {
         // diagonal of (key lane, query e): d_lo + 31 + lane - e
         const int d_lo = jw - pos - 31;
