@@ -43,7 +43,7 @@
 
 namespace wdit {
 
-int launch_rel_table_sum(const float* part, int parts, int buckets, int H, float* out, void* stream);
+int launch_rel_table_sum(const float* part, int parts, int buckets, int H, void* out, int dtype, void* stream);
 
 namespace {
 
@@ -1524,7 +1524,7 @@ int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, co
 
 template <int D, bool BF16>
 int run_bwd(const CUtensorMap (&big)[4], const CUtensorMap (&small)[4], const CUtensorMap (&out)[3], const AttnArgs& p,
-            int buckets, float* dtable, cudaStream_t st) {
+            int buckets, void* dtable, int dtable_dtype, cudaStream_t st) {
   // order of the maps: q, k, v, dO; dq, dk, dv
   static int done_q[64] = {}, done_kv[64] = {};
   const int smem = Bwd<D>::smem(p.rb);
@@ -1541,7 +1541,7 @@ int run_bwd(const CUtensorMap (&big)[4], const CUtensorMap (&small)[4], const CU
   attn_dkv_kernel<D, BF16><<<static_cast<unsigned>(gk), Bwd<D>::kThreads, smem, st>>>(big[1], big[2], small[0],
                                                                                      small[3], out[1], out[2], p);
   if ((rc = cuda_rc(cudaGetLastError()))) return rc;
-  return launch_rel_table_sum(p.table_part, p.B * q_tiles, buckets, p.H, dtable, st);
+  return launch_rel_table_sum(p.table_part, p.B * q_tiles, buckets, p.H, dtable, dtable_dtype, st);
 }
 
 long long align16(long long x) { return (x + 15) / 16 * 16; }
@@ -1620,12 +1620,14 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
                                 const long long* dout_strides, const void* out, const float* lse, int B, int H, int Lq,
                                 int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
                                 const int* bounds, int n_bounds, int bidirectional, int causal, int q_offset,
-                                float scale, void* dq, void* dk, void* dv, float* dtable, void* workspace,
+                                float scale, void* dq, void* dk, void* dv, void* dtable, int dtable_dtype,
+                                void* workspace,
                                 long long workspace_bytes, void* stream) {
   int rc = check_attn(bounds, n_bounds, B, H, Lq, Lk, D, dtype, table_dtype, q_offset, table);
   if (rc) return rc;
   if (B == 0 || Lq == 0 || Lk == 0) return WDIT_ERR_SHAPE;  // the caller knows the answer: zeros
-  if (out == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || dtable == nullptr)
+  if (out == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || dtable == nullptr ||
+      dtable_dtype < 0 || dtable_dtype > 2)
     return WDIT_ERR_ARG;
   for (const void* t : {out, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
     if ((reinterpret_cast<uintptr_t>(t) & 15) != 0) return WDIT_ERR_ALIGN;
@@ -1681,10 +1683,10 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
   const int buckets = rel_num_buckets(n_bounds, p.rb.bidirectional);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (D == 64)
-    return bf16 ? run_bwd<64, true>(big, small, outs, p, buckets, dtable, st)
-                : run_bwd<64, false>(big, small, outs, p, buckets, dtable, st);
-  return bf16 ? run_bwd<128, true>(big, small, outs, p, buckets, dtable, st)
-              : run_bwd<128, false>(big, small, outs, p, buckets, dtable, st);
+    return bf16 ? run_bwd<64, true>(big, small, outs, p, buckets, dtable, dtable_dtype, st)
+                : run_bwd<64, false>(big, small, outs, p, buckets, dtable, dtable_dtype, st);
+  return bf16 ? run_bwd<128, true>(big, small, outs, p, buckets, dtable, dtable_dtype, st)
+              : run_bwd<128, false>(big, small, outs, p, buckets, dtable, dtable_dtype, st);
 }
 
 }  // extern "C"

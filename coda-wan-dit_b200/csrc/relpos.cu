@@ -367,15 +367,26 @@ __global__ void __launch_bounds__(kRelThreads, VEC ? 2 : 3)
   }
 }
 
-// dtable[b, h] = sum over the CTAs' partial buckets, one thread each (a fixed order).
-__global__ void rel_table_sum_kernel(const float* __restrict__ part, int parts, int buckets, int H,
-                                     float* __restrict__ out) {
-  const int h = blockIdx.x;
-  for (int b = threadIdx.x; b < buckets; b += blockDim.x) {
-    const float* p = part + static_cast<size_t>(h) * parts * buckets + b;
-    float s = 0.f;
-    for (int x = 0; x < parts; ++x) s += p[static_cast<size_t>(x) * buckets];
-    out[static_cast<size_t>(b) * H + h] = s;
+// dtable[b, h] = sum over the CTAs' partial buckets, rounded once to dtype. A warp takes a bucket of
+// a head: lane l adds parts l, l + 32, ..., then the lanes are added (a fixed order).
+__global__ void __launch_bounds__(256)
+    rel_table_sum_kernel(const float* __restrict__ part, int parts, int buckets, int H, void* __restrict__ out,
+                         int dtype) {
+  const int b = blockIdx.x * 8 + (threadIdx.x >> 5), h = blockIdx.y, lane = threadIdx.x & 31;
+  if (b >= buckets) return;
+  const float* p = part + static_cast<size_t>(h) * parts * buckets + b;
+  float s = 0.f;
+  for (int x = lane; x < parts; x += 32) s += p[static_cast<size_t>(x) * buckets];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane != 0) return;
+  const size_t at = static_cast<size_t>(b) * H + h;
+  if (dtype == 0) {
+    static_cast<float*>(out)[at] = s;
+  } else if (dtype == 1) {
+    static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(s);
+  } else {
+    static_cast<__half*>(out)[at] = __float2half_rn(s);
   }
 }
 
@@ -457,8 +468,9 @@ int check_rel(const int* bounds, int n_bounds, int H, int Lq, int Lk, int q_offs
 
 }  // namespace
 
-int launch_rel_table_sum(const float* part, int parts, int buckets, int H, float* out, void* stream) {
-  rel_table_sum_kernel<<<H, 128, 0, static_cast<cudaStream_t>(stream)>>>(part, parts, buckets, H, out);
+int launch_rel_table_sum(const float* part, int parts, int buckets, int H, void* out, int dtype, void* stream) {
+  rel_table_sum_kernel<<<dim3((buckets + 7) / 8, H), 256, 0, static_cast<cudaStream_t>(stream)>>>(part, parts, buckets,
+                                                                                                 H, out, dtype);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e);
 }
@@ -493,15 +505,15 @@ long long wdit_rel_pos_bias_grad_workspace_bytes(int B, int H, int Lq, int Lk, i
 
 int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, int Lk, long long stride_b,
                            long long stride_h, long long stride_i, const int* bounds, int n_bounds, int bidirectional,
-                           int q_offset, float* dtable, void* workspace, long long workspace_bytes, void* stream) {
+                           int q_offset, void* dtable, int dtable_dtype, void* workspace, long long workspace_bytes, void* stream) {
   int rc = check_rel(bounds, n_bounds, H, Lq, Lk, q_offset, dtype);
   if (rc) return rc;
   if (B < 0) return WDIT_ERR_SHAPE;
-  if (dtable == nullptr) return WDIT_ERR_ARG;
+  if (dtable == nullptr || dtable_dtype < 0 || dtable_dtype > 2) return WDIT_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int buckets = rel_num_buckets(n_bounds, bidirectional);
   if (B == 0 || Lq == 0 || Lk == 0) {  // no cells: a zero gradient
-    const cudaError_t e = cudaMemsetAsync(dtable, 0, static_cast<size_t>(buckets) * H * 4, st);
+    const cudaError_t e = cudaMemsetAsync(dtable, 0, static_cast<size_t>(buckets) * H * (dtable_dtype == 0 ? 4 : 2), st);
     return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e);
   }
   if (dbias == nullptr) return WDIT_ERR_ARG;
@@ -524,7 +536,7 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
   rc = dtype == 0 ? go(static_cast<float*>(nullptr))
                   : (dtype == 1 ? go(static_cast<__nv_bfloat16*>(nullptr)) : go(static_cast<__half*>(nullptr)));
   if (rc) return rc;
-  return launch_rel_table_sum(part, parts, buckets, H, dtable, stream);
+  return launch_rel_table_sum(part, parts, buckets, H, dtable, dtable_dtype, stream);
 }
 
 }  // extern "C"

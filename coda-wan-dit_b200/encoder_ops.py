@@ -140,10 +140,11 @@ def _rel_pos_bias(table, q_len, k_len, bidirectional, max_distance, q_offset):
 
 
 def rel_pos_bias_grad(dbias: torch.Tensor, num_buckets: int, *, bidirectional: bool = True, max_distance: int = 128,
-                      q_offset: int = 0) -> torch.Tensor:
-    """Gradient of rel_pos_bias's table: dtable [num_buckets, H] fp32, the sum of the cells of
-    dbias ([H, Lq, Lk], or [B, H, Lq, Lk] summed over the batch the bias was broadcast to; fp32,
-    bf16 or fp16) by their bucket. Sums are fp32 in a fixed order: results repeat bit for bit."""
+                      q_offset: int = 0, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Gradient of rel_pos_bias's table: dtable [num_buckets, H], the sum of the cells of dbias
+    ([H, Lq, Lk], or [B, H, Lq, Lk] summed over the batch the bias was broadcast to; fp32, bf16
+    or fp16) by their bucket. Sums are fp32 in a fixed order (results repeat bit for bit) and
+    rounded once to dtype (fp32, bf16 or fp16)."""
     dev = _require_cuda(dbias)
     if dbias.dim() == 3:
         dbias = dbias.unsqueeze(0)
@@ -151,6 +152,8 @@ def rel_pos_bias_grad(dbias: torch.Tensor, num_buckets: int, *, bidirectional: b
         raise ValueError(f"dbias must be [H, Lq, Lk] or [B, H, Lq, Lk], got {tuple(dbias.shape)}")
     if dbias.dtype not in _DTYPE:
         raise ValueError(f"dbias must be fp32, bf16 or fp16, got {dbias.dtype}")
+    if dtype not in _DTYPE:
+        raise ValueError(f"dtype must be fp32, bf16 or fp16, got {dtype}")
     B, H, Lq, Lk = dbias.shape
     if H < 1:
         raise ValueError("dbias has no heads")
@@ -159,12 +162,12 @@ def rel_pos_bias_grad(dbias: torch.Tensor, num_buckets: int, *, bidirectional: b
     with _on_device(dev):
         if Lk > 1 and dbias.stride(3) != 1:
             dbias = dbias.contiguous()
-        out = torch.empty((num_buckets, H), dtype=torch.float32, device=dbias.device)
+        out = torch.empty((num_buckets, H), dtype=dtype, device=dbias.device)
         nbytes = _workspace_bytes(dev, "wdit_rel_pos_bias_grad_workspace_bytes", B, H, Lq, Lk, n, int(bidirectional))
         ws = _workspace(nbytes, dbias.device)
         sb, sh, si, _ = dbias.stride()
         call("wdit_rel_pos_bias_grad", dbias.data_ptr(), _DTYPE[dbias.dtype], B, H, Lq, Lk, sb, sh, si, bounds, n,
-             bidirectional, q_offset, out.data_ptr(), ptr(ws), nbytes, _stream(dev), kernels=2)
+             bidirectional, q_offset, out.data_ptr(), _DTYPE[dtype], ptr(ws), nbytes, _stream(dev), kernels=2)
     return out
 
 
@@ -179,8 +182,8 @@ class _RelPosBias(torch.autograd.Function):
     def backward(ctx, dbias):
         num_buckets, dtype, bidirectional, max_distance, q_offset = ctx.args
         dtable = rel_pos_bias_grad(dbias, num_buckets, bidirectional=bidirectional, max_distance=max_distance,
-                                   q_offset=q_offset)
-        return dtable.to(dtype), None, None, None, None, None
+                                   q_offset=q_offset, dtype=dtype)
+        return dtable, None, None, None, None, None
 
 
 def rel_pos_bias(table: torch.Tensor, q_len: int, k_len: int, *, bidirectional: bool = True, max_distance: int = 128,
@@ -421,16 +424,20 @@ class _RelPosAttention(torch.autograd.Function):
         dev = q.get_device()
         with _on_device(dev):
             g = _heads(dout)
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-            dtable = torch.empty(table.shape, dtype=torch.float32, device=table.device)
+            device = q.device
+            dq = torch.empty(q.shape, dtype=q.dtype, device=device)
+            dk = torch.empty(k.shape, dtype=q.dtype, device=device)
+            dv = torch.empty(k.shape, dtype=q.dtype, device=device)
+            dtable = torch.empty(table.shape, dtype=table.dtype, device=device)
             shape, pos = _attention_args(q, k, table, k_lens, *ctx.args)
             nbytes = _workspace_bytes(dev, "wdit_rel_attention_backward_workspace_bytes", *shape[:3], pos[5],
                                       int(pos[6]))
-            ws = _workspace(nbytes, q.device)
-            call("wdit_rel_attention_backward", ptr(q), _strides(q), ptr(k), _strides(k), ptr(v), _strides(v), ptr(g),
-                 _strides(g), ptr(out), ptr(lse), *shape, *pos, ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws), nbytes,
+            ws = _workspace(nbytes, device)
+            call("wdit_rel_attention_backward", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(),
+                 _strides(v), g.data_ptr(), _strides(g), out.data_ptr(), lse.data_ptr(), *shape, *pos, dq.data_ptr(),
+                 dk.data_ptr(), dv.data_ptr(), dtable.data_ptr(), _DTYPE[table.dtype], ws.data_ptr(), nbytes,
                  _stream(dev), kernels=3)
-        return (dq, dk, dv, dtable.to(table.dtype), *nothing)
+        return (dq, dk, dv, dtable, *nothing)
 
 
 def rel_pos_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, *,

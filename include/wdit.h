@@ -321,13 +321,14 @@ int wdit_rope_table(const double* freqs_ri, int max_pos, int f, int h, int w, in
 int wdit_rel_pos_bias(const void* table, int dtype, const int* bounds, int n_bounds, int bidirectional, int H, int Lq,
                       int Lk, int q_offset, void* out, void* stream);
 
-/* Gradient of the table: dtable[buckets, H] (fp32) = sum of dbias[b, h, i, j] over b, i, j by
+/* Gradient of the table: dtable[buckets, H] (of dtable_dtype) = sum of dbias[b, h, i, j] over b, i, j by
  * bucket. dbias of dtype with element strides (>= 0) for b, h, i and unit stride for j. The
  * workspace needs no initialization. Two launches; sums are fp32 in a fixed order. */
 long long wdit_rel_pos_bias_grad_workspace_bytes(int B, int H, int Lq, int Lk, int n_bounds, int bidirectional);
 int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, int Lk, long long stride_b,
                            long long stride_h, long long stride_i, const int* bounds, int n_bounds, int bidirectional,
-                           int q_offset, float* dtable, void* workspace, long long workspace_bytes, void* stream);
+                           int q_offset, void* dtable, int dtable_dtype, void* workspace, long long workspace_bytes,
+                           void* stream);
 
 /*
  * Attention with that bias: out[B, Lq, H, D] (contiguous) = softmax(scale q k^T + table[bucket, h]) v.
@@ -348,7 +349,7 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
 
 /*
  * Its gradients: dq [B, Lq, H, D], dk, dv [B, Lk, H, D] (contiguous, dtype; 0 for keys past
- * k_lens) and dtable [buckets, H] (fp32). out and lse are the forward's. Three launches, no atomics:
+ * k_lens) and dtable [buckets, H] (of dtable_dtype). out and lse are the forward's. Three launches, no atomics:
  * sums have a fixed order. Empty dimensions are WDIT_ERR_SHAPE (the results are zeros).
  */
 long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional);
@@ -357,7 +358,7 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
                                 const long long* dout_strides, const void* out, const float* lse, int B, int H, int Lq,
                                 int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
                                 const int* bounds, int n_bounds, int bidirectional, int causal, int q_offset,
-                                float scale, void* dq, void* dk, void* dv, float* dtable, void* workspace,
+                                float scale, void* dq, void* dk, void* dv, void* dtable, int dtable_dtype, void* workspace,
                                 long long workspace_bytes, void* stream);
 
 /*

@@ -75,11 +75,11 @@ def test_rel_pos_entry_points_validate_without_device(pkg):
     assert bias(out=ctypes.c_void_p(0x1008)) == 3
     assert bias(table=null, out=null, Lq=0) == 0 and bias(table=null, out=null, Lk=0) == 0
 
-    def grad(db=d, dtype=0, B=1, H=2, Lq=4, Lk=4, sb=32, b=bounds, n=3, off=0, out=d, ws=d, nbytes=1 << 20):
-        return lib.wdit_rel_pos_bias_grad(db, dtype, B, H, Lq, Lk, sb, 16, 4, b, n, 1, off, out, ws, nbytes, null)
+    def grad(db=d, dtype=0, B=1, H=2, Lq=4, Lk=4, sb=32, b=bounds, n=3, off=0, out=d, ddt=0, ws=d, nbytes=1 << 20):
+        return lib.wdit_rel_pos_bias_grad(db, dtype, B, H, Lq, Lk, sb, 16, 4, b, n, 1, off, out, ddt, ws, nbytes, null)
 
     assert grad(db=null) == 1 and grad(out=null) == 1 and grad(b=None) == 1 and grad(dtype=-1) == 1
-    assert grad(b=down) == 1
+    assert grad(b=down) == 1 and grad(ddt=3) == 1
     assert grad(n=0) == 2 and grad(B=-1) == 2 and grad(sb=-32) == 2
     assert grad(ws=null) == 5 and grad(nbytes=4) == 5
     assert grad(ws=ctypes.c_void_p(0x1004)) == 3
@@ -189,11 +189,12 @@ def test_attention_entry_points_validate_without_device(pkg):
     assert fwd(B=1, H=1, Lq=1, Lk=4096, ws=d, nb=need - 1) == 5
     assert lib.wdit_rel_attention_workspace_bytes(64, 64, 512, 512, 64) == 0
 
-    def back(lse=d, out=d, dq=d, dt=d, ws=d, nb=1 << 30, Lq=5, Lk=5, gs=st):
+    def back(lse=d, out=d, dq=d, dt=d, ddt=0, ws=d, nb=1 << 30, Lq=5, Lk=5, gs=st):
         return lib.wdit_rel_attention_backward(d, st, d, st, d, st, d, gs, out, lse, 2, 3, Lq, Lk, 64, 1, null, d, 0,
-                                               bounds, 3, 1, 0, 0, 1.0, dq, d, d, dt, ws, nb, null)
+                                               bounds, 3, 1, 0, 0, 1.0, dq, d, d, dt, ddt, ws, nb, null)
 
     assert back(lse=null) == 1 and back(out=null) == 1 and back(dq=null) == 1 and back(dt=null) == 1
+    assert back(ddt=-1) == 1
     assert back(Lq=0) == 2 and back(Lk=0) == 2 and back(gs=zero) == 2 and back(gs=bad) == 3
     assert back(dq=ctypes.c_void_p(0x1004)) == 3
     assert back(ws=null) == 5 and back(nb=16) == 5

@@ -109,6 +109,16 @@ def test_gradient_takes_views(pkg, make):
     assert ((got - want).abs() <= 2 * 1024 * U32 * size).all()  # the two may add in another order
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradient_is_rounded_once_to_the_type_asked_for(pkg, dtype):
+    db = torch.randn(2, 3, 70, 90, generator=torch.Generator().manual_seed(5)).to(DEV)
+    got = pkg.ops.rel_pos_bias_grad(db, 32, dtype=dtype)
+    assert got.dtype == dtype
+    assert torch.equal(got, pkg.ops.rel_pos_bias_grad(db, 32).to(dtype))
+    none = pkg.ops.rel_pos_bias_grad(db[:, :, :0], 32, dtype=dtype)
+    assert none.dtype == dtype and none.shape == (32, 3) and not none.any()
+
+
 def test_gradient_of_no_cells_is_zero(pkg):
     for shape in [(0, 2, 5, 6), (2, 2, 0, 6), (2, 2, 5, 0)]:
         got = pkg.ops.rel_pos_bias_grad(torch.empty(shape, device=DEV), 32)
