@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (lane == 0) bulk_wait_all<0>();
+    if (lane == 0) bulk_wait_read<0>();  // the stores have read shared memory
     __syncwarp();
   }
   if constexpr (SPLIT) {

@@ -19,9 +19,9 @@
 // registers and written back to TMEM in 16 bits as the A operand of the next product, so nothing
 // of size Lq x Lk leaves the SM.
 //
-//   attn_fwd_kernel  CTA = 128 query rows of one head; key tiles of 64; warp 0 loads, warp 1
-//                    issues MMAs, warps 2-5 softmax (one row per thread). With few
-//                    CTAs the keys are split over several, whose parts attn_combine_kernel joins.
+//   attn_fwd_kernel  CTA = 128 query rows of one head; key tiles of 64; one or two warps load and
+//                    issue MMAs, four are the softmax (one row per thread). With few CTAs the
+//                    keys are split over several, whose parts attn_combine_kernel joins.
 //   attn_dq_kernel   same rows; computes delta, dQ and the table's partial sums. No atomics.
 //   attn_dkv_kernel  CTA = 128 keys; runs over query tiles of 64 with the scores transposed, so
 //                    P^T and dS^T are the A operands; dK and dV stay in TMEM.
@@ -301,21 +301,26 @@ __device__ __forceinline__ int sample_len(const AttnArgs& p, int b) {
 // ---------------------------------------------------------------------------
 // Forward
 // ---------------------------------------------------------------------------
-// Six warps, two CTAs per SM. Warps 2-5 are the softmax, one row per thread: warp w reads TMEM lanes
-// [32 (w % 4), + 32). Two score buffers: the scores of t + 1 are computed while those of t are
-// exponentiated, so the softmax never waits for a product.
+// Four softmax warps, one row per thread: warp w reads TMEM lanes [32 (w % 4), + 32). NB = 2: two CTAs
+// per SM with two score buffers each; the scores of t + 1 are computed while those of t are
+// exponentiated, so the softmax never waits for a product. One more warp loads, another issues
+// MMAs. NB = 1 (D = 64): four CTAs per SM with one buffer each (128 TMEM columns, 96 registers a
+// thread) and one warp that loads and issues; a CTA's products and softmax take turns, and the
+// CTAs fill each other's gaps, starts and ends.
 //
 // The maximum in use is that of the row's first tile. Later tiles are exponentiated against it
 // without looking for theirs; only when a tile's sum passes kSumLimit is the maximum taken anew,
 // O rescaled and the tile done again. 16-bit P keeps its relative precision up to there (fp16 up
 // to 2^15 of its 65504, bf16 far beyond), and the sums are fp32.
-template <int D>
+template <int D, int NB>
 struct Fwd {
-  static constexpr int kStages = D == 64 ? 4 : 2;
-  static constexpr int kThreads = 192;
+  static constexpr int kCtas = NB == 1 ? 4 : 2;     // per SM
+  static constexpr int kControl = NB == 1 ? 1 : 2;  // warps that load and issue
+  static constexpr int kStages = D == 64 && NB == 2 ? 4 : 2;
+  static constexpr int kThreads = 32 * (kControl + 4);
   static constexpr uint32_t kQ = kRows * D * 2;
   static constexpr uint32_t kTile = kCols * D * 2;
-  static constexpr uint32_t kTmem = 256;  // two score buffers of 64 columns, O at 128
+  static constexpr uint32_t kTmem = NB == 1 ? 128 : 256;  // score buffers of 64 columns, then O
   static constexpr int kLine = 96;        // per-warp bias line (31 + 64 diagonals)
   static int smem(const RelBuckets& rb) { return 1024 + kQ + kStages * 2 * kTile + 256 + 4 * kLine * 4 + bias_smem(rb); }
 };
@@ -347,12 +352,12 @@ __device__ __forceinline__ FwdPlace fwd_place(const AttnArgs& p, int q_tiles) {
   return f;
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
+template <int D, bool BF16, int NB>
+__global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmOut,
                     const __grid_constant__ AttnArgs p) {
-  using C = Fwd<D>;
+  using C = Fwd<D, NB>;
   constexpr int ST = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     }
   }
   __syncwarp();
-  if (warp == 1) {
+  if (warp == C::kControl - 1) {
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
@@ -440,9 +445,9 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tmem_o = tmem + 2 * kCols;
+  const uint32_t tmem_o = tmem + NB * kCols;
 
-  if (warp == 0) {
+  if (NB == 2 && warp == 0) {
     if (elect_one() && n > 0) {
       int k_loaded = min(n, ST), v_loaded = k_loaded;
       for (int t = ST; t < n; ++t) {
@@ -462,7 +467,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
         wait_parity(&v_full[t % ST], (t / ST) & 1, kSiteAttn + 2, p.ctx);
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp == C::kControl - 1) {
     constexpr uint32_t id_s = idesc16(kRows, kCols, BF16, false);
     constexpr uint32_t id_o = idesc16(kRows, D, BF16, true);
     auto scores = [&](int t) {
@@ -471,20 +476,21 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
       if (elect_one()) {
-        issue_scores<D, kCols>(tmem + (t & 1) * kCols, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
-        mma_commit(&k_empty[st]);
-        mma_commit(&s_full[t & 1]);
+        issue_scores<D, kCols>(tmem + (t % NB) * kCols, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
+        if (NB == 2) mma_commit(&k_empty[st]);
+        mma_commit(&s_full[t % NB]);
       }
       __syncwarp();
       return true;
     };
     bool ok = true;
+    int loaded = min(n, ST);
     if (n > 0) {
       ok = wait_parity(q_full, 0, kSiteAttn + 4, p.ctx);
       ok = __all_sync(0xffffffffu, ok) && scores(0);
     }
     for (int t = 0; t < n && ok; ++t) {
-      if (t + 1 < n) {
+      if (NB == 2 && t + 1 < n) {
         // scores(t + 1) overwrite the buffer whose P the product of t - 1 reads: products into
         // different accumulators are ordered by their completion only
         if (t > 0) ok = __all_sync(0xffffffffu, wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 10, p.ctx));
@@ -495,16 +501,38 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       const int j0 = (t0 + t) * kCols;
       if (j0 + kCols > klen) zero_tail<D, kCols>(sV + st * C::kTile, klen - j0, lane);
-      ok = wait_parity(&p_ready[t & 1], (t >> 1) & 1, kSiteAttn + 6, p.ctx);
+      ok = wait_parity(&p_ready[t % NB], (t / NB) & 1, kSiteAttn + 6, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       if (elect_one()) {
-        issue_ts<kCols>(tmem_o, tmem + (t & 1) * kCols, smem_u32(sV + st * C::kTile), id_o, t > 0);
-        mma_commit(&v_empty[st]);
+        issue_ts<kCols>(tmem_o, tmem + (t % NB) * kCols, smem_u32(sV + st * C::kTile), id_o, t > 0);
+        if (NB == 2) mma_commit(&v_empty[st]);
         mma_commit(pv_done);
         if (t + 1 == n) mma_commit(last);
       }
       __syncwarp();
+      if (NB == 1 && t + 1 < n) {
+        // the next scores take the place of the P that this product reads; its tiles are free too
+        ok = __all_sync(0xffffffffu, wait_parity(pv_done, t & 1, kSiteAttn + 10, p.ctx));
+        if (!ok || !scores(t + 1)) break;
+        if (t + ST < n) {
+          if (elect_one()) {
+            load_k(t + ST);
+            load_v(t + ST);
+          }
+          __syncwarp();
+          loaded = t + ST + 1;
+        }
+      }
+    }
+    // Do not leave while a copy into this CTA's shared memory is in flight: all that was loaded has
+    // been waited for unless a wait ran out.
+    if (NB == 1 && !ok) {
+      wait_parity(q_full, 0, kSiteAttn + 2, p.ctx);
+      for (int t = max(0, loaded - ST); t < loaded; ++t) {
+        wait_parity(&k_full[t % ST], (t / ST) & 1, kSiteAttn + 2, p.ctx);
+        wait_parity(&v_full[t % ST], (t / ST) & 1, kSiteAttn + 2, p.ctx);
+      }
     }
   } else {
     const int wq = warp & 3;
@@ -529,7 +557,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
     const float c_left = bias.at(-bias.reach), c_right = bias.at(bias.reach);
     for (int t = 0; t < n; ++t) {
       const int j0 = (t0 + t) * kCols;
-      const uint32_t ts = tmem + lane_off + (t & 1) * kCols;
+      const uint32_t ts = tmem + lane_off + (t % NB) * kCols;
       const bool masked = t >= t_mask;
       const bool flat = !masked && (t < t_left || t >= t_right);
       const float flat_c = t < t_left ? c_left : c_right;
@@ -542,10 +570,10 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
         __syncwarp();
       }
       const float* ln = line + 31 - lane;
-      ok = wait_parity(&s_full[t & 1], (t >> 1) & 1, kSiteAttn + 7, p.ctx);
+      ok = wait_parity(&s_full[t % NB], (t / NB) & 1, kSiteAttn + 7, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       if (idle) {
-        if (lane == 0) mbar_arrive(&p_ready[t & 1]);
+        if (lane == 0) mbar_arrive(&p_ready[t % NB]);
         continue;
       }
       tc_fence_after();
@@ -557,21 +585,30 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
         const float m = m_used == -kInf ? 0.f : m_used;
         const uint64_t sub = decltype(is_flat)::value ? f2_pack(flat_c - m, flat_c - m) : f2_pack(-m, -m);
         uint64_t s2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-        uint32_t raw[2][32];
-        tmem_ld32_nowait(ts, raw[0]);
-        tmem_ld32_nowait(ts + 32, raw[1]);
-        tmem_wait_ld(raw[0]);
+        // two CTAs per SM leave the registers to load both halves at once
+        constexpr int HELD = NB == 2 ? 2 : 1;
+        uint32_t raw[HELD][32];
+        if constexpr (HELD == 2) {
+          tmem_ld32_nowait(ts, raw[0]);
+          tmem_ld32_nowait(ts + 32, raw[1]);
+          tmem_wait_ld(raw[0]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(raw[1][e]));
+          for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(raw[1][e]));
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if constexpr (HELD == 1) {
+            tmem_ld32_nowait(ts + c * 32, raw[0]);
+            tmem_wait_ld(raw[0]);
+          }
+          uint32_t* r = raw[c % HELD];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             uint64_t add = sub;
             if constexpr (!decltype(is_flat)::value)
               add = fadd2(f2_pack(ln[c * 32 + 2 * e], ln[c * 32 + 2 * e + 1]), sub);
             float x, y;
-            f2_unpack(ffma2(f2_pack(__uint_as_float(raw[c][2 * e]), __uint_as_float(raw[c][2 * e + 1])), scale2, add),
+            f2_unpack(ffma2(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), scale2, add),
                       x, y);
             if constexpr (decltype(is_masked)::value) {
               x = c * 32 + 2 * e < keep ? x : -kInf;
@@ -639,7 +676,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t & 1]);
+      if (lane == 0) mbar_arrive(&p_ready[t % NB]);
     }
     if (ok && n > 0) {
       ok = wait_parity(last, 0, kSiteAttn + 9, p.ctx);
@@ -697,7 +734,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
             tma_store_4d(&tmOut, stage + c * 16384, c * 64, h, i0 + wq * 32, b);
         }
         bulk_commit();
-        bulk_wait_all<0>();
+        bulk_wait_read<0>();  // the stores have read shared memory
       }
       __syncwarp();
     }
@@ -705,7 +742,7 @@ __global__ void __launch_bounds__(Fwd<D>::kThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, C::kTmem);
+  if (warp == C::kControl - 1) tmem_dealloc(tmem, C::kTmem);
 }
 
 // out = sum_s 2^(lse_s - lse) part_o[s], lse = log2 sum_s 2^lse_s: one warp per row.
@@ -1141,7 +1178,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     if (half < D / 64) {
       store_rows64<BF16>(&tmOut, sQ + half * 16384 + wq * 4096, tmem_acc + lane_off + half * 64, n > 0 && ok, false,
                          p.scale, lane, half * 64, h, i0 + wq * 32, b, i0 + wq * 32 < p.Lq);
-      if (lane == 0) bulk_wait_all<0>();
+      if (lane == 0) bulk_wait_read<0>();
     }
     __syncwarp();
   }
@@ -1423,7 +1460,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       store_rows64<BF16>(half == 0 ? &tmDv : &tmDk, (half == 0 ? sV : sK) + c * 16384 + wq * 4096,
                          (half == 0 ? tmem_dv : tmem_dk) + lane_off + c * 64, n > 0 && ok, !key_ok,
                          half == 0 ? 1.f : p.scale, lane, c * 64, h, jw, b, jw < p.Lk);
-    if (lane == 0) bulk_wait_all<0>();
+    if (lane == 0) bulk_wait_read<0>();
     __syncwarp();
   }
   tc_fence_before();
@@ -1454,6 +1491,17 @@ int attn_splits(int B, int H, int Lq, int Lk) {
   long long s = 2ll * attn_sms() / ctas;
   if (s > tiles / 4) s = tiles / 4;
   return s < 1 ? 1 : (s > 64 ? 64 : static_cast<int>(s));
+}
+
+// Which forward of D = 64: four CTAs per SM with one score buffer each, or two with two. Four win
+// where the CTAs outnumber two per SM and a CTA's start and end weigh (us, two / four per SM, 64
+// heads bidirectional: 2 x 512 x 512 29.7 / 27.0, 8 x 512 x 512 97 / 86; causal 8 x 512 x 512 81.6 /
+// 64.8; 80 x 12 heads x 77 x 77 29.9 / 23.0; 148 heads x 512 x 2048 72.6 / 70.6). Two win where
+// there are no more CTAs than that (74 heads x 512 x 512 16.2 / 19.6) and on long keys, whose one
+// CTA then walks twice as fast (12 heads x 8192 x 8192 337 / 355, causal 4096 x 4096 61 / 81).
+bool four_per_sm(const AttnArgs& p) {
+  const long long ctas = static_cast<long long>(p.B) * p.H * ((p.Lq + kRows - 1) / kRows);
+  return ctas > 2ll * attn_sms() && p.Lk <= 2048;
 }
 
 struct Strides {
@@ -1505,16 +1553,16 @@ int set_smem(K kernel, int bytes, int (&done)[64]) {
   return WDIT_OK;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, int NB>
 int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, const AttnArgs& p,
             cudaStream_t st) {
   static int done[64] = {};
-  const int smem = Fwd<D>::smem(p.rb);
-  int rc = set_smem(attn_fwd_kernel<D, BF16>, smem, done);
+  const int smem = Fwd<D, NB>::smem(p.rb);
+  int rc = set_smem(attn_fwd_kernel<D, BF16, NB>, smem, done);
   if (rc) return rc;
   const long long grid = static_cast<long long>((p.Lq + kRows - 1) / kRows) * p.splits * p.H * p.B;
   if (grid > 0x7fffffffll) return WDIT_ERR_SHAPE;
-  attn_fwd_kernel<D, BF16><<<static_cast<unsigned>(grid), Fwd<D>::kThreads, smem, st>>>(q, k, v, o, p);
+  attn_fwd_kernel<D, BF16, NB><<<static_cast<unsigned>(grid), Fwd<D, NB>::kThreads, smem, st>>>(q, k, v, o, p);
   rc = cuda_rc(cudaGetLastError());
   if (rc || p.splits == 1) return rc;
   const long long rows = static_cast<long long>(p.B) * p.H * p.Lq;
@@ -1604,9 +1652,11 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
       (rc = map_heads(&mo, bf16, out, B, Lq, H, D, {1ll * Lq * H * D, 1ll * H * D, D}, 32)))
     return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (D == 64)
-    return bf16 ? run_fwd<64, true>(mq, mk, mv, mo, p, st) : run_fwd<64, false>(mq, mk, mv, mo, p, st);
-  return bf16 ? run_fwd<128, true>(mq, mk, mv, mo, p, st) : run_fwd<128, false>(mq, mk, mv, mo, p, st);
+  if (D == 128)
+    return bf16 ? run_fwd<128, true, 2>(mq, mk, mv, mo, p, st) : run_fwd<128, false, 2>(mq, mk, mv, mo, p, st);
+  if (four_per_sm(p))
+    return bf16 ? run_fwd<64, true, 1>(mq, mk, mv, mo, p, st) : run_fwd<64, false, 1>(mq, mk, mv, mo, p, st);
+  return bf16 ? run_fwd<64, true, 2>(mq, mk, mv, mo, p, st) : run_fwd<64, false, 2>(mq, mk, mv, mo, p, st);
 }
 
 long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional) {

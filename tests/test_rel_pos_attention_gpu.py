@@ -201,6 +201,22 @@ def test_large_scores_and_masked_buckets(pkg):
     assert (got[0, 0, 1] == 0).all() and not got.isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Lq,Lk", [(5, 31, 300, 300), (3, 110, 130, 77), (330, 1, 1, 500), (2, 100, 257, 1)])
+def test_more_ctas_than_two_per_sm(pkg, B, H, Lq, Lk, dtype):
+    q, k, v, table = make(B, H, Lq, Lk, 64, dtype, seed=16)
+    k = (k * torch.linspace(0.1, 12, Lk, device=DEV)[None, :, None, None]).to(dtype)  # the maximum moves
+    lens = torch.tensor([[Lk, 0, Lk // 2, 65, 64][b % 5] for b in range(B)], dtype=torch.int32, device=DEV)
+    for kw in (dict(k_lens=lens), dict(causal=True, bidirectional=False, q_offset=max(0, Lk - Lq)),
+               dict(k_lens=lens, causal=True, q_offset=7, scale=0.4)):
+        want = pkg.ops.rel_pos_attention(q, k, v, table, **kw)
+        check(want, q, k, v, table, **kw)
+        if "k_lens" in kw:
+            behind = (torch.arange(Lk, device=DEV)[None] >= lens[:, None])[..., None, None]
+            k2, v2 = k.masked_fill(behind, float("nan")), v.masked_fill(behind, float("inf"))
+            assert torch.equal(pkg.ops.rel_pos_attention(q, k2, v2, table, **kw), want)
+
+
 def test_flat_scores(pkg):
     q, k, v, table = make(1, 1, 64, 3000, 128, torch.float16, seed=7)
     q.zero_(), table.zero_()
