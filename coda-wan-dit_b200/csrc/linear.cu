@@ -53,6 +53,7 @@ constexpr uint32_t kEpiBytes = 8 * (kWarpBytes + 32 * 4);  // ... and a line of 
 constexpr uint32_t kBarBytes = 512;
 constexpr uint32_t kSmemLimit = 232448;
 constexpr uint32_t kRingBudget = kSmemLimit - 1024 - kBarBytes - kEpiBytes;
+constexpr int kMaxExtent = 1 << 30;  // M, N, K: coordinates past a matrix's end stay inside 32 bits
 constexpr int kRasterRows = 8;
 constexpr long long kRasterBytes = 64ll << 20;
 
@@ -501,18 +502,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       n0 = n_blk * p.bn + c * 32;
       return row0 < p.M && n0 < p.N;
     };
+    int in_flight = -1;  // lane 0: buffer of the last residual piece asked for
     auto fetch_res = [&](int it, int c, int buf) {  // lane 0
       int row0, n0;
       if (!piece_at(it, c, row0, n0)) return;
       mbar_arrive_expect_tx(&rbar[buf], kPieceBytes);
       tma_load_2d(bufs + buf * kPieceBytes, &tmRes, &rbar[buf], n0, row0);
+      in_flight = buf;
     };
     if (has_res && lane == 0 && my_count > 0) fetch_res(0, half, 0);
-    for (int it = 0; it < my_count; ++it) {
+    bool failed = false;
+    for (int it = 0; it < my_count && !failed; ++it) {
       const int buf = it & 1;
       const uint32_t tphase = (it >> 1) & 1;
-      bool ok = wait_parity<PAIR>(&tfull_bar[buf], tphase, kSiteEpiTmemFull, p.ctx);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      failed = !__all_sync(0xffffffffu, wait_parity<PAIR>(&tfull_bar[buf], tphase, kSiteEpiTmemFull, p.ctx));
+      if (failed) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + lane_off + buf * 256;
 #pragma unroll 1
@@ -586,8 +590,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             apply_act<32>(v, p.act);
             uint8_t* mine = bufs + cur * kPieceBytes;
             if (has_res) {
-              ok = wait_parity(&rbar[cur], (rphase >> cur) & 1u, kSiteEpiCLoad, p.ctx);
-              if (!__all_sync(0xffffffffu, ok)) break;
+              failed = !__all_sync(0xffffffffu, wait_parity(&rbar[cur], (rphase >> cur) & 1u, kSiteEpiCLoad, p.ctx));
+              if (failed) break;
               rphase ^= 1u << cur;
               const uint32_t row = smem_u32(mine) + lane * 64;
 #pragma unroll
@@ -608,7 +612,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (lane == 0) bulk_wait_read<0>();  // the stores have read shared memory
+    if (lane == 0) {
+      bulk_wait_read<0>();  // the stores have read shared memory
+      // After a wait that ran out the last residual piece may still be on its way.
+      if (failed && in_flight >= 0) wait_parity(&rbar[in_flight], (rphase >> in_flight) & 1u, kSiteDrain, p.ctx);
+    }
     __syncwarp();
   }
   if constexpr (SPLIT) {
@@ -680,8 +688,11 @@ __global__ void __launch_bounds__(256)
                         float* __restrict__ part, int M, int N) {
   __shared__ float sums[8][kBackCols];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = blockIdx.x * kBackCols + lane * 8;
-  const int m0 = blockIdx.y * kBackRows;
+  const int col_blocks = (N + kBackCols - 1) / kBackCols;
+  const int chunk = blockIdx.x / col_blocks;  // (one grid dimension: rows may pass the others' 65535)
+  const int n0 = (blockIdx.x - chunk * col_blocks) * kBackCols;
+  const int n = n0 + lane * 8;
+  const int m0 = chunk * kBackRows;
   const int m1 = min(m0 + kBackRows, M);
   float acc[8];
 #pragma unroll
@@ -717,12 +728,12 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = acc[i];
   __syncthreads();
-  const int c = blockIdx.x * kBackCols + threadIdx.x;
+  const int c = n0 + threadIdx.x;
   if (c < N) {
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
-    part[static_cast<size_t>(blockIdx.y) * N + c] = s;
+    part[static_cast<size_t>(chunk) * N + c] = s;
   }
 }
 
@@ -810,7 +821,11 @@ Plan plan(int M, int N, int K, int mn_b, int sms) {
   return best;
 }
 
-int launch_error(cudaError_t e) { return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e); }
+int launch_error(cudaError_t e) {
+  if (e == cudaSuccess) return WDIT_OK;
+  cudaGetLastError();  // reported here, not by the next launch too
+  return WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+}
 
 struct Maps {
   CUtensorMap a, b, out, res, pre;
@@ -936,7 +951,7 @@ extern "C" {
 int wdit_linear_act_residual(const void* A, long long lda, int a_mn, const void* B, long long ldb, int b_mn, int M,
                              int N, int K, int dtype, const void* bias, int bias_dtype, int act, const void* res,
                              long long ldr, void* out, long long ldo, void* pre_out, long long ldp, void* stream) {
-  if (M < 0 || N < 0 || K < 0 || N % 8 != 0) return WDIT_ERR_SHAPE;
+  if (M < 0 || N < 0 || K < 0 || N % 8 != 0 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return WDIT_ERR_SHAPE;
   if (M == 0 || N == 0) return WDIT_OK;  // nothing to write
   if (K == 0) return WDIT_ERR_SHAPE;
   if (dtype != 1 && dtype != 2) return WDIT_ERR_ARG;
@@ -973,7 +988,7 @@ long long wdit_act_backward_workspace_bytes(int M, int N) {
 int wdit_act_backward(const void* dout, long long ldd, const void* pre, long long ldp, int act, int dtype, int M, int N,
                       void* dpre, long long ldq, void* dbias, int dbias_dtype, void* workspace,
                       long long workspace_bytes, void* stream) {
-  if (M < 0 || N < 0 || N % 8 != 0) return WDIT_ERR_SHAPE;
+  if (M < 0 || N < 0 || N % 8 != 0 || M > kMaxExtent || N > kMaxExtent) return WDIT_ERR_SHAPE;
   if (dtype != 1 && dtype != 2) return WDIT_ERR_ARG;
   if (act < kNone || act > kGelu || (dbias != nullptr && (dbias_dtype < 0 || dbias_dtype > 2))) return WDIT_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -991,9 +1006,10 @@ int wdit_act_backward(const void* dout, long long ldd, const void* pre, long lon
     if (workspace == nullptr || workspace_bytes < wdit_act_backward_workspace_bytes(M, N)) return WDIT_ERR_WORKSPACE;
     if (!aligned16(workspace)) return WDIT_ERR_ALIGN;
   }
-  if (chunks > 65535) return WDIT_ERR_SHAPE;
   float* part = dbias != nullptr ? static_cast<float*>(workspace) : nullptr;
-  const dim3 grid((N + kBackCols - 1) / kBackCols, chunks);
+  const long long blocks = static_cast<long long>((N + kBackCols - 1) / kBackCols) * chunks;
+  if (blocks > 0x7fffffffll) return WDIT_ERR_SHAPE;
+  const unsigned grid = static_cast<unsigned>(blocks);
   const uint16_t* g = static_cast<const uint16_t*>(dout);
   const uint16_t* x = static_cast<const uint16_t*>(pre);
   uint16_t* d = static_cast<uint16_t*>(dpre);

@@ -128,46 +128,14 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // Bounded wait for the phase with the given parity to complete.
-// kSuspend: the waiting thread is suspended by the hardware for up to kSuspendNs at a time, so that
-// it takes no issue slots from working warps; it wakes later than a polling one. (GEMM mainloops
-// gain 5-10% from it, the shorter hand-overs of attention lose as much.)
-constexpr uint32_t kSuspendNs = 100000;
-
-template <bool kCluster>
-__device__ __forceinline__ bool mbar_suspend_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  if constexpr (kCluster) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
-        : "memory");
-  }
-  return done != 0;
-}
-
-template <bool kCluster = false, bool kSuspend = false>
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_parity(uint64_t* bar, uint32_t parity, unsigned int site, const WaitCtx& ctx) {
   if (mbar_try_wait<kCluster>(bar, parity)) return true;
   const uint64_t start = globaltimer_ns();
   while (true) {
-    if constexpr (kSuspend) {
-      if (mbar_suspend_wait<kCluster>(bar, parity)) return true;
-    } else {
 #pragma unroll 1
-      for (int i = 0; i < 256; ++i) {
-        if (mbar_try_wait<kCluster>(bar, parity)) return true;
-      }
+    for (int i = 0; i < 256; ++i) {
+      if (mbar_try_wait<kCluster>(bar, parity)) return true;
     }
     if (globaltimer_ns() - start > ctx.limit_ns) {
       report_error_to(ctx.rec, kErrTimeout, site, parity);

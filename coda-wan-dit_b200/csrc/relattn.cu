@@ -1472,7 +1472,11 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-int cuda_rc(cudaError_t e) { return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e); }
+int cuda_rc(cudaError_t e) {
+  if (e == cudaSuccess) return WDIT_OK;
+  cudaGetLastError();  // reported here, not by the next launch too
+  return WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+}
 
 int attn_sms() {
   int dev = 0, n = 0;
@@ -1525,8 +1529,9 @@ int check_attn(const int* bounds, int n_bounds, int B, int H, int Lq, int Lk, in
   if (dtype != 1 && dtype != 2) return WDIT_ERR_ARG;
   if (table_dtype < 0 || table_dtype > 2) return WDIT_ERR_ARG;
   if (n_bounds < 1 || n_bounds > kMaxRelBounds) return WDIT_ERR_SHAPE;
-  if (B < 0 || H < 1 || Lq < 0 || Lk < 0 || (D != 64 && D != 128)) return WDIT_ERR_SHAPE;
-  if (q_offset < 0 || static_cast<long long>(q_offset) + Lq > (1ll << 30) || Lk > (1 << 30)) return WDIT_ERR_SHAPE;
+  if (B < 0 || H < 1 || H > 65535 || Lq < 0 || Lk < 0 || (D != 64 && D != 128)) return WDIT_ERR_SHAPE;
+  if (q_offset < 0 || static_cast<long long>(q_offset) + Lq > (1ll << 30) || Lq > (1 << 28) || Lk > (1 << 28))
+    return WDIT_ERR_SHAPE;
   return WDIT_OK;
 }
 
@@ -1540,15 +1545,20 @@ int check_heads(const void* p, const long long* s) {
   return WDIT_OK;
 }
 
+// The kernels' limit is raised once to what any table needs (always the same value, so that calls at
+// the same time do no harm).
+constexpr int kSmemMost = 176 * 1024;
+
 template <typename K>
-int set_smem(K kernel, int bytes, int (&done)[64]) {
+int set_smem(K kernel, int bytes, bool (&done)[64]) {
+  if (bytes > kSmemMost) return WDIT_ERR_SHAPE;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_rc(e);
-  if (done[dev & 63] < bytes) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (!done[dev & 63]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e != cudaSuccess) return cuda_rc(e);
-    done[dev & 63] = bytes;
+    done[dev & 63] = true;
   }
   return WDIT_OK;
 }
@@ -1556,7 +1566,7 @@ int set_smem(K kernel, int bytes, int (&done)[64]) {
 template <int D, bool BF16, int NB>
 int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, const AttnArgs& p,
             cudaStream_t st) {
-  static int done[64] = {};
+  static bool done[64] = {};
   const int smem = Fwd<D, NB>::smem(p.rb);
   int rc = set_smem(attn_fwd_kernel<D, BF16, NB>, smem, done);
   if (rc) return rc;
@@ -1574,7 +1584,7 @@ template <int D, bool BF16>
 int run_bwd(const CUtensorMap (&big)[4], const CUtensorMap (&small)[4], const CUtensorMap (&out)[3], const AttnArgs& p,
             int buckets, void* dtable, int dtable_dtype, cudaStream_t st) {
   // order of the maps: q, k, v, dO; dq, dk, dv
-  static int done_q[64] = {}, done_kv[64] = {};
+  static bool done_q[64] = {}, done_kv[64] = {};
   const int smem = Bwd<D>::smem(p.rb);
   int rc = set_smem(attn_dq_kernel<D, BF16>, smem, done_q);
   if (rc) return rc;

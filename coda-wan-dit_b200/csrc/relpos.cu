@@ -97,10 +97,12 @@ __global__ void __launch_bounds__(kRelThreads)
   __shared__ uint32_t line[E][kWords + kWords / 32 + 1];
   __shared__ int bounds[kMaxRelBounds];
   auto slot = [](int w) { return w + (w >> 5); };
-  const int h = blockIdx.z;
-  const int i0 = static_cast<int>(blockIdx.y) * rows;
+  const int col_tiles = (Lk + kBiasCols - 1) / kBiasCols;
+  const int row_tile = static_cast<int>(blockIdx.x) / col_tiles;
+  const int h = blockIdx.y;
+  const int i0 = row_tile * rows;
   const int i1 = min(i0 + rows, Lq);
-  const int j0 = static_cast<int>(blockIdx.x) * kBiasCols;
+  const int j0 = (static_cast<int>(blockIdx.x) - row_tile * col_tiles) * kBiasCols;
   const int j1 = min(j0 + kBiasCols, Lk);
   if (rb.n_bounds > kFewBounds) {
     for (int t = threadIdx.x; t < rb.n_bounds; t += kRelThreads) bounds[t] = rb.bounds[t];
@@ -390,6 +392,12 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+int cuda_rc(cudaError_t e) {
+  if (e == cudaSuccess) return WDIT_OK;
+  cudaGetLastError();  // reported here, not by the next launch too
+  return WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+}
+
 int rel_cta_target() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148 * 4;
@@ -422,11 +430,12 @@ template <typename T>
 int launch_bias(const void* table, const RelBuckets& rb, int H, int Lq, int Lk, int q_offset, void* out,
                 cudaStream_t st) {
   const int rows = Lq < kBiasRows ? Lq : kBiasRows;
-  const dim3 grid((Lk + kBiasCols - 1) / kBiasCols, (Lq + rows - 1) / rows, H);
+  const long long tiles = static_cast<long long>((Lk + kBiasCols - 1) / kBiasCols) * ((Lq + rows - 1) / rows);
+  if (tiles > 0x7fffffffll) return WDIT_ERR_SHAPE;  // (more cells than any memory holds)
+  const dim3 grid(static_cast<unsigned>(tiles), H);
   rel_bias_kernel<T><<<grid, kRelThreads, 0, st>>>(static_cast<const T*>(table), rb, H, Lq, Lk, q_offset, rows,
                                                    static_cast<T*>(out));
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+  return cuda_rc(cudaGetLastError());
 }
 
 template <typename T>
@@ -442,7 +451,7 @@ int launch_grad(const void* db, const RelBuckets& rb, int B, int H, int Lq, int 
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(rel_bias_grad_kernel<T, false>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
-    if (e != cudaSuccess) return WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+    if (e != cudaSuccess) return cuda_rc(e);
   }
   const dim3 grid(parts, H);
   const T* p = static_cast<const T*>(db);
@@ -452,8 +461,7 @@ int launch_grad(const void* db, const RelBuckets& rb, int B, int H, int Lq, int 
   else
     rel_bias_grad_kernel<T, false><<<grid, kRelThreads, smem, st>>>(p, rb, B, Lq, Lk, q_offset, sb, sh, si, buckets,
                                                                    rows, part);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+  return cuda_rc(cudaGetLastError());
 }
 
 int check_rel(const int* bounds, int n_bounds, int H, int Lq, int Lk, int q_offset, int dtype) {
@@ -471,8 +479,7 @@ int check_rel(const int* bounds, int n_bounds, int H, int Lq, int Lk, int q_offs
 int launch_rel_table_sum(const float* part, int parts, int buckets, int H, void* out, int dtype, void* stream) {
   rel_table_sum_kernel<<<dim3((buckets + 7) / 8, H), 256, 0, static_cast<cudaStream_t>(stream)>>>(part, parts, buckets,
                                                                                                  H, out, dtype);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+  return cuda_rc(cudaGetLastError());
 }
 
 }  // namespace wdit
@@ -487,8 +494,7 @@ int wdit_rel_pos_bias(const void* table, int dtype, const int* bounds, int n_bou
   if (rc) return rc;
   if (Lq == 0 || Lk == 0) return WDIT_OK;
   if (table == nullptr || out == nullptr) return WDIT_ERR_ARG;
-  if ((Lq + kBiasRows - 1) / kBiasRows > 65535) return WDIT_ERR_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0 || (reinterpret_cast<uintptr_t>(table) & 3) != 0)
+  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0 || (reinterpret_cast<uintptr_t>(table) & (dtype == 0 ? 3 : 1)) != 0)
     return WDIT_ERR_ALIGN;
   RelBuckets rb;
   if (!rel_fill(&rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
@@ -505,7 +511,8 @@ long long wdit_rel_pos_bias_grad_workspace_bytes(int B, int H, int Lq, int Lk, i
 
 int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, int Lk, long long stride_b,
                            long long stride_h, long long stride_i, const int* bounds, int n_bounds, int bidirectional,
-                           int q_offset, void* dtable, int dtable_dtype, void* workspace, long long workspace_bytes, void* stream) {
+                           int q_offset, void* dtable, int dtable_dtype, void* workspace, long long workspace_bytes,
+                           void* stream) {
   int rc = check_rel(bounds, n_bounds, H, Lq, Lk, q_offset, dtype);
   if (rc) return rc;
   if (B < 0) return WDIT_ERR_SHAPE;
@@ -513,8 +520,7 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int buckets = rel_num_buckets(n_bounds, bidirectional);
   if (B == 0 || Lq == 0 || Lk == 0) {  // no cells: a zero gradient
-    const cudaError_t e = cudaMemsetAsync(dtable, 0, static_cast<size_t>(buckets) * H * (dtable_dtype == 0 ? 4 : 2), st);
-    return e == cudaSuccess ? WDIT_OK : WDIT_ERR_CUDA_BASE + static_cast<int>(e);
+    return cuda_rc(cudaMemsetAsync(dtable, 0, static_cast<size_t>(buckets) * H * (dtable_dtype == 0 ? 4 : 2), st));
   }
   if (dbias == nullptr) return WDIT_ERR_ARG;
   if (stride_b < 0 || stride_h < 0 || stride_i < 0) return WDIT_ERR_SHAPE;

@@ -15,12 +15,16 @@ from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import call, ptr
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_BUCKETS = 256  # table rows of one direction (kMaxRelBounds + 1 in csrc/relpos.cuh)
+MAX_HEADS = 65535
+MAX_LENGTH = 1 << 28  # queries or keys
+MAX_EXTENT = 1 << 30  # M, N and K of a product (kMaxExtent in csrc/linear.cu), samples
 
 
 def _require_cuda(*ts: torch.Tensor | None) -> int:
@@ -116,13 +120,14 @@ def _bounds_arg(num_buckets: int, max_distance: int, bidirectional: bool):
 def _check_positions(q_len: int, k_len: int, q_offset: int) -> None:
     if q_len < 0 or k_len < 0 or q_offset < 0:
         raise ValueError(f"negative length or offset: q_len {q_len}, k_len {k_len}, q_offset {q_offset}")
-    if q_len + q_offset > 1 << 30 or k_len > 1 << 30:
-        raise ValueError("positions above 2^30")
+    if q_len > MAX_LENGTH or k_len > MAX_LENGTH or q_len + q_offset > 1 << 30:
+        raise ValueError(f"lengths up to 2^28 and positions up to 2^30, got q_len {q_len}, k_len {k_len}, "
+                         f"q_offset {q_offset}")
 
 
 def _check_table(table: torch.Tensor) -> None:
-    if table.dim() != 2 or table.shape[1] < 1:
-        raise ValueError(f"table must be [num_buckets, heads], got {tuple(table.shape)}")
+    if table.dim() != 2 or not 1 <= table.shape[1] <= MAX_HEADS:
+        raise ValueError(f"table must be [num_buckets, heads], 1 to {MAX_HEADS} heads, got {tuple(table.shape)}")
     if table.dtype not in _DTYPE:
         raise ValueError(f"table must be fp32, bf16 or fp16, got {table.dtype}")
 
@@ -155,8 +160,8 @@ def rel_pos_bias_grad(dbias: torch.Tensor, num_buckets: int, *, bidirectional: b
     if dtype not in _DTYPE:
         raise ValueError(f"dtype must be fp32, bf16 or fp16, got {dtype}")
     B, H, Lq, Lk = dbias.shape
-    if H < 1:
-        raise ValueError("dbias has no heads")
+    if not 1 <= H <= MAX_HEADS or B > MAX_EXTENT:
+        raise ValueError(f"1 to {MAX_HEADS} heads and at most 2^30 samples, got {H} and {B}")
     _check_positions(Lq, Lk, q_offset)
     bounds, n = _bounds_arg(num_buckets, max_distance, bidirectional)
     with _on_device(dev):
@@ -311,6 +316,8 @@ def linear_act_residual(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | N
     N, K = ws
     if N % 8 != 0 or K % 8 != 0 or N == 0 or K == 0:
         raise ValueError(f"N and K must be multiples of 8, got N {N}, K {K}")
+    if N > MAX_EXTENT or K > MAX_EXTENT or x.numel() // K > MAX_EXTENT:
+        raise ValueError(f"at most 2^30 rows, N and K, got {x.numel() // K}, {N} and {K}")
     shape = (*xs[:-1], N)
     if bias is not None and (bias.shape != (N,) or bias.dtype not in _DTYPE):
         raise ValueError(f"bias must be [{N}] of fp32, bf16 or fp16, got {tuple(bias.shape)} {bias.dtype}")
@@ -329,6 +336,7 @@ def linear_act_residual(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | N
             if not out.is_contiguous() or out.data_ptr() % 16 != 0:
                 raise ValueError("out must be contiguous and start on a 16-byte boundary")
             _check_out_overlap(out, residual, x, w, bias)
+            increment_version(out)  # autograd sees that it was written
         _linear_forward(dev, x, w, bias, act, residual, out, None)
     return out
 
@@ -457,6 +465,8 @@ def rel_pos_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
         raise ValueError(f"q [B, Lq, H, D], k and v [B, Lk, H, D] expected, got {tuple(qs)}, {tuple(ks)}, "
                          f"{tuple(v.shape)}")
     B, Lq, H, D = qs
+    if B > MAX_EXTENT:
+        raise ValueError(f"at most 2^30 samples, got {B}")
     if ks[0] != B or ks[2] != H or ks[3] != D:
         raise ValueError(f"q {tuple(qs)} and k {tuple(ks)} differ in batch, heads or head size")
     if D != 64 and D != 128:

@@ -308,7 +308,8 @@ int wdit_rope_table(const double* freqs_ri, int max_pos, int f, int h, int w, in
 
 /* ---- text-encoder operators (no reference counterpart: the reference takes the encoder's
  * output as given) ----
- * dtype codes: 0 fp32, 1 bf16, 2 fp16.
+ * dtype codes: 0 fp32, 1 bf16, 2 fp16. Limits: Lq, Lk <= 2^28, q_offset + Lq <= 2^30, H <= 65535;
+ * M, N, K <= 2^30 (WDIT_ERR_SHAPE beyond).
  *
  * Relative position buckets: relative position d = key - (query + q_offset); its distance n = |d|
  * (bidirectional != 0; keys ahead of the query, d > 0, take the upper half of the buckets) or
@@ -349,8 +350,8 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
 
 /*
  * Its gradients: dq [B, Lq, H, D], dk, dv [B, Lk, H, D] (contiguous, dtype; 0 for keys past
- * k_lens) and dtable [buckets, H] (of dtable_dtype). out and lse are the forward's. Three launches, no atomics:
- * sums have a fixed order. Empty dimensions are WDIT_ERR_SHAPE (the results are zeros).
+ * k_lens) and dtable [buckets, H] (of dtable_dtype). out and lse are the forward's. Three launches,
+ * no atomics: sums have a fixed order. Empty dimensions are WDIT_ERR_SHAPE (the results are zeros).
  */
 long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional);
 int wdit_rel_attention_backward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
@@ -358,8 +359,8 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
                                 const long long* dout_strides, const void* out, const float* lse, int B, int H, int Lq,
                                 int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
                                 const int* bounds, int n_bounds, int bidirectional, int causal, int q_offset,
-                                float scale, void* dq, void* dk, void* dv, void* dtable, int dtable_dtype, void* workspace,
-                                long long workspace_bytes, void* stream);
+                                float scale, void* dq, void* dk, void* dv, void* dtable, int dtable_dtype,
+                                void* workspace, long long workspace_bytes, void* stream);
 
 /*
  * out[M, N] = act(A . B^T + bias) + res, operands and out of dtype (bf16 or fp16), fp32 sums, one

@@ -59,6 +59,39 @@ def test_positions_refused(pkg):
         ops.rel_pos_bias(torch.zeros(32, 4, dtype=torch.float64), 4, 4)
 
 
+def test_extents_refused(pkg):
+    """Sizes past the kernels' 32-bit coordinates: refused, not wrapped (expanded tensors hold nothing)."""
+    ops, big = pkg.ops, (1 << 28) + 1
+    t = torch.zeros(32, 4)
+    for lq, lk, off in [(big, 1, 0), (1, big, 0), (1, 1, 1 << 30)]:
+        with pytest.raises(ValueError, match="lengths up to"):
+            ops.rel_pos_bias(t, lq, lk, q_offset=off)
+    with pytest.raises(ValueError, match="heads"):
+        ops.rel_pos_bias(torch.zeros(1).expand(32, 65536), 4, 4)
+    with pytest.raises(ValueError, match="at most 2\\^29"):
+        ops.rel_pos_bias(t, 4, 4, max_distance=(1 << 29) + 1)
+    with pytest.raises(ValueError, match="fp32, bf16 or fp16"):
+        ops.rel_pos_bias(t.double(), 4, 4)
+    half = torch.zeros(1, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="at most 2\\^30 rows"):
+        ops.linear_act_residual(half.expand((1 << 30) + 1, 64), half.expand(8, 64))
+    with pytest.raises(ValueError, match="at most 2\\^30 rows"):
+        ops.linear_act_residual(half.expand(1, (1 << 30) + 8), half.expand(8, (1 << 30) + 8))
+    q, k = half.expand(1, 4, 4, 64), half.expand(1, big, 4, 64)
+    with pytest.raises(ValueError, match="lengths up to"):
+        ops.rel_pos_attention(q, k, k, t)
+    lib, null, d = pkg._lib.load(), ctypes.c_void_p(None), ctypes.c_void_p(0x1000)
+    b = (ctypes.c_int * 1)(1)
+    st = (ctypes.c_longlong * 3)(64, 64, 64)
+    assert lib.wdit_rel_pos_bias(d, 0, b, 1, 1, 65536, 4, 4, 0, d, null) == 2
+    assert lib.wdit_rel_pos_bias(d, 0, b, 1, 1, 4, 4, big, 0, d, null) == 2
+    assert lib.wdit_linear_act_residual(d, 64, 0, d, 64, 0, (1 << 30) + 1, 64, 64, 1, null, 0, 0, null, 0, d, 64, null,
+                                        0, null) == 2
+    for H, lq, lk in [(65536, 1, 1), (1, big, 1), (1, 1, big)]:
+        assert lib.wdit_rel_attention(d, st, d, st, d, st, 1, H, lq, lk, 64, 1, null, d, 0, b, 1, 1, 0, 0, 1.0, d, null,
+                                      null, 0, null) == 2
+
+
 def test_rel_pos_entry_points_validate_without_device(pkg):
     lib = pkg._lib.load()
     null, d = ctypes.c_void_p(None), ctypes.c_void_p(0x1000)

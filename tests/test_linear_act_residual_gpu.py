@@ -265,3 +265,43 @@ def test_streams_and_graphs(pkg):
     torch.cuda.synchronize()
     for _, res in graphs:
         assert all(torch.equal(a, c) for a, c in zip(res, want))
+
+
+def test_out_counts_as_written(pkg):
+    """Autograd refuses a backward pass whose saved tensor out= has overwritten."""
+    x = torch.randn(8, 64, device=DEV).to(torch.bfloat16)
+    w = torch.randn(64, 64, device=DEV).to(torch.bfloat16).requires_grad_()
+    h = torch.randn(8, 64, device=DEV).to(torch.bfloat16)
+    y = pkg.ops.linear_act_residual(h, w)
+    with torch.no_grad():
+        pkg.ops.linear_act_residual(x, w, residual=h, out=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_rows_past_32_bit_offsets(pkg):
+    g = torch.Generator().manual_seed(40)
+    x = torch.randn(70, 128, generator=g).to(torch.bfloat16).to(DEV)
+    w = torch.randn(64, 128, generator=g).to(torch.bfloat16).to(DEV)
+    far = torch.empty(69 * (1 << 26) + 128, dtype=torch.bfloat16, device=DEV).as_strided((70, 128), (1 << 26, 1))
+    far.copy_(x)
+    assert torch.equal(pkg.ops.linear_act_residual(far, w, act="silu", residual=far[:, :64]),
+                       pkg.ops.linear_act_residual(x, w, act="silu", residual=x[:, :64].contiguous()))
+
+
+def test_gradients_of_more_row_chunks_than_a_grid_dimension_holds(pkg):
+    """65536 chunks of 64 rows and five more rows; only some rows carry a gradient, so that the sums
+    are exact in fp32 (small whole numbers) and every chunk boundary is met."""
+    M = 65536 * 64 + 5
+    x = torch.ones(M, 8, dtype=torch.bfloat16, device=DEV)
+    w = torch.zeros(8, 8, dtype=torch.bfloat16, device=DEV)
+    b = torch.ones(8, device=DEV)
+    xs, ws, bs = x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    dout = torch.zeros(M, 8, dtype=torch.bfloat16, device=DEV)
+    dout[::1_000_003] = 1.0
+    dout[-1] = 2.0
+    out = pkg.ops.linear_act_residual(xs, ws, bs, act="relu")  # pre = 1: act' = 1
+    dx, dw, db = torch.autograd.grad(out, [xs, ws, bs], dout)
+    total = dout.float().sum(0)
+    assert torch.equal(out, torch.ones_like(out)) and not dx.any()
+    assert torch.equal(db, total) and torch.equal(dw.float(), total[:, None].expand(8, 8))

@@ -372,3 +372,43 @@ def test_agrees_with_the_bias_tensor(pkg):
     (g2,) = torch.autograd.grad(o2, t2, dout.float())
     assert (out.float() - o2).abs().max() <= 2.0**-9 * v.abs().max()
     assert (g1 - g2).norm() <= 2.0**-9 * g2.norm() + 2.0**-9
+
+
+def test_cache_past_32_bit_offsets(pkg):
+    """Rows of a cache 2^26 elements apart: the last ones lie behind 2^32 elements."""
+    q, k, v, table = make(1, 2, 3, 70, 64, torch.bfloat16, seed=17)
+    room = torch.empty(69 * (1 << 26) + 4 * 64, dtype=torch.bfloat16, device=DEV)
+    fk, fv = (room[s:].as_strided((1, 70, 2, 64), (8, 1 << 26, 64, 1)) for s in (0, 128))
+    fk.copy_(k), fv.copy_(v)
+    kw = dict(causal=True, bidirectional=False, q_offset=67)
+    dout = torch.randn_like(q)
+    res = []
+    for kk, vv in ((k, v), (fk, fv)):
+        ts = [t.detach().requires_grad_() for t in (q, kk, vv, table)]
+        out = pkg.ops.rel_pos_attention(*ts, **kw)
+        res.append([out.detach(), *torch.autograd.grad(out, ts, dout)])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+    check(res[0], q, k, v, table, dout=dout, **kw)
+
+
+def test_two_streams_at_once(pkg):
+    """Calls that overlap on the device share nothing: key splits' workspaces, backward's partial sums."""
+    sets = [make(2, 2, 9, 3000, 64, torch.bfloat16, seed=30 + i) for i in range(2)]
+    dout = torch.randn_like(sets[0][0])
+
+    def run(ts):
+        ts = [t.detach().requires_grad_() for t in ts]
+        out = pkg.ops.rel_pos_attention(*ts)
+        return [out.detach(), *torch.autograd.grad(out, ts, dout)]
+
+    want = [run(ts) for ts in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, ts in zip(streams, sets):
+            with torch.cuda.stream(s):
+                got.append(run(ts))
+    torch.cuda.synchronize()
+    for n, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[n % 2]))

@@ -119,6 +119,35 @@ def test_gradient_is_rounded_once_to_the_type_asked_for(pkg, dtype):
     assert none.dtype == dtype and none.shape == (32, 3) and not none.any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_table_that_starts_at_any_element(pkg, dtype):
+    table = torch.randn(32, 3, generator=torch.Generator().manual_seed(6)).to(dtype).to(DEV)
+    odd = torch.empty(32 * 3 + 1, dtype=dtype, device=DEV)[1:].view(32, 3).copy_(table)
+    assert torch.equal(pkg.ops.rel_pos_bias(odd, 40, 50), pkg.ops.rel_pos_bias(table, 40, 50))
+
+
+def test_more_row_tiles_than_a_grid_dimension_holds(pkg):
+    lq = 65536 * 32 + 5
+    table = torch.randn(32, 1, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16).to(DEV)
+    got = pkg.ops.rel_pos_bias(table, lq, 3, q_offset=1)
+    for i0 in (0, 100, 65535 * 32 - 180, lq - 200):  # 200 rows each
+        where = bucket_map(200, 3, 1 + i0, 32, 128, True)
+        assert torch.equal(got[:, i0 : i0 + 200], table[where].permute(2, 0, 1))
+    db = torch.zeros(1, lq, 3, device=DEV)
+    db[0, ::100_000, 1] = 1.0
+    want = torch.zeros(32, 1, device=DEV)
+    for i in range(0, lq, 100_000):
+        want[bucket(max(1 - (i + 1), -200), 32, 128, True)] += 1.0
+    assert torch.equal(pkg.ops.rel_pos_bias_grad(db, 32, q_offset=1), want)
+
+
+def test_gradient_cells_past_32_bit_offsets(pkg):
+    db = torch.randn(70, 90, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16).to(DEV)
+    far = torch.empty(69 * (1 << 26) + 90, dtype=torch.bfloat16, device=DEV).as_strided((1, 70, 90), (0, 1 << 26, 1))
+    far[0].copy_(db)
+    assert torch.equal(pkg.ops.rel_pos_bias_grad(far, 32), pkg.ops.rel_pos_bias_grad(db[None].contiguous(), 32))
+
+
 def test_gradient_of_no_cells_is_zero(pkg):
     for shape in [(0, 2, 5, 6), (2, 2, 0, 6), (2, 2, 5, 0)]:
         got = pkg.ops.rel_pos_bias_grad(torch.empty(shape, device=DEV), 32)
