@@ -47,6 +47,7 @@ constexpr int kEpiThreads = 256;
 constexpr uint32_t kTileABytes = BM * BK * 2;
 constexpr uint32_t kTmemCols = 512;  // two accumulators of up to 256 columns
 constexpr int kMaxStages = 8;
+constexpr int kBarriers = 2 * kMaxStages + 4 + 24;  // full, empty; TMEM full, empty; residual pieces
 constexpr uint32_t kPieceBytes = 32 * 32 * 2;
 constexpr uint32_t kWarpBytes = 4 * kPieceBytes;   // three rotating pieces and one of pre-activations
 constexpr uint32_t kEpiBytes = 8 * (kWarpBytes + 32 * 4);  // ... and a line of 32 bias values
@@ -334,17 +335,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     m_blk = PAIR ? 2 * mq + cta_rank : mq;
   };
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < stages; ++i) {
-      mbar_init(&full_bar[i], 2);  // armed by the loaders of A and B
-      mbar_init(&empty_bar[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&tfull_bar[i], 1);
-      mbar_init(&tempty_bar[i], PAIR ? 2 * (kEpiThreads / 32) : kEpiThreads / 32);
-    }
-    for (int i = 0; i < 24; ++i) mbar_init(&res_bar[i], 1);
+  // One barrier a thread: set up one after the other they take as long as the first loads.
+  if (threadIdx.x < kBarriers) {
+    const int i = threadIdx.x;
+    uint32_t arrivals = 1;
+    if (i < kMaxStages) arrivals = 2;  // full_bar: armed by the loaders of A and B
+    if (i >= 2 * kMaxStages + 2 && i < 2 * kMaxStages + 4) arrivals = (PAIR ? 2 : 1) * (kEpiThreads / 32);  // tempty_bar
+    mbar_init(&full_bar[i], arrivals);
     fence_mbar_init();
+  } else if (threadIdx.x == 10 * 32) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
@@ -495,34 +494,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t rphase = 0;  // phase of each residual buffer's barrier
     int cur = 0;          // rotating piece buffer
     const bool has_res = !SPLIT && p.res != nullptr;
-    auto piece_at = [&](int it, int c, int& row0, int& n0) {  // false: outside the matrix
+    // first row of the warp and first column of a tile
+    auto place = [&](int it, int& row, int& col) {
       int m_blk, n_blk;
       coords(it, m_blk, n_blk);
-      row0 = m_blk * BM + wq * 32;
-      n0 = n_blk * p.bn + c * 32;
-      return row0 < p.M && n0 < p.N;
+      row = m_blk * BM + wq * 32;
+      col = n_blk * p.bn;
     };
     int in_flight = -1;  // lane 0: buffer of the last residual piece asked for
-    auto fetch_res = [&](int it, int c, int buf) {  // lane 0
-      int row0, n0;
-      if (!piece_at(it, c, row0, n0)) return;
+    auto fetch_res = [&](int row0, int n0, int buf) {  // lane 0
+      if (row0 >= p.M || n0 >= p.N) return;
       mbar_arrive_expect_tx(&rbar[buf], kPieceBytes);
       tma_load_2d(bufs + buf * kPieceBytes, &tmRes, &rbar[buf], n0, row0);
       in_flight = buf;
     };
-    if (has_res && lane == 0 && my_count > 0) fetch_res(0, half, 0);
+    int row0 = 0, col = 0, next_row = 0, next_col = 0;
+    if (my_count > 0) place(0, next_row, next_col);
+    if (has_res && lane == 0 && my_count > 0) fetch_res(next_row, next_col + half * 32, 0);
     bool failed = false;
     for (int it = 0; it < my_count && !failed; ++it) {
       const int buf = it & 1;
       const uint32_t tphase = (it >> 1) & 1;
+      row0 = next_row, col = next_col;
+      if (it + 1 < my_count) place(it + 1, next_row, next_col);
+      // this lane's bias of the warp's pieces, loaded while the tile is computed
+      float bias[4] = {0.f, 0.f, 0.f, 0.f};
+      if (!SPLIT && p.bias != nullptr) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = col + (half + 2 * q) * 32 + lane;
+          if (half + 2 * q < pieces && n < p.N) bias[q] = load_scalar(p.bias, n, p.bias_dtype);
+        }
+      }
       failed = !__all_sync(0xffffffffu, wait_parity<PAIR>(&tfull_bar[buf], tphase, kSiteEpiTmemFull, p.ctx));
       if (failed) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + lane_off + buf * 256;
 #pragma unroll 1
       for (int c = half; c < pieces; c += 2) {
-        int row0, n0;
-        const bool inside = piece_at(it, c, row0, n0);
+        const int n0 = col + c * 32;
+        const bool inside = row0 < p.M && n0 < p.N;
         float v[32];
         tmem_ld32(tbase + c * 32, v);
         if (c + 2 >= pieces) {
@@ -530,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) {
             if constexpr (PAIR) {
-              mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[buf]), leader));
+              mbar_arrive_tmem_cluster(mapa_shared(smem_u32(&tempty_bar[buf]), leader));
             } else {
               mbar_arrive(&tempty_bar[buf]);
             }
@@ -549,17 +560,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             bulk_wait_read<1>();  // every store but the last has left its buffer
             if (has_res) {
               if (c + 2 < pieces) {
-                fetch_res(it, c + 2, next);
+                fetch_res(row0, n0 + 64, next);
               } else if (it + 1 < my_count) {
-                fetch_res(it + 1, half, next);
+                fetch_res(next_row, next_col + half * 32, next);
               }
             }
           }
           if (inside) {
             if (p.bias != nullptr) {
-              const float bv = n0 + lane < p.N ? load_scalar(p.bias, n0 + lane, p.bias_dtype) : 0.f;
+              const int q = c >> 1;
               __syncwarp();
-              bias_line[lane] = bv;
+              bias_line[lane] = q == 0 ? bias[0] : (q == 1 ? bias[1] : (q == 2 ? bias[2] : bias[3]));
             }
             __syncwarp();
             if (p.bias != nullptr) {
@@ -947,6 +958,7 @@ int check_operand(const void* p, long long ld, long long cols) {
 using namespace wdit;
 
 extern "C" {
+
 
 int wdit_linear_act_residual(const void* A, long long lda, int a_mn, const void* B, long long ldb, int b_mn, int M,
                              int N, int K, int dtype, const void* bias, int bias_dtype, int act, const void* res,
