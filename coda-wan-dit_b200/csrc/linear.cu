@@ -64,7 +64,7 @@ struct LinArgs {
   int M, N, K;
   int m_blocks, n_blocks, k_blocks, tiles, raster_rows;
   int bn, stages, splits;
-  int a_one, b_one;  // MN-major operand whose 64-wide pieces come in one box (M or N % 64 == 0)
+  int a_one, b_one;  // MN-major operand whose 64-wide pieces come in one box (M or N and the tile % 64 == 0)
   int is_bf16, act, bias_dtype;
   const void* bias;
   const void* res;
@@ -75,6 +75,12 @@ struct LinArgs {
   long long ldp;
   WaitCtx ctx;
 };
+
+// Staged bytes of `rows` rows of a K block; MN-major ones come in whole pieces of 64 (of the last only
+// the first columns may be used: 96 rows of B in a 256 x 192 pair tile).
+__host__ __device__ __forceinline__ uint32_t operand_bytes(int rows, bool mn) {
+  return static_cast<uint32_t>(mn ? (rows + 63) / 64 * 64 : rows) * (BK * 2);
+}
 
 // MN-major tile written by TMA with the 128-byte swizzle: pieces of 64 elements (128 B) along M
 // or N, 64 K rows each. Leading offset: between pieces (64 rows x 128 B); stride offset: between
@@ -283,8 +289,8 @@ __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m
 }
 
 // Operand maps are 3-D in either storage: K-major {K, rows, 1}, box {64, rows of the tile, 1};
-// MN-major {64, K, pieces of 64} with all of a tile's pieces in one box, or, when M or N is no
-// multiple of 64, {M or N, K, 1} with one box per piece.
+// MN-major {64, K, pieces of 64} with all of a tile's pieces in one box, or, when M or N or the
+// tile is no multiple of 64, {M or N, K, 1} with one box per piece.
 template <bool PAIR, bool SPLIT, bool TA, bool TB>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int b_rows = PAIR ? p.bn / 2 : p.bn;  // B rows this CTA stages
-  const uint32_t b_bytes = static_cast<uint32_t>(b_rows) * (BK * 2);
+  const uint32_t b_bytes = operand_bytes(b_rows, TB);
   const uint32_t SB = kTileABytes + b_bytes;
   const int stages = p.stages;
   uint8_t* epi = smem + stages * SB;
@@ -372,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const CUtensorMap* map = is_a ? &tmA : &tmB;
       const bool mn = is_a ? TA : TB;
       const uint32_t bytes = is_a ? kTileABytes : b_bytes;
-      const int pieces = (is_a ? BM : b_rows) / 64;
+      const int pieces = ((is_a ? BM : b_rows) + 63) / 64;
       const bool one = (is_a ? p.a_one : p.b_one) != 0;
       const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full_bar), leader) : smem_u32(full_bar);
       uint8_t* const dst0 = smem + (is_a ? 0 : kTileABytes);
@@ -798,7 +804,9 @@ struct Plan {
 // (us; next best in brackets):   1 x 1536 x 8960 split 8 of 128 x 128 11.3 (one CTA a tile 46)
 //   256 x 1536 x 8960 split 4 15.6 (pairs, no split 47)   1024 x 1536 x 4096 128 x 128 15.6 (pairs 16.8)
 //   2048 x 1536 x 8960 pairs 256 x 192 42.5 (128 x 192 46.1)   1024 x 8960 x 1536 pairs 256 x 256 23.0
-Plan plan(int M, int N, int K, int mn_b, int sms) {
+// With B MN-major a 256 x 192 pair tile stages 128 rows of B a CTA for the 96 it uses; 5% on its blocks:
+//   4095 x 1536 x 8960 pairs 256 x 192 86.7 (256 x 256 93.5)   4096 x 5120 x 13824 256 x 256 405 (427)
+Plan plan(int M, int N, int K, bool mn_b, int sms) {
   const int kb = (K + BK - 1) / BK;
   Plan best = {0, 128, 1};
   double best_cost = 1e30;
@@ -813,9 +821,10 @@ Plan plan(int M, int N, int K, int mn_b, int sms) {
     const long long waves = (tiles + slots - 1) / slots;
     const double active = static_cast<double>(tiles < slots ? tiles : slots) * group;
     double block = 2.1 * bn;
-    const double l2 = active * (BM + (pair ? bn / 2 : bn)) * BK * 2 / 11000;
+    const double l2 = active * (kTileABytes + operand_bytes(pair ? bn / 2 : bn, mn_b)) / 11000;
     if (l2 > block) block = l2;
     if (block < 270) block = 270;
+    if (pair && mn_b && bn == 192) block *= 1.05;
     const int rows = M < BM ? M : BM;
     const double end = (s > 1 ? 4200 + 0.45 * rows * bn * (s - 1) / s : 17.0 * bn) + (pair ? 500 : 0);
     const double cost = waves * ((kb + s - 1) / s) * block + end;
@@ -827,7 +836,7 @@ Plan plan(int M, int N, int K, int mn_b, int sms) {
   for (int bn = 256; bn >= 64; bn -= 64)
     for (int s = 1; s <= 8 && s <= kb; s *= 2) {
       consider(0, bn, s);
-      if (M > BM && bn != 64 && s <= 4 && (!mn_b || bn != 192)) consider(1, bn, s);
+      if (M > BM && bn != 64 && s <= 4) consider(1, bn, s);
     }
   return best;
 }
@@ -849,7 +858,7 @@ int launch(const Maps& m, LinArgs p, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return launch_error(e);
   const int b_rows = PAIR ? p.bn / 2 : p.bn;
-  const uint32_t sb = kTileABytes + static_cast<uint32_t>(b_rows) * BK * 2;
+  const uint32_t sb = kTileABytes + operand_bytes(b_rows, TB);
   p.stages = static_cast<int>(kRingBudget / sb);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   if (!attr_set[dev & 63]) {
@@ -891,7 +900,7 @@ CUtensorMapDataType map_type(int is_bf16) {
 int map_operand(CUtensorMap* m, int is_bf16, const void* ptr, int rows, int K, long long ld, int mn, int tile,
                 int* one) {
   typedef unsigned long long u64;
-  *one = mn && rows % 64 == 0 ? 1 : 0;
+  *one = mn && rows % 64 == 0 && tile % 64 == 0 ? 1 : 0;
   const u64 row_bytes = static_cast<u64>(ld) * 2;
   if (!mn) {
     const u64 dims[3] = {static_cast<u64>(K), static_cast<u64>(rows), 1};
@@ -915,7 +924,7 @@ int map_pieces(CUtensorMap* m, int is_bf16, const void* ptr, int cols, int rows,
 
 int run_linear(const void* A, long long lda, int a_mn, const void* B, long long ldb, int b_mn, LinArgs p,
                cudaStream_t stream) {
-  const Plan pl = plan(p.M, p.N, p.K, b_mn, sm_count());
+  const Plan pl = plan(p.M, p.N, p.K, b_mn != 0, sm_count());
   p.bn = pl.bn;
   p.splits = pl.splits;
   p.m_blocks = (p.M + BM - 1) / BM;
