@@ -138,7 +138,7 @@ def _rel_pos_bias(table, q_len, k_len, bidirectional, max_distance, q_offset):
     bounds, n = _bounds_arg(nb, max_distance, bidirectional)
     with _on_device(dev):
         table = table.contiguous()
-        out = torch.empty((H, q_len, k_len), dtype=table.dtype, device=table.device)
+        out = table.new_empty((H, q_len, k_len))
         call("wdit_rel_pos_bias", table.data_ptr(), _DTYPE[table.dtype], bounds, n, bidirectional, H, q_len, k_len,
              q_offset, out.data_ptr(), _stream(dev))
     return out
@@ -249,7 +249,7 @@ class _LinearActResidual(torch.autograd.Function):
     def forward(ctx, x, w, bias, act, residual):
         dev = x.get_device()
         with _on_device(dev):
-            out = torch.empty((*x.shape[:-1], w.shape[0]), dtype=x.dtype, device=x.device)
+            out = x.new_empty((*x.shape[:-1], w.shape[0]))
             # The derivative needs pre = x W^T + bias: kept in the operands' type (half a step of
             # it moves act' by no more than rounding the gradient itself does).
             need = any(ctx.needs_input_grad[:3]) and act != "none"
@@ -273,7 +273,7 @@ class _LinearActResidual(torch.autograd.Function):
         with _on_device(dev):
             g = _rows(dout.reshape(-1, N)) if need_x or need_w or need_b else None
             if g is not None:
-                dpre = torch.empty((M, N), dtype=x.dtype, device=x.device) if pre is not None else g
+                dpre = x.new_empty((M, N)) if pre is not None else g
                 ws, nbytes = None, 0
                 if need_b:
                     db = torch.empty(N, dtype=ctx.bias_dtype, device=x.device)
@@ -284,14 +284,14 @@ class _LinearActResidual(torch.autograd.Function):
                          _DTYPE[x.dtype], M, N, ptr(dpre), _ld(dpre), ptr(db), 0 if db is None else _DTYPE[db.dtype],
                          ptr(ws), nbytes, _stream(dev), kernels=2 if need_b else 1)
                 if need_x:
-                    dx = torch.empty((M, K), dtype=x.dtype, device=x.device)
+                    dx = x.new_empty((M, K))
                     _product(dev, dpre, 0, _rows(w), 1, M, K, N, dx)
                     dx = dx.view(x.shape)
                 if need_w:
                     if M == 0:
                         dw = torch.zeros((N, K), dtype=w.dtype, device=w.device)
                     else:
-                        dw = torch.empty((N, K), dtype=w.dtype, device=w.device)
+                        dw = w.new_empty((N, K))
                         _product(dev, dpre, 1, _rows(x2), 1, N, K, M, dw)
         return dx, dw, db, None, dout if need_r else None
 
@@ -331,7 +331,7 @@ def linear_act_residual(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | N
         return _LinearActResidual.apply(x, w, bias, act, residual)
     with _on_device(dev):
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=x.device)
+            out = x.new_empty(shape)
         else:
             if not out.is_contiguous() or out.data_ptr() % 16 != 0:
                 raise ValueError("out must be contiguous and start on a 16-byte boundary")
@@ -398,7 +398,7 @@ def _attention_args(q, k, table, k_lens, bidirectional, causal, max_distance, q_
 def _attention_forward(dev, q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale, with_lse):
     B, Lq, H, D = q.shape
     device = q.device
-    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0 or Lq == 0 or k.shape[1] == 0:
         return out.zero_(), None
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=device) if with_lse else None
@@ -433,10 +433,8 @@ class _RelPosAttention(torch.autograd.Function):
         with _on_device(dev):
             g = _heads(dout)
             device = q.device
-            dq = torch.empty(q.shape, dtype=q.dtype, device=device)
-            dk = torch.empty(k.shape, dtype=q.dtype, device=device)
-            dv = torch.empty(k.shape, dtype=q.dtype, device=device)
-            dtable = torch.empty(table.shape, dtype=table.dtype, device=device)
+            dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+            dtable = torch.empty_like(table)  # (contiguous)
             shape, pos = _attention_args(q, k, table, k_lens, *ctx.args)
             nbytes = _workspace_bytes(dev, "wdit_rel_attention_backward_workspace_bytes", *shape[:3], pos[5],
                                       int(pos[6]))
