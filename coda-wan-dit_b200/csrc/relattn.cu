@@ -62,6 +62,7 @@ struct AttnArgs {
   int table_dtype;
   RelBuckets rb;
   void* out;           // [B, Lq, H, D] contiguous
+  void* out_lo;        // the same: what rounding took from out; nullable in the forward
   float* lse;          // [B, H, Lq], log2 units; nullable
   int splits;          // forward: key splits; > 1 writes part_o / part_lse instead
   float* part_o;       // [splits][B * H * Lq][D]
@@ -70,9 +71,6 @@ struct AttnArgs {
   const void* dout;    // element strides below, unit along D
   long long do_b, do_l, do_h;
   float* delta;        // [B, H, Lq]
-  void* dq;            // [B, Lq, H, D]
-  void* dk;            // [B, Lk, H, D]
-  void* dv;
   float* table_part;   // [H][B * q tiles][buckets]
   WaitCtx ctx;
 };
@@ -88,6 +86,14 @@ template <bool BF16>
 __device__ __forceinline__ float2 unpack16(uint32_t w) {
   if constexpr (BF16) return unpack_bf16x2(w);
   return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+
+// a and b rounded to 16 bits, and what that took from them.
+template <bool BF16>
+__device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack16<BF16>(a, b);
+  const float2 f = unpack16<BF16>(hi);
+  lo = pack16<BF16>(a - f.x, b - f.y);
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -356,7 +362,7 @@ template <int D, bool BF16, int NB>
 __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmOut,
-                    const __grid_constant__ AttnArgs p) {
+                    const __grid_constant__ CUtensorMap tmLo, const __grid_constant__ AttnArgs p) {
   using C = Fwd<D, NB>;
   constexpr int ST = C::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -696,8 +702,11 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
       }
     }
     // The rows go out through the query tile's shared memory (every product that reads it is
-    // done), 32 rows x 128 bytes a TMA store and warp: rows past Lq are left out by the map.
+    // done), 32 rows x 128 bytes a TMA store and warp: rows past Lq are left out by the map. What
+    // their rounding loses goes out through the K tiles' in the same way.
     uint8_t* stage = sQ + wq * 32 * 128;
+    uint8_t* stage_lo = sK + wq * 32 * 128;
+    static_assert(ST * C::kTile >= C::kQ, "place for the lost parts");
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       float o[32];
@@ -718,11 +727,17 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
         continue;
       }
       const uint32_t row = smem_u32(stage + (c >> 1) * 16384) + lane * 128;
+      const uint32_t row_lo = smem_u32(stage_lo + (c >> 1) * 16384) + lane * 128;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        st_shared_v4(row + ((((c & 1) * 4 + q) ^ (lane & 7)) << 4), pack16<BF16>(o[8 * q], o[8 * q + 1]),
-                     pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
-                     pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t at16 = (((c & 1) * 4 + q) ^ (lane & 7)) << 4;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          split16<BF16>(o[8 * q + 2 * e], o[8 * q + 2 * e + 1], hi[e], lo[e]);
+        st_shared_v4(row + at16, hi[0], hi[1], hi[2], hi[3]);
+        if (p.out_lo != nullptr) st_shared_v4(row_lo + at16, lo[0], lo[1], lo[2], lo[3]);
+      }
     }
     if (p.splits == 1) {
       fence_proxy_async_smem();
@@ -730,8 +745,10 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
       if (lane == 0) {
         if (i0 + wq * 32 < p.Lq) {
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c)
+          for (int c = 0; c < D / 64; ++c) {
             tma_store_4d(&tmOut, stage + c * 16384, c * 64, h, i0 + wq * 32, b);
+            if (p.out_lo != nullptr) tma_store_4d(&tmLo, stage_lo + c * 16384, c * 64, h, i0 + wq * 32, b);
+          }
         }
         bulk_commit();
         bulk_wait_read<0>();  // the stores have read shared memory
@@ -772,10 +789,14 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
   const int i = static_cast<int>(row % p.Lq);
   const int h = static_cast<int>(row / p.Lq % p.H);
   const long long b = row / p.Lq / p.H;
-  uint16_t* dst = static_cast<uint16_t*>(p.out) + ((b * p.Lq + i) * p.H + h) * D + lane * V;
+  const long long to = ((b * p.Lq + i) * p.H + h) * D + lane * V;
 #pragma unroll
-  for (int q = 0; q < V; q += 2)
-    *reinterpret_cast<uint32_t*>(dst + q) = pack16<BF16>(acc[q] * inv, acc[q + 1] * inv);
+  for (int q = 0; q < V; q += 2) {
+    uint32_t hi, lo;
+    split16<BF16>(acc[q] * inv, acc[q + 1] * inv, hi, lo);
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + to + q) = hi;
+    if (p.out_lo != nullptr) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out_lo) + to + q) = lo;
+  }
   if (lane == 0 && p.lse != nullptr) p.lse[row] = inv == 0.f ? -kInf : ms + log2f(total);
 }
 
@@ -928,32 +949,39 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     tmem_relinquish();
   }
   for (int t = threadIdx.x; t < 8 * nsum; t += C::kThreads) sums[t] = 0.f;
-  // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too: D / 8 lanes a row.
+  // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too: D / 8 lanes a row. O is
+  // taken before its rounding (two 16-bit parts): dP - delta is the small difference of the two
+  // where a row rests on few keys, and its error goes into every cell of the row with one sign, so
+  // into the table's sums undiminished.
   {
     constexpr int kLanes = D / 8, kAtOnce = C::kThreads / kLanes, kTurns = (kRows + kAtOnce - 1) / kAtOnce;
     const int part = threadIdx.x % kLanes;
     const uint16_t* go = static_cast<const uint16_t*>(p.dout) + b * p.do_b + h * p.do_h;
-    const uint16_t* oo = static_cast<const uint16_t*>(p.out) + (static_cast<long long>(b) * p.Lq * p.H + h) * D;
-    uint4 a[kTurns], c[kTurns];  // every row's loads are in flight together
+    const long long first = (static_cast<long long>(b) * p.Lq * p.H + h) * D;
+    const uint16_t* oo = static_cast<const uint16_t*>(p.out) + first;
+    const uint16_t* ol = static_cast<const uint16_t*>(p.out_lo) + first;
+    uint4 a[kTurns], c[kTurns], g[kTurns];  // every row's loads are in flight together
 #pragma unroll
     for (int u = 0; u < kTurns; ++u) {
       const int r = u * kAtOnce + threadIdx.x / kLanes;
       const long long i = i0 + r;
-      a[u] = c[u] = make_uint4(0u, 0u, 0u, 0u);
+      a[u] = c[u] = g[u] = make_uint4(0u, 0u, 0u, 0u);
       if (r < kRows && i < p.Lq) {
         a[u] = __ldg(reinterpret_cast<const uint4*>(go + i * p.do_l) + part);
         c[u] = __ldg(reinterpret_cast<const uint4*>(oo + i * p.H * D) + part);
+        g[u] = __ldg(reinterpret_cast<const uint4*>(ol + i * p.H * D) + part);
       }
     }
 #pragma unroll
     for (int u = 0; u < kTurns; ++u) {
       const int r = u * kAtOnce + threadIdx.x / kLanes;
       const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, cw[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+      const uint32_t gw[4] = {g[u].x, g[u].y, g[u].z, g[u].w};
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack16<BF16>(aw[e]), v = unpack16<BF16>(cw[e]);
-        s = fmaf(f.x, v.x, fmaf(f.y, v.y, s));
+        const float2 f = unpack16<BF16>(aw[e]), v = unpack16<BF16>(cw[e]), w = unpack16<BF16>(gw[e]);
+        s = fmaf(f.x, v.x + w.x, fmaf(f.y, v.y + w.y, s));
       }
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -1564,15 +1592,15 @@ int set_smem(K kernel, int bytes, bool (&done)[64]) {
 }
 
 template <int D, bool BF16, int NB>
-int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, const AttnArgs& p,
-            cudaStream_t st) {
+int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o,
+            const CUtensorMap& lo, const AttnArgs& p, cudaStream_t st) {
   static bool done[64] = {};
   const int smem = Fwd<D, NB>::smem(p.rb);
   int rc = set_smem(attn_fwd_kernel<D, BF16, NB>, smem, done);
   if (rc) return rc;
   const long long grid = static_cast<long long>((p.Lq + kRows - 1) / kRows) * p.splits * p.H * p.B;
   if (grid > 0x7fffffffll) return WDIT_ERR_SHAPE;
-  attn_fwd_kernel<D, BF16, NB><<<static_cast<unsigned>(grid), Fwd<D, NB>::kThreads, smem, st>>>(q, k, v, o, p);
+  attn_fwd_kernel<D, BF16, NB><<<static_cast<unsigned>(grid), Fwd<D, NB>::kThreads, smem, st>>>(q, k, v, o, lo, p);
   rc = cuda_rc(cudaGetLastError());
   if (rc || p.splits == 1) return rc;
   const long long rows = static_cast<long long>(p.B) * p.H * p.Lq;
@@ -1620,13 +1648,13 @@ long long wdit_rel_attention_workspace_bytes(int B, int H, int Lq, int Lk, int D
 int wdit_rel_attention(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
                        const void* v, const long long* v_strides, int B, int H, int Lq, int Lk, int D, int dtype,
                        const int* k_lens, const void* table, int table_dtype, const int* bounds, int n_bounds,
-                       int bidirectional, int causal, int q_offset, float scale, void* out, float* lse,
+                       int bidirectional, int causal, int q_offset, float scale, void* out, void* out_lo, float* lse,
                        void* workspace, long long workspace_bytes, void* stream) {
   int rc = check_attn(bounds, n_bounds, B, H, Lq, Lk, D, dtype, table_dtype, q_offset, table);
   if (rc) return rc;
   if (B == 0 || Lq == 0) return WDIT_OK;
   if (out == nullptr) return WDIT_ERR_ARG;
-  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0) return WDIT_ERR_ALIGN;
+  if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo)) & 15) != 0) return WDIT_ERR_ALIGN;
   if (Lk == 0) return WDIT_ERR_SHAPE;  // the caller knows the answer: zeros
   if ((rc = check_heads(q, q_strides)) || (rc = check_heads(k, k_strides)) || (rc = check_heads(v, v_strides)))
     return rc;
@@ -1643,6 +1671,7 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
   p.table_dtype = table_dtype;
   if (!rel_fill(&p.rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
   p.out = out;
+  p.out_lo = out_lo;
   p.lse = lse;
   p.splits = attn_splits(B, H, Lq, Lk);
   if (p.splits > 1) {
@@ -1655,18 +1684,19 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
   if ((rc = error_record_ptr(&p.ctx.rec))) return rc;
   p.ctx.limit_ns = wait_limit_ns();
   const bool bf16 = dtype == 1;
-  CUtensorMap mq, mk, mv, mo;
+  CUtensorMap mq, mk, mv, mo, ml = {};
   if ((rc = map_heads(&mq, bf16, q, B, Lq, H, D, {q_strides[0], q_strides[1], q_strides[2]}, kRows)) ||
       (rc = map_heads(&mk, bf16, k, B, Lk, H, D, {k_strides[0], k_strides[1], k_strides[2]}, kCols)) ||
       (rc = map_heads(&mv, bf16, v, B, Lk, H, D, {v_strides[0], v_strides[1], v_strides[2]}, kCols)) ||
       (rc = map_heads(&mo, bf16, out, B, Lq, H, D, {1ll * Lq * H * D, 1ll * H * D, D}, 32)))
     return rc;
+  if (out_lo != nullptr && (rc = map_heads(&ml, bf16, out_lo, B, Lq, H, D, {1ll * Lq * H * D, 1ll * H * D, D}, 32)))
+    return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (D == 128)
-    return bf16 ? run_fwd<128, true, 2>(mq, mk, mv, mo, p, st) : run_fwd<128, false, 2>(mq, mk, mv, mo, p, st);
-  if (four_per_sm(p))
-    return bf16 ? run_fwd<64, true, 1>(mq, mk, mv, mo, p, st) : run_fwd<64, false, 1>(mq, mk, mv, mo, p, st);
-  return bf16 ? run_fwd<64, true, 2>(mq, mk, mv, mo, p, st) : run_fwd<64, false, 2>(mq, mk, mv, mo, p, st);
+  auto go = [&](auto run) { return run(mq, mk, mv, mo, ml, p, st); };
+  if (D == 128) return bf16 ? go(run_fwd<128, true, 2>) : go(run_fwd<128, false, 2>);
+  if (four_per_sm(p)) return bf16 ? go(run_fwd<64, true, 1>) : go(run_fwd<64, false, 1>);
+  return bf16 ? go(run_fwd<64, true, 2>) : go(run_fwd<64, false, 2>);
 }
 
 long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional) {
@@ -1677,19 +1707,18 @@ long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int 
 
 int wdit_rel_attention_backward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
                                 const void* v, const long long* v_strides, const void* dout,
-                                const long long* dout_strides, const void* out, const float* lse, int B, int H, int Lq,
-                                int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
+                                const long long* dout_strides, const void* out, const void* out_lo, const float* lse,
+                                int B, int H, int Lq, int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
                                 const int* bounds, int n_bounds, int bidirectional, int causal, int q_offset,
                                 float scale, void* dq, void* dk, void* dv, void* dtable, int dtable_dtype,
-                                void* workspace,
-                                long long workspace_bytes, void* stream) {
+                                void* workspace, long long workspace_bytes, void* stream) {
   int rc = check_attn(bounds, n_bounds, B, H, Lq, Lk, D, dtype, table_dtype, q_offset, table);
   if (rc) return rc;
   if (B == 0 || Lq == 0 || Lk == 0) return WDIT_ERR_SHAPE;  // the caller knows the answer: zeros
-  if (out == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || dtable == nullptr ||
+  if (out == nullptr || out_lo == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || dtable == nullptr ||
       dtable_dtype < 0 || dtable_dtype > 2)
     return WDIT_ERR_ARG;
-  for (const void* t : {out, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
+  for (const void* t : {out, out_lo, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
     if ((reinterpret_cast<uintptr_t>(t) & 15) != 0) return WDIT_ERR_ALIGN;
   if ((rc = check_heads(q, q_strides)) || (rc = check_heads(k, k_strides)) || (rc = check_heads(v, v_strides)) ||
       (rc = check_heads(dout, dout_strides)))
@@ -1711,6 +1740,7 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
   p.table_dtype = table_dtype;
   if (!rel_fill(&p.rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
   p.out = const_cast<void*>(out);
+  p.out_lo = const_cast<void*>(out_lo);
   p.lse = const_cast<float*>(lse);
   p.splits = 1;
   p.dout = dout;
@@ -1719,9 +1749,6 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
   p.do_h = dout_strides[2];
   p.delta = static_cast<float*>(workspace);
   p.table_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align16(4ll * B * H * Lq));
-  p.dq = dq;
-  p.dk = dk;
-  p.dv = dv;
   if ((rc = error_record_ptr(&p.ctx.rec))) return rc;
   p.ctx.limit_ns = wait_limit_ns();
   const bool bf16 = dtype == 1;
