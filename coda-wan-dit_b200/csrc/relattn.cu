@@ -807,6 +807,7 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
 // score tile, warps 6-9 columns 32-63. D = 64: two CTAs per SM overlap each other; D = 128: one
 // CTA per SM with two score buffers.
 constexpr int kSumReach = 256;  // the table's gradient is summed by diagonal up to this last bound
+constexpr int kExactTiles = 4;  // key tiles up to which delta comes from a pass of its own
 template <int D>
 struct Bwd {
   static constexpr int kThreads = 320;
@@ -818,7 +819,7 @@ struct Bwd {
   static constexpr uint32_t kTile = kCols * D * 2;
   static constexpr int kWarp = 64 + 96 + 64;  // floats per warp: bias line, diagonals, row values
   static int smem(const RelBuckets& rb) {
-    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 8 * 4 * grad_sums(rb) + kRows * 4 +
+    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 8 * 4 * grad_sums(rb) + 2 * kRows * 4 +
            bias_smem(rb);
   }
   // Floats of a warp's sums of the table's gradient: by diagonal, or by bucket.
@@ -890,13 +891,14 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   uint64_t* ds_ready = s_full + 2;  // NB
   uint64_t* done = ds_ready + 2;
   uint64_t* last = done + 1;  // every product is done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
+  uint64_t* delta_ready = last + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(delta_ready + 1);
   float* warps = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
   const int reach = bias_reach(p.rb);
   const bool by_diag = reach <= kSumReach;
   const int nsum = C::grad_sums(p.rb);
   float* sums = warps + 8 * C::kWarp;  // [8][nsum]
-  float* sdelta = sums + 8 * nsum;     // [128]
+  float* sdelta = sums + 8 * nsum;     // [2][128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_tiles = (p.Lq + kRows - 1) / kRows;
@@ -907,8 +909,18 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   const int b = x / p.H;
   const int i0 = qt * kRows;
 
-  auto load_kv = [&](int t) {
-    const int st = t % ST;
+  const int klen = sample_len(p, b);
+  int visible = klen;
+  if (p.causal) visible = min(visible, min(i0 + kRows, p.Lq) + p.q_offset);
+  const int n = (visible + kCols - 1) / kCols;
+  // Few keys: a first pass over the tiles forms delta = rowsum(P dP) itself (see below). Steps of
+  // both passes count through; tile(step) is the key tile.
+  const int pre = n <= kExactTiles ? n : 0;
+  const int steps = pre + n;
+  auto tile = [&](int step) { return step < pre ? step : step - pre; };
+
+  auto load_kv = [&](int step) {
+    const int st = step % ST, t = tile(step);
     mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
@@ -928,12 +940,9 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     }
     mbar_init(done, 1);
     mbar_init(last, 1);
+    mbar_init(delta_ready, 8);
     fence_mbar_init();
   }
-  const int klen = sample_len(p, b);
-  int visible = klen;
-  if (p.causal) visible = min(visible, min(i0 + kRows, p.Lq) + p.q_offset);
-  const int n = (visible + kCols - 1) / kCols;
   if (threadIdx.x == 0 && n > 0) {  // the first loads run under the rest of the set-up
     mbar_arrive_expect_tx(q_full, 2 * C::kBig);
 #pragma unroll
@@ -941,7 +950,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tma_load_4d(sQ + c * 16384, &tmQ, q_full, c * 64, h, i0, b);
       tma_load_4d(sO + c * 16384, &tmO, q_full, c * 64, h, i0, b);
     }
-    for (int t = 0; t < min(n, ST); ++t) load_kv(t);
+    for (int t = 0; t < min(steps, ST); ++t) load_kv(t);
   }
   __syncwarp();
   if (warp == 1) {
@@ -950,10 +959,15 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   }
   for (int t = threadIdx.x; t < 8 * nsum; t += C::kThreads) sums[t] = 0.f;
   // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too: D / 8 lanes a row. O is
-  // taken before its rounding (two 16-bit parts): dP - delta is the small difference of the two
-  // where a row rests on few keys, and its error goes into every cell of the row with one sign, so
-  // into the table's sums undiminished.
-  {
+  // taken before its rounding (two 16-bit parts). Its sum over P rounded to 16 bits remains, which
+  // differs from rowsum(P dP) by up to half a step of each P; that error goes into every cell of
+  // the row with one sign, so into the table's sums undiminished, and is averaged away over many
+  // keys only. Up to kExactTiles tiles delta is therefore rowsum(P dP) from a pass of its own
+  // (table gradient's relative error, its own rounding 1.7e-3 among it, bf16: 5 x 2 heads x 1870 x 2 x
+  // 128 3.9e-2 with the rounded O, 1.5e-2 with its two parts, 1.4e-3 with the pass; 3 heads x 140 x
+  // 140 x 128 2.8e-3, 2.7e-3, 1.7e-3; 8 heads x 512 x 512 x 64 1.7e-3 without the pass, which
+  // takes a third of this kernel's time).
+  if (pre == 0) {
     constexpr int kLanes = D / 8, kAtOnce = C::kThreads / kLanes, kTurns = (kRows + kAtOnce - 1) / kAtOnce;
     const int part = threadIdx.x % kLanes;
     const uint16_t* go = static_cast<const uint16_t*>(p.dout) + b * p.do_b + h * p.do_h;
@@ -998,7 +1012,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     if (warp >= 2 && i < p.Lq) lse = p.lse[(static_cast<long long>(b) * p.H + h) * p.Lq + i];
     if (lse == -kInf) lse = kInf;  // no keys: every P is 0
   }
-  const BiasLine bias = load_bias(p, h, sdelta + kRows, C::kThreads);
+  const BiasLine bias = load_bias(p, h, sdelta + 2 * kRows, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1007,8 +1021,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
 
   if (warp == 0) {
     if (elect_one() && n > 0) {
-      int loaded = min(n, ST);
-      for (int t = ST; t < n; ++t) {
+      int loaded = min(steps, ST);
+      for (int t = ST; t < steps; ++t) {
         if (!wait_parity(&empty[t % ST], ((t / ST) & 1) ^ 1u, kSiteAttnDq, p.ctx)) break;
         load_kv(t);
         loaded = t + 1;
@@ -1020,18 +1034,18 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   } else if (warp == 1) {
     constexpr uint32_t id_s = idesc16(kRows, kCols, BF16, false);
     constexpr uint32_t id_acc = idesc16(kRows, D, BF16, true);
-    auto scores = [&](int t) {
-      const int st = t % ST;
-      const bool ok = wait_parity(&full[st], (t / ST) & 1, kSiteAttnDq + 2, p.ctx);
+    auto scores = [&](int step) {
+      const int st = step % ST, j0 = tile(step) * kCols;
+      const bool ok = wait_parity(&full[st], (step / ST) & 1, kSiteAttnDq + 2, p.ctx);
       if (!__all_sync(0xffffffffu, ok)) return false;
       // rows past the sample's keys would enter dQ as 0 * anything
-      if (t * kCols + kCols > klen) zero_tail<D, kCols>(sK + st * C::kTile, klen - t * kCols, lane);
+      if (j0 + kCols > klen) zero_tail<D, kCols>(sK + st * C::kTile, klen - j0, lane);
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t d = tmem + (t % NB) * 2 * kCols;
+        const uint32_t d = tmem + (step % NB) * 2 * kCols;
         issue_scores<D, kCols>(d, smem_u32(sQ), smem_u32(sK + st * C::kTile), id_s);
         issue_scores<D, kCols>(d + kCols, smem_u32(sO), smem_u32(sV + st * C::kTile), id_s);
-        mma_commit(&s_full[t % NB]);
+        mma_commit(&s_full[step % NB]);
       }
       __syncwarp();
       return true;
@@ -1041,8 +1055,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       ok = wait_parity(q_full, 0, kSiteAttnDq + 3, p.ctx);
       ok = __all_sync(0xffffffffu, ok) && scores(0);
     }
-    for (int t = 0; t < n && ok; ++t) {
-      if (NB == 2 && t + 1 < n) {
+    for (int t = 0; t < steps && ok; ++t) {
+      if (NB == 2 && t + 1 < steps) {
         // the buffer's previous content is still read until the products of t - 1 are done
         if (t > 0) ok = __all_sync(0xffffffffu, wait_parity(done, (t - 1) & 1, kSiteAttnDq + 7, p.ctx));
         if (!ok || !scores(t + 1)) break;
@@ -1052,13 +1066,14 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tc_fence_after();
       const int st = t % ST;
       if (elect_one()) {
-        issue_ts<kCols>(tmem_acc, tmem + (t % NB) * 2 * kCols, smem_u32(sK + st * C::kTile), id_acc, t > 0);
+        if (t >= pre)
+          issue_ts<kCols>(tmem_acc, tmem + (t % NB) * 2 * kCols, smem_u32(sK + st * C::kTile), id_acc, t > pre);
         mma_commit(&empty[st]);
         mma_commit(done);
-        if (t + 1 == n) mma_commit(last);
+        if (t + 1 == steps) mma_commit(last);
       }
       __syncwarp();
-      if (NB == 1 && t + 1 < n)
+      if (NB == 1 && t + 1 < steps)
         ok = __all_sync(0xffffffffu, wait_parity(done, t & 1, kSiteAttnDq + 7, p.ctx)) && scores(t + 1);
     }
   } else {
@@ -1075,7 +1090,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     const int row_end = !row_ok ? 0 : (p.causal ? min(klen, i + p.q_offset + 1) : klen);
     const int warp_first = i0 + wq * 32 + p.q_offset;
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
-    const uint64_t neg_delta = f2_pack(-sdelta[r], -sdelta[r]);
+    uint64_t neg_delta = pre == 0 ? f2_pack(-sdelta[r], -sdelta[r]) : f2_pack(0.f, 0.f);
+    float p_dp = 0.f;  // this row's sum of P dP over the warp's columns
     // The warp's tiles by kind, as in the forward kernel, for its 32 columns of each tile.
     const int t_left = (warp_first - bias.reach - 31 - half * 32 + kCols) / kCols;
     const int t_right = (warp_first + 31 + bias.ahead() - half * 32 + kCols - 1) / kCols;
@@ -1083,7 +1099,18 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     static_assert(kCols == 64, "shift above");
     const float c_left = bias.at(-bias.reach), c_right = bias.at(bias.reach);
     bool ok = true;
-    for (int t = 0; t < n; ++t) {
+    for (int step = 0; step < steps; ++step) {
+      const int t = tile(step);
+      if (pre != 0 && step == pre) {  // the other half's columns are another warp's
+        sdelta[half * kRows + r] = p_dp;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(delta_ready);
+        ok = wait_parity(delta_ready, 0, kSiteAttnDq + 8, p.ctx);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        const float delta = sdelta[r] + sdelta[kRows + r];
+        neg_delta = f2_pack(-delta, -delta);
+        if (half == 0 && row_ok) p.delta[(static_cast<long long>(b) * p.H + h) * p.Lq + i] = delta;
+      }
       const int j0 = t * kCols + half * 32;
       const int d_lo = j0 - warp_first - 31;
       const bool masked = t >= t_mask;
@@ -1095,13 +1122,13 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
         __syncwarp();
       }
       const float* ln = line + 31 - lane;
-      ok = wait_parity(&s_full[t % NB], (t / NB) & 1, kSiteAttnDq + 5, p.ctx);
+      ok = wait_parity(&s_full[step % NB], (step / NB) & 1, kSiteAttnDq + 5, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
-      const uint32_t ts = tmem + lane_off + (t % NB) * 2 * kCols + half * 32;
+      const uint32_t ts = tmem + lane_off + (step % NB) * 2 * kCols + half * 32;
       float s[32], g[32];
       tmem_ld32x2(ts, s, ts + kCols, g);
-      // dS in s
+      // dS in s (first pass: P dP)
       if (flat) {
         const float c = (t < t_left ? c_left : c_right) - lse;
         const uint64_t c2 = f2_pack(c, c);
@@ -1122,6 +1149,14 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
           for (int e = 0; e < 32; ++e) s[e] = e < keep ? s[e] : 0.f;
         }
       }
+      if (step < pre) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_ready[step % NB]);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) p_dp += s[e];
+        continue;
+      }
       uint32_t w[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) w[e] = pack16<BF16>(s[2 * e], s[2 * e + 1]);
@@ -1129,7 +1164,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_ready[t % NB]);
+      if (lane == 0) mbar_arrive(&ds_ready[step % NB]);
       // The table's gradient: the sum of dS by diagonal (the products run meanwhile).
       if (flat) {
         uint64_t a2 = f2_pack(s[0], s[1]), b2 = f2_pack(s[2], s[3]);

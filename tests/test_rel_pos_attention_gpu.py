@@ -280,6 +280,37 @@ def test_masked_buckets_have_finite_gradients(pkg):
     check((out.detach(), *grads), *(t.detach() for t in ts), dout=dout)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Lq,Lk", [(900, 1), (900, 2), (900, 5), (300, 64), (300, 65), (200, 200), (200, 256)])
+def test_table_gradient_of_few_keys(pkg, Lq, Lk, D):
+    """Most rows' cells fall into one bucket there, where their sum is 0: what is left of it are fp32
+    errors, not half steps of a 16-bit type. Per cell P (eps |dP - delta| + d(dP) + d(delta)), delta
+    the fp32 sum of P dP over the row; then the sums of the table."""
+    B, H, nb = 2, 3, 32
+    q, k, v, table = make(B, H, Lq, Lk, D, torch.bfloat16, seed=18)
+    dout = torch.randn(q.shape, generator=torch.Generator().manual_seed(19)).to(torch.bfloat16).to(DEV)
+    t = table.clone().requires_grad_()
+    (got,) = torch.autograd.grad(pkg.ops.rel_pos_attention(q, k, v, t), t, dout)
+    where = bucket_map(Lq, Lk, 0, nb, 128, True)
+    q, k, v, do = (x.double().transpose(1, 2) for x in (q, k, v, dout))
+    bias = table.double().T[:, where][None]
+    z = D**-0.5 * (q @ k.transpose(-1, -2)) + bias
+    p, dp = torch.softmax(z, -1), do @ v.transpose(-1, -2)
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    dz = (D + 4) * U * (D**-0.5 * (q.abs() @ k.abs().transpose(-1, -2)) + bias.abs() + z.amax(-1, keepdim=True).abs())
+    eps = 2 * dz.amax(-1, keepdim=True) + 2.0**-20
+    e_dp = (D + 2) * U * (do.abs() @ v.abs().transpose(-1, -2))
+    e_delta = (p * (eps * dp.abs() + e_dp)).sum(-1, keepdim=True) + (Lk + 2) * U * (p * dp.abs()).sum(-1, keepdim=True)
+    e_ds = p * (eps * (dp - delta).abs() + e_dp + e_delta)
+    depth = 32 + 16 + 5 + 2 * (Lk // 32 + 2) + 8 + B * (Lq // 128 + 1)
+    for h in range(H):
+        want, tol = (torch.zeros(nb, dtype=torch.float64, device=DEV) for _ in range(2))
+        want.index_add_(0, where.flatten(), ds[:, h].sum(0).flatten())
+        tol.index_add_(0, where.flatten(), (e_ds + depth * U * (ds.abs() + e_ds))[:, h].sum(0).flatten())
+        assert ((got[:, h].double() - want).abs() <= tol + 2.0**-24 * want.abs() + 1e-30).all()
+
+
 def test_gradient_against_differences(pkg):
     """Central differences of the op's own forward along one direction per input."""
     q, k, v, table = make(1, 2, 70, 90, 64, torch.float16, seed=11)
