@@ -14,10 +14,17 @@
 // The product is a persistent warp-specialized tcgen05 kernel: warps 0 and 10 load the tiles of A
 // and B by TMA into a shared-memory ring (128-byte swizzle, 64-wide K blocks), warp 1 issues the
 // MMAs into one of two TMEM accumulators, warps 2-9 apply the epilogue of the other: 32 x 32
-// pieces, the residual in and the result out by TMA through the warp's own shared memory. The two
-// loading threads matter: one TMA instruction with its barrier arithmetic takes a single thread
-// about 220 clocks whatever the box size (measured: 37, 74 and 125 bytes per clock and SM for
-// boxes of 8, 16 and 32 KB), so one thread that loads both operands falls behind the MMAs.
+// pieces, the residual in and the result out by TMA through the warp's own shared memory. Two
+// loading threads rather than one gain where a K block takes three loads (B MN-major in pieces:
+// 1024 x 1536 x 8960 27.2 us, one thread 28.1), nothing elsewhere. A piece takes an epilogue warp
+// about 800 clocks without an activation and 2000 with GELU, under the next tile's products; what
+// made it slow (1800 and 3000) were arrivals that release at cluster scope, which wait for all of
+// the thread's stores, bias loads piece by piece, and the tile's place computed for every piece.
+//
+// What bounds it: the tensor pipe for many rows (8192 x 13824 x 5120 fp16 with GELU 761 - 840 us by
+// the card's power, 1.4 - 1.5 PFLOP/s; 4096^3 92 us, the library's product 90), the fixed costs
+// below (1024 x 1536 x 4096 16 us, library 12: set-up 0.9 us, first loads 0.8, last epilogue 1,
+// then 270 clocks a K block at least), the weights' bytes for few (1 x 1536 x 8960 11 us).
 // Tile forms (plan()):
 //   pair    256 x bn tiles over CTA pairs (tcgen05 cta_group::2): many rows
 //   single  128 x bn tiles
@@ -800,7 +807,8 @@ struct Plan {
 // clocks at least (its issuing threads), 2.1 per column otherwise (the tensor pipe: 128 x 192 398,
 // 128 x 256 548; pairs 256 x 192 394, 256 x 256 530), and all CTAs together load about 11 KB a clock
 // from L2 (128 x 128 tiles on every SM: 418 instead of 270). The last tile's epilogue adds 17 clocks
-// per column, an exchange between splits 4200 and 0.45 per element that crosses. What that picks
+// per column (12 bare, 30 with GELU), an exchange between splits 4200 and 0.45 per element that
+// crosses. What that picks
 // (us; next best in brackets):   1 x 1536 x 8960 split 8 of 128 x 128 11.3 (one CTA a tile 46)
 //   256 x 1536 x 8960 split 4 15.6 (pairs, no split 47)   1024 x 1536 x 4096 128 x 128 15.6 (pairs 16.8)
 //   2048 x 1536 x 8960 pairs 256 x 192 42.5 (128 x 192 46.1)   1024 x 8960 x 1536 pairs 256 x 256 23.0
@@ -930,6 +938,8 @@ int run_linear(const void* A, long long lda, int a_mn, const void* B, long long 
   p.m_blocks = (p.M + BM - 1) / BM;
   p.n_blocks = (p.N + p.bn - 1) / p.bn;
   p.k_blocks = (p.K + BK - 1) / BK;
+  // Tiles go down the rows of a column, or, where B does not stay in L2, through groups of eight rows
+  // (us: B of 142 MB, 8192 x 13824 x 5120, 768 by groups, 985 without; 34 MB, 4096^3, 93 and 91).
   p.raster_rows = static_cast<long long>(p.N) * p.K * 2 > kRasterBytes ? kRasterRows : 1;
   int rc = error_record_ptr(&p.ctx.rec);
   if (rc) return rc;

@@ -10,7 +10,8 @@
 // each of the tile's rows + columns - 1 diagonals up once, keeps the table's values for them in
 // shared memory, and writes every row as a shifted window of that line with 16-byte stores. The
 // line is kept as 32-bit words (16-bit types: one copy per element parity) with a word of padding
-// every 32, so that lanes four words apart read different banks.
+// every 32, so that lanes four words apart read different banks. 64 heads x 512 x 512 bf16: 8.1 us,
+// 4.1 TB/s (launch, look-up and the first stores take half of it); 12 heads x 1 x 4097 fp32 4.7 us.
 //
 // Gradient (rel_bias_grad_kernel). A warp takes some rows of a strip of columns, and a lane's
 // accumulators are diagonals, never looked up per cell:
@@ -24,7 +25,9 @@
 // one side to the other; what lies past them goes into one sum per side. Buckets are formed once
 // per CTA. (A table whose last bound is above 512 has no room for that; its strips are added bucket
 // by bucket.) Sums are fp32, the order is fixed (no atomics), and a second small kernel adds the
-// CTAs' partial buckets.
+// CTAs' partial buckets (2 us). Aligned: 40 heads x 2048 x 2048 fp32 100 us, 6.7 TB/s; 2 x 64 heads
+// x 512 x 512 bf16 14 us, 4.7 TB/s (by the other form 148 and 38). Unaligned: 40 heads x 2047 x 2049
+// fp32 120 us, 5.6 TB/s: a seventh of its cells lie in strips that leave the row.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -42,11 +45,10 @@ constexpr int kRelThreads = 256;
 constexpr int kRelWarps = kRelThreads / 32;
 constexpr int kBiasRows = 32;    // rows of a forward tile
 constexpr int kBiasCols = 2048;  // columns of a forward tile
-constexpr int kGradRowsMin = 32;   // rows of a gradient strip: few cells ...
-constexpr int kGradRowsMax = 64;   // ... and many
+constexpr int kGradRowsMin = 32;  // rows of a gradient strip: 32, 64 or 128
+constexpr int kGradRowsMax = 128;
 constexpr int kGradCols = 256;   // columns of a gradient strip (8 per lane)
 constexpr int kGradReach = 512;  // sums per diagonal are kept up to this last bound
-constexpr int kFewBounds = 32;   // up to here bounds are counted straight from the kernel's arguments
 
 constexpr int kRing = 8;  // rows of a parallelogram strip in flight per warp
 
@@ -77,16 +79,6 @@ __device__ __forceinline__ float to_f32<__half>(__half v) {
   return __half2float(v);
 }
 
-// The bucket of d without shared memory when there are few bounds (uniform constant reads, no
-// latency chain), by binary search otherwise.
-__device__ __forceinline__ int bucket_of(const RelBuckets& rb, const int* bounds, int d) {
-  if (rb.n_bounds > kFewBounds) return rel_bucket(bounds, rb.n_bounds, rb.bidirectional, d);
-  const int n = rb.bidirectional ? (d < 0 ? -d : d) : (d < 0 ? -d : 0);
-  int c = 0;
-  for (int i = 0; i < rb.n_bounds; ++i) c += rb.bounds[i] <= n ? 1 : 0;
-  return rb.bidirectional && d > 0 ? c + rb.n_bounds + 1 : c;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kRelThreads)
     rel_bias_kernel(const T* __restrict__ table, const __grid_constant__ RelBuckets rb, int H, int Lq, int Lk,
@@ -104,14 +96,12 @@ __global__ void __launch_bounds__(kRelThreads)
   const int i1 = min(i0 + rows, Lq);
   const int j0 = (static_cast<int>(blockIdx.x) - row_tile * col_tiles) * kBiasCols;
   const int j1 = min(j0 + kBiasCols, Lk);
-  if (rb.n_bounds > kFewBounds) {
-    for (int t = threadIdx.x; t < rb.n_bounds; t += kRelThreads) bounds[t] = rb.bounds[t];
-    __syncthreads();
-  }
+  for (int t = threadIdx.x; t < rb.n_bounds; t += kRelThreads) bounds[t] = rb.bounds[t];
+  __syncthreads();
   const int d0 = j0 - (i1 - 1) - q_offset;  // the tile's first diagonal
   const int nd = (j1 - j0) + (i1 - i0) - 1;
   for (int t = threadIdx.x; t < nd; t += kRelThreads) {
-    const T v = table[static_cast<size_t>(bucket_of(rb, bounds, d0 + t)) * H + h];
+    const T v = table[static_cast<size_t>(rel_bucket(bounds, rb.n_bounds, rb.bidirectional, d0 + t)) * H + h];
     if constexpr (E == 1) {
       line[0][slot(t)] = *reinterpret_cast<const uint32_t*>(&v);
     } else {
@@ -398,32 +388,42 @@ int cuda_rc(cudaError_t e) {
   return WDIT_ERR_CUDA_BASE + static_cast<int>(e);
 }
 
-int rel_cta_target() {
+// At most 34 KB, and 65 KB of rings.
+int grad_smem(const RelBuckets& rb, int buckets, bool vec, int esize) {
+  const int reach = rb.bounds[rb.n_bounds - 1];
+  const int sums = reach <= kGradReach ? reach + (rb.bidirectional ? reach : 0) + 1 : buckets;
+  return grad_fixed_bytes(sums) + (vec ? 0 : kRelWarps * kRing * grad_row_bytes(esize));
+}
+
+int rel_sms() {
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148 * 4;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148 * 4;
-  return n * 4;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  return n;
 }
 
-// Rows of a strip: 64 when there are enough cells to give every warp two strips of that, else 32
-// (more warps with loads in flight).
-int grad_rows(int B, int H, int Lq, int Lk, int target) {
-  int rows = kGradRowsMax;
-  while (rows > kGradRowsMin && static_cast<long long>(B) * H * ((Lq + rows - 1) / rows) * grad_strips(Lk, rows, false) <
-                                    2ll * target * kRelWarps)
-    rows /= 2;
-  return rows;
-}
-
-// CTAs per head of the gradient: about four per SM over all heads, every warp the same number of
-// strips (the last may have fewer), at least one.
-int grad_parts(int B, int H, int Lq, int Lk, int target) {
-  const int rows = grad_rows(B, H, Lq, Lk, target);
-  const long long items = static_cast<long long>(B) * ((Lq + rows - 1) / rows) * grad_strips(Lk, rows, false);
-  const long long most = (target + H - 1) / H * kRelWarps;  // warps per head
-  const long long per = (items + most - 1) / most;
-  const long long x = (items + per * kRelWarps - 1) / (per * kRelWarps);
-  return x < 1 ? 1 : static_cast<int>(x);
+// Rows of a strip and CTAs per head of the gradient. All CTAs run at once (per_sm of them), a head's
+// warps share its strips. Aligned rows: the rows whose rounds of strips cost least, a strip costing
+// its rows and 24 more for its ends (us with 32 / 64 / 128 rows, bf16: 64 heads x 512 x 512 9.6 /
+// 10.9 / 15.4, twice that batch 15.9 / 15.4 / 21.3, eight times 51.5 / 49.9 / 48.7). Unaligned rows:
+// 32 (40 heads x 2047 x 2049 fp32 122 / 164 / 164, 12 heads x 333 x 333 fp16 18 / 30 / 54).
+struct GradPlan {
+  int rows, parts;
+};
+GradPlan grad_plan(int B, int H, int Lq, int Lk, bool vec, int per_sm, int sms) {
+  const long long most = sms * per_sm / H > 0 ? sms * per_sm / H : 1;
+  GradPlan best = {kGradRowsMin, 1};
+  long long best_cost = -1;
+  for (int rows = kGradRowsMin; rows <= (vec ? kGradRowsMax : kGradRowsMin); rows *= 2) {
+    const long long items = static_cast<long long>(B) * ((Lq + rows - 1) / rows) * grad_strips(Lk, rows, vec);
+    const long long rounds = (items + most * kRelWarps - 1) / (most * kRelWarps);
+    const long long cost = rounds * (rows + 24);
+    if (best_cost < 0 || cost < best_cost) {
+      best_cost = cost;
+      best = {rows, static_cast<int>((items + rounds * kRelWarps - 1) / (rounds * kRelWarps))};
+    }
+  }
+  return best;
 }
 
 template <typename T>
@@ -440,20 +440,15 @@ int launch_bias(const void* table, const RelBuckets& rb, int H, int Lq, int Lk, 
 
 template <typename T>
 int launch_grad(const void* db, const RelBuckets& rb, int B, int H, int Lq, int Lk, int q_offset, long long sb,
-                long long sh, long long si, int buckets, int parts, int rows, float* part, cudaStream_t st) {
-  constexpr long long V = 16 / static_cast<long long>(sizeof(T));
-  const bool vec = (reinterpret_cast<uintptr_t>(db) & 15) == 0 && sb % V == 0 && sh % V == 0 && si % V == 0;
-  const int reach = rb.bounds[rb.n_bounds - 1];
-  const int sums = reach <= kGradReach ? reach + (rb.bidirectional ? reach : 0) + 1 : buckets;
-  // at most 34 KB, and 65 KB of rings
-  const size_t smem =
-      grad_fixed_bytes(sums) + (vec ? 0 : kRelWarps * kRing * grad_row_bytes(static_cast<int>(sizeof(T))));
+                long long sh, long long si, int buckets, bool vec, GradPlan plan, float* part, cudaStream_t st) {
+  const int rows = plan.rows;
+  const size_t smem = grad_smem(rb, buckets, vec, static_cast<int>(sizeof(T)));
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(rel_bias_grad_kernel<T, false>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
     if (e != cudaSuccess) return cuda_rc(e);
   }
-  const dim3 grid(parts, H);
+  const dim3 grid(plan.parts, H);
   const T* p = static_cast<const T*>(db);
   if (vec)
     rel_bias_grad_kernel<T, true><<<grid, kRelThreads, smem, st>>>(p, rb, B, Lq, Lk, q_offset, sb, sh, si, buckets,
@@ -506,7 +501,14 @@ int wdit_rel_pos_bias(const void* table, int dtype, const int* bounds, int n_bou
 
 long long wdit_rel_pos_bias_grad_workspace_bytes(int B, int H, int Lq, int Lk, int n_bounds, int bidirectional) {
   if (B <= 0 || H <= 0 || Lq <= 0 || Lk <= 0 || n_bounds < 1) return 0;
-  return 4ll * grad_parts(B, H, Lq, Lk, rel_cta_target()) * H * rel_num_buckets(n_bounds, bidirectional);
+  // (the rows' alignment and the last bound are not known here: enough for any)
+  const int sms = rel_sms();
+  int parts = grad_plan(B, H, Lq, Lk, true, 2, sms).parts;
+  for (int per_sm = 2; per_sm <= 3; ++per_sm) {
+    const int n = grad_plan(B, H, Lq, Lk, false, per_sm, sms).parts;
+    parts = n > parts ? n : parts;
+  }
+  return 4ll * parts * H * rel_num_buckets(n_bounds, bidirectional);
 }
 
 int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, int Lk, long long stride_b,
@@ -532,17 +534,21 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return WDIT_ERR_ALIGN;
   RelBuckets rb;
   if (!rel_fill(&rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
-  const int parts = grad_parts(B, H, Lq, Lk, rel_cta_target());
-  const int rows = grad_rows(B, H, Lq, Lk, rel_cta_target());
+  const long long V = dtype == 0 ? 4 : 8;
+  const bool vec =
+      (reinterpret_cast<uintptr_t>(dbias) & 15) == 0 && stride_b % V == 0 && stride_h % V == 0 && stride_i % V == 0;
+  // three CTAs per SM where their shared memory fits, two of the aligned form by its registers
+  const int smem = grad_smem(rb, buckets, vec, dtype == 0 ? 4 : 2);
+  const GradPlan plan = grad_plan(B, H, Lq, Lk, vec, !vec && 3 * (smem + 1024) <= 228 * 1024 ? 3 : 2, rel_sms());
   float* part = static_cast<float*>(workspace);
   auto go = [&](auto* type) {
     return launch_grad<std::remove_pointer_t<decltype(type)>>(dbias, rb, B, H, Lq, Lk, q_offset, stride_b, stride_h,
-                                                              stride_i, buckets, parts, rows, part, st);
+                                                              stride_i, buckets, vec, plan, part, st);
   };
   rc = dtype == 0 ? go(static_cast<float*>(nullptr))
                   : (dtype == 1 ? go(static_cast<__nv_bfloat16*>(nullptr)) : go(static_cast<__half*>(nullptr)));
   if (rc) return rc;
-  return launch_rel_table_sum(part, parts, buckets, H, dtable, dtable_dtype, stream);
+  return launch_rel_table_sum(part, plan.parts, buckets, H, dtable, dtable_dtype, stream);
 }
 
 }  // extern "C"
