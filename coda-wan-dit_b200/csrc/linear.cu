@@ -243,6 +243,16 @@ __device__ __forceinline__ float load_scalar(const void* p, long long i, int dty
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
+__device__ __forceinline__ void store_scalar(void* p, long long i, int dtype, float v) {
+  if (dtype == 0) {
+    static_cast<float*>(p)[i] = v;
+  } else if (dtype == 1) {
+    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  } else {
+    static_cast<__half*>(p)[i] = __float2half_rn(v);
+  }
+}
+
 // Epilogue of eight columns of one row (n < N, N % 8 == 0): residual, stores.
 __device__ __forceinline__ void finish8(const LinArgs& p, float (&v)[8], long long row, int n) {
   if (p.pre != nullptr) {
@@ -709,7 +719,7 @@ template <bool BF16, int ACT>
 __global__ void __launch_bounds__(256)
     act_backward_kernel(const uint16_t* __restrict__ dout, long long ldd, const uint16_t* __restrict__ pre,
                         long long ldp, uint16_t* __restrict__ dpre, long long ldq,
-                        float* __restrict__ part, int M, int N) {
+                        float* __restrict__ part, void* __restrict__ dbias, int dbias_dtype, int M, int N) {
   __shared__ float sums[8][kBackCols];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col_blocks = (N + kBackCols - 1) / kBackCols;
@@ -748,7 +758,7 @@ __global__ void __launch_bounds__(256)
       for (int i = 0; i < 8; ++i) acc[i] += d[i];
     }
   }
-  if (part == nullptr) return;
+  if (part == nullptr && dbias == nullptr) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = acc[i];
   __syncthreads();
@@ -757,7 +767,11 @@ __global__ void __launch_bounds__(256)
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
-    part[static_cast<size_t>(chunk) * N + c] = s;
+    if (part != nullptr) {
+      part[static_cast<size_t>(chunk) * N + c] = s;
+    } else {  // one chunk: this is all of it
+      store_scalar(dbias, c, dbias_dtype, s);
+    }
   }
 }
 
@@ -775,13 +789,7 @@ __global__ void __launch_bounds__(256)
   if (w != 0 || n >= N) return;
 #pragma unroll
   for (int i = 1; i < 8; ++i) s += sums[i][lane];
-  if (dtype == 0) {
-    static_cast<float*>(out)[n] = s;
-  } else if (dtype == 1) {
-    static_cast<__nv_bfloat16*>(out)[n] = __float2bfloat16_rn(s);
-  } else {
-    static_cast<__half*>(out)[n] = __float2half_rn(s);
-  }
+  store_scalar(out, n, dtype, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -1012,7 +1020,7 @@ int wdit_linear_act_residual(const void* A, long long lda, int a_mn, const void*
 }
 
 long long wdit_act_backward_workspace_bytes(int M, int N) {
-  if (M <= 0 || N <= 0) return 0;
+  if (M <= kBackRows || N <= 0) return 0;  // one chunk of rows needs no second kernel
   return 4ll * ((M + kBackRows - 1) / kBackRows) * N;
 }
 
@@ -1033,11 +1041,11 @@ int wdit_act_backward(const void* dout, long long ldd, const void* pre, long lon
   if (rc) return rc;
   if (act != kNone && ((rc = check_operand(pre, ldp, N)) || (rc = check_operand(dpre, ldq, N)))) return rc;
   const int chunks = (M + kBackRows - 1) / kBackRows;
-  if (dbias != nullptr) {
+  if (dbias != nullptr && chunks > 1) {
     if (workspace == nullptr || workspace_bytes < wdit_act_backward_workspace_bytes(M, N)) return WDIT_ERR_WORKSPACE;
     if (!aligned16(workspace)) return WDIT_ERR_ALIGN;
   }
-  float* part = dbias != nullptr ? static_cast<float*>(workspace) : nullptr;
+  float* part = dbias != nullptr && chunks > 1 ? static_cast<float*>(workspace) : nullptr;
   const long long blocks = static_cast<long long>((N + kBackCols - 1) / kBackCols) * chunks;
   if (blocks > 0x7fffffffll) return WDIT_ERR_SHAPE;
   const unsigned grid = static_cast<unsigned>(blocks);
@@ -1047,9 +1055,9 @@ int wdit_act_backward(const void* dout, long long ldd, const void* pre, long lon
   auto go = [&](auto kind) {
     constexpr int A = decltype(kind)::value;
     if (dtype == 1)
-      act_backward_kernel<true, A><<<grid, 256, 0, st>>>(g, ldd, x, ldp, d, ldq, part, M, N);
+      act_backward_kernel<true, A><<<grid, 256, 0, st>>>(g, ldd, x, ldp, d, ldq, part, dbias, dbias_dtype, M, N);
     else
-      act_backward_kernel<false, A><<<grid, 256, 0, st>>>(g, ldd, x, ldp, d, ldq, part, M, N);
+      act_backward_kernel<false, A><<<grid, 256, 0, st>>>(g, ldd, x, ldp, d, ldq, part, dbias, dbias_dtype, M, N);
   };
   switch (act) {
     case kRelu: go(std::integral_constant<int, kRelu>{}); break;

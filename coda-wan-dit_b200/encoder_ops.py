@@ -33,12 +33,15 @@ def _require_cuda(*ts: torch.Tensor | None) -> int:
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError("wdit ops run on CUDA tensors only (no CPU implementation)")
         i = t.get_device()
-        if dev >= 0 and i != dev:
-            raise ValueError(f"tensors on different devices: cuda:{dev} and cuda:{i}")
-        dev = i
+        if i != dev:
+            if not t.is_cuda:
+                raise RuntimeError("wdit ops run on CUDA tensors only (no CPU implementation)")
+            if dev >= 0:
+                raise ValueError(f"tensors on different devices: cuda:{dev} and cuda:{i}")
+            dev = i
+    if dev < 0:
+        raise RuntimeError("wdit ops run on CUDA tensors only (no CPU implementation)")
     return dev
 
 
@@ -266,27 +269,28 @@ class _LinearActResidual(torch.autograd.Function):
         x, w, pre = ctx.saved_tensors
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
         N, K = w.shape
-        x2 = x.reshape(-1, K)
+        x2 = x if x.dim() == 2 else x.reshape(-1, K)
         M = x2.shape[0]
         dx = dw = db = None
         dev = x.get_device()
         with _on_device(dev):
-            g = _rows(dout.reshape(-1, N)) if need_x or need_w or need_b else None
+            g = _rows(dout if dout.dim() == 2 else dout.reshape(-1, N)) if need_x or need_w or need_b else None
             if g is not None:
                 dpre = x.new_empty((M, N)) if pre is not None else g
                 ws, nbytes = None, 0
                 if need_b:
-                    db = torch.empty(N, dtype=ctx.bias_dtype, device=x.device)
+                    db = x.new_empty(N, dtype=ctx.bias_dtype)
                     nbytes = _workspace_bytes(dev, "wdit_act_backward_workspace_bytes", M, N)
                     ws = _workspace(nbytes, x.device)
                 if need_b or pre is not None:
                     call("wdit_act_backward", ptr(g), _ld(g), ptr(pre), N, _ACT[ctx.act] if pre is not None else 0,
                          _DTYPE[x.dtype], M, N, ptr(dpre), _ld(dpre), ptr(db), 0 if db is None else _DTYPE[db.dtype],
-                         ptr(ws), nbytes, _stream(dev), kernels=2 if need_b else 1)
+                         ptr(ws), nbytes, _stream(dev), kernels=2 if nbytes > 0 else 1)
                 if need_x:
                     dx = x.new_empty((M, K))
                     _product(dev, dpre, 0, _rows(w), 1, M, K, N, dx)
-                    dx = dx.view(x.shape)
+                    if x.dim() != 2:
+                        dx = dx.view(x.shape)
                 if need_w:
                     if M == 0:
                         dw = torch.zeros((N, K), dtype=w.dtype, device=w.device)
@@ -321,11 +325,14 @@ def linear_act_residual(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | N
     shape = (*xs[:-1], N)
     if bias is not None and (bias.shape != (N,) or bias.dtype not in _DTYPE):
         raise ValueError(f"bias must be [{N}] of fp32, bf16 or fp16, got {tuple(bias.shape)} {bias.dtype}")
-    for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (t.shape != shape or t.dtype is not dtype):
-            raise ValueError(f"{name} must be {shape} of {dtype}, got {tuple(t.shape)} {t.dtype}")
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype):
+        raise ValueError(f"residual must be {shape} of {dtype}, got {tuple(residual.shape)} {residual.dtype}")
+    if out is not None and (out.shape != shape or out.dtype is not dtype):
+        raise ValueError(f"out must be {shape} of {dtype}, got {tuple(out.shape)} {out.dtype}")
     dev = _require_cuda(x, w, bias, residual, out)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual, out)):
+    if torch.is_grad_enabled() and (
+            x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad) or (out is not None and out.requires_grad)):
         if out is not None:
             raise ValueError("out= is not supported where a gradient is recorded")
         return _LinearActResidual.apply(x, w, bias, act, residual)

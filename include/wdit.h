@@ -379,7 +379,7 @@ int wdit_linear_act_residual(const void* A, long long lda, int a_mn, const void*
 /*
  * dpre[M, N] = dout * act'(pre) and, unless dbias is NULL, dbias[N] (dbias_dtype) = the column sums
  * of dpre before its rounding (fp32 sums in a fixed order). act = 0: dpre is dout, pre and dpre are
- * not looked at. The workspace (only with dbias) needs no initialization.
+ * not looked at. The workspace (only with dbias, and 0 bytes for up to 64 rows) needs no initialization.
  */
 long long wdit_act_backward_workspace_bytes(int M, int N);
 int wdit_act_backward(const void* dout, long long ldd, const void* pre, long long ldp, int act, int dtype, int M, int N,

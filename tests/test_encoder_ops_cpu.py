@@ -187,7 +187,7 @@ def test_linear_entry_points_validate_without_device(pkg):
     assert lin(lda=68) == 3 and lin(A=ctypes.c_void_p(0x1008)) == 3 and lin(res=ctypes.c_void_p(0x1002)) == 3
     assert lin(A=null, out=null, M=0) == 0
 
-    def back(dout=d, pre=d, act=3, dtype=1, M=4, N=32, dpre=d, db=d, dbt=0, ws=d, nb=1 << 20, ld=32):
+    def back(dout=d, pre=d, act=3, dtype=1, M=400, N=32, dpre=d, db=d, dbt=0, ws=d, nb=1 << 20, ld=32):
         return lib.wdit_act_backward(dout, ld, pre, ld, act, dtype, M, N, dpre, ld, db, dbt, ws, nb, null)
 
     assert back(dout=null) == 1 and back(pre=null) == 1 and back(dpre=null) == 1 and back(act=9) == 1
@@ -196,6 +196,7 @@ def test_linear_entry_points_validate_without_device(pkg):
     assert back(ld=36) == 3 and back(ws=null) == 5 and back(nb=16) == 5
     assert back(act=0, db=null, dout=null) == 0  # dpre is dout, no bias: nothing to do
     assert lib.wdit_act_backward_workspace_bytes(65, 32) == 4 * 2 * 32
+    assert lib.wdit_act_backward_workspace_bytes(64, 32) == 0
 
 
 def test_attention_entry_points_validate_without_device(pkg):
