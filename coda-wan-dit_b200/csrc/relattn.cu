@@ -51,6 +51,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kRows = 128;  // accumulator rows of a CTA
 constexpr int kCols = 64;   // columns of a score tile
+constexpr int kMaxSplits = 64;
 enum : unsigned int { kSiteAttn = 16, kSiteAttnDq = 32, kSiteAttnDkv = 48 };
 
 struct AttnArgs {
@@ -769,21 +770,42 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
   const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
-  float m = -kInf;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_lse[s * rows + row]);
-  const float ms = m == -kInf ? 0.f : m;
-  float total = 0.f;
   constexpr int V = D / 32;  // columns per lane
-  float acc[V];
+  constexpr int kAhead = 4;  // parts in flight: the first ones are loaded together with the sums
+  const float* src = p.part_o + row * D + lane * V;
+  float part[kAhead][V];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+      for (int q = 0; q < V; ++q) part[s][q] = base + s < p.splits ? src[(base + s) * rows * D + q] : 0.f;
+  };
+  load(0);
+  static_assert(kMaxSplits == 64, "two parts a lane");
+  const float lse0 = lane < p.splits ? p.part_lse[lane * rows + row] : -kInf;
+  const float lse1 = lane + 32 < p.splits ? p.part_lse[(lane + 32) * rows + row] : -kInf;
+  float m = fmaxf(lse0, lse1);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float ms = m == -kInf ? 0.f : m;
+  const float w0 = exp2f(lse0 - ms), w1 = exp2f(lse1 - ms);
+  float total = 0.f, acc[V];
 #pragma unroll
   for (int q = 0; q < V; ++q) acc[q] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float w = exp2f(p.part_lse[s * rows + row] - ms);
-    total += w;
-    const float* src = p.part_o + (s * rows + row) * D + lane * V;
-    if (w == 0.f) continue;
+  for (int base = 0; base < p.splits; base += kAhead) {
+    float now[kAhead][V];
 #pragma unroll
-    for (int q = 0; q < V; ++q) acc[q] = fmaf(w, src[q], acc[q]);
+    for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+      for (int q = 0; q < V; ++q) now[s][q] = part[s][q];
+    load(base + kAhead);
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {  // (weights past the last part are 0)
+      const float w = __shfl_sync(0xffffffffu, base < 32 ? w0 : w1, (base + s) & 31);
+      total += w;
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] = w == 0.f ? acc[q] : fmaf(w, now[s][q], acc[q]);
+    }
   }
   const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
   const int i = static_cast<int>(row % p.Lq);
@@ -1559,7 +1581,7 @@ int attn_splits(int B, int H, int Lq, int Lk) {
   if (ctas <= 0) return 1;
   long long s = 2ll * attn_sms() / ctas;
   if (s > tiles / 4) s = tiles / 4;
-  return s < 1 ? 1 : (s > 64 ? 64 : static_cast<int>(s));
+  return s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : static_cast<int>(s));
 }
 
 // Which forward of D = 64: four CTAs per SM with one score buffer each, or two with two. Four win
