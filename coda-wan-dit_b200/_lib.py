@@ -178,12 +178,12 @@ launch_counter = {"n": 0}
 def call(name: str, *args, kernels: int = 1) -> int:
     """Call a library entry point on the current torch device and raise on failure.
     `kernels`: device kernels the entry point launches (counted in launch_counter)."""
-    lib = load()
+    lib = _lib if _lib is not None else load()
     _sync_device(lib)
     if name in _LAUNCHING:
         launch_counter["n"] += kernels
     rc = getattr(lib, name)(*args)
-    if isinstance(rc, int) and not name.endswith("_bytes"):
+    if rc and not name.endswith("_bytes"):
         check(rc, name)
     return rc
 

@@ -217,34 +217,38 @@ def rel_pos_bias(table: torch.Tensor, q_len: int, k_len: int, *, bidirectional: 
 _ACT = {"none": 0, "gelu_tanh": 1, "relu": 2, "silu": 3, "gelu": 4}
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """2-D operand the kernels take as it is (unit column stride, rows on 16-byte boundaries),
-    or a contiguous copy."""
-    ld, one = t.stride()
-    if one == 1 and (t.shape[0] <= 1 or (ld % 8 == 0 and ld >= t.shape[1])) and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _rows(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
+    """2-D operand of `cols` (a multiple of 8) columns with its pointer and row stride, as the
+    kernels take it (unit column stride, rows on 16-byte boundaries), or a contiguous copy."""
+    p = t.data_ptr()
+    if p & 15 == 0:
+        if t.is_contiguous():
+            return t, p, cols
+        ld, one = t.stride()
+        if one == 1 and (t.shape[0] <= 1 or (ld % 8 == 0 and ld >= cols)):
+            return t, p, ld if t.shape[0] > 1 else cols  # a single row's stride says nothing
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), cols
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]  # a single row's stride says nothing
-
-
-def _product(dev, a, a_mn, b, b_mn, M, N, K, out, bias=None, act=0, res=None, pre=None):
-    call("wdit_linear_act_residual", a.data_ptr(), _ld(a), a_mn, b.data_ptr(), _ld(b), b_mn, M, N, K, _DTYPE[a.dtype],
-         None if bias is None else bias.data_ptr(), 0 if bias is None else _DTYPE[bias.dtype], act,
-         None if res is None else res.data_ptr(), 0 if res is None else _ld(res), out.data_ptr(), N,
-         None if pre is None else pre.data_ptr(), N, _stream(dev))
+def _product(dev, dtype, a, a_mn, b, b_mn, M, N, K, out, bias=None, act=0, res=None, pre=None):
+    """a, b, res as _rows gives them."""
+    _, pa, lda = a
+    _, pb, ldb = b
+    pr, ldr = (None, 0) if res is None else res[1:]
+    call("wdit_linear_act_residual", pa, lda, a_mn, pb, ldb, b_mn, M, N, K, _DTYPE[dtype],
+         None if bias is None else bias.data_ptr(), 0 if bias is None else _DTYPE[bias.dtype], act, pr, ldr,
+         out.data_ptr(), N, None if pre is None else pre.data_ptr(), N, _stream(dev))
 
 
 def _linear_forward(dev, x, w, bias, act, residual, out, pre):
     N, K = w.shape
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     if residual is not None:
-        residual = _rows(residual if residual.dim() == 2 else residual.reshape(-1, N))
+        residual = _rows(residual if residual.dim() == 2 else residual.reshape(-1, N), N)
     if bias is not None and bias.stride(0) != 1:
         bias = bias.contiguous()
-    _product(dev, _rows(x2), 0, _rows(w), 0, x2.shape[0], N, K, out, bias, _ACT[act], residual, pre)
+    _product(dev, x.dtype, _rows(x2, K), 0, _rows(w, K), 0, x2.shape[0], N, K, out, bias, _ACT[act], residual, pre)
 
 
 class _LinearActResidual(torch.autograd.Function):
@@ -274,21 +278,24 @@ class _LinearActResidual(torch.autograd.Function):
         dx = dw = db = None
         dev = x.get_device()
         with _on_device(dev):
-            g = _rows(dout if dout.dim() == 2 else dout.reshape(-1, N)) if need_x or need_w or need_b else None
-            if g is not None:
-                dpre = x.new_empty((M, N)) if pre is not None else g
+            if need_x or need_w or need_b:
+                g = _rows(dout if dout.dim() == 2 else dout.reshape(-1, N), N)
+                dpre = g
+                if pre is not None:
+                    t = x.new_empty((M, N))
+                    dpre = (t, t.data_ptr(), N)
                 ws, nbytes = None, 0
                 if need_b:
                     db = x.new_empty(N, dtype=ctx.bias_dtype)
                     nbytes = _workspace_bytes(dev, "wdit_act_backward_workspace_bytes", M, N)
                     ws = _workspace(nbytes, x.device)
                 if need_b or pre is not None:
-                    call("wdit_act_backward", ptr(g), _ld(g), ptr(pre), N, _ACT[ctx.act] if pre is not None else 0,
-                         _DTYPE[x.dtype], M, N, ptr(dpre), _ld(dpre), ptr(db), 0 if db is None else _DTYPE[db.dtype],
+                    call("wdit_act_backward", g[1], g[2], ptr(pre), N, _ACT[ctx.act] if pre is not None else 0,
+                         _DTYPE[x.dtype], M, N, dpre[1], dpre[2], ptr(db), 0 if db is None else _DTYPE[db.dtype],
                          ptr(ws), nbytes, _stream(dev), kernels=2 if nbytes > 0 else 1)
                 if need_x:
                     dx = x.new_empty((M, K))
-                    _product(dev, dpre, 0, _rows(w), 1, M, K, N, dx)
+                    _product(dev, x.dtype, dpre, 0, _rows(w, K), 1, M, K, N, dx)
                     if x.dim() != 2:
                         dx = dx.view(x.shape)
                 if need_w:
@@ -296,7 +303,7 @@ class _LinearActResidual(torch.autograd.Function):
                         dw = torch.zeros((N, K), dtype=w.dtype, device=w.device)
                     else:
                         dw = w.new_empty((N, K))
-                        _product(dev, dpre, 1, _rows(x2), 1, N, K, M, dw)
+                        _product(dev, x.dtype, dpre, 1, _rows(x2, K), 1, N, K, M, dw)
         return dx, dw, db, None, dout if need_r else None
 
 
@@ -377,6 +384,8 @@ def _check_out_overlap(out, residual, *inputs) -> None:
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """[B, L, H, D] the kernels take as it is (unit stride along D, the other strides positive
     multiples of 8 elements, 16-byte aligned), or a contiguous copy."""
+    if t.is_contiguous() and t.data_ptr() & 15 == 0:
+        return t
     (B, L, H, _), (sb, sl, sh, sd) = t.shape, t.stride()
     if (sd == 1 and t.data_ptr() % 16 == 0 and (B == 1 or (sb > 0 and sb % 8 == 0))
             and (L == 1 or (sl > 0 and sl % 8 == 0)) and (H == 1 or (sh > 0 and sh % 8 == 0))):
@@ -384,13 +393,14 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-_Strides = ctypes.c_longlong * 3
+@lru_cache(maxsize=1024)
+def _strides_arg(B: int, L: int, H: int, D: int, sb: int, sl: int, sh: int, _: int):
+    # a dimension of size 1 has no meaningful stride; any valid one does
+    return (ctypes.c_longlong * 3)(sb if B > 1 else D, sl if L > 1 else D, sh if H > 1 else D)
 
 
 def _strides(t: torch.Tensor):
-    # a dimension of size 1 has no meaningful stride; any valid one does
-    (B, L, H, D), (sb, sl, sh, _) = t.shape, t.stride()
-    return _Strides(sb if B > 1 else D, sl if L > 1 else D, sh if H > 1 else D)
+    return _strides_arg(*t.shape, *t.stride())
 
 
 def _attention_args(q, k, table, k_lens, bidirectional, causal, max_distance, q_offset, scale):
