@@ -305,3 +305,22 @@ def test_gradients_of_more_row_chunks_than_a_grid_dimension_holds(pkg):
     total = dout.float().sum(0)
     assert torch.equal(out, torch.ones_like(out)) and not dx.any()
     assert torch.equal(db, total) and torch.equal(dw.float(), total[:, None].expand(8, 8))
+
+
+def test_one_row_without_a_batch_dimension(pkg):
+    g = torch.Generator().manual_seed(41)
+    x, w, r = (torch.randn(*s, generator=g).to(torch.bfloat16).to(DEV) for s in ((64,), (32, 64), (32,)))
+    want = pkg.ops.linear_act_residual(x[None], w, act="relu", residual=r[None])[0]
+    assert torch.equal(pkg.ops.linear_act_residual(x, w, act="relu", residual=r), want)
+    ts = [t.clone().requires_grad_() for t in (x, w, r)]
+    out = pkg.ops.linear_act_residual(ts[0], ts[1], act="relu", residual=ts[2])
+    out.sum().backward()  # a broadcast gradient
+    assert out.shape == (32,) and all(t.grad.shape == t.shape for t in ts) and (ts[2].grad == 1).all()
+
+
+def test_the_same_tensor_as_operand_and_residual(pkg):
+    g = torch.Generator().manual_seed(42)
+    x, w = (torch.randn(*s, generator=g).to(torch.bfloat16).to(DEV) for s in ((40, 64), (64, 64)))
+    assert torch.equal(pkg.ops.linear_act_residual(x, w, residual=x), pkg.ops.linear_act_residual(x, w, residual=x.clone()))
+    with pytest.raises(ValueError, match="overlaps an operand"):
+        pkg.ops.linear_act_residual(x, w, out=x)

@@ -236,6 +236,39 @@ def test_gradients(pkg, B, H, Lq, Lk, D, dtype):
         check((out.detach(), *grads), *(t.detach() for t in (q, k, v, table)), dout=dout, **kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Lq,Lk", [(3, 110, 130, 77), (5, 31, 300, 300)])
+def test_gradients_of_more_ctas_than_two_per_sm(pkg, B, H, Lq, Lk, dtype):
+    q, k, v, table = (t.requires_grad_() for t in make(B, H, Lq, Lk, 64, dtype, seed=21))
+    lens = torch.tensor([[Lk, 0, Lk // 2, 65, 64][b % 5] for b in range(B)], dtype=torch.int32, device=DEV)
+    dout = torch.randn(q.shape, generator=torch.Generator().manual_seed(22)).to(dtype).to(DEV)
+    for kw in (dict(k_lens=lens), dict(causal=True, q_offset=5)):
+        out = pkg.ops.rel_pos_attention(q, k, v, table, **kw)
+        grads = torch.autograd.grad(out, [q, k, v, table], dout)
+        check((out.detach(), *grads), *(t.detach() for t in (q, k, v, table)), dout=dout, **kw)
+
+
+def test_gradients_of_some_inputs_and_a_summed_output(pkg):
+    """Only what is asked for is returned; the gradient of a sum arrives as a broadcast tensor; the
+    same tensor as q, k and v gets the sum of the three."""
+    q, k, v, table = make(2, 2, 70, 70, 64, torch.bfloat16, seed=23)
+    ones = torch.ones_like(q)
+    ts = [t.clone().requires_grad_() for t in (q, k, v, table)]
+    want = torch.autograd.grad(pkg.ops.rel_pos_attention(*ts), ts, ones)
+    for n in range(4):
+        args = [t.clone() for t in (q, k, v, table)]
+        args[n].requires_grad_()
+        pkg.ops.rel_pos_attention(*args).sum().backward()
+        assert torch.equal(args[n].grad, want[n])
+    x = q.clone().requires_grad_()
+    (got,) = torch.autograd.grad(pkg.ops.rel_pos_attention(x, x, x, table), x, ones)
+    three = [q.clone().requires_grad_() for _ in range(3)]
+    parts = torch.autograd.grad(pkg.ops.rel_pos_attention(*three, table), three, ones)
+    total = sum(p.double() for p in parts)
+    step = 2.0**-8 * sum(p.double().abs() for p in parts)  # two rounded adds, half a step each
+    assert ((got.double() - total).abs() <= 2 * step).all()
+
+
 @pytest.mark.parametrize("nb,md,bi", [(2, 2, False), (512, 3000, True), (8, 5, True), (64, 70, False)])
 def test_gradients_of_bucket_rules(pkg, nb, md, bi):
     q, k, v, table = (t.requires_grad_() for t in make(2, 2, 200, 330, 64, torch.bfloat16, nb=nb, seed=3))
