@@ -710,7 +710,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// dpre = dout * act'(pre), and the column sums of dpre by row chunks (bias gradient)
+// dpre = dout * act'(pre), and the column sums of dpre by row chunks (bias gradient). One pass bound
+// by HBM: 4095 x 8960 bf16 SiLU 43.5 us, 5.1 TB/s
 // ---------------------------------------------------------------------------
 constexpr int kBackRows = 64;  // rows of one block
 constexpr int kBackCols = 256;
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
   if (n < N) {
-#pragma unroll 4
+#pragma unroll 2  // (8 rows at a time take registers from other warps: 52 us, 4 47, 2 43.5)
     for (int m = m0 + warp; m < m1; m += 8) {
       const uint4 g = __ldg(reinterpret_cast<const uint4*>(dout + m * ldd + n));
       const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
