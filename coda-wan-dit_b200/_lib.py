@@ -86,10 +86,10 @@ _SIGNATURES = {
     "wdit_rel_pos_bias_grad": (c_int, [P, I, I, I, I, I, c_longlong, c_longlong, c_longlong, P, I, I, I, P, I, P,
                                        c_longlong, P]),
     "wdit_rel_attention_workspace_bytes": (c_longlong, [I, I, I, I, I]),
-    "wdit_rel_attention": (c_int, [P, P, P, P, P, P, I, I, I, I, I, I, P, P, I, P, I, I, I, I, F, P, P, P, P,
-                                   c_longlong, P]),
+    "wdit_rel_attention": (c_int, [P, P, P, P, P, P, I, I, I, I, I, I, P, P, I, P, I, I, I, I, F, P, P, P, c_longlong,
+                                   P]),
     "wdit_rel_attention_backward_workspace_bytes": (c_longlong, [I, I, I, I, I]),
-    "wdit_rel_attention_backward": (c_int, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, P, P, I, P, I, I, I, I, F,
+    "wdit_rel_attention_backward": (c_int, [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, P, P, I, P, I, I, I, I, F,
                                             P, P, P, P, I, P, c_longlong, P]),
     "wdit_linear_act_residual": (c_int, [P, c_longlong, I, P, c_longlong, I, I, I, I, I, P, I, I, P, c_longlong, P,
                                          c_longlong, P, c_longlong, P]),

@@ -4,7 +4,7 @@
 //   j <= i + q_offset when causal),  P = softmax(S) over the visible keys,  O = P v
 //   (a row that sees no key gives 0 and lse = -inf).
 //
-// Backward, with delta = rowsum(dO O) and lse kept by the forward:
+// Backward, with delta = rowsum(P dP) and lse kept by the forward:
 //   dV = P^T dO,  dP = dO v^T,  dS = P (dP - delta),  dQ = scale dS k,  dK = scale dS^T q,
 //   dtable[bucket, h] = the sum of dS over its cells.
 //
@@ -19,10 +19,18 @@
 // registers and written back to TMEM in 16 bits as the A operand of the next product, so nothing
 // of size Lq x Lk leaves the SM.
 //
+// delta is rowsum(dO O) too, but O holds its own rounding and that of P to 16 bits; the error goes into
+// every cell of a row with one sign, and so into the table's sums, whose cells cancel, undiminished
+// (table gradient off by, relative, bf16: 5 x 2 heads x 1870 queries x 2 keys x 128 3.9e-2, with O kept
+// in 32 bits still 1.5e-2, and 6e-3 at 2 heads x 2000 x 280 x 128; its own rounding alone is 1.7e-3).
+// So delta is formed from P and dP as dS is, in fp32, in a first pass over the keys: 15 of
+// attn_dq_kernel's 59 us at 2 x 64 heads x 512 x 512 x 64, 33 of 92 at 74 x 512 x 2048.
+//
 //   attn_fwd_kernel  CTA = 128 query rows of one head; key tiles of 64; one or two warps load and
 //                    issue MMAs, four are the softmax (one row per thread). With few CTAs the
 //                    keys are split over several, whose parts attn_combine_kernel joins.
-//   attn_dq_kernel   same rows; computes delta, dQ and the table's partial sums. No atomics.
+//   attn_dq_kernel   same rows, twice over the keys: first delta, then dQ and the table's partial
+//                    sums. No atomics.
 //   attn_dkv_kernel  CTA = 128 keys; runs over query tiles of 64 with the scores transposed, so
 //                    P^T and dS^T are the A operands; dK and dV stay in TMEM.
 //
@@ -63,14 +71,11 @@ struct AttnArgs {
   int table_dtype;
   RelBuckets rb;
   void* out;           // [B, Lq, H, D] contiguous
-  void* out_lo;        // the same: what rounding took from out; nullable in the forward
   float* lse;          // [B, H, Lq], log2 units; nullable
   int splits;          // forward: key splits; > 1 writes part_o / part_lse instead
   float* part_o;       // [splits][B * H * Lq][D]
   float* part_lse;     // [splits][B * H * Lq]
   // backward
-  const void* dout;    // element strides below, unit along D
-  long long do_b, do_l, do_h;
   float* delta;        // [B, H, Lq]
   float* table_part;   // [H][B * q tiles][buckets]
   WaitCtx ctx;
@@ -87,14 +92,6 @@ template <bool BF16>
 __device__ __forceinline__ float2 unpack16(uint32_t w) {
   if constexpr (BF16) return unpack_bf16x2(w);
   return __half22float2(*reinterpret_cast<__half2*>(&w));
-}
-
-// a and b rounded to 16 bits, and what that took from them.
-template <bool BF16>
-__device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack16<BF16>(a, b);
-  const float2 f = unpack16<BF16>(hi);
-  lo = pack16<BF16>(a - f.x, b - f.y);
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -363,7 +360,7 @@ template <int D, bool BF16, int NB>
 __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmOut,
-                    const __grid_constant__ CUtensorMap tmLo, const __grid_constant__ AttnArgs p) {
+                    const __grid_constant__ AttnArgs p) {
   using C = Fwd<D, NB>;
   constexpr int ST = C::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -703,11 +700,8 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
       }
     }
     // The rows go out through the query tile's shared memory (every product that reads it is
-    // done), 32 rows x 128 bytes a TMA store and warp: rows past Lq are left out by the map. What
-    // their rounding loses goes out through the K tiles' in the same way.
+    // done), 32 rows x 128 bytes a TMA store and warp: rows past Lq are left out by the map.
     uint8_t* stage = sQ + wq * 32 * 128;
-    uint8_t* stage_lo = sK + wq * 32 * 128;
-    static_assert(ST * C::kTile >= C::kQ, "place for the lost parts");
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       float o[32];
@@ -728,17 +722,11 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
         continue;
       }
       const uint32_t row = smem_u32(stage + (c >> 1) * 16384) + lane * 128;
-      const uint32_t row_lo = smem_u32(stage_lo + (c >> 1) * 16384) + lane * 128;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t at16 = (((c & 1) * 4 + q) ^ (lane & 7)) << 4;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          split16<BF16>(o[8 * q + 2 * e], o[8 * q + 2 * e + 1], hi[e], lo[e]);
-        st_shared_v4(row + at16, hi[0], hi[1], hi[2], hi[3]);
-        if (p.out_lo != nullptr) st_shared_v4(row_lo + at16, lo[0], lo[1], lo[2], lo[3]);
-      }
+      for (int q = 0; q < 4; ++q)
+        st_shared_v4(row + ((((c & 1) * 4 + q) ^ (lane & 7)) << 4), pack16<BF16>(o[8 * q], o[8 * q + 1]),
+                     pack16<BF16>(o[8 * q + 2], o[8 * q + 3]), pack16<BF16>(o[8 * q + 4], o[8 * q + 5]),
+                     pack16<BF16>(o[8 * q + 6], o[8 * q + 7]));
     }
     if (p.splits == 1) {
       fence_proxy_async_smem();
@@ -746,10 +734,8 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
       if (lane == 0) {
         if (i0 + wq * 32 < p.Lq) {
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
+          for (int c = 0; c < D / 64; ++c)
             tma_store_4d(&tmOut, stage + c * 16384, c * 64, h, i0 + wq * 32, b);
-            if (p.out_lo != nullptr) tma_store_4d(&tmLo, stage_lo + c * 16384, c * 64, h, i0 + wq * 32, b);
-          }
         }
         bulk_commit();
         bulk_wait_read<0>();  // the stores have read shared memory
@@ -811,14 +797,10 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
   const int i = static_cast<int>(row % p.Lq);
   const int h = static_cast<int>(row / p.Lq % p.H);
   const long long b = row / p.Lq / p.H;
-  const long long to = ((b * p.Lq + i) * p.H + h) * D + lane * V;
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + ((b * p.Lq + i) * p.H + h) * D + lane * V;
 #pragma unroll
-  for (int q = 0; q < V; q += 2) {
-    uint32_t hi, lo;
-    split16<BF16>(acc[q] * inv, acc[q + 1] * inv, hi, lo);
-    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + to + q) = hi;
-    if (p.out_lo != nullptr) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out_lo) + to + q) = lo;
-  }
+  for (int q = 0; q < V; q += 2)
+    *reinterpret_cast<uint32_t*>(dst + q) = pack16<BF16>(acc[q] * inv, acc[q + 1] * inv);
   if (lane == 0 && p.lse != nullptr) p.lse[row] = inv == 0.f ? -kInf : ms + log2f(total);
 }
 
@@ -829,7 +811,6 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
 // score tile, warps 6-9 columns 32-63. D = 64: two CTAs per SM overlap each other; D = 128: one
 // CTA per SM with two score buffers.
 constexpr int kSumReach = 256;  // the table's gradient is summed by diagonal up to this last bound
-constexpr int kExactTiles = 4;  // key tiles up to which delta comes from a pass of its own
 template <int D>
 struct Bwd {
   static constexpr int kThreads = 320;
@@ -935,11 +916,9 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   int visible = klen;
   if (p.causal) visible = min(visible, min(i0 + kRows, p.Lq) + p.q_offset);
   const int n = (visible + kCols - 1) / kCols;
-  // Few keys: a first pass over the tiles forms delta = rowsum(P dP) itself (see below). Steps of
-  // both passes count through; tile(step) is the key tile.
-  const int pre = n <= kExactTiles ? n : 0;
-  const int steps = pre + n;
-  auto tile = [&](int step) { return step < pre ? step : step - pre; };
+  // A first pass over the key tiles forms delta; the steps of both passes count through.
+  const int steps = 2 * n;
+  auto tile = [&](int step) { return step < n ? step : step - n; };
 
   auto load_kv = [&](int step) {
     const int st = step % ST, t = tile(step);
@@ -980,53 +959,6 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     tmem_relinquish();
   }
   for (int t = threadIdx.x; t < 8 * nsum; t += C::kThreads) sums[t] = 0.f;
-  // delta = rowsum(dO O) of the tile's rows, kept for the dK / dV kernel too: D / 8 lanes a row. O is
-  // taken before its rounding (two 16-bit parts). Its sum over P rounded to 16 bits remains, which
-  // differs from rowsum(P dP) by up to half a step of each P; that error goes into every cell of
-  // the row with one sign, so into the table's sums undiminished, and is averaged away over many
-  // keys only. Up to kExactTiles tiles delta is therefore rowsum(P dP) from a pass of its own
-  // (table gradient's relative error, its own rounding 1.7e-3 among it, bf16: 5 x 2 heads x 1870 x 2 x
-  // 128 3.9e-2 with the rounded O, 1.5e-2 with its two parts, 1.4e-3 with the pass; 3 heads x 140 x
-  // 140 x 128 2.8e-3, 2.7e-3, 1.7e-3; 8 heads x 512 x 512 x 64 1.7e-3 without the pass, which
-  // takes a third of this kernel's time).
-  if (pre == 0) {
-    constexpr int kLanes = D / 8, kAtOnce = C::kThreads / kLanes, kTurns = (kRows + kAtOnce - 1) / kAtOnce;
-    const int part = threadIdx.x % kLanes;
-    const uint16_t* go = static_cast<const uint16_t*>(p.dout) + b * p.do_b + h * p.do_h;
-    const long long first = (static_cast<long long>(b) * p.Lq * p.H + h) * D;
-    const uint16_t* oo = static_cast<const uint16_t*>(p.out) + first;
-    const uint16_t* ol = static_cast<const uint16_t*>(p.out_lo) + first;
-    uint4 a[kTurns], c[kTurns], g[kTurns];  // every row's loads are in flight together
-#pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-      const int r = u * kAtOnce + threadIdx.x / kLanes;
-      const long long i = i0 + r;
-      a[u] = c[u] = g[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < kRows && i < p.Lq) {
-        a[u] = __ldg(reinterpret_cast<const uint4*>(go + i * p.do_l) + part);
-        c[u] = __ldg(reinterpret_cast<const uint4*>(oo + i * p.H * D) + part);
-        g[u] = __ldg(reinterpret_cast<const uint4*>(ol + i * p.H * D) + part);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-      const int r = u * kAtOnce + threadIdx.x / kLanes;
-      const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, cw[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
-      const uint32_t gw[4] = {g[u].x, g[u].y, g[u].z, g[u].w};
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack16<BF16>(aw[e]), v = unpack16<BF16>(cw[e]), w = unpack16<BF16>(gw[e]);
-        s = fmaf(f.x, v.x + w.x, fmaf(f.y, v.y + w.y, s));
-      }
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (part == 0 && r < kRows) {
-        sdelta[r] = s;
-        if (i0 + r < p.Lq) p.delta[(static_cast<long long>(b) * p.H + h) * p.Lq + i0 + r] = s;
-      }
-    }
-  }
   // this compute thread's row: its lse, loaded under the set-up too
   float lse = kInf;
   {
@@ -1079,8 +1011,9 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     }
     for (int t = 0; t < steps && ok; ++t) {
       if (NB == 2 && t + 1 < steps) {
-        // the buffer's previous content is still read until the products of t - 1 are done
-        if (t > 0) ok = __all_sync(0xffffffffu, wait_parity(done, (t - 1) & 1, kSiteAttnDq + 7, p.ctx));
+        // the buffer's previous content is still read until the product of t - 1 is done (first pass:
+        // it has been read)
+        if (t > n) ok = __all_sync(0xffffffffu, wait_parity(done, (t - 1 - n) & 1, kSiteAttnDq + 7, p.ctx));
         if (!ok || !scores(t + 1)) break;
       }
       ok = wait_parity(&ds_ready[t % NB], (t / NB) & 1, kSiteAttnDq + 4, p.ctx);
@@ -1088,15 +1021,17 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tc_fence_after();
       const int st = t % ST;
       if (elect_one()) {
-        if (t >= pre)
-          issue_ts<kCols>(tmem_acc, tmem + (t % NB) * 2 * kCols, smem_u32(sK + st * C::kTile), id_acc, t > pre);
+        if (t >= n)
+          issue_ts<kCols>(tmem_acc, tmem + (t % NB) * 2 * kCols, smem_u32(sK + st * C::kTile), id_acc, t > n);
         mma_commit(&empty[st]);
-        mma_commit(done);
+        if (t >= n) mma_commit(done);
         if (t + 1 == steps) mma_commit(last);
       }
       __syncwarp();
-      if (NB == 1 && t + 1 < steps)
-        ok = __all_sync(0xffffffffu, wait_parity(done, t & 1, kSiteAttnDq + 7, p.ctx)) && scores(t + 1);
+      if (NB == 1 && t + 1 < steps) {
+        if (t >= n) ok = __all_sync(0xffffffffu, wait_parity(done, (t - n) & 1, kSiteAttnDq + 7, p.ctx));
+        ok = ok && scores(t + 1);
+      }
     }
   } else {
     const int wq = warp & 3;
@@ -1112,7 +1047,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     const int row_end = !row_ok ? 0 : (p.causal ? min(klen, i + p.q_offset + 1) : klen);
     const int warp_first = i0 + wq * 32 + p.q_offset;
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
-    uint64_t neg_delta = pre == 0 ? f2_pack(-sdelta[r], -sdelta[r]) : f2_pack(0.f, 0.f);
+    uint64_t neg_delta = f2_pack(0.f, 0.f);
     float p_dp = 0.f;  // this row's sum of P dP over the warp's columns
     // The warp's tiles by kind, as in the forward kernel, for its 32 columns of each tile.
     const int t_left = (warp_first - bias.reach - 31 - half * 32 + kCols) / kCols;
@@ -1123,7 +1058,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     bool ok = true;
     for (int step = 0; step < steps; ++step) {
       const int t = tile(step);
-      if (pre != 0 && step == pre) {  // the other half's columns are another warp's
+      if (step == n) {  // the other half's columns are another warp's
         sdelta[half * kRows + r] = p_dp;
         __syncwarp();
         if (lane == 0) mbar_arrive(delta_ready);
@@ -1150,6 +1085,11 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const uint32_t ts = tmem + lane_off + (step % NB) * 2 * kCols + half * 32;
       float s[32], g[32];
       tmem_ld32x2(ts, s, ts + kCols, g);
+      if (step < n) {  // nothing is written back: the next scores may take their place
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_ready[step % NB]);
+      }
       // dS in s (first pass: P dP)
       if (flat) {
         const float c = (t < t_left ? c_left : c_right) - lse;
@@ -1171,12 +1111,16 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
           for (int e = 0; e < 32; ++e) s[e] = e < keep ? s[e] : 0.f;
         }
       }
-      if (step < pre) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ds_ready[step % NB]);
+      if (step < n) {
+        uint64_t a2 = f2_pack(s[0], s[1]), b2 = f2_pack(s[2], s[3]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) p_dp += s[e];
+        for (int e = 4; e < 32; e += 4) {
+          a2 = fadd2(a2, f2_pack(s[e], s[e + 1]));
+          b2 = fadd2(b2, f2_pack(s[e + 2], s[e + 3]));
+        }
+        float x0, x1;
+        f2_unpack(fadd2(a2, b2), x0, x1);
+        p_dp += x0 + x1;
         continue;
       }
       uint32_t w[16];
@@ -1652,14 +1596,14 @@ int set_smem(K kernel, int bytes, bool (&done)[64]) {
 
 template <int D, bool BF16, int NB>
 int run_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o,
-            const CUtensorMap& lo, const AttnArgs& p, cudaStream_t st) {
+            const AttnArgs& p, cudaStream_t st) {
   static bool done[64] = {};
   const int smem = Fwd<D, NB>::smem(p.rb);
   int rc = set_smem(attn_fwd_kernel<D, BF16, NB>, smem, done);
   if (rc) return rc;
   const long long grid = static_cast<long long>((p.Lq + kRows - 1) / kRows) * p.splits * p.H * p.B;
   if (grid > 0x7fffffffll) return WDIT_ERR_SHAPE;
-  attn_fwd_kernel<D, BF16, NB><<<static_cast<unsigned>(grid), Fwd<D, NB>::kThreads, smem, st>>>(q, k, v, o, lo, p);
+  attn_fwd_kernel<D, BF16, NB><<<static_cast<unsigned>(grid), Fwd<D, NB>::kThreads, smem, st>>>(q, k, v, o, p);
   rc = cuda_rc(cudaGetLastError());
   if (rc || p.splits == 1) return rc;
   const long long rows = static_cast<long long>(p.B) * p.H * p.Lq;
@@ -1707,13 +1651,13 @@ long long wdit_rel_attention_workspace_bytes(int B, int H, int Lq, int Lk, int D
 int wdit_rel_attention(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
                        const void* v, const long long* v_strides, int B, int H, int Lq, int Lk, int D, int dtype,
                        const int* k_lens, const void* table, int table_dtype, const int* bounds, int n_bounds,
-                       int bidirectional, int causal, int q_offset, float scale, void* out, void* out_lo, float* lse,
+                       int bidirectional, int causal, int q_offset, float scale, void* out, float* lse,
                        void* workspace, long long workspace_bytes, void* stream) {
   int rc = check_attn(bounds, n_bounds, B, H, Lq, Lk, D, dtype, table_dtype, q_offset, table);
   if (rc) return rc;
   if (B == 0 || Lq == 0) return WDIT_OK;
   if (out == nullptr) return WDIT_ERR_ARG;
-  if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo)) & 15) != 0) return WDIT_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0) return WDIT_ERR_ALIGN;
   if (Lk == 0) return WDIT_ERR_SHAPE;  // the caller knows the answer: zeros
   if ((rc = check_heads(q, q_strides)) || (rc = check_heads(k, k_strides)) || (rc = check_heads(v, v_strides)))
     return rc;
@@ -1730,7 +1674,6 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
   p.table_dtype = table_dtype;
   if (!rel_fill(&p.rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
   p.out = out;
-  p.out_lo = out_lo;
   p.lse = lse;
   p.splits = attn_splits(B, H, Lq, Lk);
   if (p.splits > 1) {
@@ -1743,16 +1686,14 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
   if ((rc = error_record_ptr(&p.ctx.rec))) return rc;
   p.ctx.limit_ns = wait_limit_ns();
   const bool bf16 = dtype == 1;
-  CUtensorMap mq, mk, mv, mo, ml = {};
+  CUtensorMap mq, mk, mv, mo;
   if ((rc = map_heads(&mq, bf16, q, B, Lq, H, D, {q_strides[0], q_strides[1], q_strides[2]}, kRows)) ||
       (rc = map_heads(&mk, bf16, k, B, Lk, H, D, {k_strides[0], k_strides[1], k_strides[2]}, kCols)) ||
       (rc = map_heads(&mv, bf16, v, B, Lk, H, D, {v_strides[0], v_strides[1], v_strides[2]}, kCols)) ||
       (rc = map_heads(&mo, bf16, out, B, Lq, H, D, {1ll * Lq * H * D, 1ll * H * D, D}, 32)))
     return rc;
-  if (out_lo != nullptr && (rc = map_heads(&ml, bf16, out_lo, B, Lq, H, D, {1ll * Lq * H * D, 1ll * H * D, D}, 32)))
-    return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto run) { return run(mq, mk, mv, mo, ml, p, st); };
+  auto go = [&](auto run) { return run(mq, mk, mv, mo, p, st); };
   if (D == 128) return bf16 ? go(run_fwd<128, true, 2>) : go(run_fwd<128, false, 2>);
   if (four_per_sm(p)) return bf16 ? go(run_fwd<64, true, 1>) : go(run_fwd<64, false, 1>);
   return bf16 ? go(run_fwd<64, true, 2>) : go(run_fwd<64, false, 2>);
@@ -1766,18 +1707,18 @@ long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int 
 
 int wdit_rel_attention_backward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
                                 const void* v, const long long* v_strides, const void* dout,
-                                const long long* dout_strides, const void* out, const void* out_lo, const float* lse,
-                                int B, int H, int Lq, int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
-                                const int* bounds, int n_bounds, int bidirectional, int causal, int q_offset,
-                                float scale, void* dq, void* dk, void* dv, void* dtable, int dtable_dtype,
-                                void* workspace, long long workspace_bytes, void* stream) {
+                                const long long* dout_strides, const float* lse, int B, int H, int Lq, int Lk, int D,
+                                int dtype, const int* k_lens, const void* table, int table_dtype, const int* bounds,
+                                int n_bounds, int bidirectional, int causal, int q_offset, float scale, void* dq,
+                                void* dk, void* dv, void* dtable, int dtable_dtype, void* workspace,
+                                long long workspace_bytes, void* stream) {
   int rc = check_attn(bounds, n_bounds, B, H, Lq, Lk, D, dtype, table_dtype, q_offset, table);
   if (rc) return rc;
   if (B == 0 || Lq == 0 || Lk == 0) return WDIT_ERR_SHAPE;  // the caller knows the answer: zeros
-  if (out == nullptr || out_lo == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || dtable == nullptr ||
-      dtable_dtype < 0 || dtable_dtype > 2)
+  if (lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || dtable == nullptr || dtable_dtype < 0 ||
+      dtable_dtype > 2)
     return WDIT_ERR_ARG;
-  for (const void* t : {out, out_lo, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
+  for (const void* t : {dq, dk, dv})
     if ((reinterpret_cast<uintptr_t>(t) & 15) != 0) return WDIT_ERR_ALIGN;
   if ((rc = check_heads(q, q_strides)) || (rc = check_heads(k, k_strides)) || (rc = check_heads(v, v_strides)) ||
       (rc = check_heads(dout, dout_strides)))
@@ -1798,14 +1739,8 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
   p.table = table;
   p.table_dtype = table_dtype;
   if (!rel_fill(&p.rb, bounds, n_bounds, bidirectional)) return WDIT_ERR_ARG;
-  p.out = const_cast<void*>(out);
-  p.out_lo = const_cast<void*>(out_lo);
   p.lse = const_cast<float*>(lse);
   p.splits = 1;
-  p.dout = dout;
-  p.do_b = dout_strides[0];
-  p.do_l = dout_strides[1];
-  p.do_h = dout_strides[2];
   p.delta = static_cast<float*>(workspace);
   p.table_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align16(4ll * B * H * Lq));
   if ((rc = error_record_ptr(&p.ctx.rec))) return rc;

@@ -417,15 +417,14 @@ def _attention_forward(dev, q, k, v, table, k_lens, bidirectional, causal, max_d
     device = q.device
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0 or Lq == 0 or k.shape[1] == 0:
-        return out.zero_(), None, None
-    lo = torch.empty_like(out) if for_grad else None
+        return out.zero_(), None
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=device) if for_grad else None
     shape, pos = _attention_args(q, k, table, k_lens, bidirectional, causal, max_distance, q_offset, scale)
     nbytes = _workspace_bytes(dev, "wdit_rel_attention_workspace_bytes", *shape)
     ws = _workspace(nbytes, device)
     call("wdit_rel_attention", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), *shape,
-         *pos, out.data_ptr(), ptr(lo), ptr(lse), ptr(ws), nbytes, _stream(dev), kernels=1 if nbytes == 0 else 2)
-    return out, lo, lse
+         *pos, out.data_ptr(), ptr(lse), ptr(ws), nbytes, _stream(dev), kernels=1 if nbytes == 0 else 2)
+    return out, lse
 
 
 class _RelPosAttention(torch.autograd.Function):
@@ -434,16 +433,16 @@ class _RelPosAttention(torch.autograd.Function):
         dev = q.get_device()
         with _on_device(dev):
             qc, kc, vc, tc = _heads(q), _heads(k), _heads(v), table.contiguous()
-            out, lo, lse = _attention_forward(dev, qc, kc, vc, tc, k_lens, bidirectional, causal, max_distance,
-                                              q_offset, scale, True)
-        ctx.save_for_backward(qc, kc, vc, tc, k_lens, out, lo, lse)
+            out, lse = _attention_forward(dev, qc, kc, vc, tc, k_lens, bidirectional, causal, max_distance, q_offset,
+                                          scale, True)
+        ctx.save_for_backward(qc, kc, vc, tc, k_lens, lse)
         ctx.args = (bidirectional, causal, max_distance, q_offset, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, k_lens, out, lo, lse = ctx.saved_tensors
+        q, k, v, table, k_lens, lse = ctx.saved_tensors
         nothing = (None,) * 6
         if lse is None:  # no queries or no keys
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(table), *nothing)
@@ -458,7 +457,7 @@ class _RelPosAttention(torch.autograd.Function):
                                       int(pos[6]))
             ws = _workspace(nbytes, device)
             call("wdit_rel_attention_backward", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(),
-                 _strides(v), g.data_ptr(), _strides(g), out.data_ptr(), lo.data_ptr(), lse.data_ptr(), *shape, *pos, dq.data_ptr(),
+                 _strides(v), g.data_ptr(), _strides(g), lse.data_ptr(), *shape, *pos, dq.data_ptr(),
                  dk.data_ptr(), dv.data_ptr(), dtable.data_ptr(), _DTYPE[table.dtype], ws.data_ptr(), nbytes,
                  _stream(dev), kernels=3)
         return (dq, dk, dv, dtable, *nothing)

@@ -337,8 +337,7 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
  * *_strides are HOST arrays of the element strides of (b, l, h), multiples of 8 (dimensions of
  * size 1 too). k_lens (device, [B], NULL = all of Lk): valid keys per sample, clamped to [0, Lk];
  * causal != 0: key j <= i + q_offset. A row that sees no key gives 0. lse (fp32 [B, H, Lq], may be
- * NULL) receives log2 of the softmax sums (-inf for such a row), out_lo (as out, may be NULL) what
- * rounding took from out: the backward pass needs both.
+ * NULL) receives log2 of the softmax sums (-inf for such a row) for the backward pass.
  * The workspace (0 bytes unless the keys are split over several CTAs) needs no initialization.
  * Lk = 0 is WDIT_ERR_SHAPE (the result is zeros).
  */
@@ -346,22 +345,22 @@ long long wdit_rel_attention_workspace_bytes(int B, int H, int Lq, int Lk, int D
 int wdit_rel_attention(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
                        const void* v, const long long* v_strides, int B, int H, int Lq, int Lk, int D, int dtype,
                        const int* k_lens, const void* table, int table_dtype, const int* bounds, int n_bounds,
-                       int bidirectional, int causal, int q_offset, float scale, void* out, void* out_lo, float* lse,
+                       int bidirectional, int causal, int q_offset, float scale, void* out, float* lse,
                        void* workspace, long long workspace_bytes, void* stream);
 
 /*
  * Its gradients: dq [B, Lq, H, D], dk, dv [B, Lk, H, D] (contiguous, dtype; 0 for keys past
- * k_lens) and dtable [buckets, H] (of dtable_dtype). out, out_lo and lse are the forward's. Three launches,
+ * k_lens) and dtable [buckets, H] (of dtable_dtype). lse is the forward's. Three launches,
  * no atomics: sums have a fixed order. Empty dimensions are WDIT_ERR_SHAPE (the results are zeros).
  */
 long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional);
 int wdit_rel_attention_backward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
                                 const void* v, const long long* v_strides, const void* dout,
-                                const long long* dout_strides, const void* out, const void* out_lo, const float* lse,
-                                int B, int H, int Lq, int Lk, int D, int dtype, const int* k_lens, const void* table, int table_dtype,
-                                const int* bounds, int n_bounds, int bidirectional, int causal, int q_offset,
-                                float scale, void* dq, void* dk, void* dv, void* dtable, int dtable_dtype,
-                                void* workspace, long long workspace_bytes, void* stream);
+                                const long long* dout_strides, const float* lse, int B, int H, int Lq, int Lk, int D,
+                                int dtype, const int* k_lens, const void* table, int table_dtype, const int* bounds,
+                                int n_bounds, int bidirectional, int causal, int q_offset, float scale, void* dq,
+                                void* dk, void* dv, void* dtable, int dtable_dtype, void* workspace,
+                                long long workspace_bytes, void* stream);
 
 /*
  * out[M, N] = act(A . B^T + bias) + res, operands and out of dtype (bf16 or fp16), fp32 sums, one

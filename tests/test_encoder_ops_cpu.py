@@ -89,7 +89,7 @@ def test_extents_refused(pkg):
                                         0, null) == 2
     for H, lq, lk in [(65536, 1, 1), (1, big, 1), (1, 1, big)]:
         assert lib.wdit_rel_attention(d, st, d, st, d, st, 1, H, lq, lk, 64, 1, null, d, 0, b, 1, 1, 0, 0, 1.0, d, null,
-                                      null, null, 0, null) == 2
+                                      null, 0, null) == 2
 
 
 def test_rel_pos_entry_points_validate_without_device(pkg):
@@ -207,27 +207,27 @@ def test_attention_entry_points_validate_without_device(pkg):
     bad = (ctypes.c_longlong * 3)(5 * 3 * 64, 3 * 64 + 4, 64)
     zero = (ctypes.c_longlong * 3)(5 * 3 * 64, 0, 64)
 
-    def fwd(q=d, qs=st, B=2, H=3, Lq=5, Lk=5, D=64, dtype=1, table=d, td=0, b=bounds, n=3, off=0, out=d, lo=null,
-            ws=null, nb=0):
+    def fwd(q=d, qs=st, B=2, H=3, Lq=5, Lk=5, D=64, dtype=1, table=d, td=0, b=bounds, n=3, off=0, out=d, ws=null,
+            nb=0):
         return lib.wdit_rel_attention(q, qs, d, st, d, st, B, H, Lq, Lk, D, dtype, null, table, td, b, n, 1, 0, off,
-                                      1.0, out, lo, null, ws, nb, null)
+                                      1.0, out, null, ws, nb, null)
 
     assert fwd(q=null) == 1 and fwd(qs=None) == 1 and fwd(table=null) == 1 and fwd(out=null) == 1 and fwd(b=None) == 1
     assert fwd(dtype=0) == 1 and fwd(td=3) == 1
     assert fwd(D=96) == 2 and fwd(H=0) == 2 and fwd(n=0) == 2 and fwd(off=-1) == 2 and fwd(Lk=0) == 2
     assert fwd(qs=zero) == 2 and fwd(qs=bad) == 3 and fwd(q=ctypes.c_void_p(0x1008)) == 3
-    assert fwd(out=ctypes.c_void_p(0x1008)) == 3 and fwd(lo=ctypes.c_void_p(0x1008)) == 3
+    assert fwd(out=ctypes.c_void_p(0x1008)) == 3
     assert fwd(B=0, q=null, out=null) == 0 and fwd(Lq=0, q=null, out=null) == 0
     need = lib.wdit_rel_attention_workspace_bytes(1, 1, 1, 4096, 64)
     assert need > 0 and fwd(B=1, H=1, Lq=1, Lk=4096) == 5
     assert fwd(B=1, H=1, Lq=1, Lk=4096, ws=d, nb=need - 1) == 5
     assert lib.wdit_rel_attention_workspace_bytes(64, 64, 512, 512, 64) == 0
 
-    def back(lse=d, out=d, lo=d, dq=d, dt=d, ddt=0, ws=d, nb=1 << 30, Lq=5, Lk=5, gs=st):
-        return lib.wdit_rel_attention_backward(d, st, d, st, d, st, d, gs, out, lo, lse, 2, 3, Lq, Lk, 64, 1, null, d, 0,
+    def back(lse=d, dq=d, dt=d, ddt=0, ws=d, nb=1 << 30, Lq=5, Lk=5, gs=st):
+        return lib.wdit_rel_attention_backward(d, st, d, st, d, st, d, gs, lse, 2, 3, Lq, Lk, 64, 1, null, d, 0,
                                                bounds, 3, 1, 0, 0, 1.0, dq, d, d, dt, ddt, ws, nb, null)
 
-    assert back(lse=null) == 1 and back(out=null) == 1 and back(lo=null) == 1 and back(dq=null) == 1 and back(dt=null) == 1
+    assert back(lse=null) == 1 and back(dq=null) == 1 and back(dt=null) == 1
     assert back(ddt=-1) == 1
     assert back(Lq=0) == 2 and back(Lk=0) == 2 and back(gs=zero) == 2 and back(gs=bad) == 3
     assert back(dq=ctypes.c_void_p(0x1004)) == 3
