@@ -34,6 +34,14 @@
 //   attn_dkv_kernel  CTA = 128 keys; runs over query tiles of 64 with the scores transposed, so
 //                    P^T and dS^T are the A operands; dK and dV stay in TMEM.
 //
+// Measured (bf16): forward, 12 heads x 8192 x 8192 x 128 causal 187 - 205 us by the card's power, 1.0 -
+// 1.1 PFLOP/s, tensor pipe 55% and exponentials 55% busy; 2 x 64 heads x 512 x 512 x 64 with lengths
+// 512 and 227 22.4 us, of which a CTA's start and end are 4; one query over 8 x 12 heads x 8191 keys x
+// 128 66 us, 6.1 TB/s. Backward at 2 x 64 heads x 512 x 512 x 64: dQ 59 us, dK and dV 47. What bounds
+// the tiles is latency: a score tile passes from the MMAs to a warp and back over two barriers, about
+// 200 clocks each behind the other warps' exponentials, besides its TMEM reads; more CTAs per SM,
+// scores read ahead and polynomial exponentials were all slower.
+//
 // Keys past k_lens may hold anything (NaN included): their scores are replaced, and their rows of
 // an operand that is summed over are overwritten with zeros in shared memory.
 #include <cuda.h>

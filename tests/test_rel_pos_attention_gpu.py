@@ -314,7 +314,8 @@ def test_masked_buckets_have_finite_gradients(pkg):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("Lq,Lk", [(900, 1), (900, 2), (900, 5), (300, 64), (300, 65), (200, 200), (200, 256)])
+@pytest.mark.parametrize("Lq,Lk", [(900, 1), (900, 2), (900, 5), (300, 64), (300, 65), (200, 200), (200, 256),
+                                   (2000, 280), (130, 1100)])
 def test_table_gradient_of_few_keys(pkg, Lq, Lk, D):
     """Most rows' cells fall into one bucket there, where their sum is 0: what is left of it are fp32
     errors, not half steps of a 16-bit type. Per cell P (eps |dP - delta| + d(dP) + d(delta)), delta
