@@ -796,18 +796,6 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-int sm_count() {
-  static int n[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (n[dev] == 0) {
-    int v = 0;
-    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148;
-    n[dev] = v;
-  }
-  return n[dev];
-}
-
 struct Plan {
   int pair, bn, splits;
 };
@@ -981,6 +969,19 @@ int check_operand(const void* p, long long ld, long long cols) {
 }
 
 }  // namespace
+
+int sm_count() {
+  static int n[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (n[dev] == 0) {
+    int v = 0;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148;
+    n[dev] = v;
+  }
+  return n[dev];
+}
+
 }  // namespace wdit
 
 using namespace wdit;

@@ -1515,13 +1515,6 @@ int cuda_rc(cudaError_t e) {
   return WDIT_ERR_CUDA_BASE + static_cast<int>(e);
 }
 
-int attn_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-  return n;
-}
-
 // Key splits of the forward: with fewer CTAs than two per SM (a few query rows of a few heads)
 // one CTA would walk a long cache alone, so the keys are divided until the SMs are full, at least
 // four tiles a part (one query row, us with at least 1 / 4 / 16 tiles a part and undivided: 12 heads
@@ -1531,7 +1524,7 @@ int attn_splits(int B, int H, int Lq, int Lk) {
   const long long ctas = static_cast<long long>(B) * H * ((Lq + kRows - 1) / kRows);
   const int tiles = (Lk + kCols - 1) / kCols;
   if (ctas <= 0) return 1;
-  long long s = 2ll * attn_sms() / ctas;
+  long long s = 2ll * sm_count() / ctas;
   if (s > tiles / 4) s = tiles / 4;
   return s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : static_cast<int>(s));
 }
@@ -1544,7 +1537,7 @@ int attn_splits(int B, int H, int Lq, int Lk) {
 // CTA then walks twice as fast (12 heads x 8192 x 8192 337 / 355, causal 4096 x 4096 61 / 81).
 bool four_per_sm(const AttnArgs& p) {
   const long long ctas = static_cast<long long>(p.B) * p.H * ((p.Lq + kRows - 1) / kRows);
-  return ctas > 2ll * attn_sms() && p.Lk <= 2048;
+  return ctas > 2ll * sm_count() && p.Lk <= 2048;
 }
 
 struct Strides {

@@ -395,13 +395,6 @@ int grad_smem(const RelBuckets& rb, int buckets, bool vec, int esize) {
   return grad_fixed_bytes(sums) + (vec ? 0 : kRelWarps * kRing * grad_row_bytes(esize));
 }
 
-int rel_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-  return n;
-}
-
 // Rows of a strip and CTAs per head of the gradient. All CTAs run at once (per_sm of them), a head's
 // warps share its strips. Aligned rows: the rows whose rounds of strips cost least, a strip costing
 // its rows and 24 more for its ends (us with 32 / 64 / 128 rows, bf16: 64 heads x 512 x 512 9.6 /
@@ -502,7 +495,7 @@ int wdit_rel_pos_bias(const void* table, int dtype, const int* bounds, int n_bou
 long long wdit_rel_pos_bias_grad_workspace_bytes(int B, int H, int Lq, int Lk, int n_bounds, int bidirectional) {
   if (B <= 0 || H <= 0 || Lq <= 0 || Lk <= 0 || n_bounds < 1) return 0;
   // (the rows' alignment and the last bound are not known here: enough for any)
-  const int sms = rel_sms();
+  const int sms = sm_count();
   int parts = grad_plan(B, H, Lq, Lk, true, 2, sms).parts;
   for (int per_sm = 2; per_sm <= 3; ++per_sm) {
     const int n = grad_plan(B, H, Lq, Lk, false, per_sm, sms).parts;
@@ -539,7 +532,7 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
       (reinterpret_cast<uintptr_t>(dbias) & 15) == 0 && stride_b % V == 0 && stride_h % V == 0 && stride_i % V == 0;
   // three CTAs per SM where their shared memory fits, two of the aligned form by its registers
   const int smem = grad_smem(rb, buckets, vec, dtype == 0 ? 4 : 2);
-  const GradPlan plan = grad_plan(B, H, Lq, Lk, vec, !vec && 3 * (smem + 1024) <= 228 * 1024 ? 3 : 2, rel_sms());
+  const GradPlan plan = grad_plan(B, H, Lq, Lk, vec, !vec && 3 * (smem + 1024) <= 228 * 1024 ? 3 : 2, sm_count());
   float* part = static_cast<float*>(workspace);
   auto go = [&](auto* type) {
     return launch_grad<std::remove_pointer_t<decltype(type)>>(dbias, rb, B, H, Lq, Lk, q_offset, stride_b, stride_h,

@@ -90,4 +90,7 @@ int launch_rms_rope_apply(void* x, int ldx, int M, const float* part, int part_l
 int error_record_ptr(unsigned int** out);
 unsigned long long wait_limit_ns();
 
+// SMs of the current device (asked for once per device; 148 where that fails).
+int sm_count();
+
 }  // namespace wdit
