@@ -159,3 +159,29 @@ def test_cached_steps_agree_with_the_whole(pkg):
         one = pkg.ops.rel_pos_attention(q[:, n : n + 1], cache_k, cache_v, table, k_lens=lens, q_offset=n, **kw)
         tol = 2 * h * whole[:, n : n + 1].abs() + 3 * h * bound[:, n : n + 1]
         assert ((one.double() - whole[:, n : n + 1]).abs() <= tol).all(), n
+
+
+def test_layers_on_two_streams_at_once(pkg):
+    """Enough CTAs of every kernel that both streams' share the SMs and their tensor memory."""
+    L, B = 300, 40
+    g = torch.Generator().manual_seed(53)
+    p = [{n: t.requires_grad_() for n, t in parameters(torch.bfloat16, seed=s).items()} for s in (1, 2)]
+    xs = [torch.randn(B, L, C, generator=g).to(torch.bfloat16).to(DEV).requires_grad_() for _ in range(2)]
+    dout = torch.randn(B, L, C, generator=g).to(torch.bfloat16).to(DEV)
+    lens = torch.randint(0, L + 1, (B,), generator=g, dtype=torch.int32).to(DEV)
+
+    def step(i):
+        out = layer(pkg.ops, p[i], xs[i], lens)
+        return [out.detach(), *torch.autograd.grad(out, [xs[i], *p[i].values()], dout)]
+
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, step(i)))
+    torch.cuda.synchronize()
+    for i, res in got:
+        assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
