@@ -34,6 +34,8 @@ def _require_cuda(*ts: torch.Tensor | None) -> int:
         if t is None:
             continue
         i = t.get_device()
+        if i < 0:  # (a device without an index: the CPU, meta)
+            raise RuntimeError("wdit ops run on CUDA tensors only (no CPU implementation)")
         if i != dev:
             if not t.is_cuda:
                 raise RuntimeError("wdit ops run on CUDA tensors only (no CPU implementation)")
