@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 from functools import lru_cache
+from operator import index
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -86,13 +87,18 @@ def _workspace_bytes(dev: int, name: str, *shape: int) -> int:
 # ---------------------------------------------------------------------------
 # Relative position buckets
 # ---------------------------------------------------------------------------
-@lru_cache(maxsize=64)
 def rel_pos_bounds(num_buckets: int, max_distance: int, bidirectional: bool) -> tuple[int, ...]:
     """Distances at which the bucket steps up by one (the bucket of distance n is the number of
     bounds <= n): one per distance below `exact` = half of a direction's buckets, then
     logarithmic up to max_distance. Bucket exact + t begins at the least n with
     log(n / exact) / log(max_distance / exact) * T >= t, T = buckets - exact, decided in whole
     numbers as n^T >= max_distance^t * exact^(T - t)."""
+    # (whole numbers before the cache, for which 128.0 is 128)
+    return _rel_pos_bounds(index(num_buckets), index(max_distance), bool(bidirectional))
+
+
+@lru_cache(maxsize=64)
+def _rel_pos_bounds(num_buckets: int, max_distance: int, bidirectional: bool) -> tuple[int, ...]:
     if bidirectional and num_buckets % 2 != 0:
         raise ValueError(f"a bidirectional table needs an even number of buckets, got {num_buckets}")
     nb = num_buckets // 2 if bidirectional else num_buckets
