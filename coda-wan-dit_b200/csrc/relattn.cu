@@ -42,8 +42,9 @@
 // 200 clocks each behind the other warps' exponentials, besides its TMEM reads; more CTAs per SM,
 // scores read ahead and polynomial exponentials were all slower.
 //
-// Keys past k_lens may hold anything (NaN included): their scores are replaced, and their rows of
-// an operand that is summed over are overwritten with zeros in shared memory.
+// Keys past k_lens, and under a causal mask past the last query, may hold anything (NaN included):
+// their scores are replaced, and their rows of an operand that is summed over are overwritten with
+// zeros in shared memory.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -512,7 +513,8 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
       ok = wait_parity(&v_full[st], (t / ST) & 1, kSiteAttn + 5, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       const int j0 = (t0 + t) * kCols;
-      if (j0 + kCols > klen) zero_tail<D, kCols>(sV + st * C::kTile, klen - j0, lane);
+      // rows past the keys that any query of the tile sees would enter O as 0 * anything
+      if (j0 + kCols > visible) zero_tail<D, kCols>(sV + st * C::kTile, visible - j0, lane);
       ok = wait_parity(&p_ready[t % NB], (t / NB) & 1, kSiteAttn + 6, p.ctx);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
@@ -1000,8 +1002,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const int st = step % ST, j0 = tile(step) * kCols;
       const bool ok = wait_parity(&full[st], (step / ST) & 1, kSiteAttnDq + 2, p.ctx);
       if (!__all_sync(0xffffffffu, ok)) return false;
-      // rows past the sample's keys would enter dQ as 0 * anything
-      if (j0 + kCols > klen) zero_tail<D, kCols>(sK + st * C::kTile, klen - j0, lane);
+      // rows past the keys that any query of the tile sees would enter dQ as 0 * anything
+      if (j0 + kCols > visible) zero_tail<D, kCols>(sK + st * C::kTile, visible - j0, lane);
       tc_fence_after();
       if (elect_one()) {
         const uint32_t d = tmem + (step % NB) * 2 * kCols;

@@ -479,8 +479,9 @@ def rel_pos_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
     q [B, Lq, H, D], k and v [B, Lk, H, D] (bf16 or fp16, D 64 or 128; any strides, rows of a head
     contiguous and on 16-byte boundaries, others are copied); table [num_buckets, H] (fp32, bf16
     or fp16). k_lens [B] int32: sample b's first k_lens[b] keys are valid (clamped to [0, Lk]; what
-    lies behind them is not looked at). causal: query i sees the keys up to i + q_offset. A row
-    that sees no key gives 0. scale defaults to D ** -0.5. One token after a cache of n keys:
+    lies behind them is not looked at). causal: query i sees the keys up to i + q_offset (those past
+    the last query may hold anything; an infinity or NaN of a key that some query sees may reach
+    the queries before it too, as 0 times it). A row that sees no key gives 0. scale defaults to D ** -0.5. One token after a cache of n keys:
     Lq 1, q_offset n - 1 if the cache holds the token's own key, n otherwise. Differentiable in
     q, k, v and table; results repeat bit for bit."""
     qs, ks = q.shape, k.shape
