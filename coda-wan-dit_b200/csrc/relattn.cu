@@ -321,10 +321,20 @@ __device__ __forceinline__ int sample_len(const AttnArgs& p, int b) {
 // thread) and one warp that loads and issues; a CTA's products and softmax take turns, and the
 // CTAs fill each other's gaps, starts and ends.
 //
-// The maximum in use is that of the row's first tile. Later tiles are exponentiated against it
-// without looking for theirs; only when a tile's sum passes kSumLimit is the maximum taken anew,
-// O rescaled and the tile done again. 16-bit P keeps its relative precision up to there (fp16 up
-// to 2^15 of its 65504, bf16 far beyond), and the sums are fp32.
+// The maximum in use is that of the row's first tile (bf16: 2^kHeadroom above it). Later tiles are
+// exponentiated against it without looking for theirs; only when a tile's sum passes kSumLimit is
+// the maximum taken anew, O rescaled and the tile done again. What bounds the two:
+//   fp16  P up to 2^15 of its 65504; P v is then far inside fp32.
+//   bf16  v may be as large as fp32 goes, so the row's sum of P stays below 1: at most 2^22 tiles of
+//         at most 2^-22 each. The largest P of a tile whose maximum was taken is 2^-40: the row's
+//         scores may rise by a factor of 2^12 (sums of 64: 2^18) before it is taken anew, P keeps its
+//         relative precision down to 2^-86 of the largest, and O that of |v| from 2^-86 on.
+template <bool BF16>
+struct SoftmaxRange {
+  static constexpr float kHeadroom = BF16 ? 40.f : 0.f;                     // log2
+  static constexpr float kSumLimit = BF16 ? 2.3841858e-07f : 32768.f;  // 2^-22, 2^15
+};
+
 template <int D, int NB>
 struct Fwd {
   static constexpr int kCtas = NB == 1 ? 4 : 2;     // per SM
@@ -556,7 +566,7 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     const int row_end = p.causal ? min(klen, i + p.q_offset + 1) : klen;  // keys this row sees
     const int warp_first = i0 + wq * 32 + p.q_offset;                      // the warp's first position
-    constexpr float kSumLimit = BF16 ? 1.0995116e12f : 32768.f;  // 2^40, 2^15
+    using Range = SoftmaxRange<BF16>;
     float m_used = -kInf, l = 0.f;
     bool ok = true;
     // Few query rows (one token): a warp without any leaves its rows of P as they are; they only
@@ -649,7 +659,7 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
             exponentiate(yes, no);
           else
             exponentiate(no, no);
-          if (settled || !__any_sync(0xffffffffu, m_used == -kInf || sum > kSumLimit)) break;
+          if (settled || !__any_sync(0xffffffffu, m_used == -kInf || sum > Range::kSumLimit)) break;
         }
         // The row's maximum anew; everything before is rescaled to it, once the product of t - 1
         // has left O at rest.
@@ -664,7 +674,7 @@ __global__ void __launch_bounds__(Fwd<D, NB>::kThreads, Fwd<D, NB>::kCtas)
             m_tile = fmaxf(m_tile, c * 32 + e < keep ? x : -kInf);
           }
         }
-        const float m_new = fmaxf(m_used, m_tile);
+        const float m_new = fmaxf(m_used, m_tile + Range::kHeadroom);
         if (t > 0) {
           ok = wait_parity(pv_done, (t - 1) & 1, kSiteAttn + 8, p.ctx);
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -784,8 +794,15 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float ms = m == -kInf ? 0.f : m;
-  const float w0 = exp2f(lse0 - ms), w1 = exp2f(lse1 - ms);
-  float total = 0.f, acc[V];
+  float w0 = exp2f(lse0 - ms), w1 = exp2f(lse1 - ms);
+  float total = w0 + w1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  // weights that add up to 1: a sum of parts near the type's largest value stays inside it
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  w0 *= inv;
+  w1 *= inv;
+  float acc[V];
 #pragma unroll
   for (int q = 0; q < V; ++q) acc[q] = 0.f;
   for (int base = 0; base < p.splits; base += kAhead) {
@@ -798,19 +815,17 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {  // (weights past the last part are 0)
       const float w = __shfl_sync(0xffffffffu, base < 32 ? w0 : w1, (base + s) & 31);
-      total += w;
 #pragma unroll
       for (int q = 0; q < V; ++q) acc[q] = w == 0.f ? acc[q] : fmaf(w, now[s][q], acc[q]);
     }
   }
-  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
   const int i = static_cast<int>(row % p.Lq);
   const int h = static_cast<int>(row / p.Lq % p.H);
   const long long b = row / p.Lq / p.H;
   uint16_t* dst = static_cast<uint16_t*>(p.out) + ((b * p.Lq + i) * p.H + h) * D + lane * V;
 #pragma unroll
   for (int q = 0; q < V; q += 2)
-    *reinterpret_cast<uint32_t*>(dst + q) = pack16<BF16>(acc[q] * inv, acc[q + 1] * inv);
+    *reinterpret_cast<uint32_t*>(dst + q) = pack16<BF16>(acc[q], acc[q + 1]);
   if (lane == 0 && p.lse != nullptr) p.lse[row] = inv == 0.f ? -kInf : ms + log2f(total);
 }
 
