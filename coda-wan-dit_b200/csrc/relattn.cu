@@ -253,14 +253,24 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int first, int lane) {
   __syncwarp();
 }
 
-// The head's bias by diagonal: the table's values (times log2 e) and buckets of d = -reach .. reach,
+// The head's bias by diagonal: the table's values (bias_log2) and buckets of d = -reach .. reach,
 // constant past both ends, in shared memory. reach is the last bound, at most kReach: a table with
 // longer ones is searched per diagonal instead.
 constexpr int kReach = 1024;
 
+// A bias in units of log2 e. Finite ones end at 2^14 on either side: a table may hold its type's lowest
+// value (or -1e9) as a mask, and a row that sees nothing but such keys still has to tell their scores
+// apart, in fp32, in its maximum and its log-sum (half a step there is 2^-10). Next to any other
+// key the weight of such a one is 0 as before, unless their scores are more than 11356 apart.
+constexpr float kBiasMost = 16384.f;
+__device__ __forceinline__ float bias_log2(float v) {
+  const float x = v * kLog2e;
+  return fabsf(v) < kInf ? fminf(fmaxf(x, -kBiasMost), kBiasMost) : x;  // infinities and NaN stay
+}
+
 struct BiasLine {
   const int* bounds;
-  const float* col;    // [buckets] table column * log2 e
+  const float* col;    // [buckets] bias_log2 of the table's column
   const float* value;  // [2 reach + 1] unless searched
   int n_bounds, bidirectional, reach;
   bool searched;
@@ -297,7 +307,7 @@ __device__ __forceinline__ BiasLine load_bias(const AttnArgs& p, int h, void* me
   l.value = col + buckets;
   l.searched = l.reach > kReach;
   for (int t = threadIdx.x; t < p.rb.n_bounds; t += threads) bounds[t] = p.rb.bounds[t];
-  for (int t = threadIdx.x; t < buckets; t += threads) col[t] = table_value(p, t, h) * kLog2e;
+  for (int t = threadIdx.x; t < buckets; t += threads) col[t] = bias_log2(table_value(p, t, h));
   if (!l.searched) {
     __syncthreads();
     for (int t = threadIdx.x; t < 2 * l.reach + 1; t += threads) col[buckets + t] = col[l.bucket(t - l.reach)];

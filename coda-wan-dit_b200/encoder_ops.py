@@ -481,7 +481,9 @@ def rel_pos_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
     or fp16). k_lens [B] int32: sample b's first k_lens[b] keys are valid (clamped to [0, Lk]; what
     lies behind them is not looked at). causal: query i sees the keys up to i + q_offset (those past
     the last query may hold anything; an infinity or NaN of a key that some query sees may reach
-    the queries before it too, as 0 times it). A row that sees no key gives 0. scale defaults to D ** -0.5. One token after a cache of n keys:
+    the queries before it too, as 0 times it). A row that sees no key gives 0. Finite table values
+    past +-11356 count as +-11356: a mask of the type's lowest value leaves a key no weight beside
+    others, and a row of nothing but such keys is the softmax of their scores; -inf hides a key. scale defaults to D ** -0.5. One token after a cache of n keys:
     Lq 1, q_offset n - 1 if the cache holds the token's own key, n otherwise. Differentiable in
     q, k, v and table; results repeat bit for bit."""
     qs, ks = q.shape, k.shape

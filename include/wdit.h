@@ -336,7 +336,8 @@ int wdit_rel_pos_bias_grad(const void* dbias, int dtype, int B, int H, int Lq, i
  * q, k, v (and dout) are [B, L, H, D] of dtype (bf16 or fp16), D 64 or 128, unit stride along D;
  * *_strides are HOST arrays of the element strides of (b, l, h), multiples of 8 (dimensions of
  * size 1 too). k_lens (device, [B], NULL = all of Lk): valid keys per sample, clamped to [0, Lk];
- * causal != 0: key j <= i + q_offset. A row that sees no key gives 0. lse (fp32 [B, H, Lq], may be
+ * causal != 0: key j <= i + q_offset. Finite table values past +-11356 count as +-11356; -inf hides a
+ * key. A row that sees no key gives 0. lse (fp32 [B, H, Lq], may be
  * NULL) receives log2 of the softmax sums (-inf for such a row) for the backward pass.
  * The workspace (0 bytes unless the keys are split over several CTAs) needs no initialization.
  * Lk = 0 is WDIT_ERR_SHAPE (the result is zeros).

@@ -100,3 +100,60 @@ def test_keys_past_the_last_query_may_hold_anything(pkg, B, H, Lq, Lk, off, D, d
         got = out_and_gradients(pkg, q, k2, v2, table, dout, **kw)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert not want[2][:, off + Lq:].any() and not want[3][:, off + Lq:].any()
+
+
+MASKS = [(torch.float32, torch.finfo(torch.float32).min), (torch.float32, -1e9), (torch.float32, -1e30),
+         (torch.bfloat16, torch.finfo(torch.bfloat16).min), (torch.float16, torch.finfo(torch.float16).min)]
+
+
+@pytest.mark.parametrize("table_dtype,mask", MASKS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Lq,Lk,D", [(1, 2, 200, 200, 64), (2, 3, 130, 270, 128), (1, 2, 2, 3000, 64),
+                                         (8, 40, 129, 129, 64)])
+def test_masks_of_the_lowest_value(pkg, B, H, Lq, Lk, D, dtype, table_dtype, mask):
+    """Head 0: keys ahead of the query are masked. Head 1: all keys; what is left are their scores. The
+    oracle's mask is -20000, which 64 bits tell scores apart beside."""
+    q, k, v, table, dout = make(B, H, Lq, Lk, D, dtype, seed=3)
+    table[16:], table[:, 1] = mask, mask
+    table = table.to(table_dtype)
+    masked = table.double() <= -60000
+    p, _ = probabilities(pkg, q, k, torch.where(masked, -20000.0, table.double()))
+    # errors of P: as in probabilities() for the scores, with the biases that are no masks; where only
+    # masks are seen, maximum and log-sum are rounded at 2^14 (2^-10 each, twice with split keys)
+    _, eps = probabilities(pkg, q, k, torch.where(masked, 0.0, table.double()))
+    eps = eps + 2.0**-8 * torch.ones(H, device=DEV, dtype=torch.float64).index_fill(
+        0, torch.tensor([h for h in range(H) if h != 1], device=DEV), 0.0)[None, :, None, None]
+    h = torch.finfo(dtype).eps / 2
+    sub = 2.0**-25 if dtype == torch.float16 else 0.0
+    got = out_and_gradients(pkg, q, k, v, table, dout)
+    assert all(t.isfinite().all() for t in got)
+    x, do = v.double().transpose(1, 2), dout.double().transpose(1, 2)
+    want = p @ x
+    tol = (p @ x.abs()) * (h + eps + (Lk + 2) * 2.0**-23) + sub * x.abs().sum(-2, keepdim=True)
+    tol = tol + 1.01 * h * (want.abs() + tol) + torch.finfo(dtype).tiny
+    within(got[0], want.transpose(1, 2), tol.transpose(1, 2))
+    # dv = P^T dO with P to 16 bits
+    want = p.transpose(-1, -2) @ do
+    tol = (p * (eps + h) + sub + Lq * 2.0**-23 * p).transpose(-1, -2) @ do.abs()
+    tol = tol + 1.01 * h * (want.abs() + tol) + torch.finfo(dtype).tiny
+    within(got[3], want.transpose(1, 2), tol.transpose(1, 2))
+    # dq = scale dS k, dS = P (dP - delta): dP and delta are fp32 sums of D and Lk terms
+    dp = do @ x.transpose(-1, -2)
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_dp = (D + 2) * 2.0**-23 * (do.abs() @ x.abs().transpose(-1, -2))
+    e_delta = (p * ((eps + (Lk + 2) * 2.0**-23) * dp.abs() + e_dp)).sum(-1, keepdim=True)
+    e_ds = p * (eps * (dp - delta).abs() + e_dp + e_delta) * (1 + h) + h * ds.abs() + sub
+    kk, scale = k.double().transpose(1, 2), D**-0.5
+    want = scale * (ds @ kk)
+    tol = scale * ((e_ds + Lk * 2.0**-23 * ds.abs()) @ kk.abs())
+    tol = tol + 1.01 * h * (want.abs() + tol) + torch.finfo(dtype).tiny
+    within(got[1], want.transpose(1, 2), tol.transpose(1, 2))
+
+
+def test_masks_of_minus_infinity_hide_and_nan_stays(pkg):
+    q, k, v, table, dout = make(1, 2, 70, 90, 64, torch.float16, seed=4)
+    table[:, 0] = -torch.inf
+    table[3, 1] = torch.nan
+    out = pkg.ops.rel_pos_attention(q, k, v, table)
+    assert not out[:, :, 0].any() and out[:, 4:, 1].isnan().all() and out[:, :3, 1].isfinite().all()
