@@ -86,6 +86,7 @@ struct AttnArgs {
   float* part_lse;     // [splits][B * H * Lq]
   // backward
   float* delta;        // [B, H, Lq]
+  unsigned* tops;      // [B, H][4 q tiles], fp16: bounds of |dS| by 32 rows, as the bits of a float >= 0
   float* table_part;   // [H][B * q tiles][buckets]
   WaitCtx ctx;
 };
@@ -264,8 +265,10 @@ constexpr int kReach = 1024;
 // key the weight of such a one is 0 as before, unless their scores are more than 11356 apart.
 constexpr float kBiasMost = 16384.f;
 __device__ __forceinline__ float bias_log2(float v) {
-  const float x = v * kLog2e;
-  return fabsf(v) < kInf ? fminf(fmaxf(x, -kBiasMost), kBiasMost) : x;  // infinities and NaN stay
+  float x = v * kLog2e;  // infinities and NaN stay
+  if (x < -kBiasMost && v > -kInf) x = -kBiasMost;
+  if (x > kBiasMost && v < kInf) x = kBiasMost;
+  return x;
 }
 
 struct BiasLine {
@@ -846,6 +849,21 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
 // score tile, warps 6-9 columns 32-63. D = 64: two CTAs per SM overlap each other; D = 128: one
 // CTA per SM with two score buffers.
 constexpr int kSumReach = 256;  // the table's gradient is summed by diagonal up to this last bound
+
+// fp16 only: P and dS enter their products times a power of two. P is normalised (1 / Lk of flat
+// scores) and dS as small as the loss's scale makes it; below 2^-14 fp16 loses their bits one by one,
+// above 65504 it ends. P is taken times 2^14. dS is taken up to a bound of its size, 2^14 at most: for dQ
+// the row's max |P dP| + |delta|, which the first pass over the keys gives; for dK, whose sums run over the
+// rows, the largest of these of the head. So what a cell may lose is 2^-38 of that bound. A bound of 0,
+// infinity or NaN takes none; past 2^60 the gradients are below fp16 whatever their factor, and |dP| of fp16
+// operands stays below 2^39. The row's maximum and the factor cost attn_dq_kernel 5 of 63 us at 2 x 64
+// heads x 512 x 512 x 64 (99 against 91 at 74 x 512 x 2048), attn_dkv_kernel 1 of 46.
+constexpr int kPScale = 14;
+__device__ __forceinline__ float exp2_int(int e) { return __int_as_float((127 + e) << 23); }  // -126 .. 127
+__device__ __forceinline__ int grad_scale(unsigned bound_bits) {                          // log2 of dS's factor
+  const int e = static_cast<int>(bound_bits >> 23) - 127;  // bound < 2^(e + 1)
+  return bound_bits == 0 || e == 128 ? 0 : max(min(13 - e, 60), -60);
+}
 template <int D>
 struct Bwd {
   static constexpr int kThreads = 320;
@@ -857,7 +875,7 @@ struct Bwd {
   static constexpr uint32_t kTile = kCols * D * 2;
   static constexpr int kWarp = 64 + 96 + 64;  // floats per warp: bias line, diagonals, row values
   static int smem(const RelBuckets& rb) {
-    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 8 * 4 * grad_sums(rb) + 2 * kRows * 4 +
+    return 1024 + 2 * kBig + kStages * 2 * kTile + 256 + 8 * kWarp * 4 + 8 * 4 * grad_sums(rb) + 4 * kRows * 4 +
            bias_smem(rb);
   }
   // Floats of a warp's sums of the table's gradient: by diagonal, or by bucket.
@@ -937,6 +955,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   const int nsum = C::grad_sums(p.rb);
   float* sums = warps + 8 * C::kWarp;  // [8][nsum]
   float* sdelta = sums + 8 * nsum;     // [2][128]
+  float* stop = sdelta + 2 * kRows;    // [2][128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_tiles = (p.Lq + kRows - 1) / kRows;
@@ -1001,7 +1020,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     if (warp >= 2 && i < p.Lq) lse = p.lse[(static_cast<long long>(b) * p.H + h) * p.Lq + i];
     if (lse == -kInf) lse = kInf;  // no keys: every P is 0
   }
-  const BiasLine bias = load_bias(p, h, sdelta + 2 * kRows, C::kThreads);
+  const BiasLine bias = load_bias(p, h, stop + 2 * kRows, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1084,6 +1103,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     uint64_t neg_delta = f2_pack(0.f, 0.f);
     float p_dp = 0.f;  // this row's sum of P dP over the warp's columns
+    float top = 0.f;   // fp16: its largest |P dP|
+    float ds_mult = 1.f, ds_back = 1.f;  // the row's factor, and 1 / it
     // The warp's tiles by kind, as in the forward kernel, for its 32 columns of each tile.
     const int t_left = (warp_first - bias.reach - 31 - half * 32 + kCols) / kCols;
     const int t_right = (warp_first + 31 + bias.ahead() - half * 32 + kCols - 1) / kCols;
@@ -1095,6 +1116,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const int t = tile(step);
       if (step == n) {  // the other half's columns are another warp's
         sdelta[half * kRows + r] = p_dp;
+        if constexpr (!BF16) stop[half * kRows + r] = top;
         __syncwarp();
         if (lane == 0) mbar_arrive(delta_ready);
         ok = wait_parity(delta_ready, 0, kSiteAttnDq + 8, p.ctx);
@@ -1102,6 +1124,14 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
         const float delta = sdelta[r] + sdelta[kRows + r];
         neg_delta = f2_pack(-delta, -delta);
         if (half == 0 && row_ok) p.delta[(static_cast<long long>(b) * p.H + h) * p.Lq + i] = delta;
+        if constexpr (!BF16) {
+          const unsigned bound = __float_as_uint(fmaxf(stop[r], stop[kRows + r]) + fabsf(delta));
+          ds_mult = exp2_int(grad_scale(bound));
+          ds_back = exp2_int(-grad_scale(bound));
+          const unsigned all = __reduce_max_sync(0xffffffffu, bound);
+          if (half == 0 && lane == 0)
+            p.tops[((static_cast<long long>(b) * p.H + h) * q_tiles + qt) * 4 + wq] = all;
+        }
       }
       const int j0 = t * kCols + half * 32;
       const int d_lo = j0 - warp_first - 31;
@@ -1156,11 +1186,21 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
         float x0, x1;
         f2_unpack(fadd2(a2, b2), x0, x1);
         p_dp += x0 + x1;
+        if constexpr (!BF16) {
+          float most[4] = {top, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 32; ++e) most[e & 3] = fmaxf(most[e & 3], fabsf(s[e]));
+          top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        }
         continue;
       }
       uint32_t w[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) w[e] = pack16<BF16>(s[2 * e], s[2 * e + 1]);
+      for (int e = 0; e < 16; ++e) {
+        float x = s[2 * e], y = s[2 * e + 1];
+        if constexpr (!BF16) f2_unpack(fmul2(f2_pack(x, y), f2_pack(ds_mult, ds_mult)), x, y);
+        w[e] = pack16<BF16>(x, y);
+      }
       tmem_st16(ts, w);
       tmem_wait_st();
       tc_fence_before();
@@ -1241,7 +1281,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     // dQ through the query tile's shared memory: warps 2-5 write columns 0-63, 6-9 64-127.
     if (half < D / 64) {
       store_rows64<BF16>(&tmOut, sQ + half * 16384 + wq * 4096, tmem_acc + lane_off + half * 64, n > 0 && ok, false,
-                         p.scale, lane, half * 64, h, i0 + wq * 32, b, i0 + wq * 32 < p.Lq);
+                         p.scale * ds_back, lane, half * 64, h, i0 + wq * 32, b, i0 + wq * 32 < p.Lq);
       if (lane == 0) bulk_wait_read<0>();
     }
     __syncwarp();
@@ -1301,6 +1341,12 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
   // query tiles with a row that sees one of these keys
   const int q_tiles = (p.Lq + kCols - 1) / kCols;
   const int first = p.causal ? max(0, j0 - p.q_offset) / kCols : 0;
+  unsigned top = 0;
+  if constexpr (!BF16) {  // (not looked at where the sample has no keys, and the bounds no values)
+    const int n_tops = (p.Lq + kRows - 1) / kRows * 4;
+    const unsigned* src = p.tops + (static_cast<long long>(b) * p.H + h) * n_tops;
+    for (int t = threadIdx.x; t < n_tops; t += C::kThreads) top = max(top, src[t]);
+  }
 
   auto load_q = [&](int t) {
     const int st = t % ST;
@@ -1341,7 +1387,12 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
-  const BiasLine bias = load_bias(p, h, warps + 8 * C::kWarp, C::kThreads);
+  unsigned* tops = reinterpret_cast<unsigned*>(warps + 8 * C::kWarp);  // fp16: a bound of |dS| per warp
+  if constexpr (!BF16) {
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[warp] = top;
+  }
+  const BiasLine bias = load_bias(p, h, tops + 16, C::kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1415,7 +1466,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     float* rowv = line + 160;  // -lse and -delta of the half tile's 32 query rows
     const uint64_t scale2 = f2_pack(p.scale * kLog2e, p.scale * kLog2e);
     const bool key_ok = j < klen;
-    const long long hbase = (static_cast<long long>(b) * p.H + h) * p.Lq;
+    const unsigned head = static_cast<unsigned>(b) * p.H + h;
     // Row values of tile t for this lane: loaded a tile ahead, looked at when their tile begins.
     // -inf: no such row, or one without keys; every P is 0.
     float next_lse = -kInf, next_delta = 0.f;
@@ -1423,8 +1474,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const int i = (first + t) * kCols + half * 32 + lane;
       next_lse = -kInf;
       if (t < n && i < p.Lq) {
-        next_lse = p.lse[hbase + i];
-        next_delta = p.delta[hbase + i];
+        next_lse = p.lse[static_cast<long long>(head) * p.Lq + i];
+        next_delta = p.delta[static_cast<long long>(head) * p.Lq + i];
       }
     };
     load_rows(0);
@@ -1436,7 +1487,14 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     // masked: rows past Lq, keys past klen, or (causal) a row before one of the keys
     const int t_causal = p.causal ? (jw + 31 - pos0 + kCols - 1) / kCols : 0;
     const bool all_keys = jw + 32 <= klen;
-    const float c_left = bias.at(-bias.reach), c_right = bias.at(bias.reach);
+    if (lane == 0) {  // (in shared memory: registers are short)
+      line[64] = bias.at(-bias.reach);
+      line[65] = bias.at(bias.reach);
+    }
+    auto ds_scale = [&] {  // fp16: log2 of dS's factor
+      return grad_scale(__reduce_max_sync(0xffffffffu, lane < C::kThreads / 32 ? tops[lane] : 0u));
+    };
+    const float ds_mult = BF16 ? 1.f : exp2_int(ds_scale() - kPScale);  // (P carries the rest)
     bool ok = true;
     for (int t = 0; t < n; ++t) {
       const int pos = pos0 + t * kCols;
@@ -1444,8 +1502,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       const bool masked = !all_keys || t < t_causal || i_half + 32 > p.Lq;
       const bool flat = !masked && (t >= t_left || t < t_right);
       __syncwarp();
-      rowv[lane] = next_lse == -kInf ? -kInf : -next_lse;
-      rowv[32 + lane] = -next_delta;
+      rowv[lane] = next_lse == -kInf ? -kInf : BF16 ? -next_lse : kPScale - next_lse;
+      rowv[32 + lane] = BF16 ? -next_delta : -next_delta * ds_mult;
       if (!flat) {
         // diagonal of (key lane, query e): d_lo + 31 + lane - e
         const int d_lo = jw - pos - 31;
@@ -1462,7 +1520,7 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
       tmem_ld32x2(ts, s, ts + kCols, g);
       uint32_t wp[16], wd[16];
       auto transform = [&](auto is_flat, auto is_masked) {
-        const float c = t >= t_left ? c_left : c_right;
+        const float c = line[t >= t_left ? 64 : 65];
         const uint64_t c2 = f2_pack(c, c);
         const float* ln = line + 31 + lane;
         const int from = !key_ok ? 32 : (p.causal ? j - pos : 0), to = p.Lq - i_half;
@@ -1482,7 +1540,8 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
               add = fadd2(f2_pack(ln[-q], ln[-q - 1]), nl[u]);
             }
             uint64_t pr = exp2_2(ffma2(f2_pack(s[q], s[q + 1]), scale2, add));
-            uint64_t ds = fmul2(pr, fadd2(f2_pack(g[q], g[q + 1]), nd[u]));
+            const uint64_t g2 = f2_pack(g[q], g[q + 1]);
+            uint64_t ds = fmul2(pr, BF16 ? fadd2(g2, nd[u]) : ffma2(g2, f2_pack(ds_mult, ds_mult), nd[u]));
             float p0, p1, d0, d1;
             f2_unpack(pr, p0, p1);
             f2_unpack(ds, d0, d1);
@@ -1519,11 +1578,13 @@ __global__ void __launch_bounds__(Bwd<D>::kThreads, Bwd<D>::kCtas)
     }
     // Warps 2-5 write dV, warps 6-9 dK (through the tiles' shared memory); keys past the sample's
     // length get 0.
+    const float mult =
+        half == 0 ? (BF16 ? 1.f : exp2_int(-kPScale)) : (BF16 ? p.scale : p.scale * exp2_int(-ds_scale()));
 #pragma unroll 1
     for (int c = 0; c < D / 64; ++c)
       store_rows64<BF16>(half == 0 ? &tmDv : &tmDk, (half == 0 ? sV : sK) + c * 16384 + wq * 4096,
                          (half == 0 ? tmem_dv : tmem_dk) + lane_off + c * 64, n > 0 && ok, !key_ok,
-                         half == 0 ? 1.f : p.scale, lane, c * 64, h, jw, b, jw < p.Lk);
+                         mult, lane, c * 64, h, jw, b, jw < p.Lk);
     if (lane == 0) bulk_wait_read<0>();
     __syncwarp();
   }
@@ -1730,7 +1791,8 @@ int wdit_rel_attention(const void* q, const long long* q_strides, const void* k,
 long long wdit_rel_attention_backward_workspace_bytes(int B, int H, int Lq, int n_bounds, int bidirectional) {
   if (B <= 0 || H <= 0 || Lq <= 0 || n_bounds < 1) return 0;
   const long long q_tiles = (Lq + kRows - 1) / kRows;
-  return align16(4ll * B * H * Lq) + 4ll * H * B * q_tiles * rel_num_buckets(n_bounds, bidirectional);
+  return align16(4ll * B * H * Lq) + 16ll * H * B * q_tiles +
+         4ll * H * B * q_tiles * rel_num_buckets(n_bounds, bidirectional);
 }
 
 int wdit_rel_attention_backward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
@@ -1770,7 +1832,8 @@ int wdit_rel_attention_backward(const void* q, const long long* q_strides, const
   p.lse = const_cast<float*>(lse);
   p.splits = 1;
   p.delta = static_cast<float*>(workspace);
-  p.table_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align16(4ll * B * H * Lq));
+  p.tops = reinterpret_cast<unsigned*>(static_cast<char*>(workspace) + align16(4ll * B * H * Lq));
+  p.table_part = reinterpret_cast<float*>(p.tops + 4ll * B * H * ((Lq + kRows - 1) / kRows));
   if ((rc = error_record_ptr(&p.ctx.rec))) return rc;
   p.ctx.limit_ns = wait_limit_ns();
   const bool bf16 = dtype == 1;

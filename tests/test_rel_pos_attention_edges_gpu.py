@@ -157,3 +157,98 @@ def test_masks_of_minus_infinity_hide_and_nan_stays(pkg):
     table[3, 1] = torch.nan
     out = pkg.ops.rel_pos_attention(q, k, v, table)
     assert not out[:, :, 0].any() and out[:, 4:, 1].isnan().all() and out[:, :3, 1].isfinite().all()
+
+
+def significand(t, bits):
+    """Rounded to so many bits, at any exponent."""
+    m, e = torch.frexp(t)
+    return torch.ldexp(torch.round(m * 2.0**bits) * 2.0**-bits, e)
+
+
+def gradients64(pkg, q, k, v, table, dout, *, bits=None, **kw):
+    """dq, dk, dv in 64 bits; bits: P and dS rounded to that significand, at any exponent."""
+    p, _ = probabilities(pkg, q, k, table, **kw)
+    scale = kw.get("scale", q.shape[-1] ** -0.5)
+    q, k, v, do = (t.double().transpose(1, 2) for t in (q, k, v, dout))
+    dp = do @ v.transpose(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    if bits is not None:
+        p, ds = significand(p, bits), significand(ds, bits)
+    res = scale * (ds @ k), scale * (ds.transpose(-1, -2) @ q), p.transpose(-1, -2) @ do
+    return [t.transpose(1, 2) for t in res]
+
+
+def as_good_as_rounding(pkg, got, q, k, v, table, dout, **kw):
+    """fp16 gradients may be off by twice what rounding P and dS to its 11 bits (without the ends of its
+    range) and then the results to fp16 gives; errors are sums of thousands of independent roundings,
+    so their norms agree to a few per cent. fp32 sums lie far below."""
+    exact = gradients64(pkg, q, k, v, table, dout, **kw)
+    rounded = gradients64(pkg, q, k, v, table, dout, bits=11, **kw)
+    for name, g, e, r in zip(("dq", "dk", "dv"), got, exact, rounded):
+        allowed = 2 * (r.to(torch.float16).double() - e).norm()
+        assert g.isfinite().all() and e.norm() > 0, name
+        assert (g.double() - e).norm() <= allowed, (name, ((g.double() - e).norm() / e.norm()).item(),
+                                                   (allowed / e.norm()).item())
+
+
+@pytest.mark.parametrize("std", [1.0, 1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("B,H,Lq,Lk,D,kw", [
+    (1, 2, 512, 2048, 64, {}), (1, 2, 300, 4096, 128, {}), (2, 3, 257, 333, 64, dict(causal=True, q_offset=40)),
+    (1, 1, 3000, 77, 128, {}), (1, 2, 1, 1000, 64, {})])
+def test_fp16_gradients_of_any_loss_scale(pkg, B, H, Lq, Lk, D, kw, std):
+    q, k, v, table, dout = make(B, H, Lq, Lk, D, torch.float16, seed=5)
+    dout = (dout.float() * std).to(torch.float16)
+    got = out_and_gradients(pkg, q, k, v, table, dout, **kw)
+    as_good_as_rounding(pkg, got[1:4], q, k, v, table, dout, **kw)
+
+
+def test_fp16_gradients_of_rows_of_different_sizes(pkg):
+    """Each row's dq has its own factor."""
+    q, k, v, table, dout = make(1, 2, 300, 1500, 64, torch.float16, seed=6)
+    size = torch.tensor([1.0, 1e-3, 1e-4], device=DEV).repeat(100)
+    dout = (dout.float() * size[None, :, None, None]).to(torch.float16)
+    got = out_and_gradients(pkg, q, k, v, table, dout)
+    as_good_as_rounding(pkg, got[1:4], q, k, v, table, dout)
+    exact, rounded = (gradients64(pkg, q, k, v, table, dout, bits=b)[0] for b in (None, 11))
+    for n in range(3):
+        e = exact[:, n::3]
+        assert (got[1][:, n::3].double() - e).norm() <= 2 * (rounded[:, n::3].to(torch.float16).double() - e).norm(), n
+
+
+def test_fp16_gradients_of_many_flat_keys(pkg):
+    """P is 2^-16 here, below fp16's normal numbers."""
+    q, k, v, table, dout = make(1, 1, 70, 1 << 16, 64, torch.float16, seed=7)
+    got = out_and_gradients(pkg, q, k, v, table, dout, scale=0.03)
+    as_good_as_rounding(pkg, got[1:4], q, k, v, table, dout, scale=0.03)
+
+
+def test_fp16_gradients_whose_score_gradients_pass_the_type(pkg):
+    """dS reaches 10^6, dq, dk and dv do not."""
+    q, k, v, table, dout = make(1, 2, 100, 90, 64, torch.float16, seed=8)
+    q, k, v, dout = ((t.float() * f).to(torch.float16) for t, f in ((q, 2.0**-9), (k, 2.0**-9), (v, 200), (dout, 200)))
+    p, _ = probabilities(pkg, q, k, table * 3)
+    dp = dout.double().transpose(1, 2) @ v.double().permute(0, 2, 3, 1)
+    assert (p * (dp - (p * dp).sum(-1, keepdim=True))).abs().max() > 65504
+    got = out_and_gradients(pkg, q, k, v, table * 3, dout)
+    as_good_as_rounding(pkg, got[1:4], q, k, v, table * 3, dout)
+
+
+def test_fp16_gradients_beside_a_row_without_a_number(pkg):
+    """An infinity in one query's gradient reaches what that query touches and nothing else."""
+    q, k, v, table, dout = make(2, 2, 130, 150, 64, torch.float16, seed=9)
+    want = out_and_gradients(pkg, q, k, v, table, dout)
+    dout = dout.clone()
+    dout[1, 7, 0, 3] = torch.inf
+    got = out_and_gradients(pkg, q, k, v, table, dout)
+    keep = torch.ones(2, 130, 2, dtype=torch.bool, device=DEV)
+    keep[1, 7, 0] = False
+    assert torch.equal(got[1][keep], want[1][keep])
+    for n in (2, 3):
+        assert torch.equal(got[n][0], want[n][0]) and torch.equal(got[n][1, :, 1], want[n][1, :, 1])
+    assert torch.equal(got[4][:, 1], want[4][:, 1])
+
+
+def test_fp16_gradients_of_nothing_are_zero(pkg):
+    q, k, v, table, dout = make(1, 2, 70, 90, 64, torch.float16, seed=10)
+    got = out_and_gradients(pkg, q, k, v, table, torch.zeros_like(dout))
+    assert not any(t.any() for t in got[1:])
