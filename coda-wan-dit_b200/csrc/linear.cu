@@ -202,12 +202,14 @@ __device__ __forceinline__ void apply_act(float (&v)[N], int act) {
   }
 }
 
-// act'(x) of two columns. Past |x| = 20 each is 0 or 1 to fp32; the cut keeps x^2 finite (NaN passes).
+// act'(x) of two columns, cut where it is 0 or 1 in fp32 so that x, x^2 and infinities make no inf * 0
+// (NaN passes): GELU's from 20 on (at -15 both are below 2^-126), SiLU's, (1 + x) e^x on the left, from 100 on.
 template <int ACT>
 __device__ __forceinline__ uint64_t act_grad2(float a, float b) {
   if constexpr (ACT == kRelu) return f2_pack(a > 0.f ? 1.f : 0.f, b > 0.f ? 1.f : 0.f);
-  if (fabsf(a) > 20.f) a = copysignf(20.f, a);
-  if (fabsf(b) > 20.f) b = copysignf(20.f, b);
+  constexpr float kCut = ACT == kSilu ? 100.f : 20.f;
+  if (fabsf(a) > kCut) a = copysignf(kCut, a);
+  if (fabsf(b) > kCut) b = copysignf(kCut, b);
   const uint64_t x = f2_pack(a, b);
   if constexpr (ACT == kSilu) {  // s + x s (1 - s)
     const uint64_t s = rcp_2(fadd2(exp2_2(fmul2(x, splat2(-kLog2e))), splat2(1.f)));
