@@ -6,7 +6,8 @@
 * ``linear_act_residual``: act(x W^T + bias) + residual in one kernel, with its gradients.
 
 Public names are re-exported by ``ops``, beside the GEMM and position-table ops of the block.
-Differentiable ops take part in autograd (first order); the others do not.
+Differentiable ops take part in autograd (first order, reverse mode); forward-mode derivatives are
+refused.
 """
 from __future__ import annotations
 
@@ -15,6 +16,7 @@ from functools import lru_cache
 from operator import index
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -46,6 +48,14 @@ def _require_cuda(*ts: torch.Tensor | None) -> int:
     if dev < 0:
         raise RuntimeError("wdit ops run on CUDA tensors only (no CPU implementation)")
     return dev
+
+
+def _refuse_tangents(*ts: torch.Tensor | None) -> None:
+    """The ops have no forward-mode derivatives: a dual tensor's tangent would be lost silently."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("forward-mode derivatives are not implemented for the encoder ops")
 
 
 class _on_device:
@@ -162,6 +172,7 @@ def rel_pos_bias_grad(dbias: torch.Tensor, num_buckets: int, *, bidirectional: b
     or fp16) by their bucket. Sums are fp32 in a fixed order (results repeat bit for bit) and
     rounded once to dtype (fp32, bf16 or fp16)."""
     dev = _require_cuda(dbias)
+    _refuse_tangents(dbias)
     if dbias.dim() == 3:
         dbias = dbias.unsqueeze(0)
     if dbias.dim() != 4:
@@ -214,6 +225,7 @@ def rel_pos_bias(table: torch.Tensor, q_len: int, k_len: int, *, bidirectional: 
     _check_positions(q_len, k_len, q_offset)
     rel_pos_bounds(table.shape[0], max_distance, bidirectional)  # refuses what the rule does not cover
     _require_cuda(table)
+    _refuse_tangents(table)
     if torch.is_grad_enabled() and table.requires_grad:
         return _RelPosBias.apply(table, q_len, k_len, bidirectional, max_distance, q_offset)
     return _rel_pos_bias(table, q_len, k_len, bidirectional, max_distance, q_offset)
@@ -345,6 +357,7 @@ def linear_act_residual(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | N
     if out is not None and (out.shape != shape or out.dtype is not dtype):
         raise ValueError(f"out must be {shape} of {dtype}, got {tuple(out.shape)} {out.dtype}")
     dev = _require_cuda(x, w, bias, residual, out)
+    _refuse_tangents(x, w, bias, residual)
     if torch.is_grad_enabled() and (
             x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)
             or (residual is not None and residual.requires_grad) or (out is not None and out.requires_grad)):
@@ -509,6 +522,7 @@ def rel_pos_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
             raise ValueError(f"k_lens must be [{B}] int32, got {tuple(k_lens.shape)} {k_lens.dtype}")
         k_lens = k_lens.contiguous()
     dev = _require_cuda(q, k, v, table, k_lens)
+    _refuse_tangents(q, k, v, table)
     scale = D**-0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
         return _RelPosAttention.apply(q, k, v, table, k_lens, bidirectional, causal, max_distance, q_offset, scale)
