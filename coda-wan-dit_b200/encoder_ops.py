@@ -165,12 +165,43 @@ def _rel_pos_bias(table, q_len, k_len, bidirectional, max_distance, q_offset):
     return out
 
 
+def _rel_pos_bias_grad(dbias, num_buckets, bidirectional, max_distance, q_offset, dtype):
+    dev = dbias.get_device()
+    B, H, Lq, Lk = dbias.shape
+    bounds, n = _bounds_arg(num_buckets, max_distance, bidirectional)
+    with _on_device(dev):
+        if Lk > 1 and dbias.stride(3) != 1:
+            dbias = dbias.contiguous()
+        out = torch.empty((num_buckets, H), dtype=dtype, device=dbias.device)
+        nbytes = _workspace_bytes(dev, "wdit_rel_pos_bias_grad_workspace_bytes", B, H, Lq, Lk, n, int(bidirectional))
+        ws = _workspace(nbytes, dbias.device)
+        sb, sh, si, _ = dbias.stride()
+        call("wdit_rel_pos_bias_grad", dbias.data_ptr(), _DTYPE[dbias.dtype], B, H, Lq, Lk, sb, sh, si, bounds, n,
+             bidirectional, q_offset, out.data_ptr(), _DTYPE[dtype], ptr(ws), nbytes, _stream(dev), kernels=2)
+    return out
+
+
+class _RelPosBiasGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, dbias, num_buckets, bidirectional, max_distance, q_offset, dtype):
+        ctx.args = (*dbias.shape[2:], bidirectional, max_distance, q_offset)
+        ctx.batch, ctx.dtype = dbias.shape[0], dbias.dtype
+        return _rel_pos_bias_grad(dbias, num_buckets, bidirectional, max_distance, q_offset, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        # a cell's gradient is its bucket's (rounded before it is copied to the cells)
+        d = _rel_pos_bias(g.to(ctx.dtype), *ctx.args)
+        return d.expand(ctx.batch, *d.shape), None, None, None, None, None
+
+
 def rel_pos_bias_grad(dbias: torch.Tensor, num_buckets: int, *, bidirectional: bool = True, max_distance: int = 128,
                       q_offset: int = 0, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Gradient of rel_pos_bias's table: dtable [num_buckets, H], the sum of the cells of dbias
     ([H, Lq, Lk], or [B, H, Lq, Lk] summed over the batch the bias was broadcast to; fp32, bf16
     or fp16) by their bucket. Sums are fp32 in a fixed order (results repeat bit for bit) and
-    rounded once to dtype (fp32, bf16 or fp16)."""
+    rounded once to dtype (fp32, bf16 or fp16). Differentiable in dbias."""
     dev = _require_cuda(dbias)
     _refuse_tangents(dbias)
     if dbias.dim() == 3:
@@ -185,17 +216,9 @@ def rel_pos_bias_grad(dbias: torch.Tensor, num_buckets: int, *, bidirectional: b
     if not 1 <= H <= MAX_HEADS or B > MAX_EXTENT:
         raise ValueError(f"1 to {MAX_HEADS} heads and at most 2^30 samples, got {H} and {B}")
     _check_positions(Lq, Lk, q_offset)
-    bounds, n = _bounds_arg(num_buckets, max_distance, bidirectional)
-    with _on_device(dev):
-        if Lk > 1 and dbias.stride(3) != 1:
-            dbias = dbias.contiguous()
-        out = torch.empty((num_buckets, H), dtype=dtype, device=dbias.device)
-        nbytes = _workspace_bytes(dev, "wdit_rel_pos_bias_grad_workspace_bytes", B, H, Lq, Lk, n, int(bidirectional))
-        ws = _workspace(nbytes, dbias.device)
-        sb, sh, si, _ = dbias.stride()
-        call("wdit_rel_pos_bias_grad", dbias.data_ptr(), _DTYPE[dbias.dtype], B, H, Lq, Lk, sb, sh, si, bounds, n,
-             bidirectional, q_offset, out.data_ptr(), _DTYPE[dtype], ptr(ws), nbytes, _stream(dev), kernels=2)
-    return out
+    if torch.is_grad_enabled() and dbias.requires_grad:
+        return _RelPosBiasGrad.apply(dbias, num_buckets, bidirectional, max_distance, q_offset, dtype)
+    return _rel_pos_bias_grad(dbias, num_buckets, bidirectional, max_distance, q_offset, dtype)
 
 
 class _RelPosBias(torch.autograd.Function):
