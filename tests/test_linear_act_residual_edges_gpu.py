@@ -3,6 +3,7 @@ and its derivative."""
 import math
 
 import pytest
+import test_linear_act_residual_gpu as base
 import torch
 
 pytestmark = pytest.mark.gpu
@@ -65,3 +66,46 @@ def test_every_value_through_the_activation_and_its_derivative(pkg, act, dtype, 
     within(out.detach(), y, (h + 2.0**-15) * y.abs() + below + 2.0**-119)  # x to 2^7 there
     keep = slope * size < torch.finfo(dtype).max
     within(dx[keep], (slope * size)[keep], (h * slope.abs() * size + 2.0**-15 * terms * size + below + size * 2.0**-119)[keep])
+
+
+# The comparisons of test_linear_act_residual_gpu.py ask for an error above the tolerance, which NaN never
+# is: the same calls, cell by cell a number.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", base.SHAPES)
+def test_every_form_gives_numbers(pkg, m, n, k, dtype):
+    for i, act in enumerate(base.ACTS):
+        x, w, b, r = base.make(m, n, k, dtype, bias=i != 1, residual=i != 2, seed=i)
+        assert pkg.ops.linear_act_residual(x, w, b, act=act, residual=r).isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", base.ACTS)
+@pytest.mark.parametrize("m,n,k", base.GRAD_SHAPES)
+def test_gradients_are_numbers(pkg, m, n, k, act, dtype):
+    ts = [t.requires_grad_() for t in base.make(m, n, k, dtype, seed=11)]
+    dout = torch.randn(m, n, generator=torch.Generator().manual_seed(12)).to(dtype).to(DEV)
+    out = pkg.ops.linear_act_residual(ts[0], ts[1], ts[2], act=act, residual=ts[3])
+    assert all(t.isfinite().all() for t in (out.detach(), *torch.autograd.grad(out, ts, dout)))
+
+
+@pytest.mark.parametrize("m", [1, 40, 400])
+def test_views_and_bias_types_give_numbers(pkg, m):
+    for bias_dtype in (torch.float32, torch.bfloat16, torch.float16):
+        x, w, _, r = base.make(m, 264, 512, torch.bfloat16)
+        b = torch.randn(300).to(bias_dtype).to(DEV)[3:267]
+        assert pkg.ops.linear_act_residual(x, w, b, act="silu", residual=r).isfinite().all()
+    wide = torch.randn(m + 3, 600).to(torch.bfloat16).to(DEV)
+    for lo in (0, 8, 3):
+        _, w, b, r = base.make(m, 136, 520, torch.bfloat16)
+        assert pkg.ops.linear_act_residual(wide[1:m + 1, lo:lo + 520], w, b, residual=r).isfinite().all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1536, 8960), (300, 768, 1024), (513, 4608, 1536), (2049, 4104, 200)])
+def test_no_cell_is_left_unwritten(pkg, m, n, k):
+    """out= filled with NaN first, in every tile form; nothing behind it is touched."""
+    x, w, b, r = base.make(m, n, k, torch.bfloat16)
+    room = torch.full((m * n + 1024,), torch.nan, dtype=torch.bfloat16, device=DEV)
+    out = room[:m * n].view(m, n)
+    pkg.ops.linear_act_residual(x, w, b, act="gelu", residual=r, out=out)
+    assert out.isfinite().all() and room[m * n:].isnan().all()
+    base.check_forward(out, x, w, b, r, "gelu")
