@@ -35,7 +35,8 @@ def buckets(pkg, lq, lk, nb, md, bi, off):
     return torch.searchsorted(bounds, n, right=True) + (d > 0) * (nb // 2 if bi else 0)
 
 
-def probabilities(pkg, q, k, table, *, scale=None, causal=False, bidirectional=True, max_distance=128, q_offset=0):
+def probabilities(pkg, q, k, table, *, scale=None, causal=False, bidirectional=True, max_distance=128, q_offset=0,
+                  k_lens=None):
     """P in 64 bits and the error that 32-bit scores leave in it, relative (see below)."""
     B, Lq, H, D = q.shape
     Lk, scale = k.shape[1], D**-0.5 if scale is None else scale
@@ -45,11 +46,15 @@ def probabilities(pkg, q, k, table, *, scale=None, causal=False, bidirectional=T
     seen = torch.ones(Lq, Lk, dtype=torch.bool, device=DEV)
     if causal:
         seen = torch.arange(Lk, device=DEV)[None] <= torch.arange(Lq, device=DEV)[:, None] + q_offset
+    if k_lens is not None:
+        seen = seen & (torch.arange(Lk, device=DEV)[None] < k_lens[:, None])[:, None, None]
     z = torch.where(seen, z, -torch.inf)
     # a score: D fp32 adds of exact products, scaling, bias, maximum (and its power of two): a step each
-    size = abs(scale) * (q.abs() @ k.abs().transpose(-1, -2)) + bias.abs() + z.amax(-1, keepdim=True).abs() + 28
+    top = z.amax(-1, keepdim=True)
+    size = abs(scale) * (q.abs() @ k.abs().transpose(-1, -2)) + bias.abs() + top.abs() + 28
     dz = (D + 4) * 2.0**-23 * torch.where(seen, size, 0.0)
-    return torch.softmax(z, -1), 2 * dz.amax(-1, keepdim=True) + 2.0**-20
+    p = torch.where(top == -torch.inf, 0.0, torch.softmax(z, -1))  # a row without keys
+    return p, 2 * dz.amax(-1, keepdim=True) + 2.0**-20
 
 
 def within(got, want, tol):
@@ -252,3 +257,48 @@ def test_fp16_gradients_of_nothing_are_zero(pkg):
     q, k, v, table, dout = make(1, 2, 70, 90, 64, torch.float16, seed=10)
     got = out_and_gradients(pkg, q, k, v, table, torch.zeros_like(dout))
     assert not any(t.any() for t in got[1:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kw", [dict(), dict(lens=True), dict(causal=True, bidirectional=False), dict(causal=True, lens=True)])
+@pytest.mark.parametrize("B,H,Lq,Lk,D", [(2, 3, 5, 7, 128), (3, 2, 129, 257, 64), (1, 2, 64, 1000, 128), (3, 3, 640, 65, 64),
+                                         (3, 3, 900, 2, 64), (3, 3, 900, 5, 128), (2, 3, 1500, 280, 64)])
+def test_gradients_with_delta_from_fp32_sums(pkg, B, H, Lq, Lk, D, kw, dtype):
+    """delta = rowsum(P dP) is an fp32 sum of what dS is made of, not of the rounded output: no cell of dS, and
+    no bucket of the table, whose cells cancel, carries half a step of a 16-bit type of |dO| |out|."""
+    q, k, v, table, dout = make(B, H, Lq, Lk, D, dtype, seed=11)
+    kw = dict(kw, q_offset=max(0, Lk - Lq) if "causal" in kw else 0)
+    if kw.pop("lens", False):
+        kw["k_lens"] = torch.tensor([Lk, max(1, Lk // 2), 0][:B], dtype=torch.int32, device=DEV)
+    got = out_and_gradients(pkg, q, k, v, table, dout, **kw)
+    p, eps = probabilities(pkg, q, k, table, **kw)
+    where = buckets(pkg, Lq, Lk, 32, 128, kw.get("bidirectional", True), kw["q_offset"]).flatten()
+    U, h, scale = 2.0**-23, torch.finfo(dtype).eps / 2, D**-0.5
+    q, k, v, do = (t.double().transpose(1, 2) for t in (q, k, v, dout))
+    dp = do @ v.transpose(-1, -2)
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_dp = (D + 2) * U * (do.abs() @ v.abs().transpose(-1, -2))
+    e_delta = (p * ((eps + (Lk + 2) * U) * dp.abs() + e_dp)).sum(-1, keepdim=True)
+    e_ds = p * (eps * (dp - delta).abs() + e_dp + e_delta)
+    # operands of 16 bits: half a step, and in fp16 2^-38 of the bound that dS was taken up to 2^14 by
+    # (2^-39 of P, which is at most 1)
+    cell, cell_k, cell_p = h * (ds.abs() + e_ds), 0.0, 0.0
+    if dtype == torch.float16:
+        bound = (p * dp.abs()).amax(-1, keepdim=True) + delta.abs()
+        cell, cell_k, cell_p = cell + 1.1 * 2.0**-38 * bound, 1.1 * 2.0**-38 * bound.amax(-2, keepdim=True), 2.0**-39
+    tiny = torch.finfo(dtype).smallest_normal * h
+
+    def near(got, want, tol):
+        within(got, want.transpose(1, 2), (tol + 1.01 * h * (want.abs() + tol) + tiny).transpose(1, 2))
+
+    near(got[1], scale * (ds @ k), scale * ((e_ds + cell + Lk * U * ds.abs()) @ k.abs()))
+    near(got[2], scale * (ds.transpose(-1, -2) @ q),
+         scale * ((e_ds + cell + cell_k + Lq * U * ds.abs()).transpose(-1, -2) @ q.abs()))
+    near(got[3], p.transpose(-1, -2) @ do, (p * (eps + h + Lq * U) + cell_p).transpose(-1, -2) @ do.abs())
+    depth = 32 + 16 + 5 + 2 * (Lk // 32 + 2) + 8 + B * (Lq // 128 + 1)  # adds a cell of the table's sums passes
+    for head in range(H):
+        want, tol = (torch.zeros(32, dtype=torch.float64, device=DEV) for _ in range(2))
+        want.index_add_(0, where, ds[:, head].sum(0).flatten())
+        tol.index_add_(0, where, (e_ds + depth * U * (ds.abs() + e_ds))[:, head].sum(0).flatten())
+        within(got[4][:, head], want, tol + 2.0**-24 * want.abs() + 1e-30)
