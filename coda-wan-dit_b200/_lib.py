@@ -93,6 +93,7 @@ _SIGNATURES = {
                                             P, P, P, P, I, P, c_longlong, P]),
     "wdit_linear_act_residual": (c_int, [P, c_longlong, I, P, c_longlong, I, I, I, I, I, P, I, I, P, c_longlong, P,
                                          c_longlong, P, c_longlong, P]),
+    "wdit_linear_act_residual_form": (c_int, [I, I, I, I, P]),
     "wdit_act_backward_workspace_bytes": (c_longlong, [I, I]),
     "wdit_act_backward": (c_int, [P, c_longlong, P, c_longlong, I, I, I, I, P, c_longlong, P, I, P, c_longlong, P]),
     "wdit_ulysses_pack": (c_int, [P, I, I, I, I, I, I, I, P, P]),

@@ -807,12 +807,18 @@ struct Plan {
 // 128 x 256 548; pairs 256 x 192 394, 256 x 256 530), and all CTAs together load about 11 KB a clock
 // from L2 (128 x 128 tiles on every SM: 418 instead of 270). The last tile's epilogue adds 17 clocks
 // per column (12 bare, 30 with GELU), an exchange between splits 4200 and 0.45 per element that
-// crosses. What that picks
-// (us; next best in brackets):   1 x 1536 x 8960 split 8 of 128 x 128 11.3 (one CTA a tile 46)
-//   256 x 1536 x 8960 split 4 15.6 (pairs, no split 47)   1024 x 1536 x 4096 128 x 128 15.6 (pairs 16.8)
-//   2048 x 1536 x 8960 pairs 256 x 192 42.5 (128 x 192 46.1)   1024 x 8960 x 1536 pairs 256 x 256 23.0
+// crosses. What that picks (wdit_linear_act_residual_form) and what else was measured (bf16, us a launch,
+// twenty in a graph):
+//   1024 x 1536 x 4096  pairs 256 x 128 15.7 (halves of K over 128 x 192 17.3, 128 x 128 18.1, pairs 256 x 192 20.0)
+//   256 x 1536 x 8960   quarters of K over pairs 256 x 128 15.8 (over 128 x 128 16.3, halves 19.1)
+//   2048 x 1536 x 8960  pairs 256 x 192 43.8 (128 x 192 46.7, pairs 256 x 256 48.8)
+//   1024 x 8960 x 1536  pairs 256 x 256 24.8 (pairs 256 x 128 25.0)
+// and where it misses by more than a twentieth:
+//   1 x 1536 x 8960     eighths of K over 128 x 128 13.4 (over 128 x 192 11.0, over 128 x 256 11.9)
+//   1 x 4096 x 10240    quarters of K over 128 x 128 22.6 (over 128 x 256 18.6)
 // With B MN-major a 256 x 192 pair tile stages 128 rows of B a CTA for the 96 it uses; 5% on its blocks:
-//   4095 x 1536 x 8960 pairs 256 x 192 86.7 (256 x 256 93.5)   4096 x 5120 x 13824 256 x 256 405 (427)
+//   4095 x 1536 x 8960  pairs 256 x 192 87 - 97 by the card's power (128 x 192 99, pairs 256 x 256 104)
+//   4096 x 5120 x 13824 pairs 256 x 256 393 - 451 by the card's power (pairs 256 x 192 451)
 Plan plan(int M, int N, int K, bool mn_b, int sms) {
   const int kb = (K + BK - 1) / BK;
   Plan best = {0, 128, 1};
@@ -937,7 +943,7 @@ int run_linear(const void* A, long long lda, int a_mn, const void* B, long long 
   p.m_blocks = (p.M + BM - 1) / BM;
   p.n_blocks = (p.N + p.bn - 1) / p.bn;
   p.k_blocks = (p.K + BK - 1) / BK;
-  // Tiles go down the rows of a column, or, where B does not stay in L2, through groups of eight rows
+  // Tiles go along the columns of a row block (or pair), or, where B does not stay in L2, down groups of eight row blocks
   // (us: B of 142 MB, 8192 x 13824 x 5120, 768 by groups, 985 without; 34 MB, 4096^3, 93 and 91).
   p.raster_rows = static_cast<long long>(p.N) * p.K * 2 > kRasterBytes ? kRasterRows : 1;
   int rc = error_record_ptr(&p.ctx.rec);
@@ -1021,6 +1027,16 @@ int wdit_linear_act_residual(const void* A, long long lda, int a_mn, const void*
   p.pre = pre_out;
   p.ldp = ldp;
   return run_linear(A, lda, a_mn, B, ldb, b_mn, p, static_cast<cudaStream_t>(stream));
+}
+
+int wdit_linear_act_residual_form(int M, int N, int K, int b_mn, int* form) {
+  if (form == nullptr) return WDIT_ERR_ARG;
+  if (M < 1 || N < 1 || K < 1 || N % 8 != 0 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return WDIT_ERR_SHAPE;
+  const Plan pl = plan(M, N, K, b_mn != 0, sm_count());
+  form[0] = pl.pair;
+  form[1] = pl.bn;
+  form[2] = pl.splits;
+  return WDIT_OK;
 }
 
 long long wdit_act_backward_workspace_bytes(int M, int N) {

@@ -376,6 +376,10 @@ int wdit_linear_act_residual(const void* A, long long lda, int a_mn, const void*
                              int N, int K, int dtype, const void* bias, int bias_dtype, int act, const void* res,
                              long long ldr, void* out, long long ldo, void* pre_out, long long ldp, void* stream);
 
+/* The tile form that such a product takes on the current device (148 SMs without one), into form[3]:
+ * CTA pairs (1) or single CTAs (0), columns of a tile, CTAs (pairs) that share a tile's K range. */
+int wdit_linear_act_residual_form(int M, int N, int K, int b_mn, int* form);
+
 /*
  * dpre[M, N] = dout * act'(pre) and, unless dbias is NULL, dbias[N] (dbias_dtype) = the column sums
  * of dpre before its rounding (fp32 sums in a fixed order). act = 0: dpre is dout, pre and dpre are
