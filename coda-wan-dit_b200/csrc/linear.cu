@@ -21,10 +21,11 @@
 // made it slow (1800 and 3000) were arrivals that release at cluster scope, which wait for all of
 // the thread's stores, bias loads piece by piece, and the tile's place computed for every piece.
 //
-// What bounds it: the tensor pipe for many rows (8192 x 13824 x 5120 fp16 with GELU 761 - 840 us by
-// the card's power, 1.4 - 1.5 PFLOP/s; 4096^3 92 us, the library's product 90), the fixed costs
-// below (1024 x 1536 x 4096 16 us, library 12: set-up 0.9 us, first loads 0.8, last epilogue 1,
-// then 270 clocks a K block at least), the weights' bytes for few (1 x 1536 x 8960 11 us).
+// What bounds it: the tensor pipe for many rows (8192 x 13824 x 5120 fp16 with GELU and residual 836 - 846
+// us, 1.37 - 1.39 PFLOP/s, the pipe 93% busy; in a loop of nothing else 971 by the card's power; 4096^3
+// 93 us, the library's product 90), the fixed costs below (1024 x 1536 x 4096 with bias and tanh-GELU
+// 18.2 us, 15.7 bare in a graph where the library's takes 11.2: set-up 0.9 us, first loads 0.8, last
+// epilogue 1, then 270 clocks a K block at least), the weights' bytes for few (1 x 1536 x 8960 10.6 us).
 // Tile forms (plan()):
 //   pair    256 x bn tiles over CTA pairs (tcgen05 cta_group::2): many rows
 //   single  128 x bn tiles
@@ -943,8 +944,8 @@ int run_linear(const void* A, long long lda, int a_mn, const void* B, long long 
   p.m_blocks = (p.M + BM - 1) / BM;
   p.n_blocks = (p.N + p.bn - 1) / p.bn;
   p.k_blocks = (p.K + BK - 1) / BK;
-  // Tiles go along the columns of a row block (or pair), or, where B does not stay in L2, down groups of eight row blocks
-  // (us: B of 142 MB, 8192 x 13824 x 5120, 768 by groups, 985 without; 34 MB, 4096^3, 93 and 91).
+  // Tiles go along the columns of a row block (or pair), or, where B does not stay in L2, down groups of
+  // eight row blocks (us: B of 142 MB, 8192 x 13824 x 5120, 768 by groups, 985 without; 34 MB, 4096^3, 93 and 91).
   p.raster_rows = static_cast<long long>(p.N) * p.K * 2 > kRasterBytes ? kRasterRows : 1;
   int rc = error_record_ptr(&p.ctx.rec);
   if (rc) return rc;

@@ -24,7 +24,7 @@
 // (table gradient off by, relative, bf16: 5 x 2 heads x 1870 queries x 2 keys x 128 3.9e-2, with O kept
 // in 32 bits still 1.5e-2, and 6e-3 at 2 heads x 2000 x 280 x 128; its own rounding alone is 1.7e-3).
 // So delta is formed from P and dP as dS is, in fp32, in a first pass over the keys: 15 of
-// attn_dq_kernel's 59 us at 2 x 64 heads x 512 x 512 x 64, 33 of 92 at 74 x 512 x 2048.
+// attn_dq_kernel's 58 us at 2 x 64 heads x 512 x 512 x 64, 33 of 92 at 74 x 512 x 2048.
 //
 //   attn_fwd_kernel  CTA = 128 query rows of one head; key tiles of 64; one or two warps load and
 //                    issue MMAs, four are the softmax (one row per thread). With few CTAs the
@@ -35,10 +35,10 @@
 //                    P^T and dS^T are the A operands; dK and dV stay in TMEM.
 //
 // Measured (bf16): forward, 12 heads x 8192 x 8192 x 128 causal 187 - 205 us by the card's power, 1.0 -
-// 1.1 PFLOP/s, tensor pipe 55% and exponentials 55% busy; 2 x 64 heads x 512 x 512 x 64 with lengths
+// 1.1 PFLOP/s, tensor pipe and exponentials 55% busy each; 2 x 64 heads x 512 x 512 x 64 with lengths
 // 512 and 227 22.4 us, of which a CTA's start and end are 4; one query over 8 x 12 heads x 8191 keys x
-// 128 66 us, 6.1 TB/s. Backward at 2 x 64 heads x 512 x 512 x 64: dQ 59 us, dK and dV 47. What bounds
-// the tiles is latency: a score tile passes from the MMAs to a warp and back over two barriers, about
+// 128 66 us, 6.1 TB/s. Backward at 2 x 64 heads x 512 x 512 x 64: dQ 58 us (fp16 63), dK and dV 46. What
+// bounds the tiles is latency: a score tile passes from the MMAs to a warp and back over two barriers, about
 // 200 clocks each behind the other warps' exponentials, besides its TMEM reads; more CTAs per SM,
 // scores read ahead and polynomial exponentials were all slower.
 //
@@ -1605,9 +1605,9 @@ int cuda_rc(cudaError_t e) {
 
 // Key splits of the forward: with fewer CTAs than two per SM (a few query rows of a few heads)
 // one CTA would walk a long cache alone, so the keys are divided until the SMs are full, at least
-// four tiles a part (one query row, us with at least 1 / 4 / 16 tiles a part and undivided: 12 heads
-// x 8191 keys x 128 21.4 / 21.4 / 22.7 / 97, 12 x 1000 x 64 13.0 / 11.9 / 17.7 / 17.7, 8 x 12 x 8191
-// x 128 54.5 / 54.4 / 54.5 / 111).
+// four tiles a part (one query row, bf16, us with at least 1 / 4 / 16 tiles a part and undivided: 12
+// heads x 8191 keys x 128 17.3 / 17.2 / 21.2 / 97, 12 x 1000 x 64 11.0 / 11.9 / 18.2 / 18.1, 8 x 12 x
+// 8191 x 128 66 / 66 / 66 / 115, with lengths from 8191 down to 3291 57.6 / 57.6 / 57.6 / 113).
 int attn_splits(int B, int H, int Lq, int Lk) {
   const long long ctas = static_cast<long long>(B) * H * ((Lq + kRows - 1) / kRows);
   const int tiles = (Lk + kCols - 1) / kCols;
