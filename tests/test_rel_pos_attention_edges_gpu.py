@@ -302,3 +302,52 @@ def test_gradients_with_delta_from_fp32_sums(pkg, B, H, Lq, Lk, D, kw, dtype):
         want.index_add_(0, where, ds[:, head].sum(0).flatten())
         tol.index_add_(0, where, (e_ds + depth * U * (ds.abs() + e_ds))[:, head].sum(0).flatten())
         within(got[4][:, head], want, tol + 2.0**-24 * want.abs() + 1e-30)
+
+
+@pytest.mark.parametrize("nb,md,bi", [(512, 1000, True), (512, 257, True), (256, 256, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_tables_that_fill_shared_memory(pkg, nb, md, bi, dtype):
+    """The largest lines and sums of head size 128: gradients against those of a bias tensor."""
+    q, k, v, table, dout = make(1, 2, 150, 400, 128, dtype, nb=nb, seed=12)
+    kw = dict(max_distance=md, bidirectional=bi, q_offset=30)
+    got = out_and_gradients(pkg, q, k, v, table, dout, **kw)
+    assert all(t.isfinite().all() for t in got)
+    exact = gradients64(pkg, q, k, v, table, dout, **kw)
+    rounded = gradients64(pkg, q, k, v, table, dout, bits=11 if dtype == torch.float16 else 8, **kw)
+    for g, e, r in zip(got[1:4], exact, rounded):
+        assert (g.double() - e).norm() <= 2 * (r.to(dtype).double() - e).norm()
+
+
+def test_fp16_gradients_in_graphs_and_on_two_streams(pkg):
+    """The bounds of dS lie in the call's own workspace."""
+    sets = [make(2, 3, 200, 300, 64, torch.float16, seed=20 + i) for i in range(2)]
+    sets = [(*s[:4], (s[4].float() * 10.0 ** (-2 * i)).to(torch.float16)) for i, s in enumerate(sets)]
+    lens = torch.tensor([300, 111], dtype=torch.int32, device=DEV)
+    leaves = [[t.requires_grad_() for t in s[:4]] for s in sets]
+
+    def step(i):
+        out = pkg.ops.rel_pos_attention(*leaves[i], k_lens=lens)
+        return [out.detach(), *torch.autograd.grad(out, leaves[i], sets[i][4])]
+
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step(i)
+        graphs.append((g, res))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i][0].replay()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, step(i)))
+    torch.cuda.synchronize()
+    for i, res in [*enumerate(g[1] for g in graphs), *got]:
+        assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
