@@ -339,12 +339,12 @@ __device__ __forceinline__ int sample_len(const AttnArgs& p, int b) {
 // the maximum taken anew, O rescaled and the tile done again. What bounds the two:
 //   fp16  P up to 2^15 of its 65504; P v is then far inside fp32.
 //   bf16  v may be as large as fp32 goes, so the row's sum of P stays below 1: at most 2^22 tiles of
-//         at most 2^-22 each. The largest P of a tile whose maximum was taken is 2^-40: the row's
-//         scores may rise by a factor of 2^12 (sums of 64: 2^18) before it is taken anew, P keeps its
-//         relative precision down to 2^-86 of the largest, and O that of |v| from 2^-86 on.
+//         at most 2^-22 each. The largest P of a tile whose maximum was taken is 2^-40: P may rise by
+//         2^18 in one key, 2^12 in all 64 of a tile, before it is taken anew. P keeps its relative
+//         precision down to 2^-86 of the largest, and O that of |v| from 2^-86 on.
 template <bool BF16>
 struct SoftmaxRange {
-  static constexpr float kHeadroom = BF16 ? 40.f : 0.f;                     // log2
+  static constexpr float kHeadroom = BF16 ? 40.f : 0.f;                // log2
   static constexpr float kSumLimit = BF16 ? 2.3841858e-07f : 32768.f;  // 2^-22, 2^15
 };
 
